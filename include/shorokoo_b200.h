@@ -184,6 +184,124 @@ SB_API int32_t sb_session_transfer_bytes(sb_session* session, int32_t n_inputs, 
 SB_API int32_t sb_linear_noalloc(const float* x, const float* w, const float* bias, float* y, int64_t M, int64_t K,
                                  int64_t N, int32_t relu, void* stream);
 
+/* ---- Decoder-layer operators on device tensors (no counterpart in the reference interface) -----
+ * What one layer of a language model runs per step when it answers from a paged cache: a linear
+ * layer with 4-bit weights, rotary positions, the write of new keys and values into the cache and
+ * the attention that reads it. Like sb_linear_noalloc they take the caller's own device buffers and
+ * allocate nothing; unlike it they only enqueue work on `stream` (cudaStream_t of the current
+ * device, NULL = default), so they can be captured into CUDA graphs and calls on several streams
+ * may overlap as long as their outputs and workspaces are different memory. Pointers are device
+ * memory of the current device unless marked (host). Strides count elements. Element types:
+ * SB_ELEM_* (ONNX TensorProto.DataType numbering). */
+#define SB_ELEM_FLOAT 1
+#define SB_ELEM_FLOAT16 10
+#define SB_ELEM_BFLOAT16 16
+
+/* A tensor of heads: element (token, head, d) at data[token * token_stride + head * head_stride + d]. */
+typedef struct sb_heads {
+  void* data;
+  int64_t token_stride, head_stride;
+} sb_heads;
+
+/* Rotary frequencies of rotary_dim / 2 pairs in radians per position (host arrays):
+ * base^(-2i / rotary_dim), changed for contexts `factor` times the trained one by SB_ROTARY_LINEAR
+ * (every frequency divided by factor), SB_ROTARY_NTK (base times factor^(r / (r - 2))) or
+ * SB_ROTARY_BY_PARTS (a pair that turns more than beta_fast times in original_context positions
+ * keeps its frequency, one below beta_slow turns is divided by factor, those between are mixed
+ * linearly in their number of turns; *magnitude = 0.1 ln(factor) + 1, else 1). */
+#define SB_ROTARY_PLAIN 0
+#define SB_ROTARY_LINEAR 1
+#define SB_ROTARY_NTK 2
+#define SB_ROTARY_BY_PARTS 3
+SB_API int32_t sb_rotary_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor,
+                                     double original_context, double beta_fast, double beta_slow,
+                                     double* frequencies, double* magnitude);
+/* Turns per position of each frequency as 64-bit binary fractions (host arrays): what the kernels
+ * multiply positions by, exactly modulo one turn, so that positions of any size and sign keep their
+ * angle to 2^-32 of a turn. The caller copies them to the device for sb_rotary_table.phases. */
+SB_API int32_t sb_rotary_phases(const double* frequencies, int32_t pairs, uint64_t* phases);
+
+/* Pairs (2i, 2i + 1) when interleaved, (i, i + pairs) otherwise, of the first 2 * pairs elements of
+ * a head; the others are copied. Rotated values are multiplied by magnitude. */
+typedef struct sb_rotary_table {
+  const uint64_t* phases;
+  int32_t pairs;
+  int32_t interleaved;
+  float magnitude;
+} sb_rotary_table;
+
+/* y = x with every token's heads turned by its position; inverse != 0 turns by the negative angle,
+ * which is the adjoint (the gradient of x for a gradient of y). x and y: float32, float16 or
+ * bfloat16; y may be x itself, but not overlap it otherwise. positions: int32 or int64, any sign. */
+SB_API int32_t sb_rotary(const sb_heads* x, const sb_heads* y, int32_t elem_type, int64_t tokens, int32_t heads,
+                         int32_t head_dim, const void* positions, int32_t positions_int64,
+                         const sb_rotary_table* table, int32_t inverse, void* stream);
+
+/* A paged cache: position j of sequence b is row j % page_size of page
+ * page_table[b * page_table_stride + j / page_size]. context_lengths[b] counts the sequence's
+ * positions, those of the current step's tokens among them. Positions at or past
+ * max_pages * page_size, and positions whose table entry is outside [0, pages), hold nothing: they
+ * are not written, and attention leaves them out. k, v: float16 or bfloat16. */
+typedef struct sb_paged_cache {
+  void *k, *v;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const int32_t* page_table;
+  const int32_t* context_lengths;
+  int64_t page_table_stride;
+  int64_t pages;
+  int32_t elem_type;
+  int32_t page_size;
+  int32_t max_pages; /* per sequence */
+  int32_t batch;
+  int32_t kv_heads;
+  int32_t head_dim;
+} sb_paged_cache;
+
+/* The step's tokens are packed: sequence b has rows query_starts[b] .. query_starts[b + 1] - 1 of
+ * q, k, v and out (batch + 1 int32, not decreasing), its last positions in order. Rows of no
+ * sequence (before the first, behind the last) are neither read nor written. */
+
+/* Writes k and v of the step's tokens into the cache; with a table, k is turned by its position
+ * first and so is q into q_out (q and q_out NULL: keys alone; q_out may be q itself). Two rows that
+ * share a slot leave either row's values there. Same element type throughout. */
+SB_API int32_t sb_paged_append(const sb_paged_cache* cache, const sb_heads* k, const sb_heads* v, const sb_heads* q,
+                               const sb_heads* q_out, int32_t q_heads, int64_t tokens, const int32_t* query_starts,
+                               const sb_rotary_table* table, void* stream);
+
+/* out = softmax(scale * q k^T) v per query head over the positions at or before the token's own in
+ * its sequence (window > 0: the last `window` of them); query head h reads key head
+ * h / (q_heads / kv_heads). A token that sees nothing gets zeros. Positions that a token does not see
+ * do not reach its output, whatever they hold. head_dim: a multiple of 8 up to 128; data pointers
+ * 16-byte aligned and strides multiples of 8 elements. workspace: 256-byte aligned, at least
+ * sb_paged_attention_workspace bytes, not shared with a call that may overlap. */
+SB_API int32_t sb_paged_attention_workspace(const sb_paged_cache* cache, int32_t q_heads, int64_t tokens, size_t* bytes);
+SB_API int32_t sb_paged_attention(const sb_paged_cache* cache, const sb_heads* q, const sb_heads* out, int32_t q_heads,
+                                  int64_t tokens, const int32_t* query_starts, float scale, int32_t window,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Weights w[n, k] = (code[n, k] - zero[n, k / group_size]) * scale[n, k / group_size] of a linear
+ * layer, codes in 4 bits: byte k / 2 of row n of `packed` holds element k in its low half for even k
+ * and in its high half for odd k. scales [out_features, ceil(in_features / group_size)] float16 or
+ * bfloat16, the type of the layer's inputs; zeros one byte each (0 .. 15), or NULL for 8.
+ * group_size: a multiple of 32. sb_w4_layout puts them, once, into the order that the kernel reads
+ * (sb_w4_layout_bytes, 256-byte aligned); the originals are not needed afterwards. */
+typedef struct sb_w4_weights {
+  const void* data; /* written by sb_w4_layout */
+  int32_t elem_type;
+  int32_t group_size;
+  int64_t out_features, in_features;
+  int32_t has_zeros;
+} sb_w4_weights;
+SB_API int32_t sb_w4_layout_bytes(const sb_w4_weights* weights, size_t* bytes);
+SB_API int32_t sb_w4_layout(const sb_w4_weights* weights, const uint8_t* packed, int64_t packed_row_bytes,
+                            const void* scales, const uint8_t* zeros, void* data, void* stream);
+/* y[rows, out_features] = x[rows, in_features] w^T + bias (NULL: none), meant for few rows: the
+ * weights are read once for every 32 of them. x, bias and y: elem_type; rows contiguous, their
+ * strides in elements. */
+SB_API int32_t sb_linear_w4(const sb_w4_weights* weights, const void* x, int64_t x_row_stride, const void* bias, void* y,
+                            int64_t y_row_stride, int64_t rows, void* stream);
+
 /* ---- Diagnostics (no counterpart in the reference interface) ------------------------------- */
 /* Lowers and fuses the model on the host only (no device needed) for inputs given in session input
  * order, and writes a summary (one line per device op, then "separable=0|1") into buf as a

@@ -17,6 +17,27 @@ CSTR = C.c_char_p
 PSTR = C.POINTER(C.c_char_p)
 PP = C.POINTER(C.c_void_p)
 
+
+class Heads(C.Structure):   # sb_heads
+    _fields_ = [("data", P), ("token_stride", I64), ("head_stride", I64)]
+
+
+class RotaryTable(C.Structure):   # sb_rotary_table
+    _fields_ = [("phases", P), ("pairs", I32), ("interleaved", I32), ("magnitude", C.c_float)]
+
+
+class PagedCache(C.Structure):   # sb_paged_cache
+    _fields_ = [("k", P), ("v", P), ("k_page_stride", I64), ("k_token_stride", I64), ("k_head_stride", I64),
+                ("v_page_stride", I64), ("v_token_stride", I64), ("v_head_stride", I64), ("page_table", P),
+                ("context_lengths", P), ("page_table_stride", I64), ("pages", I64), ("elem_type", I32),
+                ("page_size", I32), ("max_pages", I32), ("batch", I32), ("kv_heads", I32), ("head_dim", I32)]
+
+
+class W4Weights(C.Structure):   # sb_w4_weights
+    _fields_ = [("data", P), ("elem_type", I32), ("group_size", I32), ("out_features", I64), ("in_features", I64),
+                ("has_zeros", I32)]
+
+
 # name: (restype, argtypes)
 SIGNATURES = {
     "sb_version": (I32, []),
@@ -56,6 +77,15 @@ SIGNATURES = {
     "sb_debug_narrow_bf16": (I32, [C.c_void_p, C.c_void_p, SZ, I32]),
     "sb_session_transfer_bytes": (I32, [P, I32, PSTR, PP, C.POINTER(I64), C.POINTER(I64)]),
     "sb_linear_noalloc": (I32, [P, P, P, P, I64, I64, I64, I32, P]),
+    "sb_rotary_frequencies": (I32, [I32, DBL, I32, DBL, DBL, DBL, DBL, P, C.POINTER(DBL)]),
+    "sb_rotary_phases": (I32, [P, I32, P]),
+    "sb_rotary": (I32, [P, P, I32, I64, I32, I32, P, I32, P, I32, P]),
+    "sb_paged_append": (I32, [P, P, P, P, P, I32, I64, P, P, P]),
+    "sb_paged_attention_workspace": (I32, [P, I32, I64, C.POINTER(SZ)]),
+    "sb_paged_attention": (I32, [P, P, P, I32, I64, P, C.c_float, I32, P, SZ, P]),
+    "sb_w4_layout_bytes": (I32, [P, C.POINTER(SZ)]),
+    "sb_w4_layout": (I32, [P, P, I64, P, P, P, P]),
+    "sb_linear_w4": (I32, [P, P, I64, P, P, I64, I64, P]),
 }
 
 

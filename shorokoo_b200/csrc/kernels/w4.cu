@@ -1,0 +1,305 @@
+// Linear layer with 4-bit weights for few rows: y[m, n] = sum_k x[m, k] (c[n, k] - z[n, k/g]) s[n, k/g] + b[n].
+//
+// One row of inputs needs 2 K operations per K / 2 bytes of weights: the weights' bytes bound it (HBM,
+// or L2 where they stay there). The products still go to the tensor core (mma m16n8k16, fp32
+// accumulators): 16 outputs x 8 rows per instruction costs no more than one row would, and takes the
+// multiply-adds off the issue slots, which turning codes into operands needs (about one instruction
+// per weight). c - z is a small integer and exact in either 16-bit type; the group's scale is applied
+// in fp32 to the products' sum over a group, so nothing is rounded but x (given in 16 bits) and y.
+//
+// Layout (w4_layout): tiles of 16 outputs x 64 inputs, 512 bytes each, K running fastest: one 16-byte
+// load per lane is the whole warp's operand for four k16 steps, with all 16 inputs of a step in one
+// group of 32. Lane 4g + t holds outputs g and g + 8, inputs 8t .. 8t + 7 of both 32-input halves, one
+// word each; nibble i and nibble 4 + i of a word are inputs 2i and 2i + 1, so that shifting by 4i and
+// masking gives a register of the operand with its neighbouring pair, and x needs no reordering.
+// Inputs past K and outputs past N are zero codes; x reads as zero there. Behind the tiles, scales
+// as pairs (output g, g + 8) per tile and group, then zero points likewise.
+//
+// A CTA computes 16 outputs: its warps take the 64-input blocks in turn and their sums meet in shared
+// memory, added in a fixed order.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "decoder.h"
+
+namespace sb {
+namespace k {
+namespace {
+
+struct W4Args {
+  const uint4* w;
+  const uint32_t* scales;   // [tile][group][8] pairs
+  const uint16_t* zeros;    // [tile][group][8] pairs of bytes
+  const void* x;
+  const void* bias;
+  void* y;
+  int64_t xs, ys, rows, n, k;
+  int blocks, groups, group;
+};
+
+struct W4Sizes {
+  int64_t tiles, blocks, groups;
+  size_t w, s, z;
+};
+W4Sizes sizes(const W4View& w) {
+  W4Sizes z;
+  z.tiles = (w.n + 15) / 16;
+  z.blocks = (w.k + 63) / 64;
+  z.groups = (w.k + w.group - 1) / w.group;
+  z.w = size_t(z.tiles) * z.blocks * 512;
+  z.s = (size_t(z.tiles) * z.groups * 32 + 255) / 256 * 256;
+  z.z = w.zeros ? (size_t(z.tiles) * z.groups * 16 + 255) / 256 * 256 : 0;
+  return z;
+}
+
+template <typename T> struct Half;
+template <> struct Half<__half> {
+  static constexpr uint32_t kMagic = 0x64006400u;   // 1024: a code in the low mantissa bits reads 1024 + code
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+  static __device__ __forceinline__ float2 both(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
+  static __device__ __forceinline__ float one(__half a) { return __half2float(a); }
+  static __device__ __forceinline__ __half round(float a) { return __float2half_rn(a); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Half<__nv_bfloat16> {
+  static constexpr uint32_t kMagic = 0x43004300u;   // 128: 128 + code, exact in 8 significant bits
+  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
+  static __device__ __forceinline__ float2 both(uint32_t a) {
+    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&a));
+  }
+  static __device__ __forceinline__ float one(__nv_bfloat16 a) { return __bfloat162float(a); }
+  static __device__ __forceinline__ __nv_bfloat16 round(float a) { return __float2bfloat16_rn(a); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// 8 inputs from element k of a row (zero past K); kWide: K, the row stride and the address allow 16 bytes
+template <bool kWide>
+__device__ __forceinline__ uint4 load_x(const uint16_t* row, int64_t k, int64_t kmax) {
+  if (kWide) return k < kmax ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = k + 2 * i < kmax ? row[k + 2 * i] : 0, hi = k + 2 * i + 1 < kmax ? row[k + 2 * i + 1] : 0;
+    w[i] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr int kW4Warps = 8;
+constexpr int kW4Unroll = 4;   // 64-input blocks in flight per warp
+
+// MT: row tiles of 8; kPerBlock: one group covers a 64-input block (else one per 32)
+template <typename T, int MT, bool kZeros, bool kPerBlock, bool kWide>
+__global__ void __launch_bounds__(kW4Warps * 32) linear_w4_kernel(const W4Args a) {
+  __shared__ float sums[kW4Warps][16][MT * 8 + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t tile = blockIdx.x, m0 = int64_t(blockIdx.y) * (MT * 8);
+  const uint4* w = a.w + (tile * a.blocks) * 32 + lane;
+  const uint32_t* scales = a.scales + tile * a.groups * 8 + g;
+  const uint16_t* zeros = a.zeros + tile * a.groups * 8 + g;
+  const uint16_t* x[MT];
+  bool live[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t m = m0 + i * 8 + g;
+    live[i] = m < a.rows;
+    x[i] = static_cast<const uint16_t*>(a.x) + (live[i] ? m : m0) * a.xs + t * 8;
+  }
+  float acc[MT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+
+  for (int kb0 = warp; kb0 < a.blocks; kb0 += kW4Warps * kW4Unroll) {
+    uint4 q[kW4Unroll];
+#pragma unroll
+    for (int j = 0; j < kW4Unroll; ++j) {
+      const int kb = kb0 + j * kW4Warps;
+      q[j] = kb < a.blocks ? load_once(w + int64_t(kb) * 32) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kW4Unroll; ++j) {
+      const int kb = kb0 + j * kW4Warps;
+      if (kb >= a.blocks) break;
+      const uint32_t word[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+      float part[MT][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k0 = kb * 64 + half * 32;
+        if (half == 0 || !kPerBlock) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
+        }
+        const int gi = min(k0 / a.group, a.groups - 1);   // the last block's second half may lie past K
+        uint32_t z0 = Half<T>::kMagic | 0x00080008u, z1 = z0;
+        if (kZeros) {
+          const uint32_t z = zeros[gi * 8];
+          z0 = Half<T>::kMagic | ((z & 255u) * 0x00010001u);
+          z1 = Half<T>::kMagic | ((z >> 8) * 0x00010001u);
+        }
+        uint32_t lo[4], hi[4];   // outputs g and g + 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lo[i] = Half<T>::sub(((word[2 * half] >> (4 * i)) & 0x000f000fu) | Half<T>::kMagic, z0);
+          hi[i] = Half<T>::sub(((word[2 * half + 1] >> (4 * i)) & 0x000f000fu) | Half<T>::kMagic, z1);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const uint4 b = live[i] ? load_x<kWide>(x[i], k0, a.k - t * 8) : make_uint4(0, 0, 0, 0);
+          Half<T>::mma(part[i], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+          Half<T>::mma(part[i], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
+        }
+        if (half == 1 || !kPerBlock) {
+          const float2 s = Half<T>::both(scales[gi * 8]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            acc[i][0] += s.x * part[i][0];
+            acc[i][1] += s.x * part[i][1];
+            acc[i][2] += s.y * part[i][2];
+            acc[i][3] += s.y * part[i][3];
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    sums[warp][g][i * 8 + 2 * t] = acc[i][0];
+    sums[warp][g][i * 8 + 2 * t + 1] = acc[i][1];
+    sums[warp][g + 8][i * 8 + 2 * t] = acc[i][2];
+    sums[warp][g + 8][i * 8 + 2 * t + 1] = acc[i][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MT * 8; i += kW4Warps * 32) {
+    const int64_t n = tile * 16 + (i & 15), m = m0 + (i >> 4);
+    if (n >= a.n || m >= a.rows) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < kW4Warps; ++j) s += sums[j][i & 15][i >> 4];
+    if (a.bias) s += Half<T>::one(static_cast<const T*>(a.bias)[n]);
+    static_cast<T*>(a.y)[m * a.ys + n] = Half<T>::round(s);
+  }
+}
+
+__global__ void w4_layout_kernel(const uint8_t* packed, int64_t row_bytes, const uint16_t* scales, const uint8_t* zeros, int64_t n,
+                                 int64_t k, int64_t tiles, int64_t blocks, int64_t groups, uint32_t* out_w, uint16_t* out_s,
+                                 uint8_t* out_z) {
+  const int64_t words = tiles * blocks * 128, pairs = tiles * groups * 16;
+  for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < words + pairs; i += int64_t(gridDim.x) * blockDim.x) {
+    if (i < words) {
+      const int part = int(i & 3), lane = int((i >> 2) & 31);
+      const int64_t tb = i >> 7, tile = tb / blocks, kb = tb - tile * blocks;
+      const int64_t row = tile * 16 + (lane >> 2) + (part & 1) * 8;
+      const int64_t k0 = kb * 64 + (part >> 1) * 32 + (lane & 3) * 8;
+      uint32_t word = 0;
+      for (int e = 0; e < 8; ++e) {
+        const int64_t kk = k0 + e;
+        if (row >= n || kk >= k) break;
+        const uint32_t byte = packed[row * row_bytes + kk / 2];
+        const uint32_t code = (kk & 1) ? byte >> 4 : byte & 15u;
+        word |= code << (4 * ((e >> 1) + 4 * (e & 1)));
+      }
+      out_w[i] = word;
+    } else {
+      const int64_t j = i - words;
+      const int which = int(j & 1), g = int((j >> 1) & 7);
+      const int64_t tg = j >> 4, tile = tg / groups, gi = tg - tile * groups;
+      const int64_t row = tile * 16 + g + which * 8;
+      out_s[j] = row < n ? scales[row * groups + gi] : 0;
+      if (zeros) out_z[j] = row < n ? (zeros[row * groups + gi] & 15) : 0;
+    }
+  }
+}
+
+template <typename T, int MT, bool kZeros>
+cudaError_t launch(const W4Args& a, bool per_block, bool wide, dim3 grid, cudaStream_t s) {
+  const int threads = kW4Warps * 32;
+  if (per_block && wide) linear_w4_kernel<T, MT, kZeros, true, true><<<grid, threads, 0, s>>>(a);
+  else if (per_block) linear_w4_kernel<T, MT, kZeros, true, false><<<grid, threads, 0, s>>>(a);
+  else if (wide) linear_w4_kernel<T, MT, kZeros, false, true><<<grid, threads, 0, s>>>(a);
+  else linear_w4_kernel<T, MT, kZeros, false, false><<<grid, threads, 0, s>>>(a);
+  return cudaGetLastError();
+}
+template <typename T, int MT>
+cudaError_t launch(const W4Args& a, bool zeros, bool per_block, bool wide, cudaStream_t s) {
+  const int64_t tiles = (a.n + 15) / 16, per = MT * 8;
+  // grid.y covers 65535 row blocks per launch
+  for (int64_t m = 0; m < a.rows; m += 65535 * per) {
+    W4Args b = a;
+    b.rows = std::min(a.rows - m, 65535 * per);
+    b.x = static_cast<const uint16_t*>(a.x) + m * a.xs;
+    b.y = static_cast<uint16_t*>(a.y) + m * a.ys;
+    const dim3 grid(unsigned(tiles), unsigned((b.rows + per - 1) / per));
+    const cudaError_t e = zeros ? launch<T, MT, true>(b, per_block, wide, grid, s) : launch<T, MT, false>(b, per_block, wide, grid, s);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+template <typename T>
+cudaError_t launch(const W4Args& a, bool zeros, bool per_block, bool wide, cudaStream_t s) {
+  if (a.rows <= 8) return launch<T, 1>(a, zeros, per_block, wide, s);
+  if (a.rows <= 16) return launch<T, 2>(a, zeros, per_block, wide, s);
+  return launch<T, 4>(a, zeros, per_block, wide, s);
+}
+
+}  // namespace
+
+size_t w4_layout_bytes(const W4View& w) {
+  const W4Sizes z = sizes(w);
+  return z.w + z.s + z.z;
+}
+
+cudaError_t w4_layout(const W4View& w, const uint8_t* packed, int64_t row_bytes, const void* scales, const uint8_t* zeros,
+                      void* data, cudaStream_t s) {
+  const W4Sizes z = sizes(w);
+  uint8_t* p = static_cast<uint8_t*>(data);
+  const int64_t items = z.tiles * (z.blocks * 128 + z.groups * 16);
+  const unsigned grid = unsigned(std::min<int64_t>((items + 255) / 256, 148 * 32));
+  w4_layout_kernel<<<grid, 256, 0, s>>>(packed, row_bytes, static_cast<const uint16_t*>(scales), zeros, w.n, w.k, z.tiles, z.blocks,
+                                        z.groups, reinterpret_cast<uint32_t*>(p), reinterpret_cast<uint16_t*>(p + z.w),
+                                        p + z.w + z.s);
+  return cudaGetLastError();
+}
+
+cudaError_t linear_w4(const W4View& w, const void* x, int64_t xs, const void* bias, void* y, int64_t ys, int64_t rows, int sms,
+                      cudaStream_t s) {
+  (void)sms;
+  const W4Sizes z = sizes(w);
+  const uint8_t* p = static_cast<const uint8_t*>(w.data);
+  W4Args a;
+  a.w = reinterpret_cast<const uint4*>(p);
+  a.scales = reinterpret_cast<const uint32_t*>(p + z.w);
+  a.zeros = reinterpret_cast<const uint16_t*>(p + z.w + z.s);
+  a.x = x, a.bias = bias, a.y = y, a.xs = xs, a.ys = ys, a.rows = rows, a.n = w.n, a.k = w.k;
+  a.blocks = int(z.blocks), a.groups = int(z.groups), a.group = w.group;
+  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && w.k % 8 == 0 && (xs % 8 == 0 || rows == 1);
+  const bool per_block = w.group % 64 == 0;
+  if (w.elem == 10) return launch<__half>(a, w.zeros, per_block, wide, s);
+  return launch<__nv_bfloat16>(a, w.zeros, per_block, wide, s);
+}
+
+}  // namespace k
+}  // namespace sb
