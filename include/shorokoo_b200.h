@@ -280,6 +280,11 @@ SB_API int32_t sb_paged_attention(const sb_paged_cache* cache, const sb_heads* q
                                   int64_t tokens, const int32_t* query_starts, float scale, int32_t window,
                                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* Waits for `stream` and returns SB_STATUS_CUDA_ERROR if, on the current device, a pipeline wait inside
+ * an attention call has run out (after 4 s) since the last sb_decoder_status: rows of such a call hold
+ * NaN or were not written. Not for use during stream capture. */
+SB_API int32_t sb_decoder_status(void* stream);
+
 /* Weights w[n, k] = (code[n, k] - zero[n, k / group_size]) * scale[n, k / group_size] of a linear
  * layer, codes in 4 bits: byte k / 2 of row n of `packed` holds element k in its low half for even k
  * and in its high half for odd k. scales [out_features, ceil(in_features / group_size)] float16 or

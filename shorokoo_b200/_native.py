@@ -83,6 +83,7 @@ SIGNATURES = {
     "sb_paged_append": (I32, [P, P, P, P, P, I32, I64, P, P, P]),
     "sb_paged_attention_workspace": (I32, [P, I32, I64, C.POINTER(SZ)]),
     "sb_paged_attention": (I32, [P, P, P, I32, I64, P, C.c_float, I32, P, SZ, P]),
+    "sb_decoder_status": (I32, [P]),
     "sb_w4_layout_bytes": (I32, [P, C.POINTER(SZ)]),
     "sb_w4_layout": (I32, [P, P, I64, P, P, P, P]),
     "sb_linear_w4": (I32, [P, P, I64, P, P, I64, I64, P]),

@@ -251,6 +251,15 @@ int32_t sb_paged_attention(const sb_paged_cache* cache, const sb_heads* q, const
   });
 }
 
+int32_t sb_decoder_status(void* stream) {
+  return checked("sb_decoder_status", [&] {
+    unsigned bits = 0;
+    multiprocessors();   // a current device
+    launched(k::paged_wait_errors(&bits, static_cast<cudaStream_t>(stream)));
+    SB_CHECK(bits == 0, SB_CUDA_ERROR, "an attention kernel's pipeline wait timed out (code " + std::to_string(bits) + ")");
+  });
+}
+
 int32_t sb_w4_layout_bytes(const sb_w4_weights* weights, size_t* bytes) {
   return checked("sb_w4_layout_bytes", [&] {
     need(bytes != nullptr, "bytes is null");

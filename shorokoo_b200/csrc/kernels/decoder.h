@@ -45,6 +45,9 @@ size_t paged_attention_workspace(const PagedView& c, int sms);
 cudaError_t paged_attention(const PagedView& c, int elem, HeadsView q, HeadsView out, float scale, int window, void* ws,
                             int sms, cudaStream_t s);
 
+// Waits for the stream; bits of the attention kernels' waits that ran out since the last call.
+cudaError_t paged_wait_errors(unsigned* bits, cudaStream_t s);
+
 struct W4View {
   const void* data;
   int64_t n, k;

@@ -93,7 +93,7 @@ struct RowTile {
 };
 
 template <int kRows, int kKeys>
-__host__ __device__ __forceinline__ int64_t seq_tiles(const SeqWork& s, int group, int window) {
+__device__ __forceinline__ int64_t seq_tiles(const SeqWork& s, int group, int window) {
   int64_t sum = 0;
   for (int i = 0; i * kRows < s.rows; ++i) sum += RowTile<kRows, kKeys>(s, i, group, window).tiles;
   return sum;
@@ -105,15 +105,40 @@ struct Share {
   int b, h, i, tile;
 };
 
+// Every CTA works its share out by itself (whole block; the result is the same in all threads): the
+// sequences' tiles are counted by a thread each, or by a warp each where they have many row tiles,
+// and summed; then the sequence, head and row tile that hold its first tile are looked up.
+constexpr int kCounted = 128;   // sequences whose counts are kept between the two steps
+
 template <int kRows, int kKeys, int kThreads>
 __device__ __forceinline__ Share find_share(const PagedView& c, int group, int window, int least, int cta, int ctas) {
-  __shared__ int64_t warp_sum[kThreads / 32 + 1];
+  __shared__ int64_t count[kCounted];
+  __shared__ int64_t warp_sum[kThreads / 32];
+  __shared__ int64_t found_rem;
   __shared__ Share found;
+  using Tile = RowTile<kRows, kKeys>;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t own = 0, last = 0;   // `last`: the tiles of this thread's latest sequence
-  for (int b = tid; b < c.batch; b += kThreads) {
-    last = seq_tiles<kRows, kKeys>(seq_work(c, b, group), group, window) * c.kv_heads;
-    own += last;
+  const bool kept = c.batch <= kCounted;
+  int64_t own = 0;
+  if (kept && c.tokens * group > int64_t(2 * kRows) * c.batch) {
+    for (int b = warp; b < c.batch; b += kThreads / 32) {
+      const SeqWork s = seq_work(c, b, group);
+      int64_t n = 0;
+      for (int i = lane; i * kRows < s.rows; i += 32) n += Tile(s, i, group, window).tiles;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(~0u, n, d);
+      n *= c.kv_heads;
+      if (lane == 0) {
+        count[b] = n;
+        own += n;
+      }
+    }
+  } else {
+    for (int b = tid; b < c.batch; b += kThreads) {
+      const int64_t n = seq_tiles<kRows, kKeys>(seq_work(c, b, group), group, window) * c.kv_heads;
+      if (kept) count[b] = n;
+      own += n;
+    }
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) own += __shfl_xor_sync(~0u, own, d);
@@ -131,12 +156,9 @@ __device__ __forceinline__ Share find_share(const PagedView& c, int group, int w
   int64_t before = 0;   // tiles of the sequences before this round of kThreads
   for (int b0 = 0; b0 < c.batch; b0 += kThreads) {
     const int b = b0 + tid;
-    SeqWork sw;
     int64_t mine = 0;
-    if (b < c.batch) {
-      sw = seq_work(c, b, group);
-      mine = c.batch <= kThreads ? last : seq_tiles<kRows, kKeys>(sw, group, window) * c.kv_heads;
-    }
+    if (b < c.batch)
+      mine = kept ? count[b] : seq_tiles<kRows, kKeys>(seq_work(c, b, group), group, window) * c.kv_heads;
     int64_t upto = mine;   // inclusive sum over the block's threads
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -154,23 +176,36 @@ __device__ __forceinline__ Share find_share(const PagedView& c, int group, int w
     }
     upto += before;
     if (s.u0 < upto && s.u0 >= upto - mine) {
-      const int64_t per_head = mine / c.kv_heads;
-      int64_t rem = s.u0 - (upto - mine);
+      const int64_t per_head = mine / c.kv_heads, rem = s.u0 - (upto - mine);
       s.b = b;
       s.h = int(rem / per_head);
-      rem -= s.h * per_head;
-      int i = 0;
-      for (;; ++i) {
-        const int t = RowTile<kRows, kKeys>(sw, i, group, window).tiles;
-        if (rem < t) break;
-        rem -= t;
-      }
-      s.i = i;
-      s.tile = int(rem);
       found = s;
+      found_rem = rem - s.h * per_head;
     }
     before += all;
     if (s.u0 < before) break;   // uniform
+  }
+  __syncthreads();
+  if (warp == 0) {   // 32 row tiles at a time
+    const SeqWork sw = seq_work(c, found.b, group);
+    int64_t rem = found_rem;
+    for (int i0 = 0; i0 * kRows < sw.rows; i0 += 32) {
+      const int i = i0 + lane;
+      const int64_t t = i * kRows < sw.rows ? Tile(sw, i, group, window).tiles : 0;
+      int64_t upto = t;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t v = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += v;
+      }
+      const bool here = rem < upto && rem >= upto - t;
+      if (here) {
+        found.i = i;
+        found.tile = int(rem - (upto - t));
+      }
+      if (__any_sync(~0u, here)) break;
+      rem -= __shfl_sync(~0u, upto, 31);
+    }
   }
   __syncthreads();
   return found;

@@ -11,77 +11,13 @@
 // several times the rate that the memory can feed, and needs no operand staging beyond shared memory.
 // Each of a CTA's 4 warps takes 16 of a tile's 64 positions, with its own ring of stages (cp.async, no
 // barrier between warps) and its own m, l, o, joined in shared memory at the item's end.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
-#include <atomic>
 
-#include "decoder.h"
-#include "paged.cuh"
-#include "tcgen05.cuh"
+#include "paged_attention.cuh"
 
 namespace sb {
 namespace k {
 namespace {
-
-template <typename T> struct Mma;
-template <> struct Mma<__half> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static constexpr uint32_t kExp = 0x7c00u;   // exponent bits of infinities and NaN
-  static __device__ __forceinline__ float widen(uint16_t b) { return __half2float(__ushort_as_half(b)); }
-};
-template <> struct Mma<__nv_bfloat16> {
-  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  static constexpr uint32_t kExp = 0x7f80u;
-  static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }
-};
-
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// A partial result that a cut left: slot 2c is the first piece of CTA c, slot 2c + 1 its last.
-struct PartialNote {
-  int b, h, i;
-  int more;   // > 0: the item begins here and `more` pieces follow in slots 2(c + 1), 2(c + 2), ..; else 0
-};
-
-struct PagedArgs {
-  PagedView c;
-  HeadsView q, out;
-  int group, window, ctas, least;
-  float scale_log2;
-  PartialNote* notes;   // [2 * ctas]
-  float2* ml;           // [2 * ctas][rows]: m (in units of log2), l
-  float* o;             // [2 * ctas][rows][DP]
-};
 
 constexpr int kRowsTile = 16;
 constexpr int kKeysTile = 64;
@@ -415,40 +351,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   }
 }
 
-template <typename F>
-cudaError_t launch_dependent(F kernel, dim3 grid, int threads, const PagedArgs& a, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(unsigned(threads));
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
-template <typename F>
-cudaError_t allow_smem(F kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = uint64_t(1) << (dev & 63);
-  if (done.load() & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) done.fetch_or(bit);
-  return e;
-}
-
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
-struct Space {
-  int ctas, dp;
-  size_t notes, ml, o;
-};
-Space space(const PagedView& c, int sms) {
-  Space z;
+PagedSpace space(const PagedView& c, int sms) {
+  PagedSpace z;
   z.dp = c.head_dim <= 64 ? 64 : 128;
   z.ctas = 2 * sms;
   z.notes = up256(size_t(z.ctas) * 2 * sizeof(PartialNote));
@@ -471,13 +375,14 @@ cudaError_t launch_rows(PagedArgs a, cudaStream_t s) {
 }  // namespace
 
 size_t paged_attention_workspace(const PagedView& c, int sms) {
-  const Space z = space(c, sms);
+  const PagedSpace z = paged_chunk_wanted(c) ? paged_chunk_space(c, sms) : space(c, sms);
   return z.notes + z.ml + z.o;
 }
 
 cudaError_t paged_attention(const PagedView& c, int elem, HeadsView q, HeadsView out, float scale, int window, void* ws, int sms,
                             cudaStream_t s) {
-  const Space z = space(c, sms);
+  if (paged_chunk_wanted(c)) return paged_chunk(c, elem, q, out, scale, window, ws, sms, s);
+  const PagedSpace z = space(c, sms);
   PagedArgs a;
   a.c = c, a.q = q, a.out = out;
   a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas, a.least = 2;

@@ -1,0 +1,606 @@
+// Attention of chunks of new tokens over a paged cache, on the tcgen05 tensor core (formulas:
+// paged_attention.cu). Every key byte feeds hundreds of rows, so the two products bound it, and next to
+// them the exponentials: a 128 x 128 tile of logits at head width 128 takes 1024 cycles of tensor core
+// and 1024 of the SM's 16 exponentials per cycle.
+//
+// An item is 256 query rows of one key head (rows as in paged.cuh: tokens times the query heads that
+// share the key head), as two tiles A and B of 128: while the tensor core multiplies for one, the other's
+// logits become weights. One CTA per SM, 13 warps:
+//   warps 0-3, 4-7   tiles A, B: a thread owns a query row. It loads the row's Q into shared memory (128-byte
+//                    swizzle, K-major), then per key tile reads its 128 logits from its TMEM lane twice: for
+//                    their maximum, and to write P = 2^(s - m) in 16 bits over them (columns 0-63 of the same
+//                    128), the A operand of the second product. A running maximum that grows by less than
+//                    2^8 is left as it is (P then stays below 2^8, exact in range for either type), so that O
+//                    in TMEM is rescaled a few times per row only. At the end it reads its row of O.
+//   warps 8-11       K and V tiles of 128 positions, gathered page by page with 16-byte cp.async into a ring;
+//                    rows that are not there are zero-filled, and a bit per row says so.
+//   warp 12          issues S = Q K^T (M = N = 128) and O += P V (P from TMEM, V MN-major as it lies in the
+//                    cache), in the order PV_A(j) S_A(j+1) PV_B(j) S_B(j+1): the tensor core runs its
+//                    instructions in issue order, so a commit of S(j+1) also says that PV(j) is done.
+// TMEM: S/P of A 0-127, of B 128-255, O of A 256-383, of B 384-511.
+//
+// Waits are bounded: one that runs out sets the error word, every role leaves its loop, and the rows of
+// the piece are written as NaN.
+#include <algorithm>
+
+#include "paged_attention.cuh"
+
+namespace sb {
+namespace k {
+namespace {
+
+constexpr int kChunkRows = 256;
+constexpr int kChunkKeys = 128;
+constexpr int kChunkThreads = 416;
+constexpr int kLoadWarp = 8, kMmaWarp = 12;
+template <int DP> constexpr int kRing = DP == 128 ? 5 : 8;          // stages of one K or V tile
+template <int DP> constexpr uint32_t kTileBytes = 128u * DP * 2;
+template <int DP> constexpr int kChunkSmem = int((2 + kRing<DP>) * kTileBytes<DP>) + 1024;
+constexpr int kLag = 2;          // stages that a loader keeps in flight
+constexpr int kBook = 8;         // entries of the rings of row bits and poison marks
+constexpr float kGrowth = 8.f;   // log2 of how far a weight may rise above 1 before O is rescaled
+
+__device__ unsigned chunk_error;   // bits of the waits that ran out since it was last read
+
+// byte offset of 16-byte piece `c` of row `r` in a tile of 128-byte-swizzled slabs of 64 elements
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return uint32_t(c >> 3) * 16384u + uint32_t(r) * 128u + (uint32_t((c & 7) ^ (r & 7)) << 4);
+}
+
+template <typename T> constexpr uint32_t kIdescType = 0;
+template <> constexpr uint32_t kIdescType<__nv_bfloat16> = (1u << 7) | (1u << 10);
+template <typename T> constexpr uint32_t idesc16(int M, int N) {
+  return (1u << 4) | kIdescType<T> | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+// One CTA's walk over its pieces; every role steps through the same ones.
+struct Walk {
+  const PagedView& c;
+  int group, window;
+  Share sh;
+  int64_t u;
+  int b, h, i, at;
+  SeqWork s;
+  // the piece
+  int tile_a, tile_b;   // key tiles of the pair
+  bool whole, head;     // the item in one piece; the item begins here
+  int tiles, first_tile, last_tile;
+  int slot;
+  int ta0, tb0, ta1, tb1;   // key tiles of A and B in the piece
+  int kbeg, kend;
+  int64_t all_lo, all_hi;   // positions that every row of the pair sees
+
+  __device__ __forceinline__ Walk(const PagedView& view, int g, int w, const Share& share) : c(view), group(g), window(w), sh(share) {
+    u = sh.u0, b = sh.b, h = sh.h, i = sh.i, at = sh.tile;
+    s = seq_work(c, b, group);
+    piece();
+  }
+  __device__ __forceinline__ void piece() {
+    const RowTile<kChunkRows, kChunkKeys> rt(s, i, group, window);
+    tiles = rt.tiles;
+    const int take = int(min(int64_t(tiles - at), sh.u1 - u));
+    tile_a = rt.tile0 + at;
+    tile_b = tile_a + take;
+    whole = at == 0 && take == tiles;
+    head = at == 0;
+    kbeg = rt.kbeg, kend = rt.kend;
+    all_hi = rt.pos_lo;
+    all_lo = window > 0 ? rt.pos_hi - window + 1 : 0;
+    slot = 2 * int(blockIdx.x) + (u == sh.u0 ? 0 : 1);
+    half(0, ta0, tb0);
+    half(1, ta1, tb1);
+  }
+  __device__ __forceinline__ void half(int x, int& lo, int& hi) const {
+    lo = hi = 0;
+    if ((2 * i + x) * 128 >= s.rows) return;
+    const RowTile<128, kChunkKeys> part(s, 2 * i + x, group, window);
+    if (part.kbeg >= part.kend) return;
+    lo = max(tile_a, part.tile0);
+    hi = min(tile_b, part.tile0 + part.tiles);
+    if (lo >= hi) lo = hi = 0;
+  }
+  __device__ __forceinline__ bool next() {
+    u += tile_b - tile_a;
+    at = 0;
+    if (u >= sh.u1) return false;
+    if ((++i) * kChunkRows >= s.rows) {
+      i = 0;
+      if (++h == c.kv_heads) {
+        h = 0;
+        do {
+          if (++b >= c.batch) return false;
+          s = seq_work(c, b, group);
+        } while (s.rows == 0);
+      }
+    }
+    piece();
+    return true;
+  }
+  __device__ __forceinline__ int ta(int x) const { return x ? ta1 : ta0; }
+  __device__ __forceinline__ int tb(int x) const { return x ? tb1 : tb0; }
+  __device__ __forceinline__ bool on(int x, int tile) const { return tile >= ta(x) && tile < tb(x); }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const PagedArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  constexpr int kNst = kRing<DP>;
+  constexpr uint32_t kTile = kTileBytes<DP>;
+  constexpr int kPieces = DP / 8;
+  __shared__ uint64_t full[kNst], empty[kNst], q_full[2], s_full[2], p_full[2], o_full[2];
+  __shared__ uint32_t there[kBook][4];      // which of a key tile's 128 positions are there
+  __shared__ int poison[kBook];             // number of the piece that met non-finite values in mixed positions
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;                       // Q of A, Q of B
+  uint8_t* ring = smem + 2 * kTile;
+  const PagedView& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = c.head_dim, G = a.group;
+  pdl_launch_dependents();
+
+  if (tid == 0) {
+    for (int x = 0; x < kNst; ++x) {
+      mbar_init(&full[x], 4u);
+      mbar_init(&empty[x], 1u);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], 4u);
+      mbar_init(&s_full[x], 1u);
+      mbar_init(&p_full[x], 4u);
+      mbar_init(&o_full[x], 1u);
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid < kBook) poison[tid] = 0;
+  const Share sh = find_share<kChunkRows, kChunkKeys, kChunkThreads>(c, G, a.window, a.least, blockIdx.x, a.ctas);
+  if (tid < 2) a.notes[2 * blockIdx.x + tid] = PartialNote{0, 0, 0, 0};
+  if (sh.u0 >= sh.u1) return;
+  if (warp == kMmaWarp) tmem_alloc(&tmem_holder, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  Walk w(c, G, a.window, sh);
+
+  if (warp < kLoadWarp) {
+    // ---- rows: Q, softmax, output ----
+    const int x = warp >> 2;                              // tile A or B
+    const int r = tid & 127;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + uint32_t(x * 128), to = tmem + lanes + 256u + uint32_t(x * 128);
+    uint8_t* q_at = sq + x * kTile;
+    uint32_t s_phase = 0, o_phase = 0;
+    int number = 0, book = 0;                             // pieces, key tiles before the current piece
+    do {
+      ++number;
+      const int row = w.i * kChunkRows + x * 128 + r;
+      const bool live = row < w.s.rows;
+      const int tok = live ? row / G : 0;
+      const int head = w.h * G + (live ? row - tok * G : 0);
+      const int64_t pos = w.s.ctx - w.s.n + tok;
+      // positions that the row sees: [see_lo, see_hi]
+      const int see_hi = live ? int(min(pos, int64_t(w.kend) - 1)) : -1;
+      const int see_lo = a.window > 0 ? int(max(pos - a.window + 1, int64_t(0))) : 0;
+      const bool busy = w.ta(x) < w.tb(x);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      if (busy) {
+        const T* qp = static_cast<const T*>(a.q.p) + (w.s.first + tok) * a.q.ts + int64_t(head) * a.q.hs;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (live && p * 8 < D) v = *reinterpret_cast<const uint4*>(qp + p * 8);
+          *reinterpret_cast<uint4*>(q_at + tile_off(r, p)) = v;
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[x]);
+        for (int tile = w.ta(x); tile < w.tb(x); ++tile) {
+          ok = __all_sync(~0u, mbar_wait(&s_full[x], s_phase, abort_flag, &chunk_error, 1u));
+          s_phase ^= 1u;
+          if (!ok) break;
+          tc_fence_after();
+          const int key0 = tile * kChunkKeys;
+          const uint32_t* bits = there[(book + tile - w.tile_a) % kBook];
+          const uint32_t all = bits[0] & bits[1] & bits[2] & bits[3];
+          // every row of the warp sees every position of the tile
+          const bool plain = __all_sync(~0u, all == ~0u && (!live || (see_hi >= key0 + kChunkKeys - 1 && see_lo <= key0)));
+          uint32_t seen[4];
+          if (!plain) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int lo = see_lo - key0 - g * 32, hi = see_hi - key0 - g * 32;   // in [0, 31] once clamped
+              uint32_t mask = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
+              mask &= lo <= 0 ? ~0u : lo > 31 ? 0u : ~((1u << lo) - 1u);
+              seen[g] = mask & bits[g];
+            }
+          }
+          uint32_t v[32];
+          float top = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            tmem_ld32(ts + g * 32, v);
+            if (plain) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if ((seen[g] >> j) & 1u) top = fmaxf(top, __uint_as_float(v[j]));
+            }
+          }
+          // m is the reference of the row's weights in units of the raw logits
+          const bool fresh = m == -INFINITY;
+          const bool grow = top > m && (fresh || (top - m) * a.scale_log2 > kGrowth);
+          if (__any_sync(~0u, grow)) {
+            const float f = grow ? (fresh ? 0.f : exp2_approx((m - top) * a.scale_log2)) : 1.f;
+            if (grow) m = top;
+            l *= f;
+            if (tile > w.ta(x)) {
+#pragma unroll 1
+              for (int g = 0; g < DP / 32; ++g) {
+                tmem_ld32(to + g * 32, v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+                tmem_st16(to + g * 32, v);
+                tmem_st16(to + g * 32 + 16, v + 16);
+              }
+              tmem_st_wait();
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            tmem_ld32(ts + g * 32, v);
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float p0 = exp2_approx(fmaf(__uint_as_float(v[j]), a.scale_log2, -base));
+              float p1 = exp2_approx(fmaf(__uint_as_float(v[j + 1]), a.scale_log2, -base));
+              if (!plain) {
+                p0 = (seen[g] >> j) & 1u ? p0 : 0.f;
+                p1 = (seen[g] >> (j + 1)) & 1u ? p1 : 0.f;
+              }
+              sum0 += p0;
+              sum1 += p1;
+              pk[j >> 1] = Mma<T>::pack(p0, p1);
+            }
+            tmem_st16(ts + g * 16, pk);
+          }
+          l += sum0 + sum1;
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+        if (ok) ok = __all_sync(~0u, mbar_wait(&o_full[x], o_phase, abort_flag, &chunk_error, 2u));
+        o_phase ^= 1u;
+        tc_fence_after();
+      }
+      // ---- the row's result ----
+      const bool marked = poison[number % kBook] == number;
+      const float bad = ok ? 0.f : __int_as_float(0x7fc00000);
+      const float inv = (l == 0.f ? 0.f : 1.f / l) + bad;
+#pragma unroll 1
+      for (int g = 0; g < DP / 32; ++g) {
+        uint32_t v[32];
+        __syncwarp();
+        if (busy && ok) {
+          tmem_ld32(to + g * 32, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(bad);
+        }
+        if (!live) continue;
+        if (marked) {
+          const int32_t* table = c.table + int64_t(w.b) * c.table_stride;
+          for (int key = max(w.tile_a * kChunkKeys, w.kbeg); key < min(w.tile_b * kChunkKeys, w.kend); ++key) {
+            if (key >= w.all_lo && key <= w.all_hi) {
+              key = int(min(w.all_hi, int64_t(w.kend)));   // on to the ones that not all rows see
+              continue;
+            }
+            if (key > see_hi || key < see_lo) continue;
+            const int page = table[key / c.page_size];
+            if (page < 0 || page >= c.pages) continue;
+            const uint16_t* vp = reinterpret_cast<const uint16_t*>(static_cast<const T*>(c.v) + page * c.vp +
+                                                                   (key % c.page_size) * c.vt + int64_t(w.h) * c.vh);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (g * 32 + j < D) {
+                const uint16_t bits = vp[g * 32 + j];
+                if ((bits & Mma<T>::kExp) == Mma<T>::kExp) v[j] = __float_as_uint(__uint_as_float(v[j]) + Mma<T>::widen(bits));
+              }
+          }
+        }
+        if (w.whole) {
+          T* dst = static_cast<T*>(a.out.p) + (w.s.first + tok) * a.out.ts + int64_t(head) * a.out.hs + g * 32;
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            if (g * 32 + p * 8 >= D) break;
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[e] = Mma<T>::pack(__uint_as_float(v[8 * p + 2 * e]) * inv, __uint_as_float(v[8 * p + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(dst + p * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(a.o + int64_t(w.slot) * (kChunkRows * DP)) + g * 8 * kChunkRows + x * 128 + r;
+#pragma unroll
+          for (int p = 0; p < 8; ++p)
+            dst[p * kChunkRows] = make_float4(__uint_as_float(v[4 * p]), __uint_as_float(v[4 * p + 1]), __uint_as_float(v[4 * p + 2]),
+                                              __uint_as_float(v[4 * p + 3]));
+        }
+      }
+      if (!w.whole && live) a.ml[int64_t(w.slot) * kChunkRows + x * 128 + r] = make_float2(m * a.scale_log2, l + bad);
+      if (!w.whole && w.head && tid == 0)
+        a.notes[w.slot] = PartialNote{w.b, w.h, w.i, int((w.u + w.tiles - 1) / sh.per) - int(blockIdx.x)};
+      tc_fence_before();   // these reads of O come before the next piece's products
+      book += w.tile_b - w.tile_a;
+      if (__any_sync(~0u, *abort_flag)) break;
+    } while (w.next());
+  } else if (warp < kMmaWarp) {
+    // ---- keys and values ----
+    const int lw = warp - kLoadWarp;
+    int stage = 0, number = 0, book = 0;   // stages used, pieces, key tiles before the current piece
+    bool ok = true;
+    // values of the stages in flight that have positions not every row sees: what to clean when they land
+    int clean_tile[kLag + 1], clean_slot[kLag + 1];
+#pragma unroll
+    for (int j = 0; j <= kLag; ++j) clean_tile[j] = -1, clean_slot[j] = 0;
+    int arrived = 0;                       // stages handed over
+    int page = -1, in_page = 0, page_was = -1, in_page_was = 0;
+    auto hand_over = [&](int tile, int number_of, const Walk& wk) {
+      // cleans the pieces that this thread copied, then passes the stage on
+      const int slot = arrived % kNst;
+      if (tile >= 0) {
+        bool bad = false;
+#pragma unroll 1
+        for (int j = 0; j < kPieces; ++j) {
+          const int rr = lw * 32 + j * (32 / kPieces) + lane / kPieces;
+          const int64_t key = int64_t(tile) * kChunkKeys + rr;
+          if (key <= wk.all_hi && key >= wk.all_lo) continue;
+          uint16_t* e = reinterpret_cast<uint16_t*>(ring + slot * kTile + tile_off(rr, lane % kPieces));
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if ((e[q] & Mma<T>::kExp) == Mma<T>::kExp) {
+              e[q] = 0;
+              bad = true;
+            }
+        }
+        if (bad) poison[number_of % kBook] = number_of;
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[slot]);
+      ++arrived;
+    };
+    do {
+      ++number;
+      const int32_t* table = c.table + int64_t(w.b) * c.table_stride;
+      const T* kc = static_cast<const T*>(c.k) + int64_t(w.h) * c.kh;
+      const T* vc = static_cast<const T*>(c.v) + int64_t(w.h) * c.vh;
+      // per piece: K(a), then K(j + 1), V(j) for each tile j
+      const int n = w.tile_b - w.tile_a;
+      for (int e = 0; e < 2 * n && ok; ++e) {
+        const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
+        const int tile = w.tile_a + (e == 0 ? 0 : value ? (e == 2 * n - 1 ? n - 1 : e / 2 - 1) : (e + 1) / 2);
+        const int slot = stage % kNst;
+        if (!value) {
+          page_was = page, in_page_was = in_page;
+          const int key = tile * kChunkKeys + lw * 32 + lane;
+          page = -1;
+          if (key >= w.kbeg && key < w.kend) {
+            const int page_no = key / c.page_size;
+            in_page = key - page_no * c.page_size;
+            page = table[page_no];
+            if (page < 0 || page >= c.pages) page = -1;
+          }
+        }
+        const bool last_value = e == 2 * n - 1;    // its rows are the latest looked up
+        const int pg = value && !last_value ? page_was : page, ip = value && !last_value ? in_page_was : in_page;
+        if (stage >= kNst)
+          ok = __all_sync(~0u, mbar_wait(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+        if (!ok) break;
+        if (!value) {
+          const uint32_t bits = __ballot_sync(~0u, pg >= 0);
+          if (lane == 0) there[(book + tile - w.tile_a) % kBook][lw] = bits;
+        }
+        const uint32_t dst = smem_u32(ring + slot * kTile);
+        const int piece = lane % kPieces;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+          const int rr = j * (32 / kPieces) + lane / kPieces;
+          const int p = __shfl_sync(~0u, pg, rr), ri = __shfl_sync(~0u, ip, rr);
+          const bool live = p >= 0 && piece * 8 < D;
+          const T* src = value ? vc + p * c.vp + ri * c.vt : kc + p * c.kp + ri * c.kt;
+          cp_async_16(dst + tile_off(lw * 32 + rr, piece), live ? src + piece * 8 : static_cast<const T*>(c.k), live ? 16u : 0u);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const int64_t key0 = int64_t(tile) * kChunkKeys;
+        const bool mixed = value && (key0 + kChunkKeys - 1 > w.all_hi || key0 < w.all_lo);
+#pragma unroll
+        for (int j = kLag; j > 0; --j) clean_tile[j] = clean_tile[j - 1];
+        clean_tile[0] = mixed ? tile : -1;
+        ++stage;
+        if (stage - arrived > kLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+          hand_over(clean_tile[kLag], number, w);
+        }
+      }
+      // The stages still in flight are handed over here: their cleaning needs this piece's bounds.
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      while (ok && arrived < stage) hand_over(stage - arrived == 2 ? clean_tile[1] : clean_tile[0], number, w);
+      book += n;
+      if (!ok || __any_sync(~0u, *abort_flag)) break;
+    } while (w.next());
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    // ---- products ----
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc16<T>(128, kChunkKeys), id_o = idesc16<T>(128, DP) | kMnMajorB;
+      int stage = 0;
+      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      bool ok = true;
+      auto wait_stage = [&](int st) {
+        return mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
+      };
+      auto logits = [&](int x, int st) {
+        const uint64_t qd = sw128_desc(smem_u32(sq + x * kTile)), kd = sw128_desc(smem_u32(ring + (st % kNst) * kTile));
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t step = uint64_t((kk >> 2) * 1024 + (kk & 3) * 2);   // a slab of 64 elements is 16 KB
+          umma_bf16(tmem + uint32_t(x * 128), qd + step, kd + step, id_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[x]);
+      };
+      do {
+        const int n = w.tile_b - w.tile_a;
+        // stages of this piece: K(a) is 0; K(j) is 2j - 1; V(j) is 2j + 2, but the last V is 2n - 1
+        auto k_stage = [&](int j) { return stage + (j == 0 ? 0 : 2 * j - 1); };
+        auto v_stage = [&](int j) { return stage + (j == n - 1 ? 2 * n - 1 : 2 * j + 2); };
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (ok && w.ta(x) < w.tb(x)) {
+            ok = mbar_wait(&q_full[x], q_phase[x], abort_flag, &chunk_error, 16u);
+            q_phase[x] ^= 1u;
+          }
+        ok = ok && wait_stage(k_stage(0));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (w.on(x, w.tile_a)) logits(x, k_stage(0));
+        umma_commit(&empty[k_stage(0) % kNst]);
+        for (int j = 0; j < n && ok; ++j) {
+          const int tile = w.tile_a + j;
+          if (j + 1 < n) ok = wait_stage(k_stage(j + 1));
+          ok = ok && wait_stage(v_stage(j));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = sw128_mn_desc(smem_u32(ring + (v_stage(j) % kNst) * kTile), 16384u);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (w.on(x, tile)) {
+              ok = ok && mbar_wait(&p_full[x], p_phase[x], abort_flag, &chunk_error, 32u);
+              p_phase[x] ^= 1u;
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < kChunkKeys / 16; ++kk)   // 16 positions: two 8-row groups of 1024 B
+                umma_f16_ts(tmem + 256u + uint32_t(x * 128), tmem + uint32_t(x * 128 + kk * 8), vd + uint64_t(kk * 128), id_o,
+                            tile > w.ta(x) || kk > 0 ? 1u : 0u);
+              if (tile + 1 == w.tb(x)) umma_commit(&o_full[x]);
+            }
+            if (j + 1 < n && w.on(x, tile + 1)) logits(x, k_stage(j + 1));
+          }
+          if (!ok) break;
+          umma_commit(&empty[v_stage(j) % kNst]);
+          if (j + 1 < n) umma_commit(&empty[k_stage(j + 1) % kNst]);
+        }
+        stage += 2 * n;
+      } while (ok && w.next());
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of each split item in the order of their positions: a thread per row and 4 elements.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedArgs a) {
+  pdl_wait();
+  const PartialNote n0 = a.notes[2 * blockIdx.x], n1 = a.notes[2 * blockIdx.x + 1];
+  const bool second = n1.more > 0;
+  if (!second && n0.more <= 0) return;
+  const PartialNote n = second ? n1 : n0;
+  const SeqWork s = seq_work(a.c, n.b, a.group);
+  const int r = threadIdx.x, row = n.i * kChunkRows + r;
+  if (row >= s.rows) return;
+  const int64_t first = int64_t(2 * blockIdx.x + (second ? 1 : 0)), next = 2 * (int64_t(blockIdx.x) + 1);
+  float top = -INFINITY;
+  for (int p = 0; p <= n.more; ++p) top = fmaxf(top, a.ml[(p == 0 ? first : next + 2 * (p - 1)) * kChunkRows + r].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  const int tok = row / a.group;
+  T* to = static_cast<T*>(a.out.p) + (s.first + tok) * a.out.ts + int64_t(n.h * a.group + row - tok * a.group) * a.out.hs;
+  float sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int d4 = blockIdx.y;
+  for (int p = 0; p <= n.more; ++p) {
+    const int64_t slot = p == 0 ? first : next + 2 * (p - 1);
+    const float2 ml = a.ml[slot * kChunkRows + r];
+    const float f = exp2_approx(ml.x - base);
+    const float4 o = reinterpret_cast<const float4*>(a.o + slot * (kChunkRows * DP))[d4 * kChunkRows + r];
+    sum += f * ml.y;
+    v.x += f * o.x;
+    v.y += f * o.y;
+    v.z += f * o.z;
+    v.w += f * o.w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (d4 * 4 < a.c.head_dim)
+    *reinterpret_cast<uint2*>(to + d4 * 4) = make_uint2(Mma<T>::pack(v.x * inv, v.y * inv), Mma<T>::pack(v.z * inv, v.w * inv));
+}
+
+template <typename T, int DP>
+cudaError_t launch_chunk(const PagedArgs& a, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(paged_chunk_kernel<T, DP>, kChunkSmem<DP>, done);
+  if (e != cudaSuccess) return e;
+  paged_chunk_kernel<T, DP><<<a.ctas, kChunkThreads, kChunkSmem<DP>, s>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_dependent(paged_chunk_join_kernel<T, DP>, dim3(unsigned(a.ctas), DP / 4), 256, a, s);
+}
+
+}  // namespace
+
+cudaError_t paged_wait_errors(unsigned* bits, cudaStream_t s) {
+  void* at = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&at, chunk_error);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(bits, at, sizeof(*bits), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(*bits), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  return e;
+}
+
+bool paged_chunk_wanted(const PagedView& c) {
+  return c.batch > 0 && c.tokens * (c.q_heads / c.kv_heads) >= 48 * int64_t(c.batch);
+}
+
+PagedSpace paged_chunk_space(const PagedView& c, int sms) {
+  PagedSpace z;
+  z.dp = c.head_dim <= 64 ? 64 : 128;
+  z.ctas = sms;
+  z.notes = up256(size_t(z.ctas) * 2 * sizeof(PartialNote));
+  z.ml = up256(size_t(z.ctas) * 2 * kChunkRows * sizeof(float2));
+  z.o = up256(size_t(z.ctas) * 2 * kChunkRows * z.dp * sizeof(float));
+  return z;
+}
+
+cudaError_t paged_chunk(const PagedView& c, int elem, HeadsView q, HeadsView out, float scale, int window, void* ws, int sms,
+                        cudaStream_t s) {
+  const PagedSpace z = paged_chunk_space(c, sms);
+  PagedArgs a;
+  a.c = c, a.q = q, a.out = out;
+  a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas, a.least = 4;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  uint8_t* p = static_cast<uint8_t*>(ws);
+  a.notes = reinterpret_cast<PartialNote*>(p);
+  a.ml = reinterpret_cast<float2*>(p + z.notes);
+  a.o = reinterpret_cast<float*>(p + z.notes + z.ml);
+  if (elem == 10) return z.dp == 64 ? launch_chunk<__half, 64>(a, s) : launch_chunk<__half, 128>(a, s);
+  return z.dp == 64 ? launch_chunk<__nv_bfloat16, 64>(a, s) : launch_chunk<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace k
+}  // namespace sb

@@ -137,6 +137,16 @@ __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint6
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D(tmem) (+)= A(tmem) * B(smem)^T, kind::f16: A rows are TMEM lanes, two consecutive K elements per column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -161,6 +171,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
                :
                : "memory");
 }
+
+// 16 registers of this thread's TMEM lane to columns [taddr, taddr + 16); tmem_st_wait before others read them.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // v[j] += (x, y) for the pair j, j + 1, as one packed fp32 add.
 __device__ __forceinline__ void add_pair(float (&v)[32], int j, float x, float y) {
@@ -206,6 +226,20 @@ __device__ __forceinline__ uint64_t sw32_desc(uint32_t saddr) {
   d |= uint64_t(6) << 61;                 // SWIZZLE_32B
   return d;
 }
+
+// An MN-major tile with 128-byte swizzle: one K index per 128-byte row of 64 M/N elements, 8-row groups 1024 B
+// apart (SBO), blocks of 64 M/N elements `block_bytes` apart (LBO). The instruction descriptor says which
+// operand is MN-major (kMnMajorB).
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= uint64_t((saddr & 0x3FFFFu) >> 4);
+  d |= uint64_t(block_bytes >> 4) << 16;
+  d |= uint64_t(1024 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;
+  return d;
+}
+constexpr uint32_t kMnMajorB = 1u << 16;
 
 // Instruction descriptor: D f32, A/B format (1 = bf16 for kind::f16, 2 = TF32 for kind::tf32) at
 // bits 7 and 10, both K-major, N>>3 at bit 17, M>>4 at bit 24.

@@ -261,6 +261,14 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, query_starts: torch.Tens
     return out
 
 
+def check(device="cuda") -> None:
+    """Waits for the current stream of ``device`` and raises if a pipeline wait inside an attention call
+    has run out there since the last check (its rows hold NaN or were not written)."""
+    with torch.cuda.device(device):
+        index = torch.cuda.current_device()
+        _check(_native.lib().sb_decoder_status(torch._C._cuda_getCurrentRawStream(index)))
+
+
 class W4Weights:
     """Weights (code - zero) * scale of a linear layer, codes in 4 bits, in the order the kernel reads.
 
