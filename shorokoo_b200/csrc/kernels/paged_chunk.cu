@@ -5,15 +5,19 @@
 //
 // An item is 256 query rows of one key head (rows as in paged.cuh: tokens times the query heads that
 // share the key head), as two tiles A and B of 128: while the tensor core multiplies for one, the other's
-// logits become weights. One CTA per SM, 13 warps:
+// logits become weights. One CTA per SM, 16 warps (the last three idle):
 //   warps 0-3, 4-7   tiles A, B: a thread owns a query row. It loads the row's Q into shared memory (128-byte
-//                    swizzle, K-major), then per key tile reads its 128 logits from its TMEM lane twice: for
-//                    their maximum, and to write P = 2^(s - m) in 16 bits over them (columns 0-63 of the same
+//                    swizzle, K-major), then per key tile reads its 128 logits from its TMEM lane, takes
+//                    their maximum and writes P = 2^(s - m) in 16 bits over them (columns 0-63 of the same
 //                    128), the A operand of the second product. A running maximum that grows by less than
 //                    2^8 is left as it is (P then stays below 2^8, exact in range for either type), so that O
 //                    in TMEM is rescaled a few times per row only. At the end it reads its row of O.
-//   warps 8-11       K and V tiles of 128 positions, gathered page by page with 16-byte cp.async into a ring;
-//                    rows that are not there are zero-filled, and a bit per row says so.
+//   warps 8-11       K and V tiles of 128 positions into a ring of stages; rows that are not there read as
+//                    zero, and a bit per row says so. Pages of 8, 16, 32, .. positions: warp 8 issues one TMA
+//                    box per page and 64 elements, a lane each (a page that is not there is a coordinate past
+//                    the pool, which TMA fills with zeros). Other page sizes: all four warps gather rows with
+//                    16-byte cp.async (3300 cycles a tile against the TMA boxes' few hundred).
+//                    Values in positions that not every row sees are searched for infinities and NaN.
 //   warp 12          issues S = Q K^T (M = N = 128) and O += P V (P from TMEM, V MN-major as it lies in the
 //                    cache), in the order PV_A(j) S_A(j+1) PV_B(j) S_B(j+1): the tensor core runs its
 //                    instructions in issue order, so a commit of S(j+1) also says that PV(j) is done.
@@ -22,6 +26,7 @@
 // Waits are bounded: one that runs out sets the error word, every role leaves its loop, and the rows of
 // the piece are written as NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attention.cuh"
 
@@ -31,7 +36,7 @@ namespace {
 
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 128;
-constexpr int kChunkThreads = 416;
+constexpr int kChunkThreads = 512;
 constexpr int kLoadWarp = 8, kMmaWarp = 12;
 template <int DP> constexpr int kRing = DP == 128 ? 5 : 8;          // stages of one K or V tile
 template <int DP> constexpr uint32_t kTileBytes = 128u * DP * 2;
@@ -118,16 +123,45 @@ struct Walk {
   }
   __device__ __forceinline__ int ta(int x) const { return x ? ta1 : ta0; }
   __device__ __forceinline__ int tb(int x) const { return x ? tb1 : tb0; }
+  // whether some row does not see some position of the tile
+  __device__ __forceinline__ bool mixed(int tile) const {
+    const int64_t key0 = int64_t(tile) * kChunkKeys;
+    return key0 + kChunkKeys - 1 > all_hi || key0 < all_lo;
+  }
   __device__ __forceinline__ bool on(int x, int tile) const { return tile >= ta(x) && tile < tb(x); }
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const PagedArgs a) {
+// Takes the infinities and NaNs out of one 16-byte piece of a value tile, where its position is one that
+// not every row sees: a product with a weight of zero would carry them to the rows that do not. The
+// rows that see them add them at the end.
+template <typename T>
+__device__ __forceinline__ bool clean_piece(uint8_t* tile_at, int tile, int r, int piece, const Walk& w) {
+  const int64_t key = int64_t(tile) * kChunkKeys + r;
+  if (key <= w.all_hi && key >= w.all_lo) return false;
+  bool bad = false;
+  uint16_t* e = reinterpret_cast<uint16_t*>(tile_at + tile_off(r, piece));
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if ((e[q] & Mma<T>::kExp) == Mma<T>::kExp) {
+      e[q] = 0;
+      bad = true;
+    }
+  return bad;
+}
+
+// Boxes of a whole page, or of 128 of its positions, by 64 elements; rows 0: the cache is gathered.
+struct PagedMaps {
+  CUtensorMap k, v;
+};
+
+template <typename T, int DP, bool kTma>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    paged_chunk_kernel(const PagedArgs a, const __grid_constant__ PagedMaps maps) {
   extern __shared__ uint8_t smem_raw[];
   constexpr int kNst = kRing<DP>;
   constexpr uint32_t kTile = kTileBytes<DP>;
   constexpr int kPieces = DP / 8;
-  __shared__ uint64_t full[kNst], empty[kNst], q_full[2], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t there[kBook][4];      // which of a key tile's 128 positions are there
   __shared__ int poison[kBook];             // number of the piece that met non-finite values in mixed positions
   __shared__ uint32_t tmem_holder;
@@ -143,8 +177,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
 
   if (tid == 0) {
     for (int x = 0; x < kNst; ++x) {
-      mbar_init(&full[x], 4u);
-      mbar_init(&empty[x], 1u);
+      mbar_init(&full[x], kTma ? 1u : 4u);
+      mbar_init(&clean[x], 3u);
+      mbar_init(&empty[x], kTma ? 4u : 1u);   // the products, and the three cleaning warps
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], 4u);
@@ -165,6 +200,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
   tc_fence_after();
   const uint32_t tmem = tmem_holder;
   Walk w(c, G, a.window, sh);
+
+  // 512 threads start with 128 registers each; the row warps hold 128 logits in theirs: 2 x 128 x 184 and
+  // 2 x 128 x 72 are the same 65536.
+  if (warp < kLoadWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
 
   if (warp < kLoadWarp) {
     // ---- rows: Q, softmax, output ----
@@ -209,30 +249,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
           const uint32_t all = bits[0] & bits[1] & bits[2] & bits[3];
           // every row of the warp sees every position of the tile
           const bool plain = __all_sync(~0u, all == ~0u && (!live || (see_hi >= key0 + kChunkKeys - 1 && see_lo <= key0)));
-          uint32_t seen[4];
+          uint32_t v[128];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) tmem_ld32_async(ts + g * 32, v + g * 32);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) tmem_ld_wait(v + g * 32);
           if (!plain) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const int lo = see_lo - key0 - g * 32, hi = see_hi - key0 - g * 32;   // in [0, 31] once clamped
               uint32_t mask = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
               mask &= lo <= 0 ? ~0u : lo > 31 ? 0u : ~((1u << lo) - 1u);
-              seen[g] = mask & bits[g];
+              mask &= bits[g];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[g * 32 + j] = (mask >> j) & 1u ? v[g * 32 + j] : 0xff800000u;   // -infinity
             }
           }
-          uint32_t v[32];
-          float top = -INFINITY;
+          float tops[4];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            tmem_ld32(ts + g * 32, v);
-            if (plain) {
+          for (int g = 0; g < 4; ++g) tops[g] = __uint_as_float(v[g]);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) top = fmaxf(top, __uint_as_float(v[j]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if ((seen[g] >> j) & 1u) top = fmaxf(top, __uint_as_float(v[j]));
-            }
-          }
+          for (int j = 4; j < 128; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(v[j]));
+          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           // m is the reference of the row's weights in units of the raw logits
           const bool fresh = m == -INFINITY;
           const bool grow = top > m && (fresh || (top - m) * a.scale_log2 > kGrowth);
@@ -242,37 +280,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
             l *= f;
             if (tile > w.ta(x)) {
 #pragma unroll 1
-              for (int g = 0; g < DP / 32; ++g) {
-                tmem_ld32(to + g * 32, v);
+              for (int g = 0; g < DP / 16; ++g) {
+                uint32_t o[16];
+                tmem_ld16(to + g * 16, o);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-                tmem_st16(to + g * 32, v);
-                tmem_st16(to + g * 32 + 16, v + 16);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tmem_st16(to + g * 16, o);
               }
               tmem_st_wait();
             }
           }
           const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
-          float sum0 = 0.f, sum1 = 0.f;
+          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            tmem_ld32(ts + g * 32, v);
             uint32_t pk[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              float p0 = exp2_approx(fmaf(__uint_as_float(v[j]), a.scale_log2, -base));
-              float p1 = exp2_approx(fmaf(__uint_as_float(v[j + 1]), a.scale_log2, -base));
-              if (!plain) {
-                p0 = (seen[g] >> j) & 1u ? p0 : 0.f;
-                p1 = (seen[g] >> (j + 1)) & 1u ? p1 : 0.f;
-              }
-              sum0 += p0;
-              sum1 += p1;
-              pk[j >> 1] = Mma<T>::pack(p0, p1);
+              float2 e = make_float2(__uint_as_float(v[g * 32 + j]), __uint_as_float(v[g * 32 + j + 1]));
+              e = __ffma2_rn(e, scale2, base2);
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+              if (j & 2) sum1 = __fadd2_rn(sum1, e);
+              else sum0 = __fadd2_rn(sum0, e);
+              pk[j >> 1] = Mma<T>::pack(e.x, e.y);
             }
             tmem_st16(ts + g * 16, pk);
           }
-          l += sum0 + sum1;
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -343,8 +379,97 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
       book += w.tile_b - w.tile_a;
       if (__any_sync(~0u, *abort_flag)) break;
     } while (w.next());
-  } else if (warp < kMmaWarp) {
-    // ---- keys and values ----
+  } else if (kTma && warp == kLoadWarp) {
+    // ---- keys and values: TMA ----
+    const int rows = min(c.page_size, kChunkKeys);         // of a box
+    const int per_tile = kChunkKeys / rows, boxes = per_tile * (DP / 64);
+    const int part = lane % per_tile, slab = lane / per_tile;
+    int stage = 0, book = 0;
+    bool ok = true;
+    do {
+      const int32_t* table = c.table + int64_t(w.b) * c.table_stride;
+      const int n = w.tile_b - w.tile_a;
+      int next = 0, row = 0, page = 0, page_was = 0;       // `pages` for one that is not there
+      auto look_up = [&](int tile) {
+        const int key = tile * kChunkKeys + part * rows;
+        next = int(c.pages);
+        if (tile < w.tile_b && key < w.kend && key + rows > w.kbeg) {
+          const int p = table[key / c.page_size];
+          if (p >= 0 && p < c.pages) next = p;
+        }
+      };
+      look_up(w.tile_a);
+      for (int e = 0; e < 2 * n; ++e) {
+        const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
+        const int tile = w.tile_a + (e == 0 ? 0 : value ? (e == 2 * n - 1 ? n - 1 : e / 2 - 1) : (e + 1) / 2);
+        const int slot = stage % kNst;
+        if (!value) {
+          page_was = page;
+          page = next;
+        }
+        const int from = value && e != 2 * n - 1 ? page_was : page;   // the last value's rows are the latest looked up
+        row = rows == c.page_size ? 0 : tile * kChunkKeys % c.page_size;
+        if (stage >= kNst)
+          ok = __all_sync(~0u, mbar_wait(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+        if (!ok) break;
+        if (!value) {
+          const uint32_t held = __ballot_sync(~0u, from < c.pages);   // bit p: box p's page is there
+          if (lane < 4) {
+            uint32_t bits = 0;
+            if (rows >= 32) bits = (held >> (lane * 32 / rows)) & 1u ? ~0u : 0u;
+            else
+              for (int p = 0; p < 32 / rows; ++p)
+                if ((held >> (lane * (32 / rows) + p)) & 1u) bits |= ((1u << rows) - 1u) << (p * rows);
+            there[(book + tile - w.tile_a) % kBook][lane] = bits;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(&full[slot], kTile);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(smem_u32(ring + slot * kTile) + uint32_t(slab) * 16384u + uint32_t(part * rows) * 128u, value ? &maps.v : &maps.k,
+                      slab * 64, row, w.h, from, &full[slot]);
+        if (!value) look_up(tile + 1);
+        ++stage;
+      }
+      book += n;
+      if (!ok || __any_sync(~0u, *abort_flag)) break;
+    } while (w.next());
+    // the copies in flight land before this CTA's shared memory is given up
+    volatile int not_aborted = 0;
+    for (int st = max(0, stage - kNst); st < stage; ++st)
+      mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), &not_aborted, &chunk_error, 64u);
+  } else if (kTma && warp < kMmaWarp) {
+    // ---- non-finite values that not every row sees ----
+    const int cw = warp - kLoadWarp - 1;
+    int stage = 0, number = 0;
+    bool ok = true;
+    do {
+      ++number;
+      const int n = w.tile_b - w.tile_a;
+      for (int e = 0; e < 2 * n; ++e, ++stage) {   // every stage: a wait may not skip a phase
+        const int slot = stage % kNst;
+        ok = __all_sync(~0u, mbar_wait(&full[slot], uint32_t((stage / kNst) & 1), abort_flag, &chunk_error, 128u));
+        if (!ok) break;
+        const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
+        const int tile = w.tile_a + (e == 2 * n - 1 ? n - 1 : e / 2 - 1);
+        if (value && w.mixed(tile)) {
+          bool bad = false;
+#pragma unroll 1
+          for (int p = cw * 32 + lane; p < kChunkKeys * kPieces; p += 96)
+            bad |= clean_piece<T>(ring + slot * kTile, tile, p / kPieces, p % kPieces, w);
+          if (bad) poison[number % kBook] = number;
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&clean[slot]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
+      }
+      if (!ok || __any_sync(~0u, *abort_flag)) break;
+    } while (w.next());
+  } else if (!kTma && warp >= kLoadWarp && warp < kMmaWarp) {
+    // ---- keys and values: gathered ----
     const int lw = warp - kLoadWarp;
     int stage = 0, number = 0, book = 0;   // stages used, pieces, key tiles before the current piece
     bool ok = true;
@@ -360,18 +485,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
       if (tile >= 0) {
         bool bad = false;
 #pragma unroll 1
-        for (int j = 0; j < kPieces; ++j) {
-          const int rr = lw * 32 + j * (32 / kPieces) + lane / kPieces;
-          const int64_t key = int64_t(tile) * kChunkKeys + rr;
-          if (key <= wk.all_hi && key >= wk.all_lo) continue;
-          uint16_t* e = reinterpret_cast<uint16_t*>(ring + slot * kTile + tile_off(rr, lane % kPieces));
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if ((e[q] & Mma<T>::kExp) == Mma<T>::kExp) {
-              e[q] = 0;
-              bad = true;
-            }
-        }
+        for (int j = 0; j < kPieces; ++j)
+          bad |= clean_piece<T>(ring + slot * kTile, tile, lw * 32 + j * (32 / kPieces) + lane / kPieces, lane % kPieces, wk);
         if (bad) poison[number_of % kBook] = number_of;
       }
       fence_async_smem();
@@ -386,20 +501,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
       const T* vc = static_cast<const T*>(c.v) + int64_t(w.h) * c.vh;
       // per piece: K(a), then K(j + 1), V(j) for each tile j
       const int n = w.tile_b - w.tile_a;
+      int next_page = -1, next_row = 0;       // of the key tile to load next
+      auto look_up = [&](int tile) {
+        const int key = tile * kChunkKeys + lw * 32 + lane;
+        next_page = -1;
+        if (tile < w.tile_b && key >= w.kbeg && key < w.kend) {
+          const int page_no = key / c.page_size;
+          next_row = key - page_no * c.page_size;
+          next_page = table[page_no];
+          if (next_page < 0 || next_page >= c.pages) next_page = -1;
+        }
+      };
+      look_up(w.tile_a);
       for (int e = 0; e < 2 * n && ok; ++e) {
         const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
         const int tile = w.tile_a + (e == 0 ? 0 : value ? (e == 2 * n - 1 ? n - 1 : e / 2 - 1) : (e + 1) / 2);
         const int slot = stage % kNst;
         if (!value) {
           page_was = page, in_page_was = in_page;
-          const int key = tile * kChunkKeys + lw * 32 + lane;
-          page = -1;
-          if (key >= w.kbeg && key < w.kend) {
-            const int page_no = key / c.page_size;
-            in_page = key - page_no * c.page_size;
-            page = table[page_no];
-            if (page < 0 || page >= c.pages) page = -1;
-          }
+          page = next_page, in_page = next_row;
         }
         const bool last_value = e == 2 * n - 1;    // its rows are the latest looked up
         const int pg = value && !last_value ? page_was : page, ip = value && !last_value ? in_page_was : in_page;
@@ -421,8 +541,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
           cp_async_16(dst + tile_off(lw * 32 + rr, piece), live ? src + piece * 8 : static_cast<const T*>(c.k), live ? 16u : 0u);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const int64_t key0 = int64_t(tile) * kChunkKeys;
-        const bool mixed = value && (key0 + kChunkKeys - 1 > w.all_hi || key0 < w.all_lo);
+        if (!value) look_up(tile + 1);
+        const bool mixed = value && w.mixed(tile);
 #pragma unroll
         for (int j = kLag; j > 0; --j) clean_tile[j] = clean_tile[j - 1];
         clean_tile[0] = mixed ? tile : -1;
@@ -441,10 +561,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // ---- products ----
-    if (lane == 0) {
+    if (warp == kMmaWarp && lane == 0) {
       constexpr uint32_t id_s = idesc16<T>(128, kChunkKeys), id_o = idesc16<T>(128, DP) | kMnMajorB;
       int stage = 0;
-      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, clean_phase = 0;
       bool ok = true;
       auto wait_stage = [&](int st) {
         return mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
@@ -480,6 +600,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) paged_chunk_kernel(const Pag
           const int tile = w.tile_a + j;
           if (j + 1 < n) ok = wait_stage(k_stage(j + 1));
           ok = ok && wait_stage(v_stage(j));
+          if (kTma && ok && w.mixed(tile)) {
+            const int slot = v_stage(j) % kNst;
+            ok = mbar_wait(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, &chunk_error, 256u);
+            clean_phase ^= 1u << slot;
+          }
           if (!ok) break;
           tc_fence_after();
           const uint64_t vd = sw128_mn_desc(smem_u32(ring + (v_stage(j) % kNst) * kTile), 16384u);
@@ -551,15 +676,49 @@ __global__ void __launch_bounds__(256) paged_chunk_join_kernel(const PagedArgs a
     *reinterpret_cast<uint2*>(to + d4 * 4) = make_uint2(Mma<T>::pack(v.x * inv, v.y * inv), Mma<T>::pack(v.z * inv, v.w * inv));
 }
 
-template <typename T, int DP>
-cudaError_t launch_chunk(const PagedArgs& a, cudaStream_t s) {
+// The cache as (element, position in page, head, page); false where TMA cannot describe it.
+bool encode_pages(CUtensorMap* tm, const void* base, const PagedView& c, int64_t page, int64_t token, int64_t head, bool bf16) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p) : nullptr;
+  }();
+  const int rows = std::min(c.page_size, kChunkKeys);
+  if (!fn || rows < 8 || kChunkKeys % rows != 0 || c.page_size % rows != 0 || c.pages < 1) return false;
+  const int64_t stride[3] = {token, head, page};
+  const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.page_size), cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] == 1) bytes[i] = 16;   // never stepped along
+    else if (stride[i] <= 0 || stride[i] >= (int64_t(1) << 39)) return false;
+    else bytes[i] = cuuint64_t(stride[i]) * 2;
+  }
+  const cuuint32_t box[4] = {64, cuuint32_t(rows), 1, 1}, step[4] = {1, 1, 1, 1};
+  return fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, bytes, box,
+            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DP, bool kTma>
+cudaError_t launch_chunk(const PagedArgs& a, const PagedMaps& maps, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(paged_chunk_kernel<T, DP>, kChunkSmem<DP>, done);
+  cudaError_t e = allow_smem(paged_chunk_kernel<T, DP, kTma>, kChunkSmem<DP>, done);
   if (e != cudaSuccess) return e;
-  paged_chunk_kernel<T, DP><<<a.ctas, kChunkThreads, kChunkSmem<DP>, s>>>(a);
+  paged_chunk_kernel<T, DP, kTma><<<a.ctas, kChunkThreads, kChunkSmem<DP>, s>>>(a, maps);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_dependent(paged_chunk_join_kernel<T, DP>, dim3(unsigned(a.ctas), DP / 4), 256, a, s);
+}
+
+template <typename T, int DP>
+cudaError_t launch_chunk(const PagedArgs& a, cudaStream_t s) {
+  PagedMaps maps = {};
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const PagedView& c = a.c;
+  const bool tma = encode_pages(&maps.k, c.k, c, c.kp, c.kt, c.kh, bf16) && encode_pages(&maps.v, c.v, c, c.vp, c.vt, c.vh, bf16);
+  return tma ? launch_chunk<T, DP, true>(a, maps, s) : launch_chunk<T, DP, false>(a, maps, s);
 }
 
 }  // namespace
