@@ -5,7 +5,7 @@
 //
 // An item is 256 query rows of one key head (rows as in paged.cuh: tokens times the query heads that
 // share the key head), as two tiles A and B of 128: while the tensor core multiplies for one, the other's
-// logits become weights. One CTA per SM, 16 warps (the last three idle):
+// logits become weights. One CTA per SM, 16 warps (the last two idle):
 //   warps 0-3, 4-7   tiles A, B: a thread owns a query row. It loads the row's Q into shared memory (128-byte
 //                    swizzle, K-major), then per key tile reads its 128 logits from its TMEM lane, takes
 //                    their maximum and writes P = 2^(s - m) in 16 bits over them (columns 0-63 of the same
@@ -18,9 +18,10 @@
 //                    the pool, which TMA fills with zeros). Other page sizes: all four warps gather rows with
 //                    16-byte cp.async (3300 cycles a tile against the TMA boxes' few hundred).
 //                    Values in positions that not every row sees are searched for infinities and NaN.
-//   warp 12          issues S = Q K^T (M = N = 128) and O += P V (P from TMEM, V MN-major as it lies in the
-//                    cache), in the order PV_A(j) S_A(j+1) PV_B(j) S_B(j+1): the tensor core runs its
-//                    instructions in issue order, so a commit of S(j+1) also says that PV(j) is done.
+//   warps 12, 13     issue S = Q K^T (M = N = 128) and O += P V (P from TMEM, V MN-major as it lies in the
+//                    cache) for a tile each, in the order PV(j) S(j+1): the tensor core runs a thread's
+//                    instructions in issue order, so a commit of S(j+1) also says that PV(j) is done. (One
+//                    warp for both tiles could not issue fast enough beside the row warps.)
 // TMEM: S/P of A 0-127, of B 128-255, O of A 256-383, of B 384-511.
 //
 // Waits are bounded: one that runs out sets the error word, every role leaves its loop, and the rows of
@@ -128,7 +129,6 @@ struct Walk {
     const int64_t key0 = int64_t(tile) * kChunkKeys;
     return key0 + kChunkKeys - 1 > all_hi || key0 < all_lo;
   }
-  __device__ __forceinline__ bool on(int x, int tile) const { return tile >= ta(x) && tile < tb(x); }
 };
 
 // Takes the infinities and NaNs out of one 16-byte piece of a value tile, where its position is one that
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int kNst = kRing<DP>;
   constexpr uint32_t kTile = kTileBytes<DP>;
   constexpr int kPieces = DP / 8;
-  __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
   __shared__ uint32_t there[kBook][4];      // which of a key tile's 128 positions are there
   __shared__ int poison[kBook];             // number of the piece that met non-finite values in mixed positions
   __shared__ uint32_t tmem_holder;
@@ -179,13 +179,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int x = 0; x < kNst; ++x) {
       mbar_init(&full[x], kTma ? 1u : 4u);
       mbar_init(&clean[x], 3u);
-      mbar_init(&empty[x], kTma ? 4u : 1u);   // the products, and the three cleaning warps
+      mbar_init(&empty[x], kTma ? 5u : 2u);   // both tiles' products, and the three cleaning warps
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], 4u);
-      mbar_init(&s_full[x], 1u);
-      mbar_init(&p_full[x], 4u);
-      mbar_init(&o_full[x], 1u);
+      for (int y = 0; y < 2; ++y) {
+        mbar_init(&s_full[x][y], 1u);
+        mbar_init(&p_full[x][y], 4u);
+        mbar_init(&pv_done[x][y], 1u);
+      }
     }
     abort_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -201,19 +203,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem = tmem_holder;
   Walk w(c, G, a.window, sh);
 
-  // 512 threads start with 128 registers each; the row warps hold 128 logits in theirs: 2 x 128 x 184 and
-  // 2 x 128 x 72 are the same 65536.
-  if (warp < kLoadWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-
   if (warp < kLoadWarp) {
     // ---- rows: Q, softmax, output ----
     const int x = warp >> 2;                              // tile A or B
     const int r = tid & 127;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + uint32_t(x * 128), to = tmem + lanes + 256u + uint32_t(x * 128);
+    const uint32_t ts_x = tmem + lanes + uint32_t(x * 128), to = tmem + lanes + 256u + uint32_t(x * 128);
     uint8_t* q_at = sq + x * kTile;
-    uint32_t s_phase = 0, o_phase = 0;
+    int step = 0;                                         // halves of key tiles before the current piece (even)
     int number = 0, book = 0;                             // pieces, key tiles before the current piece
     do {
       ++number;
@@ -239,24 +236,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[x]);
-        for (int tile = w.ta(x); tile < w.tb(x); ++tile) {
-          ok = __all_sync(~0u, mbar_wait(&s_full[x], s_phase, abort_flag, &chunk_error, 1u));
-          s_phase ^= 1u;
+        const int steps = 2 * (w.tb(x) - w.ta(x));
+        for (int i = 0; i < steps; ++i) {
+          const int buf = i & 1;
+          ok = __all_sync(~0u, mbar_wait(&s_full[x][buf], uint32_t((step + i) >> 1) & 1u, abort_flag, &chunk_error, 1u));
           if (!ok) break;
           tc_fence_after();
-          const int key0 = tile * kChunkKeys;
-          const uint32_t* bits = there[(book + tile - w.tile_a) % kBook];
-          const uint32_t all = bits[0] & bits[1] & bits[2] & bits[3];
-          // every row of the warp sees every position of the tile
-          const bool plain = __all_sync(~0u, all == ~0u && (!live || (see_hi >= key0 + kChunkKeys - 1 && see_lo <= key0)));
-          uint32_t v[128];
-#pragma unroll
-          for (int g = 0; g < 4; ++g) tmem_ld32_async(ts + g * 32, v + g * 32);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) tmem_ld_wait(v + g * 32);
+          const int tile = w.ta(x) + (i >> 1), key0 = tile * kChunkKeys + buf * 64;
+          const uint32_t ts = ts_x + uint32_t(buf * 64);
+          const uint32_t* bits = there[(book + tile - w.tile_a) % kBook] + buf * 2;
+          uint32_t v[64];
+          tmem_ld32_async(ts, v);
+          tmem_ld32_async(ts + 32, v + 32);
+          // every row of the warp sees every position of the half
+          const bool plain = __all_sync(~0u, (bits[0] & bits[1]) == ~0u && (!live || (see_hi >= key0 + 63 && see_lo <= key0)));
+          tmem_ld_wait(v);
+          tmem_ld_wait(v + 32);
           if (!plain) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < 2; ++g) {
               const int lo = see_lo - key0 - g * 32, hi = see_hi - key0 - g * 32;   // in [0, 31] once clamped
               uint32_t mask = hi < 0 ? 0u : hi >= 31 ? ~0u : (2u << hi) - 1u;
               mask &= lo <= 0 ? ~0u : lo > 31 ? 0u : ~((1u << lo) - 1u);
@@ -269,7 +267,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int g = 0; g < 4; ++g) tops[g] = __uint_as_float(v[g]);
 #pragma unroll
-          for (int j = 4; j < 128; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(v[j]));
+          for (int j = 4; j < 64; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(v[j]));
           const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           // m is the reference of the row's weights in units of the raw logits
           const bool fresh = m == -INFINITY;
@@ -278,7 +276,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const float f = grow ? (fresh ? 0.f : exp2_approx((m - top) * a.scale_log2)) : 1.f;
             if (grow) m = top;
             l *= f;
-            if (tile > w.ta(x)) {
+            if (i > 0) {
+              ok = __all_sync(~0u, mbar_wait(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
               for (int g = 0; g < DP / 16; ++g) {
                 uint32_t o[16];
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
           float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < 2; ++g) {
             uint32_t pk[16];
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -312,10 +313,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[x]);
+          if (lane == 0) mbar_arrive(&p_full[x][buf]);
         }
-        if (ok) ok = __all_sync(~0u, mbar_wait(&o_full[x], o_phase, abort_flag, &chunk_error, 2u));
-        o_phase ^= 1u;
+        step += steps;
+        if (ok) ok = __all_sync(~0u, mbar_wait(&pv_done[x][1], uint32_t((step - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
         tc_fence_after();
       }
       // ---- the row's result ----
@@ -560,71 +561,77 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     } while (w.next());
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
-    // ---- products ----
-    if (warp == kMmaWarp && lane == 0) {
-      constexpr uint32_t id_s = idesc16<T>(128, kChunkKeys), id_o = idesc16<T>(128, DP) | kMnMajorB;
-      int stage = 0;
-      uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, clean_phase = 0;
+    // ---- products: a warp per row tile ----
+    const int x = warp - kMmaWarp;
+    if (x < 2 && lane == 0) {
+      constexpr uint32_t id_s = idesc16<T>(128, 64), id_o = idesc16<T>(128, DP) | kMnMajorB;
+      const uint32_t ts = tmem + uint32_t(x * 128), to = tmem + 256u + uint32_t(x * 128);
+      const uint64_t qd = sw128_desc(smem_u32(sq + x * kTile));
+      int stage = 0, step = 0;
+      uint32_t q_phase = 0, clean_phase = 0;
       bool ok = true;
       auto wait_stage = [&](int st) {
         return mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
       };
-      auto logits = [&](int x, int st) {
-        const uint64_t qd = sw128_desc(smem_u32(sq + x * kTile)), kd = sw128_desc(smem_u32(ring + (st % kNst) * kTile));
+      auto logits = [&](int st, int half) {   // 64 positions
+        const uint64_t kd = sw128_desc(smem_u32(ring + (st % kNst) * kTile) + uint32_t(half) * 8192u);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t step = uint64_t((kk >> 2) * 1024 + (kk & 3) * 2);   // a slab of 64 elements is 16 KB
-          umma_bf16(tmem + uint32_t(x * 128), qd + step, kd + step, id_s, kk > 0 ? 1u : 0u);
+          const uint64_t at = uint64_t((kk >> 2) * 1024 + (kk & 3) * 2);   // a slab of 64 elements is 16 KB
+          umma_bf16(ts + uint32_t(half * 64), qd + at, kd + at, id_s, kk > 0 ? 1u : 0u);
         }
-        umma_commit(&s_full[x]);
+        umma_commit(&s_full[x][half]);
       };
       do {
-        const int n = w.tile_b - w.tile_a;
+        const int n = w.tile_b - w.tile_a, ta = w.ta(x), tb = w.tb(x);
         // stages of this piece: K(a) is 0; K(j) is 2j - 1; V(j) is 2j + 2, but the last V is 2n - 1
         auto k_stage = [&](int j) { return stage + (j == 0 ? 0 : 2 * j - 1); };
         auto v_stage = [&](int j) { return stage + (j == n - 1 ? 2 * n - 1 : 2 * j + 2); };
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (ok && w.ta(x) < w.tb(x)) {
-            ok = mbar_wait(&q_full[x], q_phase[x], abort_flag, &chunk_error, 16u);
-            q_phase[x] ^= 1u;
-          }
+        if (ta < tb) {
+          ok = mbar_wait(&q_full[x], q_phase, abort_flag, &chunk_error, 16u);
+          q_phase ^= 1u;
+        }
         ok = ok && wait_stage(k_stage(0));
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (w.on(x, w.tile_a)) logits(x, k_stage(0));
+        if (w.tile_a >= ta && w.tile_a < tb) {
+          logits(k_stage(0), 0);
+          logits(k_stage(0), 1);
+        }
         umma_commit(&empty[k_stage(0) % kNst]);
         for (int j = 0; j < n && ok; ++j) {
           const int tile = w.tile_a + j;
-          if (j + 1 < n) ok = wait_stage(k_stage(j + 1));
-          ok = ok && wait_stage(v_stage(j));
+          const bool on = tile >= ta && tile < tb, on_next = j + 1 < n && tile + 1 >= ta && tile + 1 < tb;
+          ok = wait_stage(v_stage(j));
           if (kTma && ok && w.mixed(tile)) {
             const int slot = v_stage(j) % kNst;
             ok = mbar_wait(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, &chunk_error, 256u);
             clean_phase ^= 1u << slot;
           }
           if (!ok) break;
-          tc_fence_after();
           const uint64_t vd = sw128_mn_desc(smem_u32(ring + (v_stage(j) % kNst) * kTile), 16384u);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (w.on(x, tile)) {
-              ok = ok && mbar_wait(&p_full[x], p_phase[x], abort_flag, &chunk_error, 32u);
-              p_phase[x] ^= 1u;
+          for (int half = 0; half < 2; ++half) {
+            if (on) {
+              ok = ok && mbar_wait(&p_full[x][half], uint32_t(step >> 1) & 1u, abort_flag, &chunk_error, 32u);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
-              for (int kk = 0; kk < kChunkKeys / 16; ++kk)   // 16 positions: two 8-row groups of 1024 B
-                umma_f16_ts(tmem + 256u + uint32_t(x * 128), tmem + uint32_t(x * 128 + kk * 8), vd + uint64_t(kk * 128), id_o,
-                            tile > w.ta(x) || kk > 0 ? 1u : 0u);
-              if (tile + 1 == w.tb(x)) umma_commit(&o_full[x]);
+              for (int kk = 0; kk < 4; ++kk)   // 16 positions: two 8-row groups of 1024 B
+                umma_f16_ts(to, ts + uint32_t(half * 64 + kk * 8), vd + uint64_t(half * 512 + kk * 128), id_o,
+                            tile > ta || half > 0 || kk > 0 ? 1u : 0u);
+              umma_commit(&pv_done[x][half]);
+              ++step;
             }
-            if (j + 1 < n && w.on(x, tile + 1)) logits(x, k_stage(j + 1));
+            if (half == 1) umma_commit(&empty[v_stage(j) % kNst]);
+            if (half == 0 && j + 1 < n) {
+              ok = wait_stage(k_stage(j + 1));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (on_next) logits(k_stage(j + 1), half);
           }
           if (!ok) break;
-          umma_commit(&empty[v_stage(j) % kNst]);
           if (j + 1 < n) umma_commit(&empty[k_stage(j + 1) % kNst]);
         }
         stage += 2 * n;
