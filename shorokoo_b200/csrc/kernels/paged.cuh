@@ -107,12 +107,12 @@ struct Share {
 
 // Every CTA works its share out by itself (whole block; the result is the same in all threads): the
 // sequences' tiles are counted by a thread each, or by a warp each where they have many row tiles,
-// and summed; then the sequence, head and row tile that hold its first tile are looked up.
-constexpr int kCounted = 128;   // sequences whose counts are kept between the two steps
+// and summed; then the sequence, head and row tile that hold its first tile are looked up. `count` is
+// kCounted words of shared memory that are free until then.
+constexpr int kCounted = 512;   // sequences whose counts are kept between the two steps
 
 template <int kRows, int kKeys, int kThreads>
-__device__ __forceinline__ Share find_share(const PagedView& c, int group, int window, int least, int cta, int ctas) {
-  __shared__ int64_t count[kCounted];
+__device__ __forceinline__ Share find_share(const PagedView& c, int group, int window, int least, int cta, int ctas, int64_t* count) {
   __shared__ int64_t warp_sum[kThreads / 32];
   __shared__ int64_t found_rem;
   __shared__ Share found;

@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
   const int D = c.head_dim, G = a.group;
   pdl_launch_dependents();
 
-  Share sh = find_share<kRowsTile, kKeysTile, kRowsThreads>(c, G, a.window, a.least, blockIdx.x, a.ctas);
+  Share sh = find_share<kRowsTile, kKeysTile, kRowsThreads>(c, G, a.window, a.least, blockIdx.x, a.ctas,
+                                                              reinterpret_cast<int64_t*>(smem));
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = PartialNote{0, 0, 0, 0};
   if (sh.u0 >= sh.u1) return;
   __syncthreads();

@@ -48,6 +48,32 @@ constexpr float kGrowth = 8.f;   // log2 of how far a weight may rise above 1 be
 
 __device__ unsigned chunk_error;   // bits of the waits that ran out since it was last read
 
+// mbar_wait whose attempts may sleep in hardware until the phase ends (up to 20 us each): the waiting
+// warps of the other roles share the row warps' issue slots.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err,
+                                           unsigned int code) {
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitTimeoutNs) {
+      *abort_flag = 1;
+      atomicOr(err, code);
+      return false;
+    }
+  }
+}
+
 // byte offset of 16-byte piece `c` of row `r` in a tile of 128-byte-swizzled slabs of 64 elements
 __device__ __forceinline__ uint32_t tile_off(int r, int c) {
   return uint32_t(c >> 3) * 16384u + uint32_t(r) * 128u + (uint32_t((c & 7) ^ (r & 7)) << 4);
@@ -59,9 +85,40 @@ template <typename T> constexpr uint32_t idesc16(int M, int N) {
   return (1u << 4) | kIdescType<T> | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+  return d;
+}
+
+// v = -infinity where `seen` is 0. (Volatile, so that it stays inside its branch: as selects, the 64 of a
+// row's half would be executed for tiles that need none, twice as many instructions as the rest.)
+__device__ __forceinline__ void hide(uint32_t& v, uint32_t seen) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\tselp.b32 %0, %0, 0xff800000, p;\n\t}" : "+r"(v) : "r"(seen));
+}
+
+// 2^x of a pair on the multiply-add pipe, for x <= 8 (anything below -126 counts as -126): x = n + f with n
+// the nearest integer, 2^f on [-1/2, 1/2] by the polynomial of degree 4 of least relative error (Remez
+// exchange; 2.6e-6, a hundredth of the rounding to 16 bits that follows), times 2^n made from its bits.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));   // a NaN stays one to the end
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 p = __ffma2_rn(f, make_float2(0.009570102207362652f, 0.009570102207362652f),
+                        make_float2(0.05591785907745361f, 0.05591785907745361f));
+  p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return __fmul2_rn(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+}
+constexpr int kPolyOf8 = 0;   // pairs of 8 that take it: the SM's 16 exponentials per cycle are the scarcer part
+
 // One CTA's walk over its pieces; every role steps through the same ones.
 struct Walk {
-  const PagedView& c;
   int group, window;
   Share sh;
   int64_t u;
@@ -76,7 +133,8 @@ struct Walk {
   int kbeg, kend;
   int64_t all_lo, all_hi;   // positions that every row of the pair sees
 
-  __device__ __forceinline__ Walk(const PagedView& view, int g, int w, const Share& share) : c(view), group(g), window(w), sh(share) {
+  __device__ __forceinline__ void start(const PagedView& c, int g, int win, const Share& share) {
+    group = g, window = win, sh = share;
     u = sh.u0, b = sh.b, h = sh.h, i = sh.i, at = sh.tile;
     s = seq_work(c, b, group);
     piece();
@@ -105,7 +163,7 @@ struct Walk {
     hi = min(tile_b, part.tile0 + part.tiles);
     if (lo >= hi) lo = hi = 0;
   }
-  __device__ __forceinline__ bool next() {
+  __device__ __forceinline__ bool next(const PagedView& c) {
     u += tile_b - tile_a;
     at = 0;
     if (u >= sh.u1) return false;
@@ -166,6 +224,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __shared__ int poison[kBook];             // number of the piece that met non-finite values in mixed positions
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
+  __shared__ Walk row_walk[8];              // of the row warps: their registers hold logits
   volatile int* abort_flag = &abort_word;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;                       // Q of A, Q of B
@@ -193,7 +252,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < kBook) poison[tid] = 0;
-  const Share sh = find_share<kChunkRows, kChunkKeys, kChunkThreads>(c, G, a.window, a.least, blockIdx.x, a.ctas);
+  const Share sh = find_share<kChunkRows, kChunkKeys, kChunkThreads>(c, G, a.window, a.least, blockIdx.x, a.ctas,
+                                                                     reinterpret_cast<int64_t*>(smem));
   if (tid < 2) a.notes[2 * blockIdx.x + tid] = PartialNote{0, 0, 0, 0};
   if (sh.u0 >= sh.u1) return;
   if (warp == kMmaWarp) tmem_alloc(&tmem_holder, 512);
@@ -201,10 +261,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_holder;
-  Walk w(c, G, a.window, sh);
+
+  // 512 threads start with 128 registers each; 2 x 128 x 168 and 2 x 128 x 88 are the same 65536.
+  if (warp < kLoadWarp) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 
   if (warp < kLoadWarp) {
     // ---- rows: Q, softmax, output ----
+    Walk& w = row_walk[warp];
+    {
+      Walk first;
+      first.start(c, G, a.window, sh);
+      if (lane == 0) w = first;
+      __syncwarp();
+    }
+    auto advance = [&] {
+      Walk now = w;
+      __syncwarp();
+      const bool more = now.next(c);
+      if (lane == 0) w = now;
+      __syncwarp();
+      return more;
+    };
     const int x = warp >> 2;                              // tile A or B
     const int r = tid & 127;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
@@ -236,15 +314,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[x]);
-        const int steps = 2 * (w.tb(x) - w.ta(x));
+        const int ta = w.ta(x), steps = 2 * (w.tb(x) - ta), book_a = book + ta - w.tile_a;
         for (int i = 0; i < steps; ++i) {
           const int buf = i & 1;
-          ok = __all_sync(~0u, mbar_wait(&s_full[x][buf], uint32_t((step + i) >> 1) & 1u, abort_flag, &chunk_error, 1u));
+          ok = __all_sync(~0u, wait_phase(&s_full[x][buf], uint32_t((step + i) >> 1) & 1u, abort_flag, &chunk_error, 1u));
           if (!ok) break;
           tc_fence_after();
-          const int tile = w.ta(x) + (i >> 1), key0 = tile * kChunkKeys + buf * 64;
+          const int key0 = (ta + (i >> 1)) * kChunkKeys + buf * 64;
           const uint32_t ts = ts_x + uint32_t(buf * 64);
-          const uint32_t* bits = there[(book + tile - w.tile_a) % kBook] + buf * 2;
+          const uint32_t* bits = there[(book_a + (i >> 1)) % kBook] + buf * 2;
           uint32_t v[64];
           tmem_ld32_async(ts, v);
           tmem_ld32_async(ts + 32, v + 32);
@@ -260,24 +338,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               mask &= lo <= 0 ? ~0u : lo > 31 ? 0u : ~((1u << lo) - 1u);
               mask &= bits[g];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[g * 32 + j] = (mask >> j) & 1u ? v[g * 32 + j] : 0xff800000u;   // -infinity
+              for (int j = 0; j < 32; ++j) hide(v[g * 32 + j], mask & (1u << j));
             }
           }
-          float tops[4];
+          // m is the reference of the row's weights in units of the raw logits. The weights are taken against the
+          // one of the steps before, side by side with the maximum; where that has grown too far (a row's first
+          // step, and a few after it), once more against the new one.
+          float2 sum0, sum1;
+          for (;;) {
+            const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
+            const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
+            float tops[2] = {-INFINITY, -INFINITY};
+            sum0 = sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) tops[g] = __uint_as_float(v[g]);
+            for (int g = 0; g < 2; ++g) {
+              uint32_t pk[16];
 #pragma unroll
-          for (int j = 4; j < 64; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(v[j]));
-          const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-          // m is the reference of the row's weights in units of the raw logits
-          const bool fresh = m == -INFINITY;
-          const bool grow = top > m && (fresh || (top - m) * a.scale_log2 > kGrowth);
-          if (__any_sync(~0u, grow)) {
+              for (int j = 0; j < 32; j += 2) {
+                float2 e = make_float2(__uint_as_float(v[g * 32 + j]), __uint_as_float(v[g * 32 + j + 1]));
+                tops[(j >> 1) & 1] = max3(tops[(j >> 1) & 1], e.x, e.y);
+                e = __ffma2_rn(e, scale2, base2);
+                if ((j >> 1) % 8 < kPolyOf8) {
+                  e = exp2_poly(e);
+                } else {
+                  e.x = exp2_approx(e.x);
+                  e.y = exp2_approx(e.y);
+                }
+                if (j & 2) sum1 = __fadd2_rn(sum1, e);
+                else sum0 = __fadd2_rn(sum0, e);
+                pk[j >> 1] = Mma<T>::pack(e.x, e.y);
+              }
+              tmem_st16(ts + g * 16, pk);
+            }
+            const float top = fmaxf(tops[0], tops[1]);
+            const bool fresh = m == -INFINITY;
+            const bool grow = top > m && (fresh || (top - m) * a.scale_log2 > kGrowth);
+            if (!__any_sync(~0u, grow)) break;
             const float f = grow ? (fresh ? 0.f : exp2_approx((m - top) * a.scale_log2)) : 1.f;
             if (grow) m = top;
             l *= f;
             if (i > 0) {
-              ok = __all_sync(~0u, mbar_wait(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
+              ok = __all_sync(~0u, wait_phase(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -291,24 +392,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               tmem_st_wait();
             }
           }
-          const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
-          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float2 e = make_float2(__uint_as_float(v[g * 32 + j]), __uint_as_float(v[g * 32 + j + 1]));
-              e = __ffma2_rn(e, scale2, base2);
-              e.x = exp2_approx(e.x);
-              e.y = exp2_approx(e.y);
-              if (j & 2) sum1 = __fadd2_rn(sum1, e);
-              else sum0 = __fadd2_rn(sum0, e);
-              pk[j >> 1] = Mma<T>::pack(e.x, e.y);
-            }
-            tmem_st16(ts + g * 16, pk);
-          }
+          if (!ok) break;
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
           tmem_st_wait();
           tc_fence_before();
@@ -316,7 +400,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[x][buf]);
         }
         step += steps;
-        if (ok) ok = __all_sync(~0u, mbar_wait(&pv_done[x][1], uint32_t((step - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
+        if (ok) ok = __all_sync(~0u, wait_phase(&pv_done[x][1], uint32_t((step - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
         tc_fence_after();
       }
       // ---- the row's result ----
@@ -375,13 +459,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       if (!w.whole && live) a.ml[int64_t(w.slot) * kChunkRows + x * 128 + r] = make_float2(m * a.scale_log2, l + bad);
       if (!w.whole && w.head && tid == 0)
-        a.notes[w.slot] = PartialNote{w.b, w.h, w.i, int((w.u + w.tiles - 1) / sh.per) - int(blockIdx.x)};
+        a.notes[w.slot] = PartialNote{w.b, w.h, w.i, int((w.u + w.tiles - 1) / w.sh.per) - int(blockIdx.x)};
       tc_fence_before();   // these reads of O come before the next piece's products
       book += w.tile_b - w.tile_a;
       if (__any_sync(~0u, *abort_flag)) break;
-    } while (w.next());
+    } while (advance());
   } else if (kTma && warp == kLoadWarp) {
     // ---- keys and values: TMA ----
+    Walk w;
+    w.start(c, G, a.window, sh);
     const int rows = min(c.page_size, kChunkKeys);         // of a box
     const int per_tile = kChunkKeys / rows, boxes = per_tile * (DP / 64);
     const int part = lane % per_tile, slab = lane / per_tile;
@@ -411,7 +497,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int from = value && e != 2 * n - 1 ? page_was : page;   // the last value's rows are the latest looked up
         row = rows == c.page_size ? 0 : tile * kChunkKeys % c.page_size;
         if (stage >= kNst)
-          ok = __all_sync(~0u, mbar_wait(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
         if (!ok) break;
         if (!value) {
           const uint32_t held = __ballot_sync(~0u, from < c.pages);   // bit p: box p's page is there
@@ -435,13 +521,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       book += n;
       if (!ok || __any_sync(~0u, *abort_flag)) break;
-    } while (w.next());
+    } while (w.next(c));
     // the copies in flight land before this CTA's shared memory is given up
     volatile int not_aborted = 0;
     for (int st = max(0, stage - kNst); st < stage; ++st)
-      mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), &not_aborted, &chunk_error, 64u);
+      wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), &not_aborted, &chunk_error, 64u);
   } else if (kTma && warp < kMmaWarp) {
     // ---- non-finite values that not every row sees ----
+    Walk w;
+    w.start(c, G, a.window, sh);
     const int cw = warp - kLoadWarp - 1;
     int stage = 0, number = 0;
     bool ok = true;
@@ -450,7 +538,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int n = w.tile_b - w.tile_a;
       for (int e = 0; e < 2 * n; ++e, ++stage) {   // every stage: a wait may not skip a phase
         const int slot = stage % kNst;
-        ok = __all_sync(~0u, mbar_wait(&full[slot], uint32_t((stage / kNst) & 1), abort_flag, &chunk_error, 128u));
+        ok = __all_sync(~0u, wait_phase(&full[slot], uint32_t((stage / kNst) & 1), abort_flag, &chunk_error, 128u));
         if (!ok) break;
         const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
         const int tile = w.tile_a + (e == 2 * n - 1 ? n - 1 : e / 2 - 1);
@@ -468,9 +556,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (lane == 0) mbar_arrive(&empty[slot]);
       }
       if (!ok || __any_sync(~0u, *abort_flag)) break;
-    } while (w.next());
+    } while (w.next(c));
   } else if (!kTma && warp >= kLoadWarp && warp < kMmaWarp) {
     // ---- keys and values: gathered ----
+    Walk w;
+    w.start(c, G, a.window, sh);
     const int lw = warp - kLoadWarp;
     int stage = 0, number = 0, book = 0;   // stages used, pieces, key tiles before the current piece
     bool ok = true;
@@ -525,7 +615,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool last_value = e == 2 * n - 1;    // its rows are the latest looked up
         const int pg = value && !last_value ? page_was : page, ip = value && !last_value ? in_page_was : in_page;
         if (stage >= kNst)
-          ok = __all_sync(~0u, mbar_wait(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
         if (!ok) break;
         if (!value) {
           const uint32_t bits = __ballot_sync(~0u, pg >= 0);
@@ -558,7 +648,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       while (ok && arrived < stage) hand_over(stage - arrived == 2 ? clean_tile[1] : clean_tile[0], number, w);
       book += n;
       if (!ok || __any_sync(~0u, *abort_flag)) break;
-    } while (w.next());
+    } while (w.next(c));
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     // ---- products: a warp per row tile ----
@@ -566,12 +656,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (x < 2 && lane == 0) {
       constexpr uint32_t id_s = idesc16<T>(128, 64), id_o = idesc16<T>(128, DP) | kMnMajorB;
       const uint32_t ts = tmem + uint32_t(x * 128), to = tmem + 256u + uint32_t(x * 128);
+    Walk w;
+    w.start(c, G, a.window, sh);
       const uint64_t qd = sw128_desc(smem_u32(sq + x * kTile));
       int stage = 0, step = 0;
       uint32_t q_phase = 0, clean_phase = 0;
       bool ok = true;
       auto wait_stage = [&](int st) {
-        return mbar_wait(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
+        return wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
       };
       auto logits = [&](int st, int half) {   // 64 positions
         const uint64_t kd = sw128_desc(smem_u32(ring + (st % kNst) * kTile) + uint32_t(half) * 8192u);
@@ -588,7 +680,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         auto k_stage = [&](int j) { return stage + (j == 0 ? 0 : 2 * j - 1); };
         auto v_stage = [&](int j) { return stage + (j == n - 1 ? 2 * n - 1 : 2 * j + 2); };
         if (ta < tb) {
-          ok = mbar_wait(&q_full[x], q_phase, abort_flag, &chunk_error, 16u);
+          ok = wait_phase(&q_full[x], q_phase, abort_flag, &chunk_error, 16u);
           q_phase ^= 1u;
         }
         ok = ok && wait_stage(k_stage(0));
@@ -605,7 +697,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           ok = wait_stage(v_stage(j));
           if (kTma && ok && w.mixed(tile)) {
             const int slot = v_stage(j) % kNst;
-            ok = mbar_wait(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, &chunk_error, 256u);
+            ok = wait_phase(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, &chunk_error, 256u);
             clean_phase ^= 1u << slot;
           }
           if (!ok) break;
@@ -613,7 +705,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             if (on) {
-              ok = ok && mbar_wait(&p_full[x][half], uint32_t(step >> 1) & 1u, abort_flag, &chunk_error, 32u);
+              ok = ok && wait_phase(&p_full[x][half], uint32_t(step >> 1) & 1u, abort_flag, &chunk_error, 32u);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
@@ -635,7 +727,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (j + 1 < n) umma_commit(&empty[k_stage(j + 1) % kNst]);
         }
         stage += 2 * n;
-      } while (ok && w.next());
+      } while (ok && w.next(c));
     }
     __syncwarp();
   }
