@@ -37,6 +37,7 @@ struct W4Args {
   void* y;
   int64_t xs, ys, rows, n, k;
   int blocks, groups, group;
+  int shift;   // log2 of the group size, or -1
 };
 
 struct W4Sizes {
@@ -56,7 +57,6 @@ W4Sizes sizes(const W4View& w) {
 
 template <typename T> struct Half;
 template <> struct Half<__half> {
-  static constexpr uint32_t kMagic = 0x64006400u;   // 1024: a code in the low mantissa bits reads 1024 + code
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
@@ -72,7 +72,6 @@ template <> struct Half<__half> {
   }
 };
 template <> struct Half<__nv_bfloat16> {
-  static constexpr uint32_t kMagic = 0x43004300u;   // 128: 128 + code, exact in 8 significant bits
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
@@ -98,7 +97,7 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
 
 // 8 inputs from element k of a row (zero past K); kWide: K, the row stride and the address allow 16 bytes
 template <bool kWide>
-__device__ __forceinline__ uint4 load_x(const uint16_t* row, int64_t k, int64_t kmax) {
+__device__ __forceinline__ uint4 load_x(const uint16_t* row, int k, int kmax) {
   if (kWide) return k < kmax ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
   uint32_t w[4];
 #pragma unroll
@@ -110,11 +109,46 @@ __device__ __forceinline__ uint4 load_x(const uint16_t* row, int64_t k, int64_t 
 }
 
 constexpr int kW4Warps = 8;
-constexpr int kW4Unroll = 4;   // 64-input blocks in flight per warp
 
-// MT: row tiles of 8; kPerBlock: one group covers a 64-input block (else one per 32)
+// What a warp reads of a 64-input block besides x, and has in flight for the blocks to come.
+struct Block {
+  uint4 w;
+  uint2 s;       // scale pairs (output g, g + 8) of the two halves
+  uint32_t z;    // zero points of output g, g + 8 of the first half, then of the second, a byte each
+};
+
+template <typename T> struct Codes;
+// Operand registers of 8 codes less their zero point. magic + code is exact in the type; fp16's 10 mantissa bits
+// also hold a code four bits up (1024 + 16 code), which saves the shift.
+template <> struct Codes<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x43004300u | (z * 0x00010001u); }
+  static __device__ __forceinline__ void spread(uint32_t w, uint32_t z, uint32_t (&r)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = Half<__nv_bfloat16>::sub(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, z);
+  }
+};
+template <> struct Codes<__half> {
+  static __device__ __forceinline__ uint32_t zero(uint32_t z) { return 0x64006400u | (z * 0x00010001u); }
+  static __device__ __forceinline__ void spread(uint32_t w, uint32_t z, uint32_t (&r)[4]) {
+    const __half2 z1 = *reinterpret_cast<__half2*>(&z);
+    // (1024 + 16 c) / 16 - (64 + z) = c - z, where 64 + z = (1024 + z) - 960
+    const __half2 z16 = __hsub2(__float2half2_rn(960.f), z1), sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t v = w >> (8 * i);
+      r[2 * i] = Half<__half>::sub((v & 0x000f000fu) | 0x64006400u, z);
+      uint32_t up = (v & 0x00f000f0u) | 0x64006400u;
+      const __half2 d = __hfma2(*reinterpret_cast<__half2*>(&up), sixteenth, z16);
+      r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+  }
+};
+
+// MT: row tiles of 8; kPerBlock: one group covers a 64-input block (else one per 32). kDepth: blocks in
+// flight per warp.
 template <typename T, int MT, bool kZeros, bool kPerBlock, bool kWide>
 __global__ void __launch_bounds__(kW4Warps * 32) linear_w4_kernel(const W4Args a) {
+  constexpr int kDepth = 4;
   __shared__ float sums[kW4Warps][16][MT * 8 + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t tile = blockIdx.x, m0 = int64_t(blockIdx.y) * (MT * 8);
@@ -129,57 +163,66 @@ __global__ void __launch_bounds__(kW4Warps * 32) linear_w4_kernel(const W4Args a
     live[i] = m < a.rows;
     x[i] = static_cast<const uint16_t*>(a.x) + (live[i] ? m : m0) * a.xs + t * 8;
   }
+  const int kmax = int(a.k) - t * 8;   // of this lane's pieces of x
+  auto load = [&](Block& b, int kb) {
+    b.w = load_once(w + int64_t(kb) * 32);
+    const int g0 = a.shift >= 0 ? (kb * 64) >> a.shift : kb * 64 / a.group;
+    b.s.x = scales[g0 * 8];
+    if (kZeros) b.z = zeros[g0 * 8];
+    if (!kPerBlock) {
+      // the last block's second half may lie past K
+      const int g1 = min(a.shift >= 0 ? (kb * 64 + 32) >> a.shift : (kb * 64 + 32) / a.group, a.groups - 1);
+      b.s.y = scales[g1 * 8];
+      if (kZeros) b.z |= uint32_t(zeros[g1 * 8]) << 16;
+    }
+  };
   float acc[MT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 
-  for (int kb0 = warp; kb0 < a.blocks; kb0 += kW4Warps * kW4Unroll) {
-    uint4 q[kW4Unroll];
+  Block next[kDepth];
 #pragma unroll
-    for (int j = 0; j < kW4Unroll; ++j) {
+  for (int j = 0; j < kDepth; ++j)
+    if (warp + j * kW4Warps < a.blocks) load(next[j], warp + j * kW4Warps);
+  for (int kb0 = warp; kb0 < a.blocks; kb0 += kW4Warps * kDepth) {
+#pragma unroll
+    for (int j = 0; j < kDepth; ++j) {
       const int kb = kb0 + j * kW4Warps;
-      q[j] = kb < a.blocks ? load_once(w + int64_t(kb) * 32) : make_uint4(0, 0, 0, 0);
-    }
+      if (kb < a.blocks) {
+        const Block b = next[j];
+        if (kb + kW4Warps * kDepth < a.blocks) load(next[j], kb + kW4Warps * kDepth);
+        const uint32_t word[4] = {b.w.x, b.w.y, b.w.z, b.w.w};
+        float part[MT][4];
+        uint32_t z0 = Codes<T>::zero(8u), z1 = z0;
 #pragma unroll
-    for (int j = 0; j < kW4Unroll; ++j) {
-      const int kb = kb0 + j * kW4Warps;
-      if (kb >= a.blocks) break;
-      const uint32_t word[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
-      float part[MT][4];
+        for (int half = 0; half < 2; ++half) {
+          const int k0 = kb * 64 + half * 32;
+          if (half == 0 || !kPerBlock) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k0 = kb * 64 + half * 32;
-        if (half == 0 || !kPerBlock) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
-        }
-        const int gi = min(k0 / a.group, a.groups - 1);   // the last block's second half may lie past K
-        uint32_t z0 = Half<T>::kMagic | 0x00080008u, z1 = z0;
-        if (kZeros) {
-          const uint32_t z = zeros[gi * 8];
-          z0 = Half<T>::kMagic | ((z & 255u) * 0x00010001u);
-          z1 = Half<T>::kMagic | ((z >> 8) * 0x00010001u);
-        }
-        uint32_t lo[4], hi[4];   // outputs g and g + 8
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[i] = Half<T>::sub(((word[2 * half] >> (4 * i)) & 0x000f000fu) | Half<T>::kMagic, z0);
-          hi[i] = Half<T>::sub(((word[2 * half + 1] >> (4 * i)) & 0x000f000fu) | Half<T>::kMagic, z1);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint4 b = live[i] ? load_x<kWide>(x[i], k0, a.k - t * 8) : make_uint4(0, 0, 0, 0);
-          Half<T>::mma(part[i], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-          Half<T>::mma(part[i], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-        }
-        if (half == 1 || !kPerBlock) {
-          const float2 s = Half<T>::both(scales[gi * 8]);
+            for (int i = 0; i < MT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
+            if (kZeros) {
+              z0 = Codes<T>::zero((b.z >> (16 * half)) & 255u);
+              z1 = Codes<T>::zero((b.z >> (16 * half + 8)) & 255u);
+            }
+          }
+          uint32_t lo[4], hi[4];   // outputs g and g + 8
+          Codes<T>::spread(word[2 * half], z0, lo);
+          Codes<T>::spread(word[2 * half + 1], z1, hi);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            acc[i][0] += s.x * part[i][0];
-            acc[i][1] += s.x * part[i][1];
-            acc[i][2] += s.y * part[i][2];
-            acc[i][3] += s.y * part[i][3];
+            const uint4 v = live[i] ? load_x<kWide>(x[i], k0, kmax) : make_uint4(0, 0, 0, 0);
+            Half<T>::mma(part[i], lo[0], hi[0], lo[1], hi[1], v.x, v.y);
+            Half<T>::mma(part[i], lo[2], hi[2], lo[3], hi[3], v.z, v.w);
+          }
+          if (half == 1 || !kPerBlock) {
+            const float2 s = Half<T>::both(!kPerBlock && half == 1 ? b.s.y : b.s.x);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              acc[i][0] += s.x * part[i][0];
+              acc[i][1] += s.x * part[i][1];
+              acc[i][2] += s.y * part[i][2];
+              acc[i][3] += s.y * part[i][3];
+            }
           }
         }
       }
@@ -295,6 +338,7 @@ cudaError_t linear_w4(const W4View& w, const void* x, int64_t xs, const void* bi
   a.zeros = reinterpret_cast<const uint16_t*>(p + z.w + z.s);
   a.x = x, a.bias = bias, a.y = y, a.xs = xs, a.ys = ys, a.rows = rows, a.n = w.n, a.k = w.k;
   a.blocks = int(z.blocks), a.groups = int(z.groups), a.group = w.group;
+  a.shift = (w.group & (w.group - 1)) == 0 ? __builtin_ctz(unsigned(w.group)) : -1;
   const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && w.k % 8 == 0 && (xs % 8 == 0 || rows == 1);
   const bool per_block = w.group % 64 == 0;
   if (w.elem == 10) return launch<__half>(a, w.zeros, per_block, wide, s);

@@ -17,6 +17,7 @@ compute no autograd graph and refuse inputs that require one. Errors are the bac
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -65,18 +66,32 @@ def _on(x, name: str, device: torch.device, dtype: torch.dtype, dims: int) -> No
         raise B200NotSupportedError(f"{name} requires a gradient, which these operators do not record")
 
 
-def _heads(x: torch.Tensor, name: str) -> _native.Heads:
-    token, head, last = x.stride()
-    if last != 1 and x.shape[2] != 1:
-        _bad(f"{name} must be contiguous along its last dimension")
-    return _native.Heads(x.data_ptr(), token, head)
+_pack_heads = struct.Struct("Pqq").pack   # sb_heads
+
+
+def _heads(x, name: str, device: torch.device, dtype: torch.dtype):
+    """(tokens, heads, head_dim, sb_heads) of a [tokens, heads, head_dim] tensor."""
+    try:
+        tokens, heads, dim = x.shape
+        token, head, last = x.stride()
+        if (x.dtype is dtype and x.get_device() == device.index and (last == 1 or dim == 1)
+                and not (x.requires_grad and torch.is_grad_enabled())):
+            return tokens, heads, dim, _pack_heads(x.data_ptr(), token, head)
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _on(x, name, device, dtype, 3)
+    _bad(f"{name} must be contiguous along its last dimension")
 
 
 def _starts(x, device: torch.device, batch: int) -> int:
+    try:
+        if (x.dtype is torch.int32 and x.get_device() == device.index and x.shape == (batch + 1,)
+                and (x.stride() == (1,) or batch == 0)):
+            return x.data_ptr()
+    except AttributeError:
+        pass
     _on(x, "query_starts", device, torch.int32, 1)
-    if x.shape[0] != batch + 1 or not x.is_contiguous():
-        _bad(f"query_starts must be {batch + 1} contiguous values, got {tuple(x.shape)}")
-    return x.data_ptr()
+    _bad(f"query_starts must be {batch + 1} contiguous values, got {tuple(x.shape)}")
 
 
 class RotaryTable:
@@ -134,24 +149,22 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, inverse
     (int32 or int64 [tokens], any sign). ``inverse`` turns back, which is the adjoint: the gradient of x
     for the gradient of the result. ``out`` may be x itself, but not overlap it otherwise."""
     device = _cuda(x, "x")
-    elem = _ELEM.get(x.dtype)
+    dtype = x.dtype
+    elem = _ELEM.get(dtype)
     if elem is None:
-        raise B200NotSupportedError(f"element type {x.dtype} is not supported")
-    _on(x, "x", device, x.dtype, 3)
-    tokens, heads, dim = x.shape
+        raise B200NotSupportedError(f"element type {dtype} is not supported")
+    tokens, heads, dim, xh = _heads(x, "x", device, dtype)
     if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
         _bad("positions must be an int32 or int64 tensor")
-    _on(positions, "positions", device, positions.dtype, 1)
-    if positions.shape[0] != tokens or not positions.is_contiguous():
-        _bad(f"positions must be {tokens} contiguous values, got {tuple(positions.shape)}")
+    if positions.get_device() != device.index or positions.shape != (tokens,) or not positions.is_contiguous():
+        _bad(f"positions must be {tokens} contiguous values on {device}, got {tuple(positions.shape)} on {positions.device}")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=device)
-    else:
-        _on(out, "out", device, x.dtype, 3)
-        if out.shape != x.shape:
-            _bad(f"out must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
-    _call("sb_rotary", device, C.byref(_heads(x, "x")), C.byref(_heads(out, "out")), elem, tokens, heads, dim,
-          positions.data_ptr(), positions.dtype is torch.int64, _table(table, device), bool(inverse))
+        out = torch.empty_like(x)
+    t, h, d, yh = _heads(out, "out", device, dtype)
+    if t != tokens or h != heads or d != dim:
+        _bad(f"out must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
+    _call("sb_rotary", device, xh, yh, elem, tokens, heads, dim, positions.data_ptr(), positions.dtype is torch.int64,
+          _table(table, device), bool(inverse))
     return out
 
 
@@ -205,13 +218,13 @@ class PagedCache:
             n = self._space[(heads, tokens)] = size.value
         return n
 
-    def _rows(self, x, name: str, heads: Optional[int], tokens: Optional[int]) -> _native.Heads:
-        _on(x, name, self.device, self.dtype, 3)
-        s = x.shape
-        if (tokens is not None and s[0] != tokens) or (heads is not None and s[1] != heads) or s[2] != self.head_dim:
+    def _rows(self, x, name: str, heads: Optional[int], tokens: Optional[int]):
+        """(tokens, heads, sb_heads) of a tensor of the step's rows; None: any number."""
+        t, h, d, packed = _heads(x, name, self.device, self.dtype)
+        if (tokens is not None and t != tokens) or (heads is not None and h != heads) or d != self.head_dim:
             _bad(f"{name} must have shape [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, "
-                 f"{self.head_dim}], got {tuple(s)}")
-        return _heads(x, name)
+                 f"{self.head_dim}], got {tuple(x.shape)}")
+        return t, h, packed
 
 
 def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, query_starts: torch.Tensor, *,
@@ -221,24 +234,23 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, query_star
     has rows query_starts[b] .. query_starts[b + 1] - 1 (int32 [batch + 1]), its last positions in order.
     With a table, k is turned by its position first, and so is q [tokens, heads, head_dim], which is
     returned (in ``out``, which may be q itself). Rows of no sequence are neither read nor written."""
-    kh = cache._rows(k, "k", cache.kv_heads, None)
-    tokens = k.shape[0]
-    vh = cache._rows(v, "v", cache.kv_heads, tokens)
-    starts = _starts(query_starts, cache.device, cache.batch)
-    ref = None if table is None else _table(table, cache.device)
+    device = cache.device
+    tokens, _, kh = cache._rows(k, "k", cache.kv_heads, None)
+    _, _, vh = cache._rows(v, "v", cache.kv_heads, tokens)
+    starts = _starts(query_starts, device, cache.batch)
+    ref = None if table is None else _table(table, device)
     if q is None:
         if out is not None:
             _bad("out needs q")
-        _call("sb_paged_append", cache.device, cache._ref, C.byref(kh), C.byref(vh), None, None, 0, tokens, starts, ref)
+        _call("sb_paged_append", device, cache._ref, kh, vh, None, None, 0, tokens, starts, ref)
         return None
     if table is None:
         _bad("q needs a table")
-    qh = cache._rows(q, "q", None, tokens)
+    _, heads, qh = cache._rows(q, "q", None, tokens)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
-    oh = cache._rows(out, "out", q.shape[1], tokens)
-    _call("sb_paged_append", cache.device, cache._ref, C.byref(kh), C.byref(vh), C.byref(qh), C.byref(oh), q.shape[1], tokens,
-          starts, ref)
+        out = torch.empty_like(q)
+    _, _, oh = cache._rows(out, "out", heads, tokens)
+    _call("sb_paged_append", device, cache._ref, kh, vh, qh, oh, heads, tokens, starts, ref)
     return out
 
 
@@ -248,16 +260,16 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, query_starts: torch.Tens
     over the positions of its sequence up to its own (``window`` > 0: the last ``window`` of them). Rows
     are as in ``paged_append``; query head h reads key head h // (heads // kv_heads); scale defaults to
     1 / sqrt(head_dim). A token that sees nothing gets zeros; rows of no sequence are not written."""
-    qh = cache._rows(q, "q", None, None)
-    tokens, heads, dim = q.shape
-    starts = _starts(query_starts, cache.device, cache.batch)
+    device = cache.device
+    tokens, heads, qh = cache._rows(q, "q", None, None)
+    starts = _starts(query_starts, device, cache.batch)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=cache.device)
-    oh = cache._rows(out, "out", heads, tokens)
+        out = torch.empty_like(q)
+    _, _, oh = cache._rows(out, "out", heads, tokens)
     n = cache._workspace(heads, tokens)
-    space = torch.empty(n, dtype=torch.uint8, device=cache.device)
-    _call("sb_paged_attention", cache.device, cache._ref, C.byref(qh), C.byref(oh), heads, tokens, starts,
-          dim ** -0.5 if scale is None else scale, window, space.data_ptr(), n)
+    space = torch.empty(n, dtype=torch.uint8, device=device)
+    _call("sb_paged_attention", device, cache._ref, qh, oh, heads, tokens, starts,
+          cache.head_dim ** -0.5 if scale is None else scale, window, space.data_ptr(), n)
     return out
 
 
@@ -314,23 +326,29 @@ def linear_w4(x: torch.Tensor, weights: W4Weights, bias: Optional[torch.Tensor] 
     """x [rows, in_features] times the weights' transpose, plus bias [out_features], as [rows,
     out_features]; x, bias and the result have the weights' type. Meant for few rows: the weights are
     read once for every 32 of them."""
-    device, n = weights.device, weights.out_features
-    _on(x, "x", device, weights.dtype, 2)
-    rows, k = x.shape
-    xs, last = x.stride()
-    if k != weights.in_features or (last != 1 and k > 1):
-        _bad(f"x must be [rows, {weights.in_features}] and contiguous along its rows, got {tuple(x.shape)}")
-    if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=device)
-    else:
-        _on(out, "out", device, weights.dtype, 2)
-        if out.shape != (rows, n) or (out.stride(1) != 1 and n > 1):
-            _bad(f"out must be [{rows}, {n}] and contiguous along its rows, got {tuple(out.shape)}")
+    device, dtype, n, k = weights.device, weights.dtype, weights.out_features, weights.in_features
+    rows, xs = _matrix(x, "x", device, dtype, None, k)
+    out = x.new_empty((rows, n)) if out is None else out
+    ys = _matrix(out, "out", device, dtype, rows, n)[1]
     at = None
     if bias is not None:
-        _on(bias, "bias", device, weights.dtype, 1)
-        if bias.shape[0] != n or not bias.is_contiguous():
+        if bias.dtype is not dtype or bias.get_device() != device.index or bias.shape != (n,) or not bias.is_contiguous():
+            _on(bias, "bias", device, dtype, 1)
             _bad(f"bias must be {n} contiguous values, got {tuple(bias.shape)}")
         at = bias.data_ptr()
-    _call("sb_linear_w4", device, weights._ref, x.data_ptr(), xs, at, out.data_ptr(), out.stride(0), rows)
+    _call("sb_linear_w4", device, weights._ref, x.data_ptr(), xs, at, out.data_ptr(), ys, rows)
     return out
+
+
+def _matrix(x, name: str, device: torch.device, dtype: torch.dtype, rows: Optional[int], columns: int):
+    """(rows, row stride) of a matrix whose rows are contiguous; rows None: any number."""
+    try:
+        m, n = x.shape
+        stride, last = x.stride()
+        if (x.dtype is dtype and x.get_device() == device.index and n == columns and (rows is None or m == rows)
+                and (last == 1 or n == 1) and not (x.requires_grad and torch.is_grad_enabled())):
+            return m, stride
+    except (AttributeError, TypeError, ValueError):
+        pass
+    _on(x, name, device, dtype, 2)
+    _bad(f"{name} must be [{'rows' if rows is None else rows}, {columns}] and contiguous along its rows, got {tuple(x.shape)}")
