@@ -174,12 +174,12 @@ def _weights(**kw):
 
 def test_w4_layout_bytes():
     """Tiles of 16 x 64 codes (512 bytes), then 16 scales per tile and group, then as many zero bytes,
-    the last two padded to 256 bytes."""
+    groups in whole eights."""
     n = C.c_size_t()
     assert L.sb_w4_layout_bytes(C.byref(_weights()), C.byref(n)) == 0
-    assert n.value == 3 * 4 * 512 + 512
+    assert n.value == 3 * 4 * 512 + 3 * 8 * 32
     assert L.sb_w4_layout_bytes(C.byref(_weights(has_zeros=1, out_features=49)), C.byref(n)) == 0
-    assert n.value == 4 * 4 * 512 + 512 + 256
+    assert n.value == 4 * 4 * 512 + 4 * 8 * 32 + 4 * 8 * 16
 
 
 @pytest.mark.parametrize("kw,status", [
