@@ -22,6 +22,7 @@ namespace {
 constexpr int kRowsTile = 16;
 constexpr int kKeysTile = 64;
 constexpr int kRowsThreads = 128;
+constexpr float kGrowth = 8.f;
 template <int DP> constexpr int kStages = DP == 128 ? 3 : 4;
 template <int DP> constexpr int kRowsSmem = 4 * kStages<DP> * 2 * 16 * DP * 2;
 
@@ -137,21 +138,24 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
       const uint32_t kat = ring_at + stage * kStage, vat = kat + kPart;
       const bool mixed = key0 + 15 > all_hi || key0 < all_lo;   // not every row sees every position
 
-      float sc[2][4];
+      float sc[2][4], odd[2][4];   // two sums each: half as long a chain of dependent products
 #pragma unroll
-      for (int e = 0; e < 2; ++e) sc[e][0] = sc[e][1] = sc[e][2] = sc[e][3] = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        sc[e][0] = sc[e][1] = sc[e][2] = sc[e][3] = 0.f;
+        odd[e][0] = odd[e][1] = odd[e][2] = odd[e][3] = 0.f;
+      }
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         uint32_t kf[4];
         const int r = (lane & 7) + ((lane & 16) >> 1), chunk = 2 * ks + ((lane & 8) >> 3);
         ldmatrix4(kf, kat + r * (DP * 2) + ((chunk ^ (r & 7)) << 4));
-        Mma<T>::run(sc[0], qf[ks], kf[0], kf[1]);
-        Mma<T>::run(sc[1], qf[ks], kf[2], kf[3]);
+        Mma<T>::run(ks & 1 ? odd[0] : sc[0], qf[ks], kf[0], kf[1]);
+        Mma<T>::run(ks & 1 ? odd[1] : sc[1], qf[ks], kf[2], kf[3]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[e][j] *= a.scale_log2;
+        for (int j = 0; j < 4; ++j) sc[e][j] = (sc[e][j] + odd[e][j]) * a.scale_log2;
       if (mask != 0xffffu || mixed) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -182,25 +186,26 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
         if (bad) poisoned = 1;
         __syncwarp();
       }
-      uint32_t pf[4];
-      float grow[2];
+      // The rows' references m follow their maxima only when one has grown by more than 2^8 (weights stay exact
+      // in range up to there), so that most steps need no exchange between lanes and leave o alone.
+      float top[2];
+      bool grown = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {   // rows g, g + 8
-        float top = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const float now = fmaxf(m[e], top);
-        const float base = now == -INFINITY ? 0.f : now;   // a row that has seen nothing yet
-        grow[e] = exp2_approx(m[e] - base);
-        m[e] = now;
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = exp2_approx(sc[j >> 1][2 * e + (j & 1)] - base);
-        l[e] = l[e] * grow[e] + ((p[0] + p[1]) + (p[2] + p[3]));
-        pf[e] = Mma<T>::pack(p[0], p[1]);
-        pf[e + 2] = Mma<T>::pack(p[2], p[3]);
+        top[e] = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
+        grown |= m[e] == -INFINITY ? top[e] > m[e] : top[e] - m[e] > kGrowth;
       }
-      if (__any_sync(~0u, grow[0] != 1.f || grow[1] != 1.f)) {
+      if (__any_sync(~0u, grown)) {
+        float grow[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
+          const float now = fmaxf(m[e], top[e]);
+          grow[e] = exp2_approx(m[e] - (now == -INFINITY ? 0.f : now));
+          m[e] = now;
+          l[e] *= grow[e];
+        }
 #pragma unroll
         for (int j = 0; j < DP / 8; ++j) {
           o[j][0] *= grow[0];
@@ -208,6 +213,17 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
           o[j][2] *= grow[1];
           o[j][3] *= grow[1];
         }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float base = m[e] == -INFINITY ? 0.f : m[e];   // a row that has seen nothing yet
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = exp2_approx(sc[j >> 1][2 * e + (j & 1)] - base);
+        l[e] += (p[0] + p[1]) + (p[2] + p[3]);
+        pf[e] = Mma<T>::pack(p[0], p[1]);
+        pf[e + 2] = Mma<T>::pack(p[2], p[3]);
       }
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j) {
@@ -333,15 +349,24 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
   const float base = top == -INFINITY ? 0.f : top;
   constexpr int kPer = DP / 32;
   float v[kPer] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int p = 0; p < pieces; ++p) {
-    const int64_t at = slot(p);
-    const float2 ml = a.ml[at];
-    const float f = exp2_approx(ml.x - base);
-    sum += f * ml.y;
-    const float* o = a.o + at * DP + lane * kPer;
+  for (int p0 = 0; p0 < pieces; p0 += 32) {
+    float f = 0.f, l = 0.f;   // of piece p0 + lane
+    if (p0 + lane < pieces) {
+      const float2 ml = a.ml[slot(p0 + lane)];
+      f = exp2_approx(ml.x - base);
+      l = f * ml.y;
+    }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] += f * o[j];
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+    sum += l;
+    const int count = min(32, pieces - p0);
+#pragma unroll 8
+    for (int p = 0; p < count; ++p) {
+      const float w = __shfl_sync(~0u, f, p);
+      const float* o = a.o + slot(p0 + p) * DP + lane * kPer;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) v[j] += w * o[j];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int tok = row / a.group, d = lane * kPer;

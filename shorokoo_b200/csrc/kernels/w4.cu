@@ -462,7 +462,11 @@ cudaError_t launch(const W4Args& a, bool zeros, bool per_block, bool wide, int s
     if ((a.n + 31) / 32 >= 4 * sms) return launch<T, 1, 2>(a, zeros, per_block, wide, s);
     return launch<T, 1, 1>(a, zeros, per_block, wide, s);
   }
-  if (a.rows <= 16) return launch<T, 2, 1>(a, zeros, per_block, wide, s);
+  if (a.rows <= 16) {
+    // ... and here half of what the SMs read of x, 13 rows of which are 106 KB per tile: 20.7 -> 18.5 us
+    if ((a.n + 31) / 32 >= 2 * sms) return launch<T, 2, 2>(a, zeros, per_block, wide, s);
+    return launch<T, 2, 1>(a, zeros, per_block, wide, s);
+  }
   return launch<T, 4, 1>(a, zeros, per_block, wide, s);
 }
 
