@@ -244,6 +244,12 @@ CASES = [
     ([257, 0, 1, 300], [513, 9, 0, 2000], 16, 2, 128, 64, BF16, 0, "pthd"),
     ([190, 140], [190, 640], 10, 2, 64, 16, FP16, 100, "pthd"),       # 5 heads per key head: rows of a token over two tiles
     ([300], [2500], 3, 1, 128, 16, FP16, 700, "pthd"),
+    ([200], [333], 2, 2, 64, 8, BF16, 0, "phtd"),                     # the smallest pages that are copied whole
+    ([150, 60], [700, 60], 4, 2, 128, 256, FP16, 0, "one"),           # pages longer than a tile
+    ([100, 100], [100, 900], 8, 2, 104, 128, BF16, 333, "phtd"),
+    ([90, 40], [95, 300], 16, 2, 128, 4, FP16, 0, "pthd"),            # pages too small for that: gathered
+    ([1] * 600, [1 + i % 70 for i in range(600)], 2, 1, 64, 16, BF16, 0, "pthd"),     # more sequences than are counted at once
+    ([3] * 520, [3 + i % 40 for i in range(520)], 16, 1, 64, 16, FP16, 0, "pthd"),
 ]
 
 
@@ -471,6 +477,15 @@ def linear(x, packed, scales, zeros, bias, k, group):
     (100, 80, 320, 64, BF16, True, True),
     (5, 1000, 9000, 32, FP16, True, False),
     (4, 64, 100, 4096, FP16, True, False),     # one group longer than the row
+    (1, 100, 1000, 64, FP16, True, True),      # one row: each group size, ragged ends, odd inputs
+    (1, 50, 2050, 32, BF16, True, False),
+    (1, 33, 777, 256, FP16, True, False),
+    (1, 20, 300, 96, BF16, True, True),
+    (1, 70, 5000, 1024, BF16, True, False),
+    (1, 2500, 8192, 32, FP16, True, False),
+    (1, 19000, 128, 128, BF16, False, False),  # enough outputs for the smaller CTAs
+    (7, 19100, 320, 64, FP16, True, False),    # two tiles of outputs per CTA, the last one alone
+    (12, 9500, 256, 32, BF16, True, True),
 ])
 def test_linear_w4(rows, n, k, group, dtype, zeros, bias):
     gen = torch.Generator().manual_seed(n + k)
@@ -623,6 +638,13 @@ def test_graph_replay_follows_the_lengths():
         want = step()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(out2, want)
+
+
+def test_attention_reports_no_wait_errors():
+    decoder.check()
+    p = Paged([200], [1500], 2, 64, 16, BF16)
+    decoder.paged_attention(p.gpu(), torch.zeros(200, 4, 64, dtype=BF16, device="cuda"), p.starts.cuda())
+    decoder.check()
 
 
 def test_calls_on_two_streams():
