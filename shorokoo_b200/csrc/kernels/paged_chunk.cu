@@ -189,22 +189,21 @@ struct Walk {
   }
 };
 
-// Takes the infinities and NaNs out of one 16-byte piece of a value tile, where its position is one that
-// not every row sees: a product with a weight of zero would carry them to the rows that do not. The
-// rows that see them add them at the end.
+// Takes the infinities and NaNs out of one 16-byte piece of a value tile: a product with a weight of zero
+// would carry them to rows that do not see the position. The rows that see them add them at the end. An
+// exponent of all ones carries into the sign bit when one is added to it, which finds them two at a time.
 template <typename T>
-__device__ __forceinline__ bool clean_piece(uint8_t* tile_at, int tile, int r, int piece, const Walk& w) {
-  const int64_t key = int64_t(tile) * kChunkKeys + r;
-  if (key <= w.all_hi && key >= w.all_lo) return false;
-  bool bad = false;
-  uint16_t* e = reinterpret_cast<uint16_t*>(tile_at + tile_off(r, piece));
+__device__ __forceinline__ bool clean_piece(uint8_t* tile_at, int r, int piece) {
+  constexpr uint32_t kExps = Mma<T>::kExp * 0x00010001u, kOnes = (0x8000u - Mma<T>::kExp) * 0x00010001u;
+  uint4* at = reinterpret_cast<uint4*>(tile_at + tile_off(r, piece));
+  const uint4 v = *at;
+  const uint32_t hit = ((v.x & kExps) + kOnes) | ((v.y & kExps) + kOnes) | ((v.z & kExps) + kOnes) | ((v.w & kExps) + kOnes);
+  if (!(hit & 0x80008000u)) return false;
+  uint16_t* e = reinterpret_cast<uint16_t*>(at);
 #pragma unroll
   for (int q = 0; q < 8; ++q)
-    if ((e[q] & Mma<T>::kExp) == Mma<T>::kExp) {
-      e[q] = 0;
-      bad = true;
-    }
-  return bad;
+    if ((e[q] & Mma<T>::kExp) == Mma<T>::kExp) e[q] = 0;
+  return true;
 }
 
 // Boxes of a whole page, or of 128 of its positions, by 64 elements; rows 0: the cache is gathered.
@@ -543,10 +542,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
         const int tile = w.tile_a + (e == 2 * n - 1 ? n - 1 : e / 2 - 1);
         if (value && w.mixed(tile)) {
+          // rows [0, below) and [above, 128) hold positions that not every row sees
+          const int64_t key0 = int64_t(tile) * kChunkKeys;
+          int below = int(clamp64(w.all_lo - key0, 0, kChunkKeys)), above = int(clamp64(w.all_hi + 1 - key0, 0, kChunkKeys));
+          if (below > above) below = above = 0;
+          const int gap = above - below;
           bool bad = false;
-#pragma unroll 1
-          for (int p = cw * 32 + lane; p < kChunkKeys * kPieces; p += 96)
-            bad |= clean_piece<T>(ring + slot * kTile, tile, p / kPieces, p % kPieces, w);
+#pragma unroll 1   // four at a time were 141 -> 177 us for windowed prompts: more code beside the row warps'
+          for (int p = cw * 32 + lane; p < (kChunkKeys - gap) * kPieces; p += 96) {
+            const int r = p / kPieces;
+            bad |= clean_piece<T>(ring + slot * kTile, r < below ? r : r + gap, p % kPieces);
+          }
           if (bad) poison[number % kBook] = number;
           fence_async_smem();
           __syncwarp();
@@ -577,7 +583,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         bool bad = false;
 #pragma unroll 1
         for (int j = 0; j < kPieces; ++j)
-          bad |= clean_piece<T>(ring + slot * kTile, tile, lw * 32 + j * (32 / kPieces) + lane / kPieces, lane % kPieces, wk);
+        {
+          const int r = lw * 32 + j * (32 / kPieces) + lane / kPieces;
+          const int64_t key = int64_t(tile) * kChunkKeys + r;
+          if (key > wk.all_hi || key < wk.all_lo) bad |= clean_piece<T>(ring + slot * kTile, r, lane % kPieces);
+        }
         if (bad) poison[number_of % kBook] = number_of;
       }
       fence_async_smem();
