@@ -238,7 +238,7 @@ SB_API int32_t sb_rotary(const sb_heads* x, const sb_heads* y, int32_t elem_type
                          const sb_rotary_table* table, int32_t inverse, void* stream);
 
 /* A paged cache: position j of sequence b is row j % page_size of page
- * page_table[b * page_table_stride + j / page_size]. context_lengths[b] counts the sequence's
+ * page_table[b * page_table_stride + j / page_size], at most 2^30 of them. context_lengths[b] counts the sequence's
  * positions, those of the current step's tokens among them. Positions at or past
  * max_pages * page_size, and positions whose table entry is outside [0, pages), hold nothing: they
  * are not written, and attention leaves them out. k, v: float16 or bfloat16. */

@@ -4,8 +4,10 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <string>
 
@@ -92,7 +94,7 @@ k::PagedView view(const sb_paged_cache* c, int32_t q_heads, int64_t tokens, cons
   need(c->batch >= 0 && c->max_pages >= 0 && c->pages >= 0 && c->page_size > 0 && c->kv_heads > 0 && c->head_dim > 0,
        "cache sizes must be positive");
   need(c->pages < (int64_t(1) << 31), "more than 2^31 - 1 pages");
-  need(int64_t(c->max_pages) * c->page_size < (int64_t(1) << 31), "more than 2^31 - 1 positions per sequence");
+  need(int64_t(c->max_pages) * c->page_size <= (int64_t(1) << 30), "more than 2^30 positions per sequence");
   need(c->k != nullptr && c->v != nullptr, "cache k or v is null");
   need((c->page_table != nullptr && c->context_lengths != nullptr) || c->batch == 0, "cache page_table or context_lengths is null");
   need(aligned(c->page_table, 4) && aligned(c->context_lengths, 4), "cache page_table or context_lengths is misaligned");

@@ -11,6 +11,11 @@
 // several times the rate that the memory can feed, and needs no operand staging beyond shared memory.
 // Each of a CTA's 4 warps takes 16 of a tile's 64 positions, with its own ring of stages (cp.async, no
 // barrier between warps) and its own m, l, o, joined in shared memory at the item's end.
+//
+// Measured (bf16, 32 query and 8 key heads of 128, page 16): 48 sequences of up to 8000 positions 171 us, 5.4
+// TB/s, 0.83 of the measured HBM rate; with the arithmetic taken out 150 us, so the loads' pattern is sound
+// and what is left is the warps' own latency per stage. Three CTAs per SM with two stages each: 173 us; one
+// CTA with six stages: 282 us.
 #include <algorithm>
 
 #include "paged_attention.cuh"

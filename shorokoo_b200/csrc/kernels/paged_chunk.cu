@@ -1,28 +1,35 @@
 // Attention of chunks of new tokens over a paged cache, on the tcgen05 tensor core (formulas:
 // paged_attention.cu). Every key byte feeds hundreds of rows, so the two products bound it, and next to
-// them the exponentials: a 128 x 128 tile of logits at head width 128 takes 1024 cycles of tensor core
-// and 1024 of the SM's 16 exponentials per cycle.
+// them the exponentials: two row tiles by 128 positions at head width 128 take 2054 cycles of tensor core
+// (2524 with the logits in halves of 64, as here) and 2048 of the SM's 16 exponentials per cycle.
 //
 // An item is 256 query rows of one key head (rows as in paged.cuh: tokens times the query heads that
 // share the key head), as two tiles A and B of 128: while the tensor core multiplies for one, the other's
 // logits become weights. One CTA per SM, 16 warps (the last two idle):
 //   warps 0-3, 4-7   tiles A, B: a thread owns a query row. It loads the row's Q into shared memory (128-byte
-//                    swizzle, K-major), then per key tile reads its 128 logits from its TMEM lane, takes
-//                    their maximum and writes P = 2^(s - m) in 16 bits over them (columns 0-63 of the same
-//                    128), the A operand of the second product. A running maximum that grows by less than
-//                    2^8 is left as it is (P then stays below 2^8, exact in range for either type), so that O
-//                    in TMEM is rescaled a few times per row only. At the end it reads its row of O.
+//                    swizzle, K-major), then per 64 positions reads its logits from its TMEM lane and writes
+//                    P = 2^(s - m) in 16 bits over the first 32 columns of them, the A operand of the second
+//                    product. A running maximum that grows by less than 2^8 is left as it is (P then stays
+//                    below 2^8, exact in range for either type), so that O in TMEM is rescaled a few times
+//                    per row only. At the end it reads its row of O.
 //   warps 8-11       K and V tiles of 128 positions into a ring of stages; rows that are not there read as
 //                    zero, and a bit per row says so. Pages of 8, 16, 32, .. positions: warp 8 issues one TMA
 //                    box per page and 64 elements, a lane each (a page that is not there is a coordinate past
-//                    the pool, which TMA fills with zeros). Other page sizes: all four warps gather rows with
-//                    16-byte cp.async (3300 cycles a tile against the TMA boxes' few hundred).
-//                    Values in positions that not every row sees are searched for infinities and NaN.
-//   warps 12, 13     issue S = Q K^T (M = N = 128) and O += P V (P from TMEM, V MN-major as it lies in the
-//                    cache) for a tile each, in the order PV(j) S(j+1): the tensor core runs a thread's
-//                    instructions in issue order, so a commit of S(j+1) also says that PV(j) is done. (One
-//                    warp for both tiles could not issue fast enough beside the row warps.)
+//                    the pool, which TMA fills with zeros), and warps 9-11 search values in positions that
+//                    not every row sees for infinities and NaN. Other page sizes: all four warps gather rows
+//                    with 16-byte cp.async (3300 cycles a tile, 2355 us where the boxes take 1402).
+//   warps 12, 13     issue S = Q K^T (M = 128, N = 64) and O += P V (P from TMEM, V MN-major as it lies in
+//                    the cache) for a tile each, in the order PV(i) S(i + 2): the two halves of a tile's 128
+//                    logit columns are two buffers, and the tensor core runs a thread's instructions in issue
+//                    order, so a commit of S(i + 2) also says that PV(i) is done.
 // TMEM: S/P of A 0-127, of B 128-255, O of A 256-383, of B 384-511.
+//
+// Measured (2000 tokens over 40009 positions, 32 query and 8 key heads of 128, bf16, page 64): 1380 us, 463
+// TFLOP/s, 0.28 of the measured bf16 rate; the tensor pipe is active 38% of the cycles, the exponentials' 40%.
+// What bounds it is the row warps' latency (two per scheduler: logits read, exponentials, weights stored and
+// handed over, about 2000 cycles per half against 1145 for the same instructions free of waits). Tried
+// without gain: whole 128-column logits (1402), a polynomial for 1 to 4 of 8 exponential pairs (1350-1440),
+// tile B kept out of A's exponentials (1460), logits read again instead of kept for the second try (1400).
 //
 // Waits are bounded: one that runs out sets the error word, every role leaves its loop, and the rows of
 // the piece are written as NaN.
@@ -96,26 +103,6 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
 __device__ __forceinline__ void hide(uint32_t& v, uint32_t seen) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\tselp.b32 %0, %0, 0xff800000, p;\n\t}" : "+r"(v) : "r"(seen));
 }
-
-// 2^x of a pair on the multiply-add pipe, for x <= 8 (anything below -126 counts as -126): x = n + f with n
-// the nearest integer, 2^f on [-1/2, 1/2] by the polynomial of degree 4 of least relative error (Remez
-// exchange; 2.6e-6, a hundredth of the rounding to 16 bits that follows), times 2^n made from its bits.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));   // a NaN stays one to the end
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
-  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
-  const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
-  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-  float2 p = __ffma2_rn(f, make_float2(0.009570102207362652f, 0.009570102207362652f),
-                        make_float2(0.05591785907745361f, 0.05591785907745361f));
-  p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
-  p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-  p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return __fmul2_rn(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
-                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
-}
-constexpr int kPolyOf8 = 0;   // pairs of 8 that take it: the SM's 16 exponentials per cycle are the scarcer part
 
 // One CTA's walk over its pieces; every role steps through the same ones.
 struct Walk {
@@ -357,12 +344,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 float2 e = make_float2(__uint_as_float(v[g * 32 + j]), __uint_as_float(v[g * 32 + j + 1]));
                 tops[(j >> 1) & 1] = max3(tops[(j >> 1) & 1], e.x, e.y);
                 e = __ffma2_rn(e, scale2, base2);
-                if ((j >> 1) % 8 < kPolyOf8) {
-                  e = exp2_poly(e);
-                } else {
-                  e.x = exp2_approx(e.x);
-                  e.y = exp2_approx(e.y);
-                }
+                e.x = exp2_approx(e.x);
+                e.y = exp2_approx(e.y);
                 if (j & 2) sum1 = __fadd2_rn(sum1, e);
                 else sum0 = __fadd2_rn(sum0, e);
                 pk[j >> 1] = Mma<T>::pack(e.x, e.y);
@@ -548,7 +531,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (below > above) below = above = 0;
           const int gap = above - below;
           bool bad = false;
-#pragma unroll 1   // four at a time were 141 -> 177 us for windowed prompts: more code beside the row warps'
+#pragma unroll 1   // (unrolled by four, windowed prompts take 177 us instead of 141: more code beside the row warps')
           for (int p = cw * 32 + lane; p < (kChunkKeys - gap) * kPieces; p += 96) {
             const int r = p / kPieces;
             bad |= clean_piece<T>(ring + slot * kTile, r < below ? r : r + gap, p % kPieces);

@@ -15,8 +15,12 @@
 // Inputs past K and outputs past N are zero codes; x reads as zero there. Behind the tiles, scales
 // as pairs (output g, g + 8), each pair's groups in a row; then zero points likewise.
 //
-// A CTA computes 16 outputs: its warps take the 64-input blocks in turn and their sums meet in shared
-// memory, added in a fixed order.
+// A CTA computes 16 or 32 outputs: its warps take the 64-input blocks in turn and their sums meet in shared
+// memory, added in a fixed order. One row has a kernel of its own.
+//
+// Measured (8192 inputs, 22016 outputs, groups of 32 with zero points, fp16, 104 MB): one row 31 us, 3.4 TB/s,
+// 0.52 of the measured HBM rate (its loads alone take 27 us, its arithmetic alone about 14 us of issue slots);
+// with the kernel for several rows 51 us. 13 rows by 4096 inputs and 11000 outputs, groups of 64: 18.5 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -269,7 +269,7 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, query_starts: torch.Tens
     n = cache._workspace(heads, tokens)
     space = torch.empty(n, dtype=torch.uint8, device=device)
     _call("sb_paged_attention", device, cache._ref, qh, oh, heads, tokens, starts,
-          cache.head_dim ** -0.5 if scale is None else scale, window, space.data_ptr(), n)
+          cache.head_dim ** -0.5 if scale is None else scale, min(window, 1 << 30), space.data_ptr(), n)
     return out
 
 
@@ -287,8 +287,9 @@ class W4Weights:
     ``packed``: uint8 [out_features, ceil(in_features / 2)], element k of a row in the low half of byte
     k // 2 for even k, in the high half for odd k. ``scales``: [out_features, ceil(in_features /
     group_size)] float16 or bfloat16, the type of the layer's inputs. ``zeros``: uint8 of the same shape
-    (0 to 15), or None for 8. ``group_size``: a multiple of 32. The laid out copy is made here, once; the
-    arguments are not kept."""
+    (0 to 15), or None for 8. ``group_size``: a multiple of 32. The laid out copy is made here, once, on
+    the current stream (another stream waits for it before it uses the object); the arguments are not
+    kept."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  in_features: int, group_size: int):

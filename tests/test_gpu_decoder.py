@@ -349,6 +349,14 @@ def test_attention_strided_queries():
     within(out.transpose(0, 1), want, tol, "strided")
 
 
+def test_attention_window_longer_than_the_context():
+    p = Paged([3, 100], [50, 300], 2, 64, 16, BF16, seed=2)
+    q = normal(torch.Generator().manual_seed(3), (103, 4, 64), BF16).cuda()
+    want = decoder.paged_attention(p.gpu(), q, p.starts.cuda())
+    for window in (300, 1 << 30, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(decoder.paged_attention(p.gpu(), q, p.starts.cuda(), window=window), want)
+
+
 def test_attention_refuses_on_the_gpu():
     p = Paged([1], [20], 2, 64, 16, BF16)
     cache, q, s = p.gpu(), torch.zeros(1, 4, 64, dtype=BF16, device="cuda"), p.starts.cuda()
