@@ -63,7 +63,7 @@ template <typename T, int V> struct alignas(V * sizeof(T)) Piece { T e[V]; };
 
 // V: elements per memory access (a 16-byte piece, or 1 where alignment, strides or sizes allow no more)
 template <typename T, int V, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads, kAppend ? 4 : 8) rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turns[];   // [per_cta][pairs] magnitude * (cos, sin)
   __shared__ int64_t position[kMostTokensPerCta];
   __shared__ int64_t k_slot[kMostTokensPerCta], v_slot[kMostTokensPerCta];   // element offsets in the cache
@@ -142,18 +142,16 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
     if (it.ib >= 0) *reinterpret_cast<P*>(dst + it.ib) = xb;
   };
 
-  // The first item's pieces are under way while the positions are looked up and the angles computed (append of
-  // 5000 tokens 41 -> 35 us; two items: 39 us, for their registers).
-  constexpr int kEarly = 1;
+  // An append's first item is under way while the slots are looked up (5000 tokens: 41 -> 35 us; two items: 39
+  // us, for their registers). Without slots to wait for, 4099 tokens of 32 heads take 16.4 us without it, 19.9 with.
+  constexpr int kEarly = kAppend ? 1 : 0;
   const int first = blockIdx.y * kRotaryThreads + tid;
-  Item early[kEarly];
-  P ea[kEarly], eb[kEarly];
-#pragma unroll
-  for (int e = 0; e < kEarly; ++e)
-    if (first + e * stride < items) {
-      early[e] = item(first + e * stride);
-      fetch(early[e], ea[e], eb[e]);
-    }
+  Item early;
+  P ea, eb;
+  if (kEarly && first < items) {
+    early = item(first);
+    fetch(early, ea, eb);
+  }
   if (kAppend) {
     const int w = tid >> 5;
     if (w < count) {
@@ -195,9 +193,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
     turns[i] = make_float2(a.magnitude * cs, a.magnitude * a.sign * sn);
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEarly; ++e)
-    if (first + e * stride < items) finish(early[e], ea[e], eb[e]);
+  if (kEarly && first < items) finish(early, ea, eb);
   for (int i = first + kEarly * stride; i < items; i += stride) {
     const Item it = item(i);
     P xa, xb;
