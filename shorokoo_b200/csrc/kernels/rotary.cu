@@ -63,7 +63,7 @@ template <typename T, int V> struct alignas(V * sizeof(T)) Piece { T e[V]; };
 
 // V: elements per memory access (a 16-byte piece, or 1 where alignment, strides or sizes allow no more)
 template <typename T, int V, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kRotaryThreads, kAppend ? 4 : 8) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turns[];   // [per_cta][pairs] magnitude * (cos, sin)
   __shared__ int64_t position[kMostTokensPerCta];
   __shared__ int64_t k_slot[kMostTokensPerCta], v_slot[kMostTokensPerCta];   // element offsets in the cache
@@ -142,13 +142,13 @@ __global__ void __launch_bounds__(kRotaryThreads, kAppend ? 4 : 8) rotary_kernel
     if (it.ib >= 0) *reinterpret_cast<P*>(dst + it.ib) = xb;
   };
 
-  // An append's first item is under way while the slots are looked up (5000 tokens: 41 -> 35 us; two items: 39
-  // us, for their registers). Without slots to wait for, 4099 tokens of 32 heads take 16.4 us without it, 19.9 with.
-  constexpr int kEarly = kAppend ? 1 : 0;
+  // An append's first item is under way while the slots are looked up (5600 tokens: 41 -> 35 us; two items: 39
+  // us, for their registers). Without slots to wait for, the plain loop at the end is faster (4099 tokens of 32
+  // heads of 128: 16.4 us against 19.9).
   const int first = blockIdx.y * kRotaryThreads + tid;
   Item early;
   P ea, eb;
-  if (kEarly && first < items) {
+  if (kAppend && first < items) {
     early = item(first);
     fetch(early, ea, eb);
   }
@@ -193,12 +193,47 @@ __global__ void __launch_bounds__(kRotaryThreads, kAppend ? 4 : 8) rotary_kernel
     turns[i] = make_float2(a.magnitude * cs, a.magnitude * a.sign * sn);
   }
   __syncthreads();
-  if (kEarly && first < items) finish(early, ea, eb);
-  for (int i = first + kEarly * stride; i < items; i += stride) {
-    const Item it = item(i);
-    P xa, xb;
-    fetch(it, xa, xb);
-    finish(it, xa, xb);
+  if constexpr (kAppend) {
+    if (first < items) finish(early, ea, eb);
+    for (int i = first + stride; i < items; i += stride) {
+      const Item it = item(i);
+      P xa, xb;
+      fetch(it, xa, xb);
+      finish(it, xa, xb);
+    }
+  } else
+  for (int i = first; i < items; i += stride) {
+    const int w = count == 1 ? 0 : i / per_token;
+    const int r = i - w * per_token, h = r / units, u = r - h * units;
+    const T* src = static_cast<const T*>(a.q.p) + (t0 + w) * a.q.ts + h * a.q.hs;
+    T* dst = static_cast<T*>(a.qo.p) + (t0 + w) * a.qo.ts + h * a.qo.hs;
+    if (u >= a.rot_units) {   // behind the rotated part
+      const int at = 2 * a.pairs + (u - a.rot_units) * V;
+      *reinterpret_cast<P*>(dst + at) = *reinterpret_cast<const P*>(src + at);
+    } else if (kInter && V > 1) {
+      const int at = u * V;
+      P x = *reinterpret_cast<const P*>(src + at);
+      const float2* cs = turns + w * a.pairs + at / 2;
+#pragma unroll
+      for (int e = 0; e + 1 < V; e += 2) {
+        const float va = Elem<T>::load(x.e[e]), vb = Elem<T>::load(x.e[e + 1]);
+        x.e[e] = Elem<T>::store(va * cs[e / 2].x - vb * cs[e / 2].y);
+        x.e[e + 1] = Elem<T>::store(va * cs[e / 2].y + vb * cs[e / 2].x);
+      }
+      *reinterpret_cast<P*>(dst + at) = x;
+    } else {
+      const int ia = kInter ? 2 * u : u * V, ib = kInter ? 2 * u + 1 : a.pairs + u * V;
+      P xa = *reinterpret_cast<const P*>(src + ia), xb = *reinterpret_cast<const P*>(src + ib);
+      const float2* cs = turns + w * a.pairs + u * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float va = Elem<T>::load(xa.e[e]), vb = Elem<T>::load(xb.e[e]);
+        xa.e[e] = Elem<T>::store(va * cs[e].x - vb * cs[e].y);
+        xb.e[e] = Elem<T>::store(va * cs[e].y + vb * cs[e].x);
+      }
+      *reinterpret_cast<P*>(dst + ia) = xa;
+      *reinterpret_cast<P*>(dst + ib) = xb;
+    }
   }
 }
 
