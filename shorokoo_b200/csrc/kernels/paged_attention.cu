@@ -2,8 +2,9 @@
 // a running maximum and sum per query row (base 2: scale * log2(e) is folded into the exponent):
 //   m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),  o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j
 // Two partial results over disjoint keys join the same way, which is what splits a context over CTAs.
-// m, l and o are fp32; 2^(s - m) is rounded to the operands' 16-bit type for the second product (relative
-// 2^-9 or 2^-12 per weight, at random, under the rounding of the result itself).
+// m, l and o are fp32; the weights are rounded to the operands' 16-bit type for the second product, by at most
+// 2^-8 (bf16) or 2^-11 (fp16) of each weight, in either direction, as the result itself is: the tensor core takes no
+// wider operand with 16-bit values. (Reference in paged_attention.cuh: how fp16's range is kept from losing weights.)
 //
 // paged_rows_kernel: 16 query rows per item, for decode steps (the q_heads / kv_heads query heads that
 // share a key head, times a few tokens). Each byte of the cache feeds 2 x rows operations: reading keys
@@ -27,7 +28,6 @@ namespace {
 constexpr int kRowsTile = 16;
 constexpr int kKeysTile = 64;
 constexpr int kRowsThreads = 128;
-constexpr float kGrowth = 8.f;
 template <int DP> constexpr int kStages = DP == 128 ? 3 : 4;
 template <int DP> constexpr int kRowsSmem = 4 * kStages<DP> * 2 * 16 * DP * 2;
 
@@ -191,22 +191,28 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
         if (bad) poisoned = 1;
         __syncwarp();
       }
-      // The rows' references m follow their maxima only when one has grown by more than 2^8 (weights stay exact
-      // in range up to there), so that most steps need no exchange between lanes and leave o alone.
+      // The rows' references m move only when one has to, so that most steps need no exchange between lanes and
+      // leave o alone.
       float top[2];
-      bool grown = false;
+      bool moves = false;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {   // rows g, g + 8
         top[e] = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
-        grown |= m[e] == -INFINITY ? top[e] > m[e] : top[e] - m[e] > kGrowth;
+        moves |= rises<T>(top[e] - m[e]) || falls<T>(top[e] - m[e]);
       }
-      if (__any_sync(~0u, grown)) {
+      if (__any_sync(~0u, moves)) {
         float grow[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
           top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
-          const float now = fmaxf(m[e], top[e]);
+          float now = fmaxf(m[e], top[e]);
+          if (Reference<T>::kFalls) {
+            float sum = l[e];
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            if (falls<T>(top[e] - m[e]) && sum < kMostSum) now = fmaxf(top[e] + kBack, m[e] - kDeepest);
+          }
           grow[e] = exp2_approx(m[e] - (now == -INFINITY ? 0.f : now));
           m[e] = now;
           l[e] *= grow[e];
@@ -222,7 +228,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2) paged_rows_kernel(const Paged
       uint32_t pf[4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float base = m[e] == -INFINITY ? 0.f : m[e];   // a row that has seen nothing yet
+        const float base = m[e] == -INFINITY ? 0.f : m[e] - Reference<T>::kLift;   // a row that has seen nothing yet
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) p[j] = exp2_approx(sc[j >> 1][2 * e + (j & 1)] - base);

@@ -42,6 +42,33 @@ template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }
 };
 
+// The weights of a step of positions are 2^(s - m + kLift), s and m in units of log2, rounded to the operands' type.
+// m is a reference near the running maximum, the same for o and l, which are fp32; any value serves that keeps the
+// step's own weights within the type. A step's maximum more than kGrowth above m becomes m, so that o is rescaled
+// a few times per row only and weights stay below 2^(kLift + kGrowth).
+// fp16 has full precision from 2^-14 to 2^15 only, far less than what softmax weights span: after a leading position
+// 17 nats above the others all of theirs would be below 2^-24 of it, and thousands of them gone from o but not from
+// l. So m is lifted to the top of that range, and brought down to kBack above a step's maximum that is more than
+// kFall below it: a step's largest weight is 2^-2 or more, and a weight is off by 2^-11 of itself or 2^-23 of the
+// largest of its step. At most kDeepest at a time and while l < kMostSum, so that o (65504 l) stays in fp32;
+// what is weighted less than 2^-39 of the largest then may be lost.
+template <typename T> struct Reference {   // bf16: the range of fp32
+  static constexpr float kLift = 0.f, kGrowth = 8.f;
+  static constexpr bool kFalls = false;
+};
+template <> struct Reference<__half> {
+  static constexpr float kLift = 11.f, kGrowth = 4.f;
+  static constexpr bool kFalls = true;
+};
+constexpr float kFall = 13.f, kBack = 10.f, kDeepest = 40.f, kMostSum = 1125899906842624.f;   // 2^50
+
+// Whether a step whose maximum is `above` (its distance from m) needs another reference. Not where m or the
+// maximum is infinite, but for a row's first logits.
+template <typename T> __device__ __forceinline__ bool rises(float above) { return above > Reference<T>::kGrowth; }
+template <typename T> __device__ __forceinline__ bool falls(float above) {
+  return Reference<T>::kFalls && above < -kFall && above > -INFINITY;
+}
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");

@@ -9,9 +9,8 @@
 //   warps 0-3, 4-7   tiles A, B: a thread owns a query row. It loads the row's Q into shared memory (128-byte
 //                    swizzle, K-major), then per 64 positions reads its logits from its TMEM lane and writes
 //                    P = 2^(s - m) in 16 bits over the first 32 columns of them, the A operand of the second
-//                    product. A running maximum that grows by less than 2^8 is left as it is (P then stays
-//                    below 2^8, exact in range for either type), so that O in TMEM is rescaled a few times
-//                    per row only. At the end it reads its row of O.
+//                    product. The reference m moves a few times per row only (Reference in
+//                    paged_attention.cuh), since O in TMEM is rescaled with it. At the end it reads its row of O.
 //   warps 8-11       K and V tiles of 128 positions into a ring of stages; rows that are not there read as
 //                    zero, and a bit per row says so. Pages of 8, 16, 32, .. positions: warp 8 issues one TMA
 //                    box per page and 64 elements, a lane each (a page that is not there is a coordinate past
@@ -51,7 +50,6 @@ template <int DP> constexpr uint32_t kTileBytes = 128u * DP * 2;
 template <int DP> constexpr int kChunkSmem = int((2 + kRing<DP>) * kTileBytes<DP>) + 1024;
 constexpr int kLag = 2;          // stages that a loader keeps in flight
 constexpr int kBook = 8;         // entries of the rings of row bits and poison marks
-constexpr float kGrowth = 8.f;   // log2 of how far a weight may rise above 1 before O is rescaled
 
 __device__ unsigned chunk_error;   // bits of the waits that ran out since it was last read
 
@@ -327,12 +325,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               for (int j = 0; j < 32; ++j) hide(v[g * 32 + j], mask & (1u << j));
             }
           }
-          // m is the reference of the row's weights in units of the raw logits. The weights are taken against the
-          // one of the steps before, side by side with the maximum; where that has grown too far (a row's first
-          // step, and a few after it), once more against the new one.
+          // The weights are taken against the reference of the steps before, side by side with the maximum; where
+          // that is too far from it (a row's first step, and a few after it), once more against a new one.
           float2 sum0, sum1;
-          for (;;) {
-            const float base = m == -INFINITY ? 0.f : m * a.scale_log2;
+          for (bool moved = false;; moved = true) {
+            const float base = m == -INFINITY ? 0.f : m - Reference<T>::kLift;
             const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
             float tops[2] = {-INFINITY, -INFINITY};
             sum0 = sum1 = make_float2(0.f, 0.f);
@@ -352,12 +349,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               }
               tmem_st16(ts + g * 16, pk);
             }
-            const float top = fmaxf(tops[0], tops[1]);
-            const bool fresh = m == -INFINITY;
-            const bool grow = top > m && (fresh || (top - m) * a.scale_log2 > kGrowth);
-            if (!__any_sync(~0u, grow)) break;
-            const float f = grow ? (fresh ? 0.f : exp2_approx((m - top) * a.scale_log2)) : 1.f;
-            if (grow) m = top;
+            const float top = fmaxf(tops[0], tops[1]) * a.scale_log2;
+            const bool rise = rises<T>(top - m), fall = falls<T>(top - m) && l < kMostSum;
+            if (moved || !__any_sync(~0u, rise || fall)) break;
+            const float now = rise ? top : fall ? fmaxf(top + kBack, m - kDeepest) : m;
+            const float f = rise || fall ? exp2_approx(m - now) : 1.f;   // 0 on a row's first
+            m = now;
             l *= f;
             if (i > 0) {
               ok = __all_sync(~0u, wait_phase(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
@@ -439,7 +436,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                               __uint_as_float(v[4 * p + 3]));
         }
       }
-      if (!w.whole && live) a.ml[int64_t(w.slot) * kChunkRows + x * 128 + r] = make_float2(m * a.scale_log2, l + bad);
+      if (!w.whole && live) a.ml[int64_t(w.slot) * kChunkRows + x * 128 + r] = make_float2(m, l + bad);
       if (!w.whole && w.head && tid == 0)
         a.notes[w.slot] = PartialNote{w.b, w.h, w.i, int((w.u + w.tiles - 1) / w.sh.per) - int(blockIdx.x)};
       tc_fence_before();   // these reads of O come before the next piece's products

@@ -1,0 +1,88 @@
+"""GPU tests of the decoder-layer operators where they can go wrong at the edges: weights far below a
+row's largest. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+import pytest
+import torch
+
+from shorokoo_b200 import decoder
+from test_gpu_decoder import BF16, FP16, Paged, attended, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- softmax weights far below the largest -----------------------------------------------------
+
+def given_logits(logits, values, new, dtype, page=16):
+    """A cache of one key head of 64 whose keys give logit j at scale 1 for queries (1, 0, 0, ..), and the queries
+    of its last `new` tokens."""
+    p = Paged([new], [len(logits)], 1, 64, page, dtype, poison=False)
+    j = torch.arange(len(logits))
+    at = p.table[0][j // page].long(), j % page
+    p.k.zero_()
+    p.k[at[0], at[1], 0, 0] = logits.to(dtype)
+    p.v[at[0], at[1], 0] = values.to(dtype)
+    q = torch.zeros(new, 1, 64, dtype=dtype)
+    q[:, :, 0] = 1
+    return p, q
+
+
+def fp16_weights(p, q, block):
+    """What fp16 weights add to the tolerance of `attended` at scale 1. A block of positions is weighted against
+    one reference, by which its largest weight becomes 2^-2 or more, and 2^11 or more where it is the largest of
+    the row; fp16 below 2^-14 is off by up to 2^-25."""
+    c, n = p.context[0], p.new[0]
+    k, v, _ = p.gather(0)
+    s = k[:, 0] @ q[0, 0].double()
+    more = torch.zeros(n, 1, 64, dtype=torch.float64)
+    for i in range(n):
+        w = torch.softmax(s[: c - n + i + 1], 0)
+        mass = v[: len(w), 0].abs()
+        for a in range(0, len(w), block):
+            top = w[a: a + block].max()
+            off = 2.0 ** -25 / (2.0 ** 11 if top == w.max() else 2.0 ** -2)
+            more[i, 0] += off * top * mass[a: a + block].sum(0)
+    return more
+
+
+@pytest.mark.parametrize("new", [1, 40])          # the 16-row kernel's, the tensor core's
+@pytest.mark.parametrize("gap,length", [(8, 8000), (14, 8000), (15, 8000), (17, 8000), (19, 30000)])
+def test_attention_keeps_a_long_tail_of_small_weights(gap, length, new):
+    """A leading position with nothing in its value, as the first of a text often is, and thousands of equal
+    ones `gap` nats below it: the result is theirs."""
+    gen = torch.Generator().manual_seed(gap)
+    logits, values = torch.zeros(length), 1 + 0.25 * torch.randn((length, 64), generator=gen)
+    logits[0], values[0] = gap, 0
+    p, q = given_logits(logits, values, new, FP16)
+    want, tol = attended(p, q, 0, 1.0)
+    got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda(), scale=1.0)
+    within(got, want, tol + fp16_weights(p, q, 16 if new == 1 else 64), f"gap {gap}")
+
+
+@pytest.mark.parametrize("new,dtype", [(1, FP16), (40, FP16), (1, BF16), (40, BF16)])
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_attention_follows_levels_up_and_down(seed, new, dtype):
+    """Stretches of positions at four levels down to 19 nats, in a random order, with values that make each
+    level's share of the result alike."""
+    gen = torch.Generator().manual_seed(seed)
+    level = torch.tensor([0.0, -5.0, -12.0, -19.0])[torch.randint(0, 4, (40,), generator=gen)]
+    level = level.repeat_interleave(100)
+    logits = level + 0.25 * torch.randn(4000, generator=gen)
+    values = torch.exp(-level).clamp(max=30000)[:, None] * 2 ** -8 * torch.randn((4000, 64), generator=gen)
+    p, q = given_logits(logits, values, new, dtype)
+    want, tol = attended(p, q, 0, 1.0)
+    if dtype is FP16:
+        tol = tol + fp16_weights(p, q, 16 if new == 1 else 64)
+    got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda(), scale=1.0)
+    within(got, want, tol, f"levels {seed}")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_attention_of_a_split_context_with_a_leading_position(new):
+    """The same over a context that is cut over the whole card, so that most pieces do not hold the leader."""
+    length = 100003
+    gen = torch.Generator().manual_seed(7)
+    logits, values = torch.zeros(length), 1 + 0.25 * torch.randn((length, 64), generator=gen)
+    logits[5], values[5] = 17.5, 0
+    p, q = given_logits(logits, values, new, FP16, page=64)
+    want, tol = attended(p, q, 0, 1.0)
+    got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda(), scale=1.0)
+    within(got, want, tol + fp16_weights(p, q, 16 if new == 1 else 64), "split")
