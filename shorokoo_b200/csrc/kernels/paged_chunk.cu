@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int kPieces = DP / 8;
   __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
   __shared__ uint32_t there[kBook][4];      // which of a key tile's 128 positions are there
-  __shared__ int poison[kBook];             // number of the piece that met non-finite values in mixed positions
+  __shared__ int poison[kBook];             // number of the last piece that met non-finite values in mixed positions
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_word;
   __shared__ Walk row_walk[8];              // of the row warps: their registers hold logits
@@ -383,7 +383,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tc_fence_after();
       }
       // ---- the row's result ----
-      const bool marked = poison[number % kBook] == number;
+      // The mark may be a later piece's by now: nothing holds the other roles back while this tile has no keys in the
+      // pieces after this one. A later one only means that this piece is searched too.
+      const bool marked = poison[number % kBook] >= number;
       const float bad = ok ? 0.f : __int_as_float(0x7fc00000);
       const float inv = (l == 0.f ? 0.f : 1.f / l) + bad;
 #pragma unroll 1

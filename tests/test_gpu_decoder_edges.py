@@ -1,10 +1,12 @@
 """GPU tests of the decoder-layer operators where they can go wrong at the edges: weights far below a
-row's largest. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+row's largest, non-finite values over long walks. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+import math
+
 import pytest
 import torch
 
 from shorokoo_b200 import decoder
-from test_gpu_decoder import BF16, FP16, Paged, attended, within
+from test_gpu_decoder import BF16, FP16, U, Paged, attended, half, normal, within
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +88,40 @@ def test_attention_of_a_split_context_with_a_leading_position(new):
     want, tol = attended(p, q, 0, 1.0)
     got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda(), scale=1.0)
     within(got, want, tol + fp16_weights(p, q, 16 if new == 1 else 64), "split")
+
+
+# ---- many items to a CTA -------------------------------------------------------------------------
+
+def attended_in_order(p, q):
+    """`attended` for one head per key head, without window or missing pages, whole sequences at a time."""
+    want, tol = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    h, d = half(q.dtype), q.shape[2]
+    for b, n in enumerate(p.new):
+        k, v, _ = p.gather(b)
+        rows, c = slice(int(p.starts[b]), int(p.starts[b]) + n), p.context[b]
+        seen = torch.arange(c) <= torch.arange(c - n, c)[:, None]
+        for x in range(q.shape[1]):
+            qx = q[rows, x].double()
+            w = torch.softmax((qx @ k[:, x].t() * d ** -0.5).masked_fill(~seen, -math.inf), 1)
+            delta = (d + 4) * U * (qx.abs() @ k[:, x].abs().t()).amax(1, keepdim=True) * d ** -0.5
+            want[rows, x] = w @ v[:, x]
+            tol[rows, x] = h * want[rows, x].abs() + (h + 2 * delta + (c / 16 + 32) * U) * (w @ v[:, x].abs())
+    return want, tol
+
+
+@pytest.mark.parametrize("page", [16, 24])      # copied whole, gathered
+def test_nonfinite_values_in_some_of_many_short_items(page):
+    """About ten items per CTA, most of which leave its second row tile without keys, every third with a NaN among
+    the new tokens' own values: it reaches the tokens after it in its sequence, no other row."""
+    new = [150 if b % 9 == 0 else 40 for b in range(1500)]
+    p = Paged(new, new, 1, 64, page, BF16, seed=5, poison=False)
+    q = normal(torch.Generator().manual_seed(6), (sum(new), 1, 64), BF16)
+    want, tol = attended_in_order(p, q)
+    lost = torch.zeros(q.shape, dtype=torch.bool)
+    for b in range(0, len(new), 3):
+        at = new[b] // 2
+        p.v[p.table[b, at // page], at % page, 0, 3] = math.nan
+        lost[int(p.starts[b]) + at: int(p.starts[b]) + new[b], 0, 3] = True
+    got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda()).double().cpu()
+    assert torch.equal(torch.isnan(got), lost)
+    within(got[~lost], want[~lost], tol[~lost], "items")
