@@ -89,6 +89,12 @@ struct PartialNote {
   int more;   // > 0: the item begins here and `more` pieces follow in slots 2(c + 1), 2(c + 2), ..; else 0
 };
 
+// How long a wait of the chunk kernel may last, and one attempt of it.
+struct WaitLimit {
+  uint64_t ns;
+  uint32_t sleep_ns;
+};
+
 struct PagedArgs {
   PagedView c;
   HeadsView q, out;
@@ -97,6 +103,7 @@ struct PagedArgs {
   PartialNote* notes;   // [2 * ctas]
   float2* ml;           // [2 * ctas][rows]: m (in units of log2), l
   float* o;             // [2 * ctas][rows][DP]; chunks: [2 * ctas][DP / 4][rows][4]
+  WaitLimit wait;       // chunks
 };
 
 template <typename F>

@@ -30,9 +30,10 @@
 // without gain: whole 128-column logits (1402), a polynomial for 1 to 4 of 8 exponential pairs (1350-1440),
 // tile B kept out of A's exponentials (1460), logits read again instead of kept for the second try (1400).
 //
-// Waits are bounded: one that runs out sets the error word, every role leaves its loop, and the rows of
-// the piece are written as NaN.
+// Waits are bounded: one that runs out sets the error word, every role leaves its loop, the rows of the
+// piece are written as NaN, and the CTA ends once its copies and products in flight have.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "paged_attention.cuh"
@@ -53,9 +54,12 @@ constexpr int kBook = 8;         // entries of the rings of row bits and poison 
 
 __device__ unsigned chunk_error;   // bits of the waits that ran out since it was last read
 
+constexpr uint32_t kSleepNs = 20000;
+constexpr WaitLimit kEndWait = {kWaitTimeoutNs, kSleepNs};   // of what was issued, whatever the other waits' limit
+
 // mbar_wait whose attempts may sleep in hardware until the phase ends (up to 20 us each): the waiting
 // warps of the other roles share the row warps' issue slots.
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err,
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_flag, WaitLimit limit,
                                            unsigned int code) {
   uint64_t t0 = 0;
   while (true) {
@@ -65,15 +69,15 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(limit.sleep_ns)
         : "memory");
     if (ok) return true;
     if (*abort_flag) return false;
     const uint64_t now = global_timer_ns();
     if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitTimeoutNs) {
+    if (now - t0 > limit.ns) {
       *abort_flag = 1;
-      atomicOr(err, code);
+      atomicOr(&chunk_error, code);
       return false;
     }
   }
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int kNst = kRing<DP>;
   constexpr uint32_t kTile = kTileBytes<DP>;
   constexpr int kPieces = DP / 8;
-  __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2];
+  __shared__ uint64_t full[kNst], empty[kNst], clean[kNst], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], ended[2];
   __shared__ uint32_t there[kBook][4];      // which of a key tile's 128 positions are there
   __shared__ int poison[kBook];             // number of the last piece that met non-finite values in mixed positions
   __shared__ uint32_t tmem_holder;
@@ -226,6 +230,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&q_full[x], 4u);
+      mbar_init(&ended[x], 1u);
       for (int y = 0; y < 2; ++y) {
         mbar_init(&s_full[x][y], 1u);
         mbar_init(&p_full[x][y], 4u);
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int ta = w.ta(x), steps = 2 * (w.tb(x) - ta), book_a = book + ta - w.tile_a;
         for (int i = 0; i < steps; ++i) {
           const int buf = i & 1;
-          ok = __all_sync(~0u, wait_phase(&s_full[x][buf], uint32_t((step + i) >> 1) & 1u, abort_flag, &chunk_error, 1u));
+          ok = __all_sync(~0u, wait_phase(&s_full[x][buf], uint32_t((step + i) >> 1) & 1u, abort_flag, a.wait, 1u));
           if (!ok) break;
           tc_fence_after();
           const int key0 = (ta + (i >> 1)) * kChunkKeys + buf * 64;
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             m = now;
             l *= f;
             if (i > 0) {
-              ok = __all_sync(~0u, wait_phase(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
+              ok = __all_sync(~0u, wait_phase(&pv_done[x][buf ^ 1], uint32_t((step + i - 1) >> 1) & 1u, abort_flag, a.wait, 2u));
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[x][buf]);
         }
         step += steps;
-        if (ok) ok = __all_sync(~0u, wait_phase(&pv_done[x][1], uint32_t((step - 1) >> 1) & 1u, abort_flag, &chunk_error, 2u));
+        if (ok) ok = __all_sync(~0u, wait_phase(&pv_done[x][1], uint32_t((step - 1) >> 1) & 1u, abort_flag, a.wait, 2u));
         tc_fence_after();
       }
       // ---- the row's result ----
@@ -445,6 +450,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       book += w.tile_b - w.tile_a;
       if (__any_sync(~0u, *abort_flag)) break;
     } while (advance());
+    tmem_st_wait();   // weights of a step that a wait broke off
   } else if (kTma && warp == kLoadWarp) {
     // ---- keys and values: TMA ----
     Walk w;
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int from = value && e != 2 * n - 1 ? page_was : page;   // the last value's rows are the latest looked up
         row = rows == c.page_size ? 0 : tile * kChunkKeys % c.page_size;
         if (stage >= kNst)
-          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, a.wait, 4u));
         if (!ok) break;
         if (!value) {
           const uint32_t held = __ballot_sync(~0u, from < c.pages);   // bit p: box p's page is there
@@ -506,7 +512,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // the copies in flight land before this CTA's shared memory is given up
     volatile int not_aborted = 0;
     for (int st = max(0, stage - kNst); st < stage; ++st)
-      wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), &not_aborted, &chunk_error, 64u);
+      wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), &not_aborted, kEndWait, 64u);
   } else if (kTma && warp < kMmaWarp) {
     // ---- non-finite values that not every row sees ----
     Walk w;
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int n = w.tile_b - w.tile_a;
       for (int e = 0; e < 2 * n; ++e, ++stage) {   // every stage: a wait may not skip a phase
         const int slot = stage % kNst;
-        ok = __all_sync(~0u, wait_phase(&full[slot], uint32_t((stage / kNst) & 1), abort_flag, &chunk_error, 128u));
+        ok = __all_sync(~0u, wait_phase(&full[slot], uint32_t((stage / kNst) & 1), abort_flag, a.wait, 128u));
         if (!ok) break;
         const bool value = e == 2 * n - 1 || (e > 0 && (e & 1) == 0);
         const int tile = w.tile_a + (e == 2 * n - 1 ? n - 1 : e / 2 - 1);
@@ -607,7 +613,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool last_value = e == 2 * n - 1;    // its rows are the latest looked up
         const int pg = value && !last_value ? page_was : page, ip = value && !last_value ? in_page_was : in_page;
         if (stage >= kNst)
-          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, &chunk_error, 4u));
+          ok = __all_sync(~0u, wait_phase(&empty[slot], uint32_t((stage / kNst - 1) & 1), abort_flag, a.wait, 4u));
         if (!ok) break;
         if (!value) {
           const uint32_t bits = __ballot_sync(~0u, pg >= 0);
@@ -655,7 +661,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       uint32_t q_phase = 0, clean_phase = 0;
       bool ok = true;
       auto wait_stage = [&](int st) {
-        return wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, &chunk_error, 8u);
+        return wait_phase(&full[st % kNst], uint32_t((st / kNst) & 1), abort_flag, a.wait, 8u);
       };
       auto logits = [&](int st, int half) {   // 64 positions
         const uint64_t kd = sw128_desc(smem_u32(ring + (st % kNst) * kTile) + uint32_t(half) * 8192u);
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         auto k_stage = [&](int j) { return stage + (j == 0 ? 0 : 2 * j - 1); };
         auto v_stage = [&](int j) { return stage + (j == n - 1 ? 2 * n - 1 : 2 * j + 2); };
         if (ta < tb) {
-          ok = wait_phase(&q_full[x], q_phase, abort_flag, &chunk_error, 16u);
+          ok = wait_phase(&q_full[x], q_phase, abort_flag, a.wait, 16u);
           q_phase ^= 1u;
         }
         ok = ok && wait_stage(k_stage(0));
@@ -689,7 +695,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           ok = wait_stage(v_stage(j));
           if (kTma && ok && w.mixed(tile)) {
             const int slot = v_stage(j) % kNst;
-            ok = wait_phase(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, &chunk_error, 256u);
+            ok = wait_phase(&clean[slot], (clean_phase >> slot) & 1u, abort_flag, a.wait, 256u);
             clean_phase ^= 1u << slot;
           }
           if (!ok) break;
@@ -697,7 +703,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             if (on) {
-              ok = ok && wait_phase(&p_full[x][half], uint32_t(step >> 1) & 1u, abort_flag, &chunk_error, 32u);
+              ok = ok && wait_phase(&p_full[x][half], uint32_t(step >> 1) & 1u, abort_flag, a.wait, 32u);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
@@ -720,11 +726,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         stage += 2 * n;
       } while (ok && w.next(c));
+      // The products in flight, and the arrivals of the last releases, come before this CTA's memory is given up.
+      volatile int not_aborted = 0;
+      umma_commit(&ended[x]);
+      wait_phase(&ended[x], 0u, &not_aborted, kEndWait, 512u);
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
+  // Items that begin here and end elsewhere are not joined if some of this CTA's warps left before their last piece.
+  if (tid < 2 && abort_word) a.notes[2 * blockIdx.x + tid].more = 0;
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -812,6 +824,16 @@ cudaError_t launch_chunk(const PagedArgs& a, cudaStream_t s) {
   return tma ? launch_chunk<T, DP, true>(a, maps, s) : launch_chunk<T, DP, false>(a, maps, s);
 }
 
+// SHOROKOO_B200_WAIT_NS: a limit by which a test sees waits run out
+WaitLimit wait_limit() {
+  static const uint64_t ns = [] {
+    const char* e = std::getenv("SHOROKOO_B200_WAIT_NS");
+    const unsigned long long v = e ? std::strtoull(e, nullptr, 10) : 0;
+    return v > 0 && v < kWaitTimeoutNs ? uint64_t(v) : kWaitTimeoutNs;
+  }();
+  return {ns, uint32_t(std::min<uint64_t>(ns, kSleepNs))};
+}
+
 }  // namespace
 
 cudaError_t paged_wait_errors(unsigned* bits, cudaStream_t s) {
@@ -846,6 +868,7 @@ cudaError_t paged_chunk(const PagedView& c, int elem, HeadsView q, HeadsView out
   PagedArgs a;
   a.c = c, a.q = q, a.out = out;
   a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas, a.least = 4;
+  a.wait = wait_limit();
   a.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* p = static_cast<uint8_t*>(ws);
   a.notes = reinterpret_cast<PartialNote*>(p);

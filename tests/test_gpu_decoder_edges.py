@@ -1,6 +1,9 @@
 """GPU tests of the decoder-layer operators where they can go wrong at the edges: weights far below a
-row's largest, non-finite values over long walks. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+row's largest, non-finite values over long walks, waits that run out. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -125,3 +128,47 @@ def test_nonfinite_values_in_some_of_many_short_items(page):
     got = decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda()).double().cpu()
     assert torch.equal(torch.isnan(got), lost)
     within(got[~lost], want[~lost], tol[~lost], "items")
+
+
+# ---- waits that run out --------------------------------------------------------------------------
+
+RUN_OUT = """
+import torch
+from shorokoo_b200 import B200InvalidOperationError, decoder
+from test_gpu_decoder import BF16, Paged, attended, normal, within
+for page in (16, 24):                     # copied whole, gathered
+    for new, context in (([300, 40, 200], [3000, 40, 900]), ([600], [20000])):
+        p = Paged(new, context, 2, 128, page, BF16, seed=1)
+        q = normal(torch.Generator().manual_seed(2), (sum(new) + 2, 4, 128), BF16).cuda()
+        cache, starts = p.gpu(), p.starts.cuda()
+        out = torch.full(q.shape, 5.0, dtype=BF16, device="cuda")
+        decoder.paged_attention(cache, q, starts, out=out)
+        try:
+            decoder.check()
+            raise SystemExit("no wait ran out")
+        except B200InvalidOperationError as e:
+            assert "timed out" in str(e), e
+        decoder.check()                   # reported once
+        rows = out[: sum(new)]
+        lost = torch.isnan(rows).any(2) | (rows == 5.0).all(2)
+        assert lost.any() and (out[sum(new):] == 5.0).all()
+        if sum(context) < 10000:          # rows that were done before are right
+            want, tol = attended(p, q.cpu())
+            keep = ~lost.cpu()
+            within(rows.cpu()[keep], want[: sum(new)][keep], tol[: sum(new)][keep], "kept")
+p = Paged([1, 1], [900, 70], 2, 128, 16, BF16)      # the device goes on
+q = normal(torch.Generator().manual_seed(2), (2, 4, 128), BF16)
+want, tol = attended(p, q)
+within(decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda()), want, tol, "after")
+decoder.check()
+print("ran out and went on")
+"""
+
+
+def test_waits_that_run_out_are_reported_and_end():
+    """With a limit of a nanosecond every wait that is not over at once runs out: the call returns, its rows are NaN
+    or not written, and the status says so once."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, SHOROKOO_B200_WAIT_NS="1", PYTHONPATH=os.pathsep.join([os.path.dirname(here), here]))
+    r = subprocess.run([sys.executable, "-c", RUN_OUT], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ran out and went on" in r.stdout, r.stdout + r.stderr
