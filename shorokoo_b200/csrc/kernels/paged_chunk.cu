@@ -824,6 +824,8 @@ cudaError_t launch_chunk(const PagedArgs& a, cudaStream_t s) {
   return tma ? launch_chunk<T, DP, true>(a, maps, s) : launch_chunk<T, DP, false>(a, maps, s);
 }
 
+__global__ void forget_errors_kernel(unsigned bits) { atomicAnd(&chunk_error, ~bits); }
+
 // SHOROKOO_B200_WAIT_NS: a limit by which a test sees waits run out
 WaitLimit wait_limit() {
   static const uint64_t ns = [] {
@@ -836,11 +838,15 @@ WaitLimit wait_limit() {
 
 }  // namespace
 
+// Clears no more than it reports: a wait on another stream may run out in between.
 cudaError_t paged_wait_errors(unsigned* bits, cudaStream_t s) {
   void* at = nullptr;
   cudaError_t e = cudaGetSymbolAddress(&at, chunk_error);
   if (e == cudaSuccess) e = cudaMemcpyAsync(bits, at, sizeof(*bits), cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof(*bits), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess || *bits == 0) return e;
+  forget_errors_kernel<<<1, 1, 0, s>>>(*bits);
+  e = cudaGetLastError();
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   return e;
 }
