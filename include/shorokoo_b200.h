@@ -272,7 +272,8 @@ SB_API int32_t sb_paged_append(const sb_paged_cache* cache, const sb_heads* k, c
 /* out = softmax(scale * q k^T) v per query head over the positions at or before the token's own in
  * its sequence (window > 0: the last `window` of them); query head h reads key head
  * h / (q_heads / kv_heads). A token that sees nothing gets zeros. Positions that a token does not see
- * do not reach its output, whatever they hold. head_dim: a multiple of 8 up to 128; data pointers
+ * do not reach its output, whatever they hold. head_dim: a multiple of 8 up to 128;
+ * tokens * q_heads / kv_heads: at most 2^30; data pointers
  * 16-byte aligned and strides multiples of 8 elements. workspace: 256-byte aligned, at least
  * sb_paged_attention_workspace bytes, not shared with a call that may overlap. */
 SB_API int32_t sb_paged_attention_workspace(const sb_paged_cache* cache, int32_t q_heads, int64_t tokens, size_t* bytes);

@@ -121,7 +121,8 @@ void check_attention(const k::PagedView& p) {
        std::to_string(p.q_heads) + " query heads are not a multiple of " + std::to_string(p.kv_heads) + " key heads");
   supported(p.head_dim % 8 == 0 && p.head_dim <= 128,
             "head_dim " + std::to_string(p.head_dim) + " (a multiple of 8 up to 128)");
-  need(p.tokens * (p.q_heads / p.kv_heads) < (int64_t(1) << 31), "tokens x query heads out of range");
+  // the kernels count a sequence's rows in 32 bits, in steps of up to 32 tiles past the last one
+  need(p.tokens * (p.q_heads / p.kv_heads) <= (int64_t(1) << 30), "more than 2^30 tokens x query heads of a key head");
 }
 
 k::W4View view(const sb_w4_weights* w) {

@@ -166,6 +166,14 @@ def test_attention_refuses():
     assert L.sb_paged_attention_workspace(None, 8, 3, C.byref(n)) == 1
 
 
+@pytest.mark.parametrize("tokens,heads", [((1 << 28) - 4, 32), ((1 << 27) + 1, 32), ((1 << 30), 8)])
+def test_attention_refuses_rows_that_its_counters_cannot_hold(tokens, heads):
+    c, h, n = _cache(), _heads(), C.c_size_t()
+    assert L.sb_paged_attention(C.byref(c), C.byref(h), C.byref(h), heads, tokens, PTR, 0.125, 0, PTR, 1 << 40, None) == 1
+    assert b"2^30" in L.sb_last_error()
+    assert L.sb_paged_attention_workspace(C.byref(c), heads, tokens, C.byref(n)) == 1
+
+
 def _weights(**kw):
     d = dict(data=PTR, elem_type=16, group_size=64, out_features=48, in_features=200, has_zeros=0)
     d.update(kw)
