@@ -61,14 +61,15 @@ int multiprocessors() {
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// |stride| * count stays far from 63 bits, so that the kernels' products cannot wrap
+// No buffer of a device spans as many elements, so that a stride beyond is a mistake.
 constexpr int64_t kMostStride = int64_t(1) << 40;
+bool usable(int64_t stride) { return stride > -kMostStride && stride < kMostStride; }
 constexpr int64_t kMostTokens = int64_t(1) << 30;
 
 k::HeadsView view(const sb_heads* h, const char* name, size_t esz) {
   need(h != nullptr && h->data != nullptr, std::string(name) + " is null");
   need(aligned(h->data, esz), std::string(name) + " is not aligned to its element type");
-  need(std::llabs(h->token_stride) < kMostStride && std::llabs(h->head_stride) < kMostStride,
+  need(usable(h->token_stride) && usable(h->head_stride),
        std::string(name) + ": stride out of range");
   return {h->data, h->token_stride, h->head_stride};
 }
@@ -101,7 +102,7 @@ k::PagedView view(const sb_paged_cache* c, int32_t q_heads, int64_t tokens, cons
   need(aligned(c->k, 2) && aligned(c->v, 2), "cache k or v is misaligned");
   for (int64_t s : {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride, c->v_token_stride,
                     c->v_head_stride, c->page_table_stride})
-    need(std::llabs(s) < kMostStride, "cache stride out of range");
+    need(usable(s), "cache stride out of range");
   need(tokens >= 0 && tokens <= kMostTokens, "token count out of range");
   need((starts != nullptr && aligned(starts, 4)) || tokens == 0 || c->batch == 0, "query_starts is null or misaligned");
   k::PagedView p;
@@ -290,7 +291,7 @@ int32_t sb_linear_w4(const sb_w4_weights* weights, const void* x, int64_t x_row_
     if (rows == 0) return;
     need(w.data != nullptr && aligned(w.data, 256), "weights data is null or misaligned");
     need(x != nullptr && y != nullptr && aligned(x, 2) && aligned(y, 2) && aligned(bias, 2), "x, y or bias is null or misaligned");
-    need(std::llabs(x_row_stride) < kMostStride && std::llabs(y_row_stride) < kMostStride, "row stride out of range");
+    need(usable(x_row_stride) && usable(y_row_stride), "row stride out of range");
     need(rows == 1 || std::llabs(y_row_stride) >= w.n, "rows of y overlap");
     launched(k::linear_w4(w, x, x_row_stride, bias, y, y_row_stride, rows, multiprocessors(), static_cast<cudaStream_t>(stream)));
   });

@@ -174,6 +174,21 @@ def test_attention_refuses_rows_that_its_counters_cannot_hold(tokens, heads):
     assert L.sb_paged_attention_workspace(C.byref(c), heads, tokens, C.byref(n)) == 1
 
 
+def test_the_most_negative_stride_is_out_of_range():
+    """Its magnitude does not fit 64 bits."""
+    low, c, h = -(1 << 63), _cache(), _heads()
+    for bad in (_heads(ts=low), _heads(hs=low)):
+        assert _rotary(x=bad) == 1 and _rotary(y=bad) == 1
+        assert L.sb_paged_append(C.byref(c), C.byref(bad), C.byref(h), None, None, 0, 3, PTR, None, None) == 1
+        assert L.sb_paged_attention(C.byref(c), C.byref(bad), C.byref(h), 8, 3, PTR, 0.125, 0, PTR, 1 << 40, None) == 1
+    for name in ("k_page_stride", "k_token_stride", "k_head_stride", "v_page_stride", "v_token_stride", "v_head_stride",
+                 "page_table_stride"):
+        bad = _cache(**{name: low})
+        assert L.sb_paged_attention(C.byref(bad), C.byref(h), C.byref(h), 8, 3, PTR, 0.125, 0, PTR, 1 << 40, None) == 1, name
+    for xs, ys in ((low, 48), (200, low)):
+        assert L.sb_linear_w4(C.byref(_weights()), PTR, xs, None, PTR, ys, 2, None) == 1
+
+
 def _weights(**kw):
     d = dict(data=PTR, elem_type=16, group_size=64, out_features=48, in_features=200, has_zeros=0)
     d.update(kw)
