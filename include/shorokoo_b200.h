@@ -197,7 +197,8 @@ SB_API int32_t sb_linear_noalloc(const float* x, const float* w, const float* bi
 #define SB_ELEM_FLOAT16 10
 #define SB_ELEM_BFLOAT16 16
 
-/* A tensor of heads: element (token, head, d) at data[token * token_stride + head * head_stride + d]. */
+/* A tensor of heads: element (token, head, d) at data[token * token_stride + head * head_stride + d].
+ * Inputs may repeat memory (strides of 0); no two elements of a result may share it. */
 typedef struct sb_heads {
   void* data;
   int64_t token_stride, head_stride;

@@ -74,6 +74,12 @@ k::HeadsView view(const sb_heads* h, const char* name, size_t esz) {
   return {h->data, h->token_stride, h->head_stride};
 }
 
+// A result's: writes of the same element by several rows would leave any of them.
+void apart(const k::HeadsView& v, const char* name, int64_t tokens, int64_t heads, int64_t head_dim) {
+  if ((tokens > 1 && std::llabs(v.ts) < head_dim) || (heads > 1 && std::llabs(v.hs) < head_dim))
+    need(false, std::string("rows of ") + name + " overlap");
+}
+
 void wide(const k::HeadsView& h, const char* name) {
   supported(aligned(h.p, 16) && h.ts % 8 == 0 && h.hs % 8 == 0,
             std::string(name) + " needs 16-byte alignment and strides of whole 8-element pieces");
@@ -198,6 +204,7 @@ int32_t sb_rotary(const sb_heads* x, const sb_heads* y, int32_t elem_type, int64
     if (tokens == 0 || heads == 0) return;
     const size_t esz = dtype_size(elem_type);
     const k::HeadsView xv = view(x, "x", esz), yv = view(y, "y", esz);
+    apart(yv, "y", tokens, heads, head_dim);
     need(positions != nullptr && aligned(positions, positions_int64 ? 8 : 4), "positions are null or misaligned");
     launched(k::rotary(xv, yv, elem_type, tokens, heads, head_dim, positions, positions_int64 ? 1 : 0, t,
                        multiprocessors(), static_cast<cudaStream_t>(stream)));
@@ -217,7 +224,7 @@ int32_t sb_paged_append(const sb_paged_cache* cache, const sb_heads* k, const sb
     if (tokens == 0 || c.batch == 0) return;
     const k::HeadsView kv = view(k, "k", 2), vv = view(v, "v", 2);
     k::HeadsView qv = {nullptr, 0, 0}, ov = {nullptr, 0, 0};
-    if (q) qv = view(q, "q", 2), ov = view(q_out, "q_out", 2);
+    if (q) qv = view(q, "q", 2), ov = view(q_out, "q_out", 2), apart(ov, "q_out", tokens, q_heads, c.head_dim);
     launched(k::paged_append(c, cache->elem_type, kv, vv, qv, ov, t, multiprocessors(), static_cast<cudaStream_t>(stream)));
   });
 }
@@ -244,6 +251,7 @@ int32_t sb_paged_attention(const sb_paged_cache* cache, const sb_heads* q, const
     const k::HeadsView qv = view(q, "q", 2), ov = view(out, "out", 2);
     wide(qv, "q");
     wide(ov, "out");
+    apart(ov, "out", tokens, q_heads, c.head_dim);
     wide({c.k, c.kt, c.kh}, "cache k");
     wide({c.v, c.vt, c.vh}, "cache v");
     supported(c.kp % 8 == 0 && c.vp % 8 == 0, "cache page strides need whole 8-element pieces");

@@ -189,6 +189,17 @@ def test_the_most_negative_stride_is_out_of_range():
         assert L.sb_linear_w4(C.byref(_weights()), PTR, xs, None, PTR, ys, 2, None) == 1
 
 
+@pytest.mark.parametrize("bad", [_heads(ts=0), _heads(hs=0), _heads(ts=56), _heads(hs=-56), _heads(ts=-8, hs=512)],
+                         ids=["tokens on one", "heads on one", "tokens", "heads", "tokens backwards"])
+def test_results_whose_rows_overlap_are_refused(bad):
+    c, h, t = _cache(), _heads(), _table()
+    assert _rotary(y=bad) == 1 and b"overlap" in L.sb_last_error()
+    assert L.sb_paged_append(C.byref(c), C.byref(h), C.byref(h), C.byref(h), C.byref(bad), 8, 3, PTR, C.byref(t), None) == 1
+    assert b"overlap" in L.sb_last_error()
+    assert L.sb_paged_attention(C.byref(c), C.byref(h), C.byref(bad), 8, 3, PTR, 0.125, 0, PTR, 1 << 40, None) == 1
+    assert b"overlap" in L.sb_last_error()
+
+
 def _weights(**kw):
     d = dict(data=PTR, elem_type=16, group_size=64, out_features=48, in_features=200, has_zeros=0)
     d.update(kw)
