@@ -333,10 +333,15 @@ def linear_w4(x: torch.Tensor, weights: W4Weights, bias: Optional[torch.Tensor] 
     ys = _matrix(out, "out", device, dtype, rows, n)[1]
     at = None
     if bias is not None:
-        if bias.dtype is not dtype or bias.get_device() != device.index or bias.shape != (n,) or not bias.is_contiguous():
+        try:
+            if (bias.dtype is dtype and bias.get_device() == device.index and bias.shape == (n,) and bias.is_contiguous()
+                    and not (bias.requires_grad and torch.is_grad_enabled())):
+                at = bias.data_ptr()
+        except AttributeError:
+            pass
+        if at is None:
             _on(bias, "bias", device, dtype, 1)
             _bad(f"bias must be {n} contiguous values, got {tuple(bias.shape)}")
-        at = bias.data_ptr()
     _call("sb_linear_w4", device, weights._ref, x.data_ptr(), xs, at, out.data_ptr(), ys, rows)
     return out
 

@@ -1,5 +1,6 @@
 """GPU tests of the decoder-layer operators where they can go wrong at the edges: weights far below a
-row's largest, non-finite values over long walks, waits that run out. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+row's largest, non-finite values over long walks, waits that run out,
+gradients that the operators do not record. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
 import math
 import os
 import subprocess
@@ -8,7 +9,7 @@ import sys
 import pytest
 import torch
 
-from shorokoo_b200 import decoder
+from shorokoo_b200 import B200ArgumentError, B200NotSupportedError, decoder
 from test_gpu_decoder import BF16, FP16, U, Paged, attended, half, normal, within
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +173,51 @@ def test_waits_that_run_out_are_reported_and_end():
     env = dict(os.environ, SHOROKOO_B200_WAIT_NS="1", PYTHONPATH=os.pathsep.join([os.path.dirname(here), here]))
     r = subprocess.run([sys.executable, "-c", RUN_OUT], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "ran out and went on" in r.stdout, r.stdout + r.stderr
+
+
+# ---- gradients that are not recorded ------------------------------------------------------------
+
+def small_layer():
+    packed = torch.zeros(8, 32, dtype=torch.uint8, device="cuda")
+    w = decoder.W4Weights(packed, torch.ones(8, 1, dtype=BF16, device="cuda"), in_features=64, group_size=64)
+    p = Paged([2], [20], 2, 64, 16, BF16, poison=False)
+    zeros = lambda *shape: torch.zeros(*shape, dtype=BF16, device="cuda")
+    return dict(w=w, cache=p.gpu(), starts=p.starts.cuda(), table=decoder.RotaryTable(64, device="cuda"), x=zeros(2, 64),
+                bias=zeros(8), q=zeros(2, 4, 64), k=zeros(2, 2, 64), v=zeros(2, 2, 64), pos=torch.zeros(2, dtype=torch.int64, device="cuda"))
+
+
+CALLS = {
+    "linear_w4 x": ("x", lambda s, t: decoder.linear_w4(t, s["w"])),
+    "linear_w4 bias": ("bias", lambda s, t: decoder.linear_w4(s["x"], s["w"], t)),
+    "linear_w4 out": ("y", lambda s, t: decoder.linear_w4(s["x"], s["w"], out=t)),
+    "rotary x": ("q", lambda s, t: decoder.rotary(t, s["pos"], s["table"])),
+    "rotary out": ("q", lambda s, t: decoder.rotary(s["q"], s["pos"], s["table"], out=t)),
+    "append k": ("k", lambda s, t: decoder.paged_append(s["cache"], t, s["v"], s["starts"])),
+    "append v": ("v", lambda s, t: decoder.paged_append(s["cache"], s["k"], t, s["starts"])),
+    "append q": ("q", lambda s, t: decoder.paged_append(s["cache"], s["k"], s["v"], s["starts"], q=t, table=s["table"])),
+    "append out": ("q", lambda s, t: decoder.paged_append(s["cache"], s["k"], s["v"], s["starts"], q=s["q"], table=s["table"], out=t)),
+    "attention q": ("q", lambda s, t: decoder.paged_attention(s["cache"], t, s["starts"])),
+    "attention out": ("q", lambda s, t: decoder.paged_attention(s["cache"], s["q"], s["starts"], out=t)),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tensors_that_require_a_gradient_are_refused(name):
+    """Every tensor argument, and the same call without recording, which has to pass."""
+    s = small_layer()
+    s["y"] = torch.zeros(2, 8, dtype=BF16, device="cuda")
+    which, call = CALLS[name]
+    t = s[which].clone().requires_grad_()
+    with pytest.raises(B200NotSupportedError, match="gradient"):
+        call(s, t)
+    with torch.no_grad():
+        call(s, t)
+    call(s, t.detach())
+
+
+@pytest.mark.parametrize("name", [n for n in CALLS if not n.endswith("out")])
+def test_arguments_that_are_no_tensors_are_refused(name):
+    s = small_layer()
+    for t in (1.0, [0.0] * 8):
+        with pytest.raises(B200ArgumentError):
+            CALLS[name][1](s, t)
