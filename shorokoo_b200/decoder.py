@@ -11,7 +11,7 @@ answers from a paged cache (the sb_rotary*, sb_paged_* and sb_*w4* entry points 
 Tensors are torch CUDA tensors. Every call enqueues its kernels on torch's current stream of the
 tensors' device and returns; nothing waits, and results are new tensors of torch's allocator unless
 ``out`` is given, so calls can be captured into CUDA graphs and run on several streams. The operators
-compute no autograd graph and refuse inputs that require one. Errors are the backend's
+compute no autograd graph and no tangents, and refuse tensors that require either. Errors are the backend's
 (``B200ArgumentError`` and so on).
 """
 from __future__ import annotations
@@ -21,6 +21,7 @@ import struct
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .backend import B200ArgumentError, B200NotSupportedError, _check
@@ -55,6 +56,12 @@ def _cuda(x, name: str) -> torch.device:
     return x.device
 
 
+def _derived(x) -> bool:
+    """Whether autograd would have to record what is computed from x, backward or forward."""
+    return (x.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0
+                                                             and forward_ad.unpack_dual(x).tangent is not None)
+
+
 def _on(x, name: str, device: torch.device, dtype: torch.dtype, dims: int) -> None:
     if not isinstance(x, torch.Tensor) or x.device != device:
         _bad(f"{name} must be a tensor on {device}")
@@ -62,8 +69,8 @@ def _on(x, name: str, device: torch.device, dtype: torch.dtype, dims: int) -> No
         _bad(f"{name} must be {dtype}, got {x.dtype}")
     if x.dim() != dims:
         _bad(f"{name} must have {dims} dimensions, got shape {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise B200NotSupportedError(f"{name} requires a gradient, which these operators do not record")
+    if _derived(x):
+        raise B200NotSupportedError(f"{name} requires a gradient or has a tangent, which these operators do not record")
 
 
 _pack_heads = struct.Struct("Pqq").pack   # sb_heads
@@ -74,8 +81,7 @@ def _heads(x, name: str, device: torch.device, dtype: torch.dtype):
     try:
         tokens, heads, dim = x.shape
         token, head, last = x.stride()
-        if (x.dtype is dtype and x.get_device() == device.index and (last == 1 or dim == 1)
-                and not (x.requires_grad and torch.is_grad_enabled())):
+        if x.dtype is dtype and x.get_device() == device.index and (last == 1 or dim == 1) and not _derived(x):
             return tokens, heads, dim, _pack_heads(x.data_ptr(), token, head)
     except (AttributeError, TypeError, ValueError):
         pass
@@ -335,7 +341,7 @@ def linear_w4(x: torch.Tensor, weights: W4Weights, bias: Optional[torch.Tensor] 
     if bias is not None:
         try:
             if (bias.dtype is dtype and bias.get_device() == device.index and bias.shape == (n,) and bias.is_contiguous()
-                    and not (bias.requires_grad and torch.is_grad_enabled())):
+                    and not _derived(bias)):
                 at = bias.data_ptr()
         except AttributeError:
             pass
@@ -352,7 +358,7 @@ def _matrix(x, name: str, device: torch.device, dtype: torch.dtype, rows: Option
         m, n = x.shape
         stride, last = x.stride()
         if (x.dtype is dtype and x.get_device() == device.index and n == columns and (rows is None or m == rows)
-                and (last == 1 or n == 1) and not (x.requires_grad and torch.is_grad_enabled())):
+                and (last == 1 or n == 1) and not _derived(x)):
             return m, stride
     except (AttributeError, TypeError, ValueError):
         pass

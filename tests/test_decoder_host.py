@@ -252,3 +252,20 @@ def test_tensors_off_the_gpu_are_refused():
         decoder.PagedCache(x[None], x[None], torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
     with pytest.raises(B200ArgumentError, match="CUDA"):
         decoder.W4Weights(torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.float16), in_features=64, group_size=64)
+
+
+def test_what_autograd_would_have_to_record():
+    import torch
+    from torch.autograd import forward_ad
+    x = torch.ones(3)
+    assert not decoder._derived(x) and decoder._derived(x.clone().requires_grad_())
+    with torch.no_grad():
+        assert not decoder._derived(x.clone().requires_grad_())
+    with forward_ad.dual_level():
+        assert not decoder._derived(x) and decoder._derived(forward_ad.make_dual(x, x))
+        with torch.no_grad():          # which leaves tangents alone
+            assert decoder._derived(forward_ad.make_dual(x, x))
+    seen = []
+    torch.func.jvp(lambda z: (seen.append(decoder._derived(z)), z)[1], (x,), (x,))
+    torch.func.grad(lambda z: (seen.append(decoder._derived(z)), z.sum())[1])(x)
+    assert seen == [True, True]

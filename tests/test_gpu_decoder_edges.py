@@ -8,6 +8,7 @@ import sys
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from shorokoo_b200 import B200ArgumentError, B200NotSupportedError, decoder
 from test_gpu_decoder import BF16, FP16, U, Paged, attended, half, normal, within
@@ -221,3 +222,18 @@ def test_arguments_that_are_no_tensors_are_refused(name):
     for t in (1.0, [0.0] * 8):
         with pytest.raises(B200ArgumentError):
             CALLS[name][1](s, t)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tensors_with_a_tangent_are_refused(name):
+    """Forward-mode derivatives, by a dual tensor and by torch.func.jvp."""
+    s = small_layer()
+    s["y"] = torch.zeros(2, 8, dtype=BF16, device="cuda")
+    which, call = CALLS[name]
+    t = s[which]
+    with forward_ad.dual_level():
+        with pytest.raises(B200NotSupportedError, match="tangent"):
+            call(s, forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+        call(s, t)
+    with pytest.raises(B200NotSupportedError, match="tangent"):
+        torch.func.jvp(lambda z: call(s, z), (t.clone(),), (torch.ones_like(t),))
