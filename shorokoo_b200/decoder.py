@@ -233,6 +233,14 @@ class PagedCache:
         return t, h, packed
 
 
+def _device(cache) -> torch.device:
+    if not isinstance(cache, PagedCache):
+        _bad("cache must be a PagedCache")
+    if _derived(cache.k_pages) or _derived(cache.v_pages):   # since it was made, or made without recording
+        raise B200NotSupportedError("the cache's pages require a gradient or have a tangent, which these operators do not record")
+    return cache.device
+
+
 def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, query_starts: torch.Tensor, *,
                  q: Optional[torch.Tensor] = None, table: Optional[RotaryTable] = None,
                  out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -240,7 +248,7 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, query_star
     has rows query_starts[b] .. query_starts[b + 1] - 1 (int32 [batch + 1]), its last positions in order.
     With a table, k is turned by its position first, and so is q [tokens, heads, head_dim], which is
     returned (in ``out``, which may be q itself). Rows of no sequence are neither read nor written."""
-    device = cache.device
+    device = _device(cache)
     tokens, _, kh = cache._rows(k, "k", cache.kv_heads, None)
     _, _, vh = cache._rows(v, "v", cache.kv_heads, tokens)
     starts = _starts(query_starts, device, cache.batch)
@@ -266,7 +274,7 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, query_starts: torch.Tens
     over the positions of its sequence up to its own (``window`` > 0: the last ``window`` of them). Rows
     are as in ``paged_append``; query head h reads key head h // (heads // kv_heads); scale defaults to
     1 / sqrt(head_dim). A token that sees nothing gets zeros; rows of no sequence are not written."""
-    device = cache.device
+    device = _device(cache)
     tokens, heads, qh = cache._rows(q, "q", None, None)
     starts = _starts(query_starts, device, cache.batch)
     if out is None:
@@ -333,6 +341,8 @@ def linear_w4(x: torch.Tensor, weights: W4Weights, bias: Optional[torch.Tensor] 
     """x [rows, in_features] times the weights' transpose, plus bias [out_features], as [rows,
     out_features]; x, bias and the result have the weights' type. Meant for few rows: the weights are
     read once for every 32 of them."""
+    if not isinstance(weights, W4Weights):
+        _bad("weights must be W4Weights")
     device, dtype, n, k = weights.device, weights.dtype, weights.out_features, weights.in_features
     rows, xs = _matrix(x, "x", device, dtype, None, k)
     out = x.new_empty((rows, n)) if out is None else out

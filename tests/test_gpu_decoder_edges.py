@@ -237,3 +237,24 @@ def test_tensors_with_a_tangent_are_refused(name):
         call(s, t)
     with pytest.raises(B200NotSupportedError, match="tangent"):
         torch.func.jvp(lambda z: call(s, z), (t.clone(),), (torch.ones_like(t),))
+
+
+@pytest.mark.parametrize("which", ["k_pages", "v_pages"])
+def test_pages_that_require_a_gradient_later_are_refused(which):
+    s = small_layer()
+    getattr(s["cache"], which).requires_grad_()
+    calls = (lambda: decoder.paged_attention(s["cache"], s["q"], s["starts"]),
+             lambda: decoder.paged_append(s["cache"], s["k"], s["v"], s["starts"]))
+    for call in calls:
+        with pytest.raises(B200NotSupportedError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+def test_objects_of_another_kind_are_refused():
+    s = small_layer()
+    for call in (lambda: decoder.linear_w4(s["x"], s["x"]), lambda: decoder.paged_attention(s["w"], s["q"], s["starts"]),
+                 lambda: decoder.paged_append(None, s["k"], s["v"], s["starts"]), lambda: decoder.rotary(s["q"], s["pos"], s["w"])):
+        with pytest.raises(B200ArgumentError):
+            call()
