@@ -1,6 +1,6 @@
 """GPU tests of the decoder-layer operators where they can go wrong at the edges: weights far below a
-row's largest, non-finite values over long walks, waits that run out,
-gradients that the operators do not record. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
+row's largest, non-finite values over long walks, waits that run out, gradients
+that the operators do not record, index arrays that no caller should pass. Formulas, caches and tolerances are those of test_gpu_decoder.py."""
 import math
 import os
 import subprocess
@@ -98,7 +98,7 @@ def test_attention_of_a_split_context_with_a_leading_position(new):
 # ---- many items to a CTA -------------------------------------------------------------------------
 
 def attended_in_order(p, q):
-    """`attended` for one head per key head, without window or missing pages, whole sequences at a time."""
+    """`attended` without window or missing pages, whole sequences at a time."""
     want, tol = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
     h, d = half(q.dtype), q.shape[2]
     for b, n in enumerate(p.new):
@@ -106,11 +106,11 @@ def attended_in_order(p, q):
         rows, c = slice(int(p.starts[b]), int(p.starts[b]) + n), p.context[b]
         seen = torch.arange(c) <= torch.arange(c - n, c)[:, None]
         for x in range(q.shape[1]):
-            qx = q[rows, x].double()
-            w = torch.softmax((qx @ k[:, x].t() * d ** -0.5).masked_fill(~seen, -math.inf), 1)
-            delta = (d + 4) * U * (qx.abs() @ k[:, x].abs().t()).amax(1, keepdim=True) * d ** -0.5
-            want[rows, x] = w @ v[:, x]
-            tol[rows, x] = h * want[rows, x].abs() + (h + 2 * delta + (c / 16 + 32) * U) * (w @ v[:, x].abs())
+            qx, kx, vx = (y.double() for y in (q[rows, x], k[:, x * p.kv // q.shape[1]], v[:, x * p.kv // q.shape[1]]))
+            w = torch.softmax((qx @ kx.t() * d ** -0.5).masked_fill(~seen, -math.inf), 1)
+            delta = (d + 4) * U * (qx.abs() @ kx.abs().t()).amax(1, keepdim=True) * d ** -0.5
+            want[rows, x] = w @ vx
+            tol[rows, x] = h * want[rows, x].abs() + (h + 2 * delta + (c / 16 + 32) * U) * (w @ vx.abs())
     return want, tol
 
 
@@ -258,3 +258,68 @@ def test_objects_of_another_kind_are_refused():
                  lambda: decoder.paged_append(None, s["k"], s["v"], s["starts"]), lambda: decoder.rotary(s["q"], s["pos"], s["w"])):
         with pytest.raises(B200ArgumentError):
             call()
+
+
+# ---- sequences of many row tiles -----------------------------------------------------------------
+
+@pytest.mark.parametrize("new,heads,kv", [
+    ([1] * 60 + [600] + [1] * 60, 2, 2),      # 38 row tiles in the 16-row kernel
+    ([4200, 30], 4, 2),                       # 33 in the tensor core's
+])
+def test_attention_of_sequences_with_more_row_tiles_than_a_warp_has_lanes(new, heads, kv):
+    context = [n + 37 for n in new]
+    p = Paged(new, context, kv, 64, 16, BF16, seed=9)
+    q = normal(torch.Generator().manual_seed(6), (sum(new), heads, 64), BF16)
+    want, tol = attended_in_order(p, q)
+    within(decoder.paged_attention(p.gpu(), q.cuda(), p.starts.cuda()), want, tol, "tiles")
+
+
+# ---- index arrays that no caller should pass ------------------------------------------------------
+
+GUARD = 1 << 16    # bytes on either side
+
+
+def guarded(shape, dtype, fill):
+    """A tensor in the middle of a buffer, and a check that the buffer around it is as it was."""
+    n = math.prod(shape) * dtype.itemsize
+    whole = torch.full((n + 2 * GUARD,), 0xA5, dtype=torch.uint8, device="cuda")
+    inner = whole[GUARD: GUARD + n].view(dtype).view(shape)
+    if fill is not None:
+        inner.copy_(fill)
+
+    def untouched():
+        assert (whole[:GUARD] == 0xA5).all() and (whole[GUARD + n:] == 0xA5).all()
+    return inner, untouched
+
+
+@pytest.mark.parametrize("tokens", [3, 200])          # the 16-row kernel's, the tensor core's
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("starts,context", [
+    ((0, -5, 1.0), (40, 30)), ((0.7, 0, 0.3), (300, 30)), ((0, 100, 0.5), (40, 400)), ((1.0, 1.0, 1.0), (40, 30)),
+    ((5, 1, 1.0), (40, 30)), ((0, 0.5, 1.0), (-3, (1 << 31) - 1)), ((-(1 << 31), (1 << 31) - 1, 7), (1 << 30, 1)),
+])
+def test_index_arrays_out_of_order_write_nothing_outside(tokens, page, starts, context):
+    """Row starts that decrease or leave the rows, contexts that no table holds, table entries of any value: what
+    surrounds the result, the pages and the workspace stays as it was, and so does a page that no entry names."""
+    p = Paged([1, 1], [40, 30], 2, 64, page, BF16, poison=False, width=6)
+    p.table[0, 4], p.table[1, 4:] = 1 << 30, -(1 << 31)
+    named = set(int(x) for x in p.table.flatten() if 0 <= x < p.pages)
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (normal(gen, (tokens, x, 64), BF16).cuda() for x in (4, 2, 2))
+    s = torch.tensor([int(x * tokens) if isinstance(x, float) else x for x in starts], dtype=torch.int32).cuda()
+    kp, k_untouched = guarded(p.k.shape, BF16, p.k)
+    vp, v_untouched = guarded(p.v.shape, BF16, p.v)
+    out, out_untouched = guarded(q.shape, BF16, torch.zeros(q.shape))
+    cache = decoder.PagedCache(kp, vp, p.table.cuda(), torch.tensor(context, dtype=torch.int32).cuda())
+    decoder.paged_append(cache, k, v, s, q=q, table=decoder.RotaryTable(64, device="cuda"), out=out)
+    n = cache._workspace(4, tokens)
+    space, space_untouched = guarded((n,), torch.uint8, None)
+    qh, oh = (cache._rows(x, "rows", 4, tokens)[2] for x in (q, out))
+    for window in (0, 20):
+        decoder._call("sb_paged_attention", cache.device, cache._ref, qh, oh, 4, tokens, s.data_ptr(), 0.125, window,
+                      space.data_ptr(), n)
+    for check in (k_untouched, v_untouched, out_untouched, space_untouched):
+        check()
+    for page_no in set(range(p.pages)) - named:
+        assert torch.equal(kp[page_no].cpu(), p.k[page_no]) and torch.equal(vp[page_no].cpu(), p.v[page_no])
+    decoder.check()
