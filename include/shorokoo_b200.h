@@ -209,7 +209,8 @@ typedef struct sb_heads {
  * (every frequency divided by factor), SB_ROTARY_NTK (base times factor^(r / (r - 2))) or
  * SB_ROTARY_BY_PARTS (a pair that turns more than beta_fast times in original_context positions
  * keeps its frequency, one below beta_slow turns is divided by factor, those between are mixed
- * linearly in their number of turns; *magnitude = 0.1 ln(factor) + 1, else 1). */
+ * linearly in their number of turns, not in the pair's index; *magnitude = 0.1 ln(factor) + 1,
+ * else 1). */
 #define SB_ROTARY_PLAIN 0
 #define SB_ROTARY_LINEAR 1
 #define SB_ROTARY_NTK 2
@@ -218,8 +219,9 @@ SB_API int32_t sb_rotary_frequencies(int32_t rotary_dim, double base, int32_t sc
                                      double original_context, double beta_fast, double beta_slow,
                                      double* frequencies, double* magnitude);
 /* Turns per position of each frequency as 64-bit binary fractions (host arrays): what the kernels
- * multiply positions by, exactly modulo one turn, so that positions of any size and sign keep their
- * angle to 2^-32 of a turn. The caller copies them to the device for sb_rotary_table.phases. */
+ * multiply positions by, modulo one turn. An angle is off by about 2^-26 of a turn and 2^-65 of a
+ * turn per position (and the frequency's own rounding): positions of either sign below about 2^38
+ * keep it to 2^-25 of a turn. The caller copies them to the device for sb_rotary_table.phases. */
 SB_API int32_t sb_rotary_phases(const double* frequencies, int32_t pairs, uint64_t* phases);
 
 /* Pairs (2i, 2i + 1) when interleaved, (i, i + pairs) otherwise, of the first 2 * pairs elements of
@@ -232,7 +234,8 @@ typedef struct sb_rotary_table {
 } sb_rotary_table;
 
 /* y = x with every token's heads turned by its position; inverse != 0 turns by the negative angle,
- * which is the adjoint (the gradient of x for a gradient of y). x and y: float32, float16 or
+ * which is the adjoint (the gradient of x for a gradient of y; the inverse too where the table's
+ * magnitude is 1). x and y: float32, float16 or
  * bfloat16; y may be x itself, but not overlap it otherwise. positions: int32 or int64, any sign. */
 SB_API int32_t sb_rotary(const sb_heads* x, const sb_heads* y, int32_t elem_type, int64_t tokens, int32_t heads,
                          int32_t head_dim, const void* positions, int32_t positions_int64,
@@ -261,7 +264,7 @@ typedef struct sb_paged_cache {
 
 /* The step's tokens are packed: sequence b has rows query_starts[b] .. query_starts[b + 1] - 1 of
  * q, k, v and out (batch + 1 int32, not decreasing), its last positions in order. Rows of no
- * sequence (before the first, behind the last) are neither read nor written. */
+ * sequence (before the first, behind the last) are not written, and what they hold has no effect. */
 
 /* Writes k and v of the step's tokens into the cache; with a table, k is turned by its position
  * first and so is q into q_out (q and q_out NULL: keys alone; q_out may be q itself). Two rows that

@@ -13,10 +13,10 @@
 // Each of a CTA's 4 warps takes 16 of a tile's 64 positions, with its own ring of stages (cp.async, no
 // barrier between warps) and its own m, l, o, joined in shared memory at the item's end.
 //
-// Measured (bf16, 32 query and 8 key heads of 128, page 16): 48 sequences of up to 8000 positions 171 us, 5.4
-// TB/s, 0.83 of the measured HBM rate; with the arithmetic taken out 150 us, so the loads' pattern is sound
-// and what is left is the warps' own latency per stage. Three CTAs per SM with two stages each: 173 us; one
-// CTA with six stages: 282 us.
+// Measured (bf16, 32 query and 8 key heads of 128, page 16): 48 sequences of up to 8000 positions 168 us replayed
+// from a graph, 5.5 TB/s, 0.85 of the measured HBM rate (170 to 180 called from Python); with the arithmetic taken
+// out of the first version's 171 us 150, so the loads' pattern is sound and what is left is the warps' own latency
+// per stage. Three CTAs per SM with two stages each: 173 us; one CTA with six stages: 282 us.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -422,7 +422,10 @@ cudaError_t paged_attention(const PagedView& c, int elem, HeadsView q, HeadsView
   const PagedSpace z = space(c, sms);
   PagedArgs a;
   a.c = c, a.q = q, a.out = out;
-  a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas, a.least = 2;
+  a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas;
+  // Key tiles of a CTA, at least: one sequence over 1500 positions 18.8, 15.4, 15.3 and 19.7 us with 1, 2, 4 and 8;
+  // over 256 positions 10.5, 10.9, 11.4 and 17.8.
+  a.least = 2;
   a.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* p = static_cast<uint8_t*>(ws);
   a.notes = reinterpret_cast<PartialNote*>(p);

@@ -23,11 +23,11 @@
 //                    order, so a commit of S(i + 2) also says that PV(i) is done.
 // TMEM: S/P of A 0-127, of B 128-255, O of A 256-383, of B 384-511.
 //
-// Measured (2000 tokens over 40009 positions, 32 query and 8 key heads of 128, bf16, page 64): 1380 us, 463
-// TFLOP/s, 0.28 of the measured bf16 rate; the tensor pipe is active 38% of the cycles, the exponentials' 40%.
-// What bounds it is the row warps' latency (two per scheduler: logits read, exponentials, weights stored and
+// Measured (2000 tokens over 40009 positions, 32 query and 8 key heads of 128, bf16, page 64): 1480 to 1560 us
+// on several cards, 820 to 865 TFLOP/s, 0.52 of the measured bf16 rate; the tensor pipe is active 49% of the
+// cycles, the exponentials' as much. What bounds it is the row warps' latency (two per scheduler: logits read, exponentials, weights stored and
 // handed over, about 2000 cycles per half against 1145 for the same instructions free of waits). Tried
-// without gain: whole 128-column logits (1402), a polynomial for 1 to 4 of 8 exponential pairs (1350-1440),
+// without gain, on a card that took 1380: whole 128-column logits (1402), a polynomial for 1 to 4 of 8 exponential pairs (1350-1440),
 // tile B kept out of A's exponentials (1460), logits read again instead of kept for the second try (1400).
 //
 // Waits are bounded: one that runs out sets the error word, every role leaves its loop, the rows of the
@@ -851,7 +851,8 @@ cudaError_t paged_wait_errors(unsigned* bits, cudaStream_t s) {
   return e;
 }
 
-// More than 32 query rows per sequence and key head, on average. 16 sequences over 4000 positions (32 query, 8 key
+// More than 32 query rows per sequence and key head, on average over the batch: the host knows no more, so that a
+// step of single tokens and a prompt's chunk goes to one kernel as a whole. 16 sequences, all alike, over 4000 positions (32 query, 8 key
 // heads of 128): at 12 rows the 16-row kernel takes 62 us and this one 101, at 24 and 32 both 101 (it reads the
 // cache once per 16 rows), at 48 rows 152 and 102.
 bool paged_chunk_wanted(const PagedView& c) {
@@ -873,7 +874,11 @@ cudaError_t paged_chunk(const PagedView& c, int elem, HeadsView q, HeadsView out
   const PagedSpace z = paged_chunk_space(c, sms);
   PagedArgs a;
   a.c = c, a.q = q, a.out = out;
-  a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas, a.least = 4;
+  a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas;
+  // Key tiles of a CTA, at least: 300 tokens over 8000 positions 81.5 us with 1 to 8; 100 over 2000 29.2, 29.3, 32.5
+  // and 41.9 with 1, 2, 4 and 8; a prompt of 500 38.9, 38.9, 52.0 and 79.8. (Short
+  // prompts would be faster with 2.)
+  a.least = 4;
   a.wait = wait_limit();
   a.scale_log2 = scale * 1.4426950408889634f;
   uint8_t* p = static_cast<uint8_t*>(ws);

@@ -6,8 +6,10 @@
 //
 // The angle: 32-bit products lose it at far positions (position 10^6 in fp32 is off by 0.06 rad), so a
 // frequency is held as the 64-bit binary fraction of a turn per position and the product with the
-// position is taken modulo 2^64, that is exactly modulo one turn; its top 32 bits, as a signed number
-// in [-1, 1) half turns, go to sincospif.
+// position is taken modulo 2^64, that is exactly modulo one turn: the fraction's own rounding costs 2^-65 of a
+// turn per position, nothing else grows with it. Its top 32 bits, as a signed number in [-1, 1) half turns, are
+// rounded to fp32 for sincospif: about 2^-26 of a turn, 2^-25 pi radians, no more than what the results' own fp32
+// products lose (fp32 error against 64 bits 3.8e-8 of the values; 3.0e-8 with angles in 64 bits).
 //
 // Every value is read and written once: the kernels are bound by memory bandwidth (and, for a decode
 // step of some tens of tokens, by launch latency). A CTA takes one or a few tokens: the angles of its
@@ -251,7 +253,8 @@ cudaError_t launch(RotaryArgs a, bool inter, bool vec, int sms, cudaStream_t s) 
   const int64_t per_token = int64_t(a.q_heads + (kAppend ? 2 * a.kv_heads : 0)) * (a.rot_units + a.copy_units);
   if (per_token > (int64_t(1) << 27)) return cudaErrorInvalidValue;
   // Tokens of few pieces share a CTA (two pieces per thread) while the card stays full; tokens of many
-  // are split over CTAs while it is not.
+  // are split over CTAs while it is not. Replayed from a graph: 5000 tokens of 2 heads of 64 in bf16 9.5 us one to a
+  // CTA, 3.6 eight to a CTA (1200 tokens: 3.4 and 2.5); 32 tokens of 64 heads of 128 in fp32 5.1 us whole, 3.1 split.
   int per_cta = 1;
   while (per_cta < kMostTokensPerCta && per_cta * 2 * per_token <= 2 * kRotaryThreads &&
          a.tokens >= int64_t(per_cta) * 2 * 4 * sms && int64_t(per_cta) * 2 * a.pairs <= 4096)

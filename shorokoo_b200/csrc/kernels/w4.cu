@@ -20,7 +20,9 @@
 //
 // Measured (8192 inputs, 22016 outputs, groups of 32 with zero points, fp16, 104 MB): one row 31 us, 3.4 TB/s,
 // 0.52 of the measured HBM rate (its loads alone take 27 us, its arithmetic alone about 14 us of issue slots);
-// with the kernel for several rows 51 us. 13 rows by 4096 inputs and 11000 outputs, groups of 64: 18.5 us.
+// with the kernel for several rows 51 us. 13 rows by 4096 inputs and 11000 outputs, groups of 64, zero points: 21 us
+// (19.6 replayed from a graph); 125 registers leave two CTAs per SM, so that its 344 CTAs take two waves.
+// The figures at the choices below are replayed from a graph, 4096 inputs, weights from HBM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -449,7 +451,9 @@ template <typename T>
 cudaError_t launch_row(const W4Args& a, bool zeros, bool wide, int sms, cudaStream_t s) {
   const int64_t tiles = (a.n + 15) / 16;
   const int supers = (a.blocks + 3) / 4;
-  // Small CTAs end at different times and leave no SM idle; where there are few of them, more warps per tile.
+  // Small CTAs end at different times and leave no SM idle; where there are few of them, more warps per tile. Groups
+  // of 128: 22016 outputs 19.0 us with four warps, 22.2 with eight; 4096 outputs 6.4 and 6.0. (Between, four are ahead
+  // already: 11000 outputs 11.1 and 12.7.)
   const int threads = 32 * std::max(1, std::min(tiles >= 8 * sms ? 4 : 8, supers));
   const unsigned grid = unsigned(tiles);
   if (zeros && wide) linear_w4_row_kernel<T, true, true><<<grid, threads, 0, s>>>(a);
@@ -462,15 +466,19 @@ template <typename T>
 cudaError_t launch(const W4Args& a, bool zeros, bool per_block, bool wide, int sms, cudaStream_t s) {
   if (a.rows == 1 && a.shift >= 5) return launch_row<T>(a, zeros, wide, sms, s);
   if (a.rows <= 8) {
-    // Two tiles of outputs per CTA share the loads of x, where that leaves several CTAs per SM
+    // Two tiles of outputs per CTA share the loads of x, where that leaves several CTAs per SM: 8 rows, 22016 outputs,
+    // groups of 128, 18.8 us against 23.5 with one; 4 rows with zero points, groups of 64, 24.4 and 24.3 there, 23.5
+    // and 20.6 at 19000 outputs, 16.2 and 13.5 at 11000.
     if ((a.n + 31) / 32 >= 4 * sms) return launch<T, 1, 2>(a, zeros, per_block, wide, s);
     return launch<T, 1, 1>(a, zeros, per_block, wide, s);
   }
   if (a.rows <= 16) {
-    // ... and here half of what the SMs read of x, 13 rows of which are 106 KB per tile: 20.7 -> 18.5 us
+    // ... and here half of what the SMs read of x. 13 rows with zero points, groups of 64: 11000 outputs 19.6 us
+    // against 22.8 with one tile, 16384 outputs 22.6 and 30.3, but 4096 outputs 10.2 and 9.7.
     if ((a.n + 31) / 32 >= 2 * sms) return launch<T, 2, 2>(a, zeros, per_block, wide, s);
     return launch<T, 2, 1>(a, zeros, per_block, wide, s);
   }
+  // 11000 outputs, groups of 64: 17 rows 24.5 us, 32 rows 28.2; as two passes of 16 rows 38.2 and 40.1
   return launch<T, 4, 1>(a, zeros, per_block, wide, s);
 }
 

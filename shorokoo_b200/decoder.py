@@ -107,8 +107,9 @@ class RotaryTable:
     contexts ``factor`` times the trained one: "linear" divides every frequency by factor, "ntk"
     multiplies base by factor^(r / (r - 2)), "by_parts" keeps pairs that turn more than beta_fast times
     in original_context positions, divides those below beta_slow turns by factor, mixes those between
-    linearly in their turns and multiplies rotated values by 0.1 ln(factor) + 1.
-    ``from_frequencies`` takes any other frequencies (radians per position)."""
+    linearly in their turns and multiplies rotated values by 0.1 ln(factor) + 1. Checkpoints whose scaling
+    mixes linearly in the pair's index need ``from_frequencies``, which takes any frequencies (radians per
+    position)."""
 
     def __init__(self, rotary_dim: int, base: float = 10000.0, *, interleaved: bool = False, scaling: str = "none",
                  factor: float = 1.0, original_context: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
@@ -152,8 +153,8 @@ def _table(table, device: torch.device):
 def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, inverse: bool = False,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [tokens, heads, head_dim] (float32, float16, bfloat16) with each token turned by its position
-    (int32 or int64 [tokens], any sign). ``inverse`` turns back, which is the adjoint: the gradient of x
-    for the gradient of the result. ``out`` may be x itself, but not overlap it otherwise."""
+    (int32 or int64 [tokens], any sign). ``inverse`` turns back and multiplies by the table's magnitude all
+    the same, which is the adjoint: the gradient of x for the gradient of the result. ``out`` may be x itself, but not overlap it otherwise."""
     device = _cuda(x, "x")
     dtype = x.dtype
     elem = _ELEM.get(dtype)
@@ -247,7 +248,8 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, query_star
     """Writes the step's keys and values (k, v [tokens, kv_heads, head_dim]) into the cache. Sequence b
     has rows query_starts[b] .. query_starts[b + 1] - 1 (int32 [batch + 1]), its last positions in order.
     With a table, k is turned by its position first, and so is q [tokens, heads, head_dim], which is
-    returned (in ``out``, which may be q itself). Rows of no sequence are neither read nor written."""
+    returned (in ``out``, which may be q itself). Rows of no sequence are not written, and what they hold
+    has no effect."""
     device = _device(cache)
     tokens, _, kh = cache._rows(k, "k", cache.kv_heads, None)
     _, _, vh = cache._rows(v, "v", cache.kv_heads, tokens)
