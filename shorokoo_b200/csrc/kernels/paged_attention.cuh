@@ -50,8 +50,8 @@ template <> struct Mma<__nv_bfloat16> {
 // 17 nats above the others all of theirs would be below 2^-24 of it, and thousands of them gone from o but not from
 // l. So m is lifted to the top of that range, and brought down to kBack above a step's maximum that is more than
 // kFall below it: a step's largest weight is 2^-2 or more, and a weight is off by 2^-11 of itself or 2^-23 of the
-// largest of its step. At most kDeepest at a time and while l < kMostSum, so that o (65504 l) stays in fp32;
-// what is weighted less than 2^-39 of the largest then may be lost.
+// largest of its step. At most kDeepest at a time and while l < kMostSum, so that o (up to 65504 l) stays in
+// fp32. A weight that is lost then is below 2^-75 of l, and 2^30 of them with values of 65504 round to zero.
 template <typename T> struct Reference {   // bf16: the range of fp32
   static constexpr float kLift = 0.f, kGrowth = 8.f;
   static constexpr bool kFalls = false;

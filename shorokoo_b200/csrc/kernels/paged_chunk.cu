@@ -876,8 +876,8 @@ cudaError_t paged_chunk(const PagedView& c, int elem, HeadsView q, HeadsView out
   a.c = c, a.q = q, a.out = out;
   a.group = c.q_heads / c.kv_heads, a.window = window, a.ctas = z.ctas;
   // Key tiles of a CTA, at least: 300 tokens over 8000 positions 81.5 us with 1 to 8; 100 over 2000 29.2, 29.3, 32.5
-  // and 41.9 with 1, 2, 4 and 8; a prompt of 500 38.9, 38.9, 52.0 and 79.8. (Short
-  // prompts would be faster with 2.)
+  // and 41.9 with 1, 2, 4 and 8; a prompt of 500 38.9, 38.9, 52.0 and 79.8. (Short prompts
+  // would be faster with 2.)
   a.least = 4;
   a.wait = wait_limit();
   a.scale_log2 = scale * 1.4426950408889634f;

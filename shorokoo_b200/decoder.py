@@ -154,7 +154,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: RotaryTable, inverse
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [tokens, heads, head_dim] (float32, float16, bfloat16) with each token turned by its position
     (int32 or int64 [tokens], any sign). ``inverse`` turns back and multiplies by the table's magnitude all
-    the same, which is the adjoint: the gradient of x for the gradient of the result. ``out`` may be x itself, but not overlap it otherwise."""
+    the same, which is the adjoint: the gradient of x for the gradient of the result. ``out`` may be x
+    itself, but not overlap it otherwise."""
     device = _cuda(x, "x")
     dtype = x.dtype
     elem = _ELEM.get(dtype)
