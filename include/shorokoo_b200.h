@@ -312,6 +312,70 @@ SB_API int32_t sb_w4_layout(const sb_w4_weights* weights, const uint8_t* packed,
 SB_API int32_t sb_linear_w4(const sb_w4_weights* weights, const void* x, int64_t x_row_stride, const void* bias, void* y,
                             int64_t y_row_stride, int64_t rows, void* stream);
 
+/* The norms around a block's residual, for each row of `width` elements:
+ *   t = norm(x) post_weight + post_bias   (post_weight NULL: t = x)
+ *   h = residual + scale * gate * t       (residual NULL: 0; gate NULL: 1)
+ *   y = norm(h) weight + bias
+ * norm(z) = z / sqrt(mean(z^2) + eps) or, with layer_norm, the same of z - mean(z). weight_offset is added to
+ * weight and post_weight (checkpoints that hold them less 1). x, gate and y have elem_type (float32, float16 or
+ * bfloat16), residual and sum (where h goes; NULL: nowhere) elem_type or float32, weights and biases elem_type or
+ * float32. y NULL: h alone; weight belongs to y. gate_row_stride 0: one gate for all rows. Sums are fp32: of squares, so
+ * that fp32 values beyond 10^18 overflow. sum may be residual or x itself and y may be x itself; they may not overlap
+ * an input otherwise. width: at most 32768. */
+typedef struct sb_residual_norm_args {
+  const void *x, *residual, *gate;
+  void *sum, *y;
+  int64_t x_row_stride, residual_row_stride, gate_row_stride, sum_row_stride, y_row_stride;
+  const void *weight, *bias, *post_weight, *post_bias;
+  int64_t rows, width;
+  int32_t elem_type, sum_type, weight_type, layer_norm;
+  float scale, eps, weight_offset;
+} sb_residual_norm_args;
+SB_API int32_t sb_residual_norm(const sb_residual_norm_args* args, void* stream);
+
+/* A mixture-of-experts layer. Scores of a token: s = softmax(l) or 1 / (1 + e^-l) of l = router x; its experts are the
+ * top_k with the largest s + selection_bias (NULL: 0; equal ones: the lower expert first), the shares s, divided by
+ * their sum over the token's experts when normalize, times scale, and
+ *   y = sum over its experts of share * down[e] (act(gate_up[e][:inner] x) * (gate_up[e][inner:] x))
+ * with act(z) = z / (1 + e^-z) or z Phi(z). router [experts][width] (elem_type or float32), gate_up
+ * [experts][2 * inner][width], down [experts][width][inner] (elem_type: float16 or bfloat16), rows contiguous and the
+ * other strides in elements; selection_bias float32. Meant for few tokens: an expert's weights are read once for every
+ * 32 of its tokens. experts: at most 512; top_k: at most 32; width and inner: multiples of 8; pointers
+ * 16-byte aligned and strides multiples of 8 elements. Hidden values are rounded to elem_type. */
+#define SB_MOE_SOFTMAX 0
+#define SB_MOE_SIGMOID 1
+#define SB_MOE_SILU 0
+#define SB_MOE_GELU 1
+typedef struct sb_moe_weights {
+  const void *router, *gate_up, *down;
+  const float* selection_bias;
+  int64_t router_row_stride, gate_up_expert_stride, gate_up_row_stride, down_expert_stride, down_row_stride;
+  int64_t experts, width, inner;
+  int32_t elem_type, router_type, top_k, scoring, normalize, activation;
+  float scale;
+} sb_moe_weights;
+SB_API int32_t sb_moe_workspace(const sb_moe_weights* weights, int64_t tokens, size_t* bytes);
+/* x, y [tokens][width] of elem_type; y may be x itself. workspace: 256-byte aligned, at least
+ * sb_moe_workspace bytes, not shared with a call that may overlap. A cooperative launch. */
+SB_API int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_row_stride, void* y, int64_t y_row_stride,
+                      int64_t tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The next token of each row of logits [rows][vocab] (float32, float16 or bfloat16, NaN as -inf): with
+ * w = exp((l - max) / temperature), kept are w >= min_p, of these the top_k largest, of these the fewest largest
+ * whose sum is at least top_p of theirs (equal logits: the lower index first); tokens[row] is the first index at
+ * which the running sum of the kept w, in order of the index, exceeds uniform[row] (float32, [0, 1)) times their sum.
+ * Settings of each row (device arrays) or, where the array is NULL, of all. temperature 0 (or less, or NaN): the first
+ * of the largest. top_k 0 (or less): any number. top_p 1 (or more, or NaN) and min_p 0 (or less, or NaN): no filter;
+ * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0. */
+typedef struct sb_sampling {
+  const float *temperature_of, *top_p_of, *min_p_of;
+  const int32_t* top_k_of;
+  float temperature, top_p, min_p;
+  int32_t top_k;
+} sb_sampling;
+SB_API int32_t sb_sample(const void* logits, int64_t logits_row_stride, int32_t elem_type, int64_t rows, int64_t vocab,
+                         const float* uniform, const sb_sampling* by, int64_t* tokens, void* stream);
+
 /* ---- Diagnostics (no counterpart in the reference interface) ------------------------------- */
 /* Lowers and fuses the model on the host only (no device needed) for inputs given in session input
  * order, and writes a summary (one line per device op, then "separable=0|1") into buf as a

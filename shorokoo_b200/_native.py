@@ -38,6 +38,25 @@ class W4Weights(C.Structure):   # sb_w4_weights
                 ("has_zeros", I32)]
 
 
+class ResidualNorm(C.Structure):   # sb_residual_norm_args
+    _fields_ = [("x", P), ("residual", P), ("gate", P), ("sum", P), ("y", P), ("x_row_stride", I64), ("residual_row_stride", I64),
+                ("gate_row_stride", I64), ("sum_row_stride", I64), ("y_row_stride", I64), ("weight", P), ("bias", P),
+                ("post_weight", P), ("post_bias", P), ("rows", I64), ("width", I64), ("elem_type", I32), ("sum_type", I32),
+                ("weight_type", I32), ("layer_norm", I32), ("scale", C.c_float), ("eps", C.c_float), ("weight_offset", C.c_float)]
+
+
+class MoEWeights(C.Structure):   # sb_moe_weights
+    _fields_ = [("router", P), ("gate_up", P), ("down", P), ("selection_bias", P), ("router_row_stride", I64),
+                ("gate_up_expert_stride", I64), ("gate_up_row_stride", I64), ("down_expert_stride", I64), ("down_row_stride", I64),
+                ("experts", I64), ("width", I64), ("inner", I64), ("elem_type", I32), ("router_type", I32), ("top_k", I32),
+                ("scoring", I32), ("normalize", I32), ("activation", I32), ("scale", C.c_float)]
+
+
+class Sampling(C.Structure):   # sb_sampling
+    _fields_ = [("temperature_of", P), ("top_p_of", P), ("min_p_of", P), ("top_k_of", P), ("temperature", C.c_float),
+                ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", I32)]
+
+
 # name: (restype, argtypes)
 SIGNATURES = {
     "sb_version": (I32, []),
@@ -87,6 +106,10 @@ SIGNATURES = {
     "sb_w4_layout_bytes": (I32, [P, C.POINTER(SZ)]),
     "sb_w4_layout": (I32, [P, P, I64, P, P, P, P]),
     "sb_linear_w4": (I32, [P, P, I64, P, P, I64, I64, P]),
+    "sb_residual_norm": (I32, [P, P]),
+    "sb_moe_workspace": (I32, [P, I64, C.POINTER(SZ)]),
+    "sb_moe": (I32, [P, P, I64, P, I64, I64, P, SZ, P]),
+    "sb_sample": (I32, [P, I64, I32, I64, I64, P, P, P, P]),
 }
 
 

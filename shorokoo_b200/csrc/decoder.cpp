@@ -142,6 +142,37 @@ k::W4View view(const sb_w4_weights* w) {
   return {w->data, w->out_features, w->in_features, w->group_size, w->has_zeros ? 1 : 0, w->elem_type};
 }
 
+k::MoEView view(const sb_moe_weights* w) {
+  need(w != nullptr, "weights are null");
+  supported(w->elem_type == DT_FLOAT16 || w->elem_type == DT_BFLOAT16,
+            std::string("element type ") + dtype_name(w->elem_type) + " (float16 or bfloat16)");
+  need(w->router_type == w->elem_type || w->router_type == DT_FLOAT, "router_type must be elem_type or float32");
+  need(w->experts > 0 && w->width > 0 && w->inner > 0, "sizes must be positive");
+  supported(w->experts <= 512, std::to_string(w->experts) + " experts (at most 512)");
+  need(w->top_k > 0 && w->top_k <= w->experts, "top_k " + std::to_string(w->top_k) + " of " + std::to_string(w->experts) + " experts");
+  supported(w->top_k <= 32, "top_k " + std::to_string(w->top_k) + " (at most 32)");
+  supported(w->width % 8 == 0 && w->inner % 8 == 0 && w->width < (1 << 20) && w->inner < (1 << 20),
+            "width and inner must be multiples of 8 below 2^20");
+  need(w->scoring == SB_MOE_SOFTMAX || w->scoring == SB_MOE_SIGMOID, "unknown scoring");
+  need(w->activation == SB_MOE_SILU || w->activation == SB_MOE_GELU, "unknown activation");
+  need(std::isfinite(w->scale), "scale must be finite");
+  need(w->router != nullptr && w->gate_up != nullptr && w->down != nullptr, "router, gate_up or down is null");
+  supported(aligned(w->router, 16) && aligned(w->gate_up, 16) && aligned(w->down, 16), "weights need 16-byte alignment");
+  need(aligned(w->selection_bias, 4), "selection_bias is misaligned");
+  for (int64_t s : {w->router_row_stride, w->gate_up_expert_stride, w->gate_up_row_stride, w->down_expert_stride, w->down_row_stride}) {
+    need(usable(s), "stride of the weights out of range");
+    supported(s % 8 == 0, "weights need strides of whole 8-element pieces");
+  }
+  k::MoEView v = {};
+  v.router = w->router, v.gate_up = w->gate_up, v.down = w->down, v.selection_bias = w->selection_bias;
+  v.router_row = w->router_row_stride, v.up_expert = w->gate_up_expert_stride, v.up_row = w->gate_up_row_stride;
+  v.down_expert = w->down_expert_stride, v.down_row = w->down_row_stride;
+  v.elem = w->elem_type, v.router_elem = w->router_type, v.experts = int(w->experts), v.width = int(w->width);
+  v.inner = int(w->inner), v.top_k = w->top_k, v.softmax = w->scoring == SB_MOE_SOFTMAX, v.normalize = w->normalize != 0;
+  v.gelu = w->activation == SB_MOE_GELU, v.scale = w->scale;
+  return v;
+}
+
 }  // namespace
 
 extern "C" {
@@ -302,6 +333,93 @@ int32_t sb_linear_w4(const sb_w4_weights* weights, const void* x, int64_t x_row_
     need(usable(x_row_stride) && usable(y_row_stride), "row stride out of range");
     need(rows == 1 || std::llabs(y_row_stride) >= w.n, "rows of y overlap");
     launched(k::linear_w4(w, x, x_row_stride, bias, y, y_row_stride, rows, multiprocessors(), static_cast<cudaStream_t>(stream)));
+  });
+}
+
+int32_t sb_residual_norm(const sb_residual_norm_args* args, void* stream) {
+  return checked("sb_residual_norm", [&] {
+    need(args != nullptr, "args is null");
+    const sb_residual_norm_args& a = *args;
+    const int32_t t = a.elem_type;
+    supported(t == DT_FLOAT || t == DT_FLOAT16 || t == DT_BFLOAT16, std::string("element type ") + dtype_name(t));
+    need(a.sum_type == t || a.sum_type == DT_FLOAT, "sum_type must be elem_type or float32");
+    need(a.weight_type == t || a.weight_type == DT_FLOAT, "weight_type must be elem_type or float32");
+    need(a.rows >= 0 && a.rows <= kMostTokens && a.width > 0, "sizes out of range");
+    supported(a.width <= 32768, "width " + std::to_string(a.width) + " (at most 32768)");
+    need(std::isfinite(a.scale) && std::isfinite(a.weight_offset), "scale and weight_offset must be finite");
+    need(std::isfinite(a.eps) && a.eps >= 0, "eps must not be negative");
+    if (a.rows == 0) return;   // whose tensors are null
+    need(a.y != nullptr || a.sum != nullptr, "y and sum are both null");
+    need((a.y != nullptr) == (a.weight != nullptr), "y and weight go together");
+    need(a.bias == nullptr || a.weight != nullptr, "bias needs weight");
+    need(a.post_bias == nullptr || a.post_weight != nullptr, "post_bias needs post_weight");
+    need(a.x != nullptr, "x is null");
+    need(a.y == nullptr || a.y != a.sum, "y and sum are the same");
+    const size_t size = dtype_size(t), sum = dtype_size(a.sum_type), weight = dtype_size(a.weight_type);
+    need(aligned(a.x, size) && aligned(a.gate, size) && aligned(a.y, size) && aligned(a.residual, sum) && aligned(a.sum, sum) &&
+             aligned(a.weight, weight) && aligned(a.bias, weight) && aligned(a.post_weight, weight) && aligned(a.post_bias, weight),
+         "a tensor is not aligned to its element type");
+    for (int64_t s : {a.x_row_stride, a.residual_row_stride, a.gate_row_stride, a.sum_row_stride, a.y_row_stride})
+      need(usable(s), "row stride out of range");
+    need(a.rows == 1 || ((a.y == nullptr || std::llabs(a.y_row_stride) >= a.width) &&
+                         (a.sum == nullptr || std::llabs(a.sum_row_stride) >= a.width)),
+         "rows of y or sum overlap");
+    k::ResidualNormArgs v = {};
+    v.x = a.x, v.residual = a.residual, v.gate = a.gate, v.sum = a.sum, v.y = a.y;
+    v.xs = a.x_row_stride, v.rs = a.residual_row_stride, v.gs = a.gate_row_stride, v.ss = a.sum_row_stride, v.ys = a.y_row_stride;
+    v.weight = a.weight, v.bias = a.bias, v.post_weight = a.post_weight, v.post_bias = a.post_bias;
+    v.rows = a.rows, v.width = int(a.width), v.weight_elem = a.weight_type, v.layer = a.layer_norm != 0;
+    v.scale = a.scale, v.eps = a.eps, v.offset = a.weight_offset;
+    launched(k::residual_norm(v, t, a.sum_type, multiprocessors(), static_cast<cudaStream_t>(stream)));
+  });
+}
+
+int32_t sb_moe_workspace(const sb_moe_weights* weights, int64_t tokens, size_t* bytes) {
+  return checked("sb_moe_workspace", [&] {
+    need(bytes != nullptr, "bytes is null");
+    need(tokens >= 0 && tokens <= kMostTokens, "token count out of range");
+    *bytes = k::moe_workspace(view(weights), tokens);
+  });
+}
+
+int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_row_stride, void* y, int64_t y_row_stride, int64_t tokens,
+               void* workspace, size_t workspace_bytes, void* stream) {
+  return checked("sb_moe", [&] {
+    const k::MoEView w = view(weights);
+    need(tokens >= 0 && tokens <= kMostTokens, "token count out of range");
+    if (tokens == 0) return;
+    need(x != nullptr && y != nullptr, "x or y is null");
+    need(usable(x_row_stride) && usable(y_row_stride), "row stride out of range");
+    supported(aligned(x, 16) && aligned(y, 16) && x_row_stride % 8 == 0 && y_row_stride % 8 == 0,
+              "x and y need 16-byte alignment and strides of whole 8-element pieces");
+    need(tokens == 1 || std::llabs(y_row_stride) >= w.width, "rows of y overlap");
+    const size_t bytes = k::moe_workspace(w, tokens);
+    need(workspace != nullptr && aligned(workspace, 256), "workspace is null or not 256-byte aligned");
+    need(workspace_bytes >= bytes, "workspace has " + std::to_string(workspace_bytes) + " of " + std::to_string(bytes) + " bytes");
+    launched(k::moe(w, x, x_row_stride, y, y_row_stride, tokens, workspace, multiprocessors(), static_cast<cudaStream_t>(stream)));
+  });
+}
+
+int32_t sb_sample(const void* logits, int64_t logits_row_stride, int32_t elem_type, int64_t rows, int64_t vocab, const float* uniform,
+                  const sb_sampling* by, int64_t* tokens, void* stream) {
+  return checked("sb_sample", [&] {
+    supported(elem_type == DT_FLOAT || elem_type == DT_FLOAT16 || elem_type == DT_BFLOAT16,
+              std::string("element type ") + dtype_name(elem_type));
+    need(by != nullptr, "by is null");
+    need(rows >= 0 && rows <= (int64_t(1) << 26) && vocab > 0, "sizes out of range");
+    supported(vocab <= (1 << 24), "vocab " + std::to_string(vocab) + " (at most 2^24)");
+    need(by->temperature_of != nullptr || !std::isnan(by->temperature), "temperature is NaN");
+    need(by->top_p_of != nullptr || !std::isnan(by->top_p), "top_p is NaN");
+    need(by->min_p_of != nullptr || !std::isnan(by->min_p), "min_p is NaN");
+    if (rows == 0) return;
+    need(logits != nullptr && uniform != nullptr && tokens != nullptr, "logits, uniform or tokens is null");
+    need(aligned(logits, dtype_size(elem_type)) && aligned(uniform, 4) && aligned(tokens, 8) && aligned(by->temperature_of, 4) &&
+             aligned(by->top_p_of, 4) && aligned(by->min_p_of, 4) && aligned(by->top_k_of, 4),
+         "a tensor is not aligned to its element type");
+    need(usable(logits_row_stride), "row stride out of range");
+    const k::SamplingView v = {by->temperature_of, by->top_p_of, by->min_p_of, by->top_k_of, by->temperature, by->top_p, by->min_p, by->top_k};
+    launched(k::sample(logits, logits_row_stride, elem_type, rows, int(vocab), uniform, v, tokens, multiprocessors(),
+                       static_cast<cudaStream_t>(stream)));
   });
 }
 

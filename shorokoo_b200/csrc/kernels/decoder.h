@@ -1,5 +1,5 @@
-// Launch interface of the decoder-layer kernels (rotary.cu, w4.cu, paged_attention.cu): what
-// ../decoder.cpp checks and passes on. Arguments are valid when they get here.
+// Launch interface of the decoder-layer kernels (rotary.cu, w4.cu, paged_attention.cu, residual_norm.cu, moe.cu,
+// sample.cu): what ../decoder.cpp checks and passes on. Arguments are valid when they get here.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -58,6 +58,40 @@ cudaError_t w4_layout(const W4View& w, const uint8_t* packed, int64_t row_bytes,
                       void* data, cudaStream_t s);
 cudaError_t linear_w4(const W4View& w, const void* x, int64_t xs, const void* bias, void* y, int64_t ys, int64_t rows,
                       int sms, cudaStream_t s);
+
+// Rows of width elements; strides between them in elements. Null: not there.
+struct ResidualNormArgs {
+  const void *x, *residual, *gate;
+  void *sum, *y;
+  int64_t xs, rs, gs, ss, ys;
+  const void *weight, *bias, *post_weight, *post_bias;
+  int64_t rows;
+  int width, weight_elem, layer;   // layer: the mean is taken off
+  float scale, eps, offset;        // offset: added to the weights
+  float per_width;                 // 1 / width, set by residual_norm
+};
+cudaError_t residual_norm(const ResidualNormArgs& a, int elem, int sum_elem, int sms, cudaStream_t s);
+
+struct MoEView {
+  const void *router, *gate_up, *down;   // [experts][width], [experts][2 inner][width], [experts][width][inner]
+  const float* selection_bias;           // [experts] or null
+  int64_t router_row, up_expert, up_row, down_expert, down_row;
+  int elem, router_elem, experts, width, inner, top_k;
+  int softmax, normalize, gelu;
+  float scale;
+};
+size_t moe_workspace(const MoEView& w, int64_t tokens);
+cudaError_t moe(const MoEView& w, const void* x, int64_t xs, void* y, int64_t ys, int64_t tokens, void* ws, int sms, cudaStream_t s);
+
+// Settings of all rows, or (not null) of each.
+struct SamplingView {
+  const float *temperature_of, *top_p_of, *min_p_of;
+  const int32_t* top_k_of;
+  float temperature, top_p, min_p;
+  int top_k;
+};
+cudaError_t sample(const void* logits, int64_t stride, int elem, int64_t rows, int vocab, const float* uniform, const SamplingView& by,
+                   int64_t* tokens, int sms, cudaStream_t s);
 
 }  // namespace k
 }  // namespace sb

@@ -1,0 +1,571 @@
+// A mixture-of-experts layer for a few tokens, in one cooperative kernel:
+//   l = x R^T,  s = softmax(l) or 1 / (1 + e^-l),  the top_k largest s (+ selection bias), share_e = s_e (/ their sum) scale
+//   y = sum over the chosen e of share_e D_e (act(G_e x) * (U_e x))
+//
+// Few tokens read each chosen expert's weights for a handful of columns: the weights' bytes bound it. The products
+// go to the tensor core (mma m16n8k16, fp32 accumulators) with the weights as the 16-row operand and up to 8 tokens
+// as its columns, so that a token more costs next to nothing. Its inputs' order in k does not matter as long as both
+// operands have the same, so a lane takes 8 neighbouring inputs of a row as its part of two products: weights come as
+// they lie in memory, in 16-byte pieces that only the lane that copied them reads (a cp.async ring per warp, without
+// barriers; it runs on over the ends of tiles and is filled for the second product while the grid waits for the first).
+// A tile of the first product holds 8 rows of G and the same 8 of U: a lane has gate and input of one feature.
+//
+// The phases, with the grid's barrier between them: the router's dot products; the choice, by every CTA for itself
+// where there are few tokens, and the lists of tokens per expert; the first product over (expert, features), its
+// k split over a CTA's warps; the second over (expert, outputs, part of k) into partial sums; their sum in the order
+// of a token's experts. No atomics decide an order: results repeat.
+// The router sums pieces of 8 products in fp32 and the pieces in fp64: a choice between experts whose scores are next
+// to each other hangs on it. Hidden values are rounded to the weights' type, the second product's operand; the rest
+// stays in fp32.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "decoder.h"
+
+namespace sb {
+namespace k {
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kBlock = 64;          // inputs of a step
+constexpr int kMostExperts = 512;   // of a lane's 16 scores
+
+struct Entry { int expert, row, count, pad; };   // up to 8 NT rows of one expert
+
+struct MoEArgs {
+  MoEView w;
+  const void* x;
+  void* y;
+  int64_t xs, ys;
+  int tokens, rows;        // rows: tokens * top_k
+  int words, entries;      // mask words of an expert; room for entries
+  int splits;              // of the second product's k
+  double* logits;          // [tokens][experts]
+  int* chosen;             // [rows]
+  float* share;            // [rows]
+  void* hidden;            // [rows][inner]
+  float* partial;          // [splits][rows][width]
+};
+
+template <typename T> struct Op;
+template <> struct Op<__half> {
+  static __device__ __forceinline__ float2 both(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+  static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Op<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 both(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+  static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {   // zeros where it is not
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
+// A score as an integer of the same order, NaN below all and 0 for none
+__device__ __forceinline__ uint32_t ordered(float v) {
+  if (v != v) return 1u;
+  const uint32_t b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One dot product of the router, by a warp.
+template <typename T>
+__device__ __forceinline__ double router_dot(const MoEArgs& a, int t, int e, int lane) {
+  const uint16_t* x = static_cast<const uint16_t*>(a.x) + t * a.xs;
+  double sum = 0;
+  if (a.w.router_elem == 1) {
+    const float* r = static_cast<const float*>(a.w.router) + e * a.w.router_row;
+#pragma unroll 4
+    for (int k = lane * 8; k < a.w.width; k += 256) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + k);
+      const float4 p = *reinterpret_cast<const float4*>(r + k), q = *reinterpret_cast<const float4*>(r + k + 4);
+      const float2 v0 = Op<T>::both(v.x), v1 = Op<T>::both(v.y), v2 = Op<T>::both(v.z), v3 = Op<T>::both(v.w);
+      sum += double(v0.x) * p.x + double(v0.y) * p.y + double(v1.x) * p.z + double(v1.y) * p.w;
+      sum += double(v2.x) * q.x + double(v2.y) * q.y + double(v3.x) * q.z + double(v3.y) * q.w;
+    }
+  } else {
+    const uint16_t* r = static_cast<const uint16_t*>(a.w.router) + e * a.w.router_row;
+#pragma unroll 8
+    for (int k = lane * 8; k < a.w.width; k += 256) {
+      const uint4 v = *reinterpret_cast<const uint4*>(x + k), q = *reinterpret_cast<const uint4*>(r + k);
+      const float2 v0 = Op<T>::both(v.x), v1 = Op<T>::both(v.y), v2 = Op<T>::both(v.z), v3 = Op<T>::both(v.w);
+      const float2 q0 = Op<T>::both(q.x), q1 = Op<T>::both(q.y), q2 = Op<T>::both(q.z), q3 = Op<T>::both(q.w);
+      float p = v0.x * q0.x;
+      p += v0.y * q0.y, p += v1.x * q1.x, p += v1.y * q1.y, p += v2.x * q2.x, p += v2.y * q2.y, p += v3.x * q3.x, p += v3.y * q3.y;
+      sum += p;
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+  return sum;
+}
+
+// The experts of a token and their shares, by a warp; equal scores go to the lower expert.
+__device__ __forceinline__ void choose(const MoEArgs& a, int t, int lane, int* chosen, float* share) {
+  const MoEView& w = a.w;
+  const double* l = a.logits + int64_t(t) * w.experts;
+  uint32_t key[kMostExperts / 32];
+  double top = -INFINITY, all = 0;
+  const bool sums = w.softmax && (w.selection_bias != nullptr || !w.normalize);   // needs the sum over all experts
+  if (w.softmax) {
+    for (int e = lane; e < w.experts; e += 32) top = fmax(top, __ldcg(l + e));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, d));
+    if (sums) {
+      for (int e = lane; e < w.experts; e += 32) all += exp(__ldcg(l + e) - top);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+    }
+  }
+  auto score = [&](double v) { return w.softmax ? exp(v - top) : 1.0 / (1.0 + exp(-v)); };
+#pragma unroll
+  for (int j = 0; j < kMostExperts / 32; ++j) {
+    const int e = j * 32 + lane;
+    key[j] = 0;
+    if (j * 32 < w.experts && e < w.experts) {
+      const double v = __ldcg(l + e);
+      if (w.selection_bias) key[j] = ordered(float((w.softmax ? score(v) / all : score(v)) + double(w.selection_bias[e])));
+      else key[j] = ordered(float(v));
+    }
+  }
+  int mine = 0;   // lane r: the r-th chosen
+  for (int r = 0; r < w.top_k; ++r) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int j = 0; j < kMostExperts / 32; ++j)
+      if (j * 32 < w.experts) best = max(best, key[j]);
+    const uint32_t most = __reduce_max_sync(~0u, best);
+    uint32_t e = ~0u;
+#pragma unroll
+    for (int j = kMostExperts / 32 - 1; j >= 0; --j)
+      if (j * 32 < w.experts && key[j] == most) e = j * 32 + lane;
+    e = __reduce_min_sync(~0u, e);
+#pragma unroll
+    for (int j = 0; j < kMostExperts / 32; ++j)
+      if (e == uint32_t(j * 32 + lane)) key[j] = 0;
+    if (lane == r) mine = int(e);
+  }
+  double s = lane < w.top_k ? score(__ldcg(l + mine)) : 0.0;
+  if (w.normalize) {
+    double sum = s;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    s /= sum;
+  } else if (w.softmax) {
+    s /= all;
+  }
+  if (lane < w.top_k) {
+    chosen[t * w.top_k + lane] = mine;
+    share[t * w.top_k + lane] = float(s * double(w.scale));
+  }
+}
+
+// What a CTA knows of the step's rows, in shared memory.
+struct Lists {
+  uint32_t* mask;      // [experts][words] tokens of each expert
+  int* base;           // [experts] its first row
+  Entry* entry;        // [entries]
+  int* chosen;         // [rows] by token and rank
+  float* share;
+  uint16_t* token;     // [rows] of a row
+  uint16_t* row;       // [rows] of a token and rank
+  int* count;          // entries in use
+};
+__host__ __device__ inline size_t lists_bytes(int experts, int words, int entries, int rows) {
+  return size_t(entries) * sizeof(Entry) + size_t(experts) * (words + 1) * 4 + size_t(rows) * 12 + 16;
+}
+
+// The two products. Units: (entry, tile of rows, part of k); a CTA takes every gridDim.x-th.
+template <typename T, int NT, int MT, int S, bool kFirst>
+struct Product {
+  const MoEArgs& a;
+  const Lists& at;
+  const uint32_t ring;   // this warp's
+  float* sums;           // [2][kWarps][4 MT NT][32]
+  const int lane, warp, g, t;
+  int units, tiles, parts, blocks, depth, out_rows;   // blocks of k in a part; depth: k; out_rows: rows of the weights (of each half)
+  int64_t expert_stride, row_stride, second;          // second: from a row to the one 8 further in the tile
+  const uint16_t* weights;
+  int copy_unit, copy_block, copy_end;   // the next step to copy
+  const uint16_t* copy_from;
+  uint32_t copy_there;                   // bit 2 m + r: those rows exist
+  int stage_in, stage_out;
+
+  __device__ __forceinline__ Product(const MoEArgs& args, const Lists& lists, uint32_t ring_at, float* sums_at, int lane_no, int warp_no)
+      : a(args), at(lists), ring(ring_at), sums(sums_at), lane(lane_no), warp(warp_no), g(lane_no >> 2), t(lane_no & 3) {
+    depth = kFirst ? a.w.width : a.w.inner;
+    out_rows = kFirst ? a.w.inner : a.w.width;
+    parts = kFirst ? 1 : a.splits;
+    const int all = (depth + kBlock - 1) / kBlock;
+    blocks = (all + parts - 1) / parts;
+    tiles = (out_rows + kTile - 1) / kTile;
+    units = *at.count * tiles * parts;
+    expert_stride = kFirst ? a.w.up_expert : a.w.down_expert;
+    row_stride = kFirst ? a.w.up_row : a.w.down_row;
+    second = (kFirst ? int64_t(a.w.inner) : 8) * row_stride;
+    weights = static_cast<const uint16_t*>(kFirst ? a.w.gate_up : a.w.down);
+    stage_in = stage_out = 0;
+    copy_unit = blockIdx.x - gridDim.x;
+    copy_block = copy_end = 0;
+    next_unit();
+  }
+  static constexpr int kTile = kFirst ? 8 * MT : 16 * MT;   // rows (features) of a unit
+  static constexpr int kApart = kFirst ? 8 : 16;            // between a unit's products
+
+  struct Unit { int entry, first, part; };
+  __device__ __forceinline__ Unit unit(int u) const {
+    Unit v;
+    const int e = u / parts;
+    v.part = u - e * parts;
+    v.entry = e / tiles;
+    v.first = (e - v.entry * tiles) * kTile;
+    return v;
+  }
+  __device__ __forceinline__ int end_of(const Unit& v) const {
+    return min((v.part + 1) * blocks, (depth + kBlock - 1) / kBlock);
+  }
+
+  __device__ __forceinline__ void next_unit() {   // to the next unit in which this warp has a step
+    do {
+      copy_unit += gridDim.x;
+      if (copy_unit >= units) return;
+      const Unit v = unit(copy_unit);
+      copy_block = v.part * blocks + warp;
+      copy_end = end_of(v);
+      copy_from = weights + at.entry[v.entry].expert * expert_stride + (v.first + g) * row_stride + 8 * t;
+      copy_there = 0;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (v.first + m * kApart + g < out_rows) copy_there |= 1u << (2 * m);
+        if (v.first + m * kApart + g + (kFirst ? 0 : 8) < out_rows) copy_there |= 2u << (2 * m);
+      }
+    } while (copy_block >= copy_end);
+  }
+  __device__ __forceinline__ void copy_step() {
+    if (copy_unit < units) {
+      const uint32_t to = ring + stage_in * (MT * 2048) + lane * 16;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = copy_block * kBlock + h * 32;
+            const bool there = (copy_there >> (2 * m + r) & 1) && k + 8 * t < depth;
+            copy16(to + ((m * 2 + r) * 2 + h) * 512, there ? copy_from + m * kApart * row_stride + r * second + k : weights, there);
+          }
+      copy_block += kWarps;
+      if (copy_block >= copy_end) next_unit();
+    }
+    commit();
+    stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
+  }
+  __device__ __forceinline__ void fill() {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy_step();
+  }
+
+  __device__ __forceinline__ void run() {
+    int turn = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const Unit v = unit(u);
+      const Entry en = at.entry[v.entry];
+      const int used = (en.count + 7) / 8;   // column tiles
+      const uint16_t* column[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int c = n * 8 + g;
+        column[n] = nullptr;
+        if (c < en.count)
+          column[n] = kFirst ? static_cast<const uint16_t*>(a.x) + at.token[en.row + c] * a.xs
+                             : static_cast<const uint16_t*>(a.hidden) + int64_t(en.row + c) * a.w.inner;
+      }
+      auto fetch = [&](uint4 (&b)[NT][2], int block) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = block * kBlock + h * 32 + 8 * t;
+            b[n][h] = make_uint4(0, 0, 0, 0);
+            if (column[n] != nullptr && k < depth) b[n][h] = *reinterpret_cast<const uint4*>(column[n] + k);
+          }
+      };
+      float d[NT][MT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[n][m][i] = 0.f;
+      const int end = end_of(v);
+      uint4 b[NT][2];
+      int block = v.part * blocks + warp;
+      if (block < end) fetch(b, block);
+      for (; block < end; block += kWarps) {
+        wait<S - 2>();
+        const uint32_t from = ring + stage_out * (MT * 2048) + lane * 16;
+        stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
+        uint4 w[MT][2][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[m][r][h] = shared16(from + ((m * 2 + r) * 2 + h) * 512);
+        copy_step();   // into the stage read in the step before
+        uint4 ahead[NT][2];
+        if (block + kWarps < end) fetch(ahead, block + kWarps);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (NT > 1 && n >= used) break;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              Op<T>::mma(d[n][m], w[m][0][h].x, w[m][1][h].x, w[m][0][h].y, w[m][1][h].y, b[n][h].x, b[n][h].y);
+              Op<T>::mma(d[n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b[n][h].z, b[n][h].w);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) b[n][h] = ahead[n][h];
+      }
+      // The warps' sums meet; two buffers in turn, so that one barrier is enough.
+      constexpr int kEach = NT * MT * 4 * 32;
+      float* all = sums + turn * kWarps * kEach;
+      turn ^= 1;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (NT > 1 && n >= used) break;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) all[warp * kEach + ((n * MT + m) * 4 + i) * 32 + lane] = d[n][m][i];
+      }
+      __syncthreads();
+      auto total = [&](int q) {
+        float s = all[q];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) s += all[w * kEach + q];
+        return s;
+      };
+      if (kFirst) {
+        for (int i = threadIdx.x; i < used * MT * 64; i += kThreads) {
+          const int l = i & 31, odd = i >> 5 & 1, nm = i >> 6, n = nm / MT, m = nm - n * MT;
+          const int c = n * 8 + (l & 3) * 2 + odd, f = v.first + m * kApart + (l >> 2);
+          if (c < en.count && f < out_rows) {
+            const float gate = total((nm * 4 + odd) * 32 + l), up = total((nm * 4 + odd + 2) * 32 + l);
+            const float act = a.w.gelu ? 0.5f * gate * (1.f + erff(gate * 0.70710678f)) : gate / (1.f + expf(-gate));
+            static_cast<T*>(a.hidden)[int64_t(en.row + c) * a.w.inner + f] = Op<T>::round(act * up);
+          }
+        }
+      } else {
+        for (int i = threadIdx.x; i < used * MT * 128; i += kThreads) {
+          const int l = i & 31, q = i >> 5 & 3, nm = i >> 7, n = nm / MT, m = nm - n * MT;
+          const int c = n * 8 + (l & 3) * 2 + (q & 1), r = v.first + m * kApart + (q >> 1) * 8 + (l >> 2);
+          if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + en.row + c) * out_rows + r] = total((nm * 4 + q) * 32 + l);
+        }
+      }
+    }
+  }
+};
+
+template <typename T, int NT, int MT, int S>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const MoEArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const auto grid = cooperative_groups::this_grid();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int experts = a.w.experts, top_k = a.w.top_k;
+  constexpr int kRing = kWarps * S * MT * 2048, kSums = 2 * kWarps * NT * MT * 128 * 4;
+
+  for (int i = warp * gridDim.x + blockIdx.x; i < a.tokens * experts; i += kWarps * gridDim.x) {   // spread over the SMs first
+    const double v = router_dot<T>(a, i / experts, i % experts, lane);
+    if (lane == 0) a.logits[i] = v;
+  }
+  grid.sync();
+
+  Lists at;
+  {
+    uint8_t* p = smem + kRing + kSums;
+    at.entry = reinterpret_cast<Entry*>(p), p += a.entries * sizeof(Entry);
+    at.mask = reinterpret_cast<uint32_t*>(p), p += size_t(experts) * a.words * 4;
+    at.base = reinterpret_cast<int*>(p), p += size_t(experts) * 4;
+    at.chosen = reinterpret_cast<int*>(p), p += size_t(a.rows) * 4;
+    at.share = reinterpret_cast<float*>(p), p += size_t(a.rows) * 4;
+    at.count = reinterpret_cast<int*>(p), p += 16;
+    at.token = reinterpret_cast<uint16_t*>(p), p += size_t(a.rows) * 2;
+    at.row = reinterpret_cast<uint16_t*>(p);
+  }
+  for (int i = tid; i < experts * a.words; i += kThreads) at.mask[i] = 0;
+  if (a.tokens <= 2 * kWarps) {   // every CTA chooses for itself: cheaper than another barrier
+    for (int t = warp; t < a.tokens; t += kWarps) choose(a, t, lane, at.chosen, at.share);
+  } else {
+    for (int t = warp * gridDim.x + blockIdx.x; t < a.tokens; t += kWarps * gridDim.x) choose(a, t, lane, a.chosen, a.share);
+    grid.sync();
+    for (int i = tid; i < a.rows; i += kThreads) at.chosen[i] = __ldcg(a.chosen + i), at.share[i] = __ldcg(a.share + i);
+  }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kThreads) {
+    const int t = i / top_k;
+    atomicOr(at.mask + at.chosen[i] * a.words + (t >> 5), 1u << (t & 31));
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int rows = 0, entries = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0;
+      if (e < experts)
+        for (int i = 0; i < a.words; ++i) n += __popc(at.mask[e * a.words + i]);
+      const int mine = (n + 8 * NT - 1) / (8 * NT);
+      int r = n, m = mine;   // sums up to this lane
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int pr = __shfl_up_sync(~0u, r, d), pm = __shfl_up_sync(~0u, m, d);
+        if (lane >= d) r += pr, m += pm;
+      }
+      const int row = rows + r - n;
+      if (e < experts) at.base[e] = row;
+      for (int i = 0; i < mine; ++i) at.entry[entries + m - mine + i] = {e, row + i * 8 * NT, min(8 * NT, n - i * 8 * NT), 0};
+      rows += __shfl_sync(~0u, r, 31);
+      entries += __shfl_sync(~0u, m, 31);
+    }
+    if (lane == 0) *at.count = entries;
+  }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kThreads) {
+    const int t = i / top_k, e = at.chosen[i];
+    int row = at.base[e];
+    for (int j = 0; j < t >> 5; ++j) row += __popc(at.mask[e * a.words + j]);
+    row += __popc(at.mask[e * a.words + (t >> 5)] & ((1u << (t & 31)) - 1));
+    at.token[row] = uint16_t(t);
+    at.row[i] = uint16_t(row);
+  }
+  __syncthreads();
+
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S * MT * 2048;
+  float* sums = reinterpret_cast<float*>(smem + kRing);
+  {
+    Product<T, NT, MT, S, true> first(a, at, ring, sums, lane, warp);
+    first.fill();
+    first.run();
+    wait<0>();
+    Product<T, NT, MT, S, false> second(a, at, ring, sums, lane, warp);
+    second.fill();   // weights, while the grid finishes the hidden values
+    grid.sync();
+    second.run();
+    wait<0>();
+  }
+  grid.sync();
+
+  const int quads = a.w.width / 4;
+  for (int i = blockIdx.x * kThreads + tid; i < a.tokens * quads; i += gridDim.x * kThreads) {
+    const int t = i / quads, h = (i - t * quads) * 4;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < top_k; ++r) {
+      const float s = at.share[t * top_k + r];
+      const float* p = a.partial + int64_t(at.row[t * top_k + r]) * a.w.width + h;
+      float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+      for (int j = 1; j < a.splits; ++j) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(p + int64_t(j) * a.rows * a.w.width));
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      }
+      y.x += s * v.x, y.y += s * v.y, y.z += s * v.z, y.w += s * v.w;
+    }
+    alignas(8) T out[4] = {Op<T>::round(y.x), Op<T>::round(y.y), Op<T>::round(y.z), Op<T>::round(y.w)};
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.y) + t * a.ys + h) = *reinterpret_cast<const uint2*>(out);
+  }
+}
+
+// Sizes of one launch over up to `tokens` tokens.
+struct Sizes {
+  int tokens, words, entries, splits, columns;
+  size_t logits, chosen, hidden, partial, total;
+};
+Sizes sizes(const MoEView& w, int64_t tokens) {
+  Sizes z;
+  z.tokens = int(std::min<int64_t>(std::max<int64_t>(tokens, 1), std::min(256, 2048 / w.top_k)));
+  const int rows = z.tokens * w.top_k;
+  z.columns = z.tokens <= 8 ? 8 : 32;
+  z.words = (z.tokens + 31) / 32;
+  z.entries = std::min(w.experts, rows) + rows / z.columns;
+  // Parts of the second product's k where (expert, tile) pairs are few, of 256 inputs or more
+  const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + 15) / 16);
+  z.splits = 1;
+  while (z.splits < 8 && units * z.splits < 1024 && w.inner / (z.splits * 2) >= 256) z.splits *= 2;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  z.logits = up(size_t(z.tokens) * w.experts * 8);
+  z.chosen = up(size_t(rows) * 4);
+  z.hidden = up(size_t(rows) * w.inner * 2);
+  z.partial = up(size_t(z.splits) * rows * w.width * 4);
+  z.total = z.logits + 2 * z.chosen + z.hidden + z.partial;
+  return z;
+}
+
+template <typename T, int NT, int MT, int S>
+cudaError_t launch(MoEArgs a, int sms, cudaStream_t s) {
+  const size_t smem = size_t(kWarps) * S * MT * 2048 + size_t(2) * kWarps * NT * MT * 512 + lists_bytes(a.w.experts, a.words, a.entries, a.rows);
+  const void* kernel = reinterpret_cast<const void*>(moe_kernel<T, NT, MT, S>);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e != cudaSuccess) return e;
+  int each = 0;
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, kThreads, smem);
+  if (e != cudaSuccess) return e;
+  if (each < 1) return cudaErrorInvalidConfiguration;
+  void* args[] = {&a};
+  return cudaLaunchCooperativeKernel(kernel, dim3(unsigned(each * sms)), dim3(kThreads), args, smem, s);
+}
+
+}  // namespace
+
+size_t moe_workspace(const MoEView& w, int64_t tokens) {
+  const Sizes z = sizes(w, tokens);
+  return std::max(z.total, sizes(w, tokens % z.tokens).total);
+}
+
+cudaError_t moe(const MoEView& w, const void* x, int64_t xs, void* y, int64_t ys, int64_t tokens, void* ws, int sms, cudaStream_t s) {
+  // More tokens than a launch takes go through in pieces.
+  const Sizes most = sizes(w, tokens);
+  for (int64_t t0 = 0; t0 < tokens; t0 += most.tokens) {
+    const Sizes z = sizes(w, std::min<int64_t>(most.tokens, tokens - t0));
+    MoEArgs a;
+    a.w = w;
+    a.x = static_cast<const uint16_t*>(x) + t0 * xs, a.y = static_cast<uint16_t*>(y) + t0 * ys, a.xs = xs, a.ys = ys;
+    a.tokens = z.tokens, a.rows = z.tokens * w.top_k, a.words = z.words, a.entries = z.entries, a.splits = z.splits;
+    uint8_t* p = static_cast<uint8_t*>(ws);
+    a.logits = reinterpret_cast<double*>(p), p += z.logits;
+    a.chosen = reinterpret_cast<int*>(p), p += z.chosen;
+    a.share = reinterpret_cast<float*>(p), p += z.chosen;
+    a.hidden = p, p += z.hidden;
+    a.partial = reinterpret_cast<float*>(p);
+    cudaError_t e;
+    if (w.elem == 10) e = z.columns == 8 ? launch<__half, 1, 1, 6>(a, sms, s) : launch<__half, 4, 2, 4>(a, sms, s);
+    else e = z.columns == 8 ? launch<__nv_bfloat16, 1, 1, 6>(a, sms, s) : launch<__nv_bfloat16, 4, 2, 4>(a, sms, s);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace k
+}  // namespace sb

@@ -1,5 +1,6 @@
-"""Decoder-layer operators on device tensors: what one layer of a language model runs per step when it
-answers from a paged cache (the sb_rotary*, sb_paged_* and sb_*w4* entry points of the library's C ABI).
+"""Decoder-layer operators on device tensors: what a language model runs per step when it answers from a
+paged cache (the sb_rotary*, sb_paged_*, sb_*w4*, sb_residual_norm, sb_moe* and sb_sample entry points of the
+library's C ABI).
 
     weights = W4Weights(packed, scales, zeros, in_features=4096, group_size=128)     # once
     table = RotaryTable(128, 500000.0)                                               # once
@@ -7,6 +8,10 @@ answers from a paged cache (the sb_rotary*, sb_paged_* and sb_*w4* entry points 
     qkv = linear_w4(x, weights)
     q = paged_append(cache, k, v, query_starts, q=q, table=table)
     o = paged_attention(cache, q, query_starts)
+    y, h = residual_norm(linear_w4(o.flatten(1), projection), weight, residual=h)
+    experts = MoEWeights(router, gate_up, down, top_k=8)                             # once
+    y, h = residual_norm(moe(y, experts), weight, residual=h)
+    tokens = sample(linear_w4(y, head), uniform, temperature=0.7, top_p=0.9)
 
 Tensors are torch CUDA tensors. Every call enqueues its kernels on torch's current stream of the
 tensors' device and returns; nothing waits, and results are new tensors of torch's allocator unless
@@ -365,15 +370,214 @@ def linear_w4(x: torch.Tensor, weights: W4Weights, bias: Optional[torch.Tensor] 
     return out
 
 
-def _matrix(x, name: str, device: torch.device, dtype: torch.dtype, rows: Optional[int], columns: int):
-    """(rows, row stride) of a matrix whose rows are contiguous; rows None: any number."""
+def _matrix(x, name: str, device: torch.device, dtype: torch.dtype, rows: Optional[int], columns: Optional[int]):
+    """(rows, row stride) of a matrix whose rows are contiguous; rows or columns None: any number."""
     try:
         m, n = x.shape
         stride, last = x.stride()
-        if (x.dtype is dtype and x.get_device() == device.index and n == columns and (rows is None or m == rows)
+        if (x.dtype is dtype and x.get_device() == device.index and (columns is None or n == columns) and (rows is None or m == rows)
                 and (last == 1 or n == 1) and not _derived(x)):
             return m, stride
     except (AttributeError, TypeError, ValueError):
         pass
     _on(x, name, device, dtype, 2)
-    _bad(f"{name} must be [{'rows' if rows is None else rows}, {columns}] and contiguous along its rows, got {tuple(x.shape)}")
+    _bad(f"{name} must be [{'rows' if rows is None else rows}, {'width' if columns is None else columns}] and contiguous along its rows, got {tuple(x.shape)}")
+
+
+def _vector(x, name: str, device: torch.device, dtypes, n: int):
+    """(address, type) of n contiguous values of one of the types; (None, None) of None."""
+    if x is None:
+        return None, None
+    try:
+        dtype = x.dtype
+        if dtype in dtypes and x.get_device() == device.index and x.shape == (n,) and (x.stride() == (1,) or n == 1) and not _derived(x):
+            return x.data_ptr(), dtype
+    except AttributeError:
+        pass
+    _on(x, name, device, getattr(x, "dtype", None) if getattr(x, "dtype", None) in dtypes else dtypes[0], 1)
+    _bad(f"{name} must be {n} contiguous values, got {tuple(x.shape)}")
+
+
+def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Optional[torch.Tensor] = None,
+                  residual: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
+                  post_bias: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, scale: float = 1.0, kind: str = "rms",
+                  eps: float = 1e-6, weight_offset: float = 0.0, out: Optional[torch.Tensor] = None,
+                  residual_out: Optional[torch.Tensor] = None):
+    """The norms around a block's residual, for each row of x [rows, width] (float32, float16, bfloat16):
+
+        t = norm(x) post_weight + post_bias     (x without a post_weight)
+        h = residual + scale gate t
+        y = norm(h) weight + bias
+
+    as (y, h). norm(z) is z / sqrt(mean(z^2) + eps) or, with kind "layer", the same of z less its mean.
+    ``residual`` [rows, width] has x's type or float32, and so has h; ``gate`` is [width] or [rows, width] of x's
+    type; weights and biases [width] have x's type or float32, all of them the same one; ``weight_offset`` is added
+    to both weights. Without residual, gate, post_weight and scale h is x itself; without a weight y is None. y is
+    taken of h before h is rounded. ``out`` may be x, and ``residual_out`` x or residual; they may not overlap an
+    input otherwise."""
+    device = _cuda(x, "x")
+    dtype = x.dtype
+    elem = _ELEM.get(dtype)
+    if elem is None:
+        raise B200NotSupportedError(f"element type {dtype} is not supported")
+    if kind != "rms" and kind != "layer":
+        _bad(f"kind must be 'rms' or 'layer', got {kind!r}")
+    rows, xs = _matrix(x, "x", device, dtype, None, None)
+    n = x.shape[1]
+    a = _native.ResidualNorm()
+    sum_type, rs = dtype, 0
+    if residual is not None:
+        sum_type = torch.float32 if getattr(residual, "dtype", None) is torch.float32 else dtype
+        rs = _matrix(residual, "residual", device, sum_type, rows, n)[1]
+        a.residual = residual.data_ptr()
+    elif residual_out is not None:
+        sum_type = torch.float32 if getattr(residual_out, "dtype", None) is torch.float32 else dtype
+    gs = 0
+    if gate is not None:
+        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
+            a.gate = _vector(gate, "gate", device, (dtype,), n)[0]
+        else:
+            gs = _matrix(gate, "gate", device, dtype, rows, n)[1]
+            a.gate = gate.data_ptr()
+    weights = (dtype, torch.float32)
+    kinds = set()
+    for name, v in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
+        if v is not None:
+            at, t = _vector(v, name, device, weights, n)
+            setattr(a, name, at)
+            kinds.add(t)
+    if len(kinds) > 1:
+        _bad("weights and biases must have the same type")
+    if weight is None and (bias is not None or out is not None):
+        _bad("bias and out need a weight")
+    if post_weight is None and post_bias is not None:
+        _bad("post_bias needs a post_weight")
+    changed = residual is not None or gate is not None or post_weight is not None or scale != 1.0
+    if weight is None and not changed:
+        _bad("there is nothing to compute")
+    h = x
+    if changed or residual_out is not None:
+        h = residual_out if residual_out is not None else torch.empty((rows, n), dtype=sum_type, device=device)
+        a.sum_row_stride = _matrix(h, "residual_out", device, sum_type, rows, n)[1]
+        a.sum = h.data_ptr()
+    y = None
+    if weight is not None:
+        y = out if out is not None else torch.empty((rows, n), dtype=dtype, device=device)
+        a.y_row_stride = _matrix(y, "out", device, dtype, rows, n)[1]
+        a.y = y.data_ptr()
+    a.x, a.x_row_stride, a.residual_row_stride, a.gate_row_stride = x.data_ptr(), xs, rs, gs
+    a.rows, a.width, a.elem_type, a.sum_type = rows, n, elem, _ELEM[sum_type]
+    a.weight_type = _ELEM[kinds.pop()] if kinds else elem
+    a.layer_norm, a.scale, a.eps, a.weight_offset = kind == "layer", scale, eps, weight_offset
+    _call("sb_residual_norm", device, C.byref(a))
+    return y, h
+
+
+class MoEWeights:
+    """Weights of a mixture-of-experts layer, and how a token chooses: ``router`` [experts, width] (the weights' type or
+    float32), ``gate_up`` [experts, 2 * inner, width] (the gates' rows first), ``down`` [experts, width, inner],
+    float16 or bfloat16, of any strides (multiples of 8) along all but the last dimension. A token's scores are the
+    softmax (``scoring`` "softmax") or the sigmoids ("sigmoid") of router x; its experts the ``top_k`` largest of
+    score + ``selection_bias`` (float32 [experts]; equal ones: the lower first), their shares the scores, divided by
+    their sum with ``normalize``, times ``scale``. ``activation`` of the gates: "silu" or "gelu". The object keeps the
+    tensors; their contents may change between calls."""
+
+    def __init__(self, router: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, *, top_k: int, scoring: str = "softmax",
+                 normalize: bool = True, scale: float = 1.0, selection_bias: Optional[torch.Tensor] = None, activation: str = "silu"):
+        device = _cuda(gate_up, "gate_up")
+        dtype = gate_up.dtype
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise B200NotSupportedError(f"element type {dtype} is not supported")
+        _on(gate_up, "gate_up", device, dtype, 3)
+        _on(down, "down", device, dtype, 3)
+        _on(router, "router", device, torch.float32 if getattr(router, "dtype", None) is torch.float32 else dtype, 2)
+        experts, wide, width = gate_up.shape
+        inner = wide // 2
+        if wide != 2 * inner or tuple(down.shape) != (experts, width, inner) or tuple(router.shape) != (experts, width):
+            _bad(f"router, gate_up and down must be [experts, width], [experts, 2 * inner, width] and [experts, width, inner], got "
+                 f"{tuple(router.shape)}, {tuple(gate_up.shape)} and {tuple(down.shape)}")
+        for name, p in (("router", router), ("gate_up", gate_up), ("down", down)):
+            if p.stride(-1) != 1 and p.shape[-1] > 1:
+                _bad(f"{name} must be contiguous along its last dimension")
+        if scoring not in ("softmax", "sigmoid"):
+            _bad(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+        if activation not in ("silu", "gelu"):
+            _bad(f"activation must be 'silu' or 'gelu', got {activation!r}")
+        bias = _vector(selection_bias, "selection_bias", device, (torch.float32,), experts)[0]
+        self.router, self.gate_up, self.down, self.selection_bias = router, gate_up, down, selection_bias
+        self.device, self.dtype, self.experts, self.width, self.inner, self.top_k = device, dtype, experts, width, inner, int(top_k)
+        self._c = _native.MoEWeights(router.data_ptr(), gate_up.data_ptr(), down.data_ptr(), bias, router.stride(0), gate_up.stride(0),
+                                     gate_up.stride(1), down.stride(0), down.stride(1), experts, width, inner, _ELEM[dtype],
+                                     _ELEM[router.dtype], self.top_k, int(scoring == "sigmoid"), int(bool(normalize)),
+                                     int(activation == "gelu"), float(scale))
+        self._ref = C.byref(self._c)
+        self._space = {}
+        self._workspace(1)   # refuses what the layer does not support
+
+    def _workspace(self, tokens: int) -> int:
+        n = self._space.get(tokens)
+        if n is None:
+            size = C.c_size_t()
+            _check(_native.lib().sb_moe_workspace(self._ref, tokens, C.byref(size)))
+            if len(self._space) > 64:
+                self._space.clear()
+            n = self._space[tokens] = size.value
+        return n
+
+
+def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The mixture-of-experts layer of x [tokens, width], of the weights' type: for each token the sum over its
+    experts of share * down (act(gate x) * (up x)). Meant for few tokens: an expert's weights are read once for every
+    32 of its tokens. Hidden values are rounded to the weights' type. ``out`` may be x itself. A cooperative launch."""
+    if not isinstance(weights, MoEWeights):
+        _bad("weights must be MoEWeights")
+    for name in ("router", "gate_up", "down"):   # since the object was made, or made without recording
+        if _derived(getattr(weights, name)):
+            raise B200NotSupportedError(f"{name} requires a gradient or has a tangent, which these operators do not record")
+    device, dtype = weights.device, weights.dtype
+    tokens, xs = _matrix(x, "x", device, dtype, None, weights.width)
+    out = torch.empty((tokens, weights.width), dtype=dtype, device=device) if out is None else out
+    ys = _matrix(out, "out", device, dtype, tokens, weights.width)[1]
+    n = weights._workspace(tokens)
+    space = torch.empty(n, dtype=torch.uint8, device=device)
+    _call("sb_moe", device, weights._ref, x.data_ptr(), xs, out.data_ptr(), ys, tokens, space.data_ptr(), n)
+    return out
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The next token of each row of logits [rows, vocab] (float32, float16, bfloat16; NaN counts as -inf), int64
+    [rows], from the row's number in ``uniform`` (float32 [rows], in [0, 1)). With w = exp((l - max) / temperature),
+    kept are w >= min_p, of these the top_k largest, of these the fewest largest whose sum is at least top_p of theirs
+    (equal logits: the lower index first); the token is the first index at which the running sum of the kept w, in order
+    of the index, exceeds uniform times their sum. Each setting is a number or a tensor of one per row (float32, top_k
+    int32). Temperature 0 (or less): the first of the largest; top_k 0 (or less), top_p 1 (or more) and min_p 0 (or
+    less) filter nothing. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0."""
+    device = _cuda(logits, "logits")
+    dtype = logits.dtype
+    elem = _ELEM.get(dtype)
+    if elem is None:
+        raise B200NotSupportedError(f"element type {dtype} is not supported")
+    rows, stride = _matrix(logits, "logits", device, dtype, None, None)
+    at = _vector(uniform, "uniform", device, (torch.float32,), rows)[0]
+    by = _native.Sampling()
+    if isinstance(temperature, torch.Tensor):
+        by.temperature_of = _vector(temperature, "temperature", device, (torch.float32,), rows)[0]
+    else:
+        by.temperature = temperature
+    if isinstance(top_k, torch.Tensor):
+        by.top_k_of = _vector(top_k, "top_k", device, (torch.int32,), rows)[0]
+    else:
+        by.top_k = min(max(int(top_k), 0), 0x7fffffff)
+    if isinstance(top_p, torch.Tensor):
+        by.top_p_of = _vector(top_p, "top_p", device, (torch.float32,), rows)[0]
+    else:
+        by.top_p = top_p
+    if isinstance(min_p, torch.Tensor):
+        by.min_p_of = _vector(min_p, "min_p", device, (torch.float32,), rows)[0]
+    else:
+        by.min_p = min_p
+    out = torch.empty(rows, dtype=torch.int64, device=device) if out is None else out
+    _call("sb_sample", device, logits.data_ptr(), stride, elem, rows, logits.shape[1], at, C.byref(by),
+          _vector(out, "out", device, (torch.int64,), rows)[0])
+    return out
