@@ -6,8 +6,15 @@
 // bandwidth bounds many rows, and the chain load, sums, store a single one. y is taken of h before h is
 // rounded to its type. The variance of a layer norm is the mean square of differences from the mean, in a
 // second sum over the registers: the difference of two large sums would lose it where the mean is large.
+//
+// Threads take pieces of 8 elements that begin where memory has 16-byte boundaries: with a row that begins s elements
+// behind one, the first piece has s elements before the row, which count as none. Rows of an odd width so come in wide
+// accesses too (element by element, 11001 in fp16 with a residual in fp32, 777 rows took 95 us); only the weights, which lie
+// otherwise, are shifted into place. Tensors whose rows begin unlike each other go element by element.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "decoder.h"
 
@@ -24,22 +31,129 @@ template <> __device__ __forceinline__ float narrow(float x) { return x; }
 template <> __device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
 
-// V elements as they lie in memory: 16-byte accesses for V = 8, single elements for V = 1
-template <typename T, int V> struct alignas(V == 8 ? 16 : sizeof(T)) Piece { T e[V]; };
+// Words of two 16-bit elements or one of 32 bits
+template <typename T> __device__ __forceinline__ float2 unpack(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-template <int V> __device__ __forceinline__ void load_vector(float (&to)[V], const void* p, int64_t at, int elem, float add) {
-  if (elem == 1) {
-    const Piece<float, V> v = *reinterpret_cast<const Piece<float, V>*>(static_cast<const float*>(p) + at);
+// V elements as they lie in memory: 16-byte accesses for V = 8, single elements for V = 1
+template <typename T, int V> struct alignas(V == 8 ? 16 : sizeof(T)) Piece {
+  T e[V];
+  __device__ __forceinline__ void widened(float (&z)[V]) const {
+    if constexpr (V == 8 && sizeof(T) == 2) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(e);
 #pragma unroll
-    for (int e = 0; e < V; ++e) to[e] = v.e[e] + add;
-  } else if (elem == 10) {
-    const Piece<__half, V> v = *reinterpret_cast<const Piece<__half, V>*>(static_cast<const __half*>(p) + at);
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack<T>(w[i]);
+        z[2 * i] = f.x, z[2 * i + 1] = f.y;
+      }
+    } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) to[e] = __half2float(v.e[e]) + add;
+      for (int i = 0; i < V; ++i) z[i] = widen<T>(e[i]);
+    }
+  }
+  __device__ __forceinline__ void narrowed(const float (&z)[V]) {
+    if constexpr (V == 8 && sizeof(T) == 2) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = pack<T>(z[2 * i], z[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = narrow<T>(z[i]);
+    }
+  }
+};
+
+// Which of a piece's elements are in the row: `at` is the index of its first, below the width. Without edges, pieces
+// begin with the row and the width is a whole number of them.
+template <int V, bool kEdges> __device__ __forceinline__ bool whole(int at, int width) { return V == 1 || !kEdges || (at >= 0 && at + V <= width); }
+__device__ __forceinline__ bool inside(int i, int width) { return i >= 0 && i < width; }
+
+// (Not inline: code that only a row's first and last piece run, at every access.)
+template <typename T> __device__ __noinline__ Piece<T, 8> load_part(const T* row, int at, int width) {
+  Piece<T, 8> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v.e[e] = inside(at + e, width) ? row[at + e] : narrow<T>(0.f);
+  return v;
+}
+template <typename T> __device__ __noinline__ void store_part(T* row, int at, int width, Piece<T, 8> v) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (inside(at + e, width)) row[at + e] = v.e[e];
+}
+template <typename T, int V, bool kEdges> __device__ __forceinline__ Piece<T, V> load(const T* row, int at, int width) {
+  if constexpr (V == 8 && kEdges)
+    if (!whole<V, kEdges>(at, width)) return load_part<T>(row, at, width);
+  return *reinterpret_cast<const Piece<T, V>*>(row + at);
+}
+template <typename T, int V, bool kEdges> __device__ __forceinline__ void store(T* row, int at, int width, const float (&z)[V]) {
+  Piece<T, V> v;
+  v.narrowed(z);
+  if constexpr (V == 8 && kEdges)
+    if (!whole<V, kEdges>(at, width)) return store_part<T>(row, at, width, v);
+  *reinterpret_cast<Piece<T, V>*>(row + at) = v;
+}
+
+// A piece of weights, which are aligned as a whole, from any element: `skip` elements into the 16 from the boundary
+// before it. (Read-only loads: they need not wait for the stores before them.)
+template <typename W> __device__ __forceinline__ Piece<W, 8> shifted(const W* p, int skip) {
+  Piece<W, 8> v;
+  uint32_t* w = reinterpret_cast<uint32_t*>(v.e);
+  auto words = [](uint32_t* to, const W* from, int n) {
+#pragma unroll
+    for (int i = 0; i < n; i += 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(from) + i / 4);
+      to[i] = q.x, to[i + 1] = q.y, to[i + 2] = q.z, to[i + 3] = q.w;
+    }
+  };
+  if constexpr (sizeof(W) == 4) {
+    if (skip % 4 == 0) {
+      words(w, p, 8);
+    } else {
+      uint32_t x[12];
+      words(x, p - skip % 4, 12);
+#pragma unroll
+      for (int e = 0; e < 10; ++e) x[e] = skip & 2 ? x[e + 2] : x[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = skip & 1 ? x[e + 1] : x[e];
+    }
   } else {
-    const Piece<__nv_bfloat16, V> v = *reinterpret_cast<const Piece<__nv_bfloat16, V>*>(static_cast<const __nv_bfloat16*>(p) + at);
+    if (skip == 0) {
+      words(w, p, 4);
+    } else {
+      uint32_t x[8];
+      words(x, p - skip, 8);
 #pragma unroll
-    for (int e = 0; e < V; ++e) to[e] = __bfloat162float(v.e[e]) + add;
+      for (int i = 0; i < 6; ++i) x[i] = skip & 4 ? x[i + 2] : x[i];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) x[i] = skip & 2 ? x[i + 1] : x[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(x[i], x[i + 1], (skip & 1) * 16);
+    }
+  }
+  return v;
+}
+template <typename W, int V, bool kEdges> __device__ __forceinline__ void weights(float (&to)[V], const void* p, int at, int width) {
+  const W* w = static_cast<const W*>(p);
+  if constexpr (V == 1) {
+    to[0] = widen<W>(__ldg(w + at));
+  } else if constexpr (!kEdges) {
+    shifted<W>(w + at, 0).widened(to);
+  } else {
+    const int skip = at & 7;
+    if (at >= skip && at + (skip ? 16 - skip : 8) <= width) shifted<W>(w + at, skip).widened(to);
+    else load_part<W>(w, at, width).widened(to);
   }
 }
 
@@ -64,144 +178,286 @@ template <bool kWarp> struct Row {
   }
 };
 
-// Mean to subtract and factor to multiply by, of the row's values; those past the width are 0.
-template <int V, int P, bool kWarp>
-__device__ __forceinline__ float2 moments(const float (&z)[P][V], const ResidualNormArgs& a, Row<kWarp>& row, int tid, int stride) {
-  float mean = 0.f;
+// Mean to subtract and factor to multiply by, of the row's values; those outside it are 0.
+template <int V, int P, bool kEdges, bool kWarp>
+__device__ __forceinline__ float2 moments(const float (&z)[P][V], const ResidualNormArgs& a, Row<kWarp>& row, int first, int stride) {
+  float mean = 0.f, s = 0.f;
   if (a.layer) {
-    float s = 0.f;
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < V; ++e) s += z[p][e];
     mean = row.sum(s) * a.per_width;
-  }
-  float s = 0.f;
+    s = 0.f;
 #pragma unroll
-  for (int p = 0; p < P; ++p)
-    if ((tid + p * stride) * V < a.width) {
+    for (int p = 0; p < P; ++p) {
+      const int at = first + p * stride;
+      if (at >= a.width) continue;
+      if (whole<V, kEdges>(at, a.width)) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s += (z[p][e] - mean) * (z[p][e] - mean);
+        for (int e = 0; e < V; ++e) s += (z[p][e] - mean) * (z[p][e] - mean);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (inside(at + e, a.width)) s += (z[p][e] - mean) * (z[p][e] - mean);
+      }
     }
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += z[p][e] * z[p][e];
+  }
   return make_float2(mean, rsqrtf(row.sum(s) * a.per_width + a.eps));
 }
 
-// P pieces of V elements per thread; S: the type of residual and sum; kMost: threads of a row, at most. 32: a row per
-// warp, else per CTA.
-template <typename T, typename S, int V, int P, int kMost>
+// z becomes (z - mean) factor w + b; elements outside the row stay 0.
+template <typename W, int V, int P, bool kEdges>
+__device__ __forceinline__ void apply(float (&z)[P][V], float2 c, const void* w, const void* b, const ResidualNormArgs& a, int first, int stride) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int at = first + p * stride;
+    if (at >= a.width) continue;
+    float f[V], g[V];
+    weights<W, V, kEdges>(f, w, at, a.width);
+    if (b) weights<W, V, kEdges>(g, b, at, a.width);
+    if (a.layer) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] -= c.x;
+    }
+    if (a.offset != 0.f) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = whole<V, kEdges>(at, a.width) || inside(at + e, a.width) ? f[e] + a.offset : 0.f;
+    }
+    if (b) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] = fmaf(z[p][e] * c.y, f[e], g[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] = z[p][e] * c.y * f[e];
+    }
+  }
+}
+
+// A row from its x in z on; residual and gate come by r(p, at) and g(p, at).
+template <typename T, typename S, typename W, int V, int P, bool kEdges, bool kWarp, typename R, typename G>
+__device__ __forceinline__ void finish(float (&z)[P][V], const ResidualNormArgs& a, int64_t m, Row<kWarp>& row, int first, int stride, R&& r, G&& g) {
+  if (a.post_weight) apply<W, V, P, kEdges>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), a.post_weight, a.post_bias, a, first, stride);
+  S* sum = static_cast<S*>(a.sum) + m * a.ss;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int at = first + p * stride;
+    if (at >= a.width) continue;
+    if (a.scale != 1.f) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] *= a.scale;
+    }
+    float f[V];
+    if (a.gate) {
+      if (a.gs == 0) weights<T, V, kEdges>(f, a.gate, at, a.width);
+      else g(p, at).widened(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] *= f[e];
+    }
+    if (a.residual) {
+      r(p, at).widened(f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[p][e] += f[e];
+    }
+    if (a.sum) store<S, V, kEdges>(sum, at, a.width, z[p]);
+  }
+  if (!a.y) return;
+  apply<W, V, P, kEdges>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), a.weight, a.bias, a, first, stride);
+  T* y = static_cast<T*>(a.y) + m * a.ys;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int at = first + p * stride;
+    if (at < a.width) store<T, V, kEdges>(y, at, a.width, z[p]);
+  }
+}
+
+// Elements of row m before its first 16-byte boundary: -at of the first piece.
+template <typename T, bool kEdges> __device__ __forceinline__ int overhang(const ResidualNormArgs& a, int64_t m) {
+  constexpr int kEach = 16 / sizeof(T);
+  return !kEdges ? 0 : int(reinterpret_cast<uintptr_t>(static_cast<const T*>(a.x) + m * a.xs) / sizeof(T) % kEach);
+}
+
+// Few rows, or short ones. P pieces of V elements per thread; S: the type of residual and sum; W: of the weights; kMost:
+// threads of a row, at most. 32: a row per warp, else per CTA.
+template <typename T, typename S, typename W, int V, int P, bool kEdges, int kMost>
 __global__ void __launch_bounds__(kMost == 32 ? 128 : kMost) residual_norm_kernel(const ResidualNormArgs a) {
   constexpr bool kWarp = kMost == 32;
   __shared__ float slots[kWarp ? 1 : 64];
   Row<kWarp> row{slots};
-  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, stride = kWarp ? 32 : blockDim.x;
+  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x, stride = (kWarp ? 32 : blockDim.x) * V;
   const int64_t m = kWarp ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (m >= a.rows) return;   // whole warps
-  using PT = Piece<T, V>;
-  using PS = Piece<S, V>;
-  PT x[P], g[P];
-  PS r[P];
+  const int first = tid * V - overhang<T, kEdges>(a, m);
+  Piece<T, V> g[P];
+  Piece<S, V> r[P];
   float z[P][V];
-  const T* xr = static_cast<const T*>(a.x) + m * a.xs;
-  const S* rr = static_cast<const S*>(a.residual) + m * a.rs;
-  const T* gr = static_cast<const T*>(a.gate) + m * a.gs;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = (tid + p * stride) * V;
-    if (at >= a.width) continue;
-    x[p] = *reinterpret_cast<const PT*>(xr + at);
-    if (a.residual) r[p] = *reinterpret_cast<const PS*>(rr + at);
-    if (a.gate) g[p] = *reinterpret_cast<const PT*>(gr + at);
-  }
-#pragma unroll
-  for (int p = 0; p < P; ++p)
-#pragma unroll
-    for (int e = 0; e < V; ++e) z[p][e] = (tid + p * stride) * V < a.width ? widen<T>(x[p].e[e]) : 0.f;
-  if (a.post_weight) {
-    const float2 c = moments<V, P, kWarp>(z, a, row, tid, stride);
+  {
+    Piece<T, V> x[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const int at = (tid + p * stride) * V;
+      const int at = first + p * stride;
       if (at >= a.width) continue;
-      float w[V], b[V];
-      load_vector<V>(w, a.post_weight, at, a.weight_elem, a.offset);
-      if (a.post_bias) load_vector<V>(b, a.post_bias, at, a.weight_elem, 0.f);
+      x[p] = load<T, V, kEdges>(static_cast<const T*>(a.x) + m * a.xs, at, a.width);
+      if (a.residual) r[p] = load<S, V, kEdges>(static_cast<const S*>(a.residual) + m * a.rs, at, a.width);
+      if (a.gate && a.gs != 0) g[p] = load<T, V, kEdges>(static_cast<const T*>(a.gate) + m * a.gs, at, a.width);
+    }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        z[p][e] = (z[p][e] - c.x) * c.y * w[e];
-        if (a.post_bias) z[p][e] += b[e];
+    for (int p = 0; p < P; ++p) {
+      if (first + p * stride < a.width) {
+        x[p].widened(z[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[p][e] = 0.f;
       }
     }
   }
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = (tid + p * stride) * V;
-    if (at >= a.width) continue;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float v = z[p][e] * a.scale;
-      if (a.gate) v *= widen<T>(g[p].e[e]);
-      z[p][e] = a.residual ? widen<S>(r[p].e[e]) + v : v;
-    }
-    if (a.sum) {
-      PS h;
-#pragma unroll
-      for (int e = 0; e < V; ++e) h.e[e] = narrow<S>(z[p][e]);
-      *reinterpret_cast<PS*>(static_cast<S*>(a.sum) + m * a.ss + at) = h;
-    }
-  }
-  if (!a.y) return;
-  const float2 c = moments<V, P, kWarp>(z, a, row, tid, stride);
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int at = (tid + p * stride) * V;
-    if (at >= a.width) continue;
-    float w[V], b[V];
-    load_vector<V>(w, a.weight, at, a.weight_elem, a.offset);
-    if (a.bias) load_vector<V>(b, a.bias, at, a.weight_elem, 0.f);
-    PT y;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float v = (z[p][e] - c.x) * c.y * w[e];
-      y.e[e] = narrow<T>(a.bias ? v + b[e] : v);
-    }
-    *reinterpret_cast<PT*>(static_cast<T*>(a.y) + m * a.ys + at) = y;
+  finish<T, S, W, V, P, kEdges, kWarp>(z, a, m, row, first, stride, [&](int p, int) { return r[p]; }, [&](int p, int) { return g[p]; });
+}
+
+// Many rows: CTAs that stay and take every gridDim.x-th row, whose inputs arrive in shared memory (cp.async, a ring of
+// rows) while the rows before are computed. A row comes as the 16-byte pieces of memory that it lies in (the bytes before
+// it in the first piece are of the same allocation, those behind it are not read).
+__device__ __forceinline__ void copy_row(uint8_t* to, const uint8_t* from, int bytes, int tid, int threads) {
+  const int head = int(reinterpret_cast<uintptr_t>(from) % 16);
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  for (int q = tid * 16; q < head + bytes; q += threads * 16) {
+    const int n = min(16, head + bytes - q);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + q), "l"(from - head + q), "r"(n) : "memory");
   }
 }
 
-template <typename T, typename S, int V, int P>
-void start(const ResidualNormArgs& a, int threads, cudaStream_t s) {
+struct RowRing {
+  int stages, r, g, bytes;   // offsets of residual and gate in a stage, and a stage's bytes
+};
+
+template <typename T, typename S, typename W, int P, bool kEdges, int kMost, int kCtas>
+__global__ void __launch_bounds__(kMost, kCtas) residual_norm_stream(const ResidualNormArgs a, const RowRing ring) {
+  constexpr int V = 8;
+  extern __shared__ __align__(16) uint8_t held[];
+  __shared__ float slots[64];
+  Row<false> row{slots};
+  const int tid = threadIdx.x, stride = blockDim.x * V;
+  const bool gates = a.gate && a.gs != 0;   // rows of them
+  auto row_of = [](const void* p, int64_t m, int64_t s, int size) { return static_cast<const uint8_t*>(p) + m * s * size; };
+  auto copy = [&](int64_t m, int stage) {
+    if (m < a.rows) {
+      uint8_t* to = held + stage * ring.bytes;
+      copy_row(to, row_of(a.x, m, a.xs, sizeof(T)), a.width * int(sizeof(T)), tid, blockDim.x);
+      if (a.residual) copy_row(to + ring.r, row_of(a.residual, m, a.rs, sizeof(S)), a.width * int(sizeof(S)), tid, blockDim.x);
+      if (gates) copy_row(to + ring.g, row_of(a.gate, m, a.gs, sizeof(T)), a.width * int(sizeof(T)), tid, blockDim.x);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int i = 0; i < ring.stages - 1; ++i) copy(blockIdx.x + int64_t(i) * gridDim.x, i);
+  int in = ring.stages - 1, out = 0;
+  for (int64_t m = blockIdx.x; m < a.rows; m += gridDim.x) {
+    if (ring.stages == 2) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (ring.stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+    __syncthreads();   // the row is there, and the one before it done with
+    copy(m + int64_t(ring.stages - 1) * gridDim.x, in);
+    in = in + 1 == ring.stages ? 0 : in + 1;
+    const uint8_t* from = held + out * ring.bytes;
+    out = out + 1 == ring.stages ? 0 : out + 1;
+    auto begin = [](const uint8_t* p) { return int(reinterpret_cast<uintptr_t>(p) % 16); };
+    const T* x = reinterpret_cast<const T*>(from + begin(row_of(a.x, m, a.xs, sizeof(T))));
+    const S* r = reinterpret_cast<const S*>(from + ring.r + begin(row_of(a.residual, m, a.rs, sizeof(S))));
+    const T* g = reinterpret_cast<const T*>(from + ring.g + begin(row_of(a.gate, m, a.gs, sizeof(T))));
+    const int first = tid * V - overhang<T, kEdges>(a, m);
+    float z[P][V];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int at = first + p * stride;
+      if (at < a.width) {
+        load<T, V, kEdges>(x, at, a.width).widened(z[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) z[p][e] = 0.f;
+      }
+    }
+    finish<T, S, W, V, P, kEdges, false>(z, a, m, row, first, stride, [&](int, int at) { return load<S, V, kEdges>(r, at, a.width); },
+                                         [&](int, int at) { return load<T, V, kEdges>(g, at, a.width); });
+  }
+}
+
+template <typename T, typename S, typename W, int P, bool kEdges, int kMost, int kCtas>
+cudaError_t stream(const ResidualNormArgs& a, RowRing ring, int threads, int ctas, int sms, cudaStream_t s) {
+  const auto kernel = residual_norm_stream<T, S, W, P, kEdges, kMost, kCtas>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  if (e != cudaSuccess) return e;
+  const int64_t grid = std::min<int64_t>(a.rows, int64_t(ctas) * sms);
+  kernel<<<unsigned(grid), threads, size_t(ring.stages) * ring.bytes, s>>>(a, ring);
+  return cudaGetLastError();
+}
+
+template <typename T, typename S, typename W, int V, int P, bool kEdges>
+cudaError_t start(const ResidualNormArgs& a, int threads, cudaStream_t s) {
   if (threads == 32) {
     constexpr int kRows = 4;   // of a CTA
-    residual_norm_kernel<T, S, V, P, 32><<<unsigned((a.rows + kRows - 1) / kRows), 32 * kRows, 0, s>>>(a);
+    residual_norm_kernel<T, S, W, V, P, kEdges, 32><<<unsigned((a.rows + kRows - 1) / kRows), 32 * kRows, 0, s>>>(a);
   } else if (threads <= 256) {
-    residual_norm_kernel<T, S, V, P, 256><<<unsigned(a.rows), threads, 0, s>>>(a);
+    residual_norm_kernel<T, S, W, V, P, kEdges, 256><<<unsigned(a.rows), threads, 0, s>>>(a);
   } else {
-    residual_norm_kernel<T, S, V, P, 1024><<<unsigned(a.rows), threads, 0, s>>>(a);
-  }
-}
-
-template <typename T, typename S>
-cudaError_t launch(const ResidualNormArgs& a, bool wide, int sms, cudaStream_t s) {
-  const int v = wide ? 8 : 1;
-  const int pieces = (a.width + v - 1) / v;
-  // Pieces per thread: with rows for every SM, four 16-byte pieces (or 16 elements), so that a row takes few
-  // warps; otherwise one (four), so that it takes many.
-  const bool many = a.rows >= 2 * int64_t(sms);
-  int each = wide ? (many ? 4 : 1) : (many ? 16 : 4);
-  const int most = wide ? 4 : 32;
-  while (each < most && pieces > 1024 * each) each *= 2;
-  int threads = 32;
-  while (threads < 1024 && threads * each < pieces) threads *= 2;
-  if (wide) {
-    if (each == 1) start<T, S, 8, 1>(a, threads, s);
-    else if (each == 2) start<T, S, 8, 2>(a, threads, s);
-    else start<T, S, 8, 4>(a, threads, s);
-  } else {
-    if (each == 4) start<T, S, 1, 4>(a, threads, s);
-    else if (each <= 16) start<T, S, 1, 16>(a, threads, s);
-    else start<T, S, 1, 32>(a, threads, s);
+    residual_norm_kernel<T, S, W, V, P, kEdges, 1024><<<unsigned(a.rows), threads, 0, s>>>(a);
   }
   return cudaGetLastError();
+}
+
+// Pieces of 8 elements, or single ones where rows begin unlike each other.
+template <typename T, typename S, typename W, bool kEdges>
+cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
+  const int pieces = (a.width + 7) / 8 + (kEdges ? 1 : 0);
+  // Many rows of 1024 elements or more: two pieces per thread (4099 rows of 4096 in bf16 with both norms and a gate: 41 us,
+  // one piece 45, four 47; without the ring 97). Shorter rows go a warp each without it (12608 of 768 in fp32: 36 us, 39 with).
+  constexpr int kEach = 2;
+  RowRing ring;
+  const int pad = kEdges ? 32 : 0;   // a row that begins and ends inside a piece
+  auto up = [](int n) { return (n + 15) / 16 * 16; };
+  ring.r = up(a.width * int(sizeof(T))) + pad;
+  ring.g = ring.r + (a.residual ? up(a.width * int(sizeof(S))) + pad : 0);
+  ring.bytes = ring.g + (a.gate && a.gs != 0 ? up(a.width * int(sizeof(T))) + pad : 0);
+  int threads = 128;
+  while (threads * kEach < pieces) threads *= 2;
+  const int kRing = 216 * 1024;
+  const int ctas = std::min(1024 / threads, kRing / (2 * ring.bytes));
+  if (pieces >= 128 && threads <= 1024 && ctas > 0 && a.rows >= 2 * int64_t(ctas) * sms) {
+    ring.stages = std::min(4, kRing / (ctas * ring.bytes));
+    if (threads <= 256) return stream<T, S, W, kEach, kEdges, 256, 4>(a, ring, threads, ctas, sms, s);
+    return stream<T, S, W, kEach, kEdges, 1024, 1>(a, ring, threads, ctas, sms, s);
+  }
+  // Pieces per thread: with rows for every SM four, so that a row takes few warps; otherwise one, so that it takes many.
+  int each = a.rows >= 2 * int64_t(sms) || pieces > 1024 ? 4 : 1;
+  threads = 32;
+  while (threads < 1024 && threads * each < pieces) threads *= 2;
+  if (each == 1) return start<T, S, W, 8, 1, kEdges>(a, threads, s);
+  if (kEdges && pieces > 4096) return start<T, S, W, 8, 5, kEdges>(a, threads, s);   // 32768 elements and an overhang
+  return start<T, S, W, 8, 4, kEdges>(a, threads, s);
+}
+
+template <typename T, typename S, typename W>
+cudaError_t launch_single(const ResidualNormArgs& a, int sms, cudaStream_t s) {
+  const int each = a.width > 16384 ? 32 : a.rows >= 2 * int64_t(sms) || a.width > 4096 ? 16 : 4;
+  int threads = 32;
+  while (threads < 1024 && threads * each < a.width) threads *= 2;
+  if (each == 4) return start<T, S, W, 1, 4, false>(a, threads, s);
+  if (each == 16) return start<T, S, W, 1, 16, false>(a, threads, s);
+  return start<T, S, W, 1, 32, false>(a, threads, s);
+}
+
+enum Form { kSingle, kPieces, kWithEdges };
+template <typename T, typename S, typename W>
+cudaError_t launch_form(const ResidualNormArgs& a, Form form, int sms, cudaStream_t s) {
+  if (form == kPieces) return launch_wide<T, S, W, false>(a, sms, s);
+  return form == kWithEdges ? launch_wide<T, S, W, true>(a, sms, s) : launch_single<T, S, W>(a, sms, s);
+}
+template <typename T, typename S>
+cudaError_t launch(const ResidualNormArgs& a, Form form, int sms, cudaStream_t s) {
+  return a.weight_elem == 1 ? launch_form<T, S, float>(a, form, sms, s) : launch_form<T, S, T>(a, form, sms, s);
 }
 
 }  // namespace
@@ -209,16 +465,21 @@ cudaError_t launch(const ResidualNormArgs& a, bool wide, int sms, cudaStream_t s
 cudaError_t residual_norm(const ResidualNormArgs& args, int elem, int sum_elem, int sms, cudaStream_t s) {
   ResidualNormArgs a = args;
   a.per_width = 1.f / float(a.width);
-  // 16-byte pieces: 8 elements, of each row, of whatever type
-  auto fits = [&](const void* p, int64_t stride) {
-    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride % 8 == 0 || a.rows == 1));
+  // Rows begin alike, in elements from a 16-byte boundary: 8 elements apart for the 16-bit types, 4 for 32-bit ones.
+  const int per = elem == 1 ? 4 : 8, sum_per = sum_elem == 1 ? 4 : 8;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x) / (16 / per);
+  auto alike = [&](const void* p, int64_t stride, int n) {
+    return p == nullptr || ((reinterpret_cast<uintptr_t>(p) / (16 / n) - begin) % n == 0 && (a.rows == 1 || (stride - a.xs) % n == 0));
   };
-  const bool wide = a.width % 8 == 0 && fits(a.x, a.xs) && fits(a.residual, a.rs) && fits(a.sum, a.ss) &&
-                    fits(a.y, a.ys) && fits(a.gate, a.gs) && fits(a.weight, 0) && fits(a.bias, 0) &&
-                    fits(a.post_weight, 0) && fits(a.post_bias, 0);
-  if (elem == 1) return launch<float, float>(a, wide, sms, s);
-  if (elem == 10) return sum_elem == 1 ? launch<__half, float>(a, wide, sms, s) : launch<__half, __half>(a, wide, sms, s);
-  return sum_elem == 1 ? launch<__nv_bfloat16, float>(a, wide, sms, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, wide, sms, s);
+  auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool wide = alike(a.residual, a.rs, sum_per) && alike(a.sum, a.ss, sum_per) && alike(a.y, a.ys, per) &&
+                    (a.gs == 0 ? whole(a.gate) : alike(a.gate, a.gs, per)) && whole(a.weight) && whole(a.bias) && whole(a.post_weight) &&
+                    whole(a.post_bias);
+  const bool edges = a.width % 8 != 0 || begin % per != 0 || (a.rows > 1 && a.xs % per != 0);
+  const Form form = !wide ? kSingle : edges ? kWithEdges : kPieces;
+  if (elem == 1) return launch_form<float, float, float>(a, form, sms, s);
+  if (elem == 10) return sum_elem == 1 ? launch<__half, float>(a, form, sms, s) : launch<__half, __half>(a, form, sms, s);
+  return sum_elem == 1 ? launch<__nv_bfloat16, float>(a, form, sms, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, form, sms, s);
 }
 
 }  // namespace k

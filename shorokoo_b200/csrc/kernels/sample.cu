@@ -7,13 +7,14 @@
 // CTAs that hold its slices in shared memory: the logits are read from memory once, whatever the passes, and a few
 // rows still spread over the card.
 //
-// Weights are integers, 2^40 exp(.) in 64 bits from an exponential in fp64: their sums do not depend on an order, so that
-// results repeat and all CTAs of a cluster come to the same decisions, and are off by 2^-41 of the largest weight per
-// token. In fp32 the sums would be off by about as much as the gap between neighbours of a flat row.
+// Weights are integers, exp(.) in units of 2^-40 in 64 bits: their sums do not depend on an order, so that results repeat and
+// all CTAs of a cluster come to the same decisions. They are off by about 2^-30 of themselves; from fp32 arithmetic the
+// sums of a flat row of 10^5 tokens would be off by 10^-4 to 10^-3 of a token, and so would the choice.
 //
 // The filters keep what lies above a border in (logit, index). It is found without sorting: a histogram of 512 bins over
 // the range that holds it, of counts for top_k and of weights for top_p, then over the border's bin alone, until that is one
-// logit: bins of equal width in the logit first (even for what a model gives), of equal numbers of floats afterwards.
+// logit: bins of equal width in the logit first (even for what a model gives), of equal numbers of floats afterwards. The
+// first bin's candidates are listed, and later rounds go over the list.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,12 +29,19 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = kThreads;         // one thread merges and scans one bin
+#ifndef ST
+#define ST 256
+#define SB 4
+#define SK 64
+#endif
+constexpr int kThreads = ST, kWarps = kThreads / 32;
+constexpr int kBins = 256;
 constexpr int kMostCtas = 8;            // of a cluster
-constexpr int kHeld = 200 * 1024;       // bytes of a slice that fit shared memory
-constexpr int kMostRounds = 6;          // 512 bins, then at least 256 each of what is left of 2^32 floats
-constexpr double kOne = 1099511627776.0;   // 2^40: the largest weight
+constexpr int kHeld = 192 * 1024;       // bytes of a slice that fit shared memory
+constexpr int kCoarse = 128;            // bins of the first round of weights, per warp
+constexpr int kListBytes = 8192;        // of a list of candidates
+constexpr int kMostRounds = 6;          // 128 or 256 bins, then at least 128 each of what is left of 2^32 floats
+constexpr int kSteps = 64;              // table of 2^(-j / 64)
 
 struct SampleArgs {
   const void* logits;
@@ -48,6 +56,26 @@ template <typename T> __device__ __forceinline__ float value(T x);
 template <> __device__ __forceinline__ float value(float x) { return x; }
 template <> __device__ __forceinline__ float value(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T lowest();   // -inf
+template <> __device__ __forceinline__ float lowest() { return -INFINITY; }
+template <> __device__ __forceinline__ __half lowest() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xff80); }
+
+// The largest of a piece, NaN passed over.
+template <typename T> __device__ __forceinline__ float largest(uint4 v);
+template <> __device__ __forceinline__ float largest<float>(uint4 v) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+template <> __device__ __forceinline__ float largest<__half>(uint4 v) {
+  const __half2* e = reinterpret_cast<const __half2*>(&v);
+  const float2 m = __half22float2(__hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3])));
+  return fmaxf(m.x, m.y);
+}
+template <> __device__ __forceinline__ float largest<__nv_bfloat16>(uint4 v) {
+  const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3])));
+  return fmaxf(m.x, m.y);
+}
 
 // Logits as integers of the same order; NaN below all others, the zeros equal.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -57,47 +85,103 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-struct Shared {   // each CTA's, read by the others of its cluster
-  unsigned long long mass[2][kBins];
-  uint32_t count[2][kBins];
-  float most, least;
+struct alignas(16) Shared {
+  // read by the other CTAs of the cluster; what rounds write anew is there twice and used in turn
+  uint32_t low[2][kBins], high[2][kBins];   // halves of the bins' sums
+  uint32_t least[2], most[2];               // keys of the candidates
+  float top;
+  int lowest;
   unsigned long long warp_mass[kWarps];
   uint32_t warp_ties[kWarps];
   // this CTA's own
-  unsigned long long scan[kWarps];
-  unsigned long long found_above;
-  float found[2][kWarps];
-  uint32_t range[2];
-  int low;
+  uint32_t power[kSteps];                   // 2^(30 - j / 64)
+  uint32_t part_low[kWarps][kCoarse], part_high[kWarps][kCoarse];   // sums of each warp's part of the slice
+  uint4 list[2][kListBytes / 16];
+  int listed[2];
+  unsigned long long scan[2][kWarps];
+  float warp_top[kWarps];
+  // what its first warp found out
+  unsigned long long all, target, above, before, ties_before, tie;
+  double wide_rate;
+  float most_of_row, rate, rate_low;
+  uint32_t lo;
+  int near, outcome, bin, chosen;
 };
 
-// The bins of a range of keys: bin 0 holds the largest.
-struct Bins {
-  uint32_t lo, hi;
-  bool even;      // of equal width in the logit
-  float half, scale;
+constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: sums with it are rounded to integers, in their low bits
+
+// exp((v - top) / T) in units of 2^-40 for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
+// floats, k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms
+// of its series (the next is 2^-34), in integers: off by about 2^-30 of itself, where expf would be off by up to 2^-21
+// (the difference top - v alone by 2^-20) and exp in fp64 takes three times as long.
+__device__ __noinline__ unsigned long long wide_exp(double d, double rate) {   // any finite d and temperature
+  return __double2ull_rn(exp(d * rate) * 1099511627776.0);
+}
+// kShort: v and top have 16 bits, and top - v is as good as exact: what it loses (of logits below 2^-7) is 2^-25 of it.
+template <bool kShort> struct NearWeights {   // temperatures and logits that are floats like others
+  float top, rate, rate_low;   // log2(e) / T
+  const uint32_t* power;
+  __device__ __forceinline__ unsigned long long operator()(float v) const {
+    const float d = top - v;
+    const float y = d * rate;
+    float y_low = fmaf(d, rate_low, fmaf(d, rate, -y));
+    if (!kShort) {
+      const float b = d - top;
+      y_low = fmaf((top - (d - b)) - (v + b), rate, y_low);   // what d lost
+    }
+    const float shifted = fmaf(y, float(kSteps), kMagic);
+    const uint32_t k = __float_as_uint(shifted);
+    const float g = fmaf(shifted - kMagic, -1.f / kSteps, y) + y_low;
+    const float z = g * fmaf(-g, fmaf(-g, 0.0555041087f, 0.240226507f), 0.693147181f);
+    const int zi = int(__float_as_uint(fmaf(z, 536870912.f, kMagic)) - 0x4b400000u);   // in units of 2^-29
+    const uint32_t p = power[k % kSteps];
+    const uint32_t w = p - uint32_t(__mulhi(int(p), zi * 8));
+    return (static_cast<unsigned long long>(w) << 10) >> (k / kSteps & 63);
+  }
+};
+struct FarWeights {   // any others
+  float top;
+  double rate;   // 1 / T
+  __device__ __forceinline__ unsigned long long operator()(float v) const {
+    return v == top ? 1ull << 40 : wide_exp(double(v) - double(top), rate);
+  }
+};
+
+// Bins of equal width in the logit, over a range of floats: 0 holds the largest, n - 1 or n - 2 the least (`start` is a whole
+// number, so that the largest comes to lie within half a bin of 0).
+struct EvenBins {
+  float slope, start;
+  __device__ __forceinline__ bool set(float l, float h, int n) {
+    const float width = 0.5f * h - 0.5f * l;
+    slope = -0.5f * float(n - 2) / width;
+    start = fmaf(-slope, h, kMagic);
+    return width > 0.f && slope < 0.f && slope > -1e30f && fabsf(slope * h) < 1e6f && fabsf(slope * l) < 1e6f;
+  }
+  __device__ __forceinline__ int operator()(float v) const { return int(__float_as_uint(fmaf(v, slope, start)) & 0x3ffu); }
+};
+
+// Bins of a range of keys, of equal numbers of them: 0 holds the largest.
+struct KeyBins {
+  uint32_t hi;
   int shift;
-  __device__ __forceinline__ void set(uint32_t l, uint32_t h, bool by_value) {
-    lo = l, hi = h;
-    half = 0.5f * of_key(h);
-    const float width = half - 0.5f * of_key(l);
-    scale = float(kBins) / width;
-    even = by_value && h - l >= uint32_t(kBins) && width > 0.f && scale < INFINITY && scale > 0.f;
-    shift = max(0, 32 - __clz(h - l) - 9);   // (h - l) >> shift is below 512
+  __device__ __forceinline__ void set(uint32_t l, uint32_t h, int n) {
+    hi = h;
+    shift = max(0, 32 - __clz(h - l) - (31 - __clz(n)));   // (h - l) >> shift is below n, a power of two
   }
-  __device__ __forceinline__ int bin(uint32_t k, float v) const {
-    return even ? min(kBins - 1, int((half - 0.5f * v) * scale)) : int((hi - k) >> shift);
-  }
+  __device__ __forceinline__ int operator()(float v) const { return int((hi - key_of(v)) >> shift); }
 };
 
-template <typename T> struct Slice {
-  const T* p;
-  int count;
-  __device__ __forceinline__ float at(int i) const { return value<T>(p[i]); }
-};
+__device__ __forceinline__ unsigned long long sum_upto(unsigned long long v, int lane) {   // of the lanes up to this one
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long p = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += p;
+  }
+  return v;
+}
 
 template <typename T, bool kHold>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -105,61 +189,71 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / ctas;
 
-  // ---- the slice, its largest and least logit
-  const int begin = min(rank * a.slice, a.vocab);
-  Slice<T> z;
-  z.count = min(a.slice, a.vocab - begin);
+  // ---- the slice, in 16-byte pieces as they lie in memory (the first begins `shift` elements before it), and its largest
+  constexpr int kV = 16 / sizeof(T);
+  const int begin = min(rank * a.slice, a.vocab), count = min(a.slice, a.vocab - begin);
   const T* from = static_cast<const T*>(a.logits) + row * a.stride + begin;
-  float most = -INFINITY, least = INFINITY;
-  {
-    constexpr int kV = 16 / sizeof(T);
-    const int shift = int(reinterpret_cast<uintptr_t>(from) / sizeof(T) % kV);   // kept in shared memory: 16-byte copies
-    T* held = reinterpret_cast<T*>(raw + (sizeof(Shared) + 15) / 16 * 16);
-    z.p = kHold ? held + shift : from;
-    auto see = [&](float v) {
-      if (v > -INFINITY) most = fmaxf(most, v), least = fminf(least, v);   // not NaN
-    };
-    const int pieces = (z.count + shift + kV - 1) / kV;
-#pragma unroll 4
-    for (int q = tid; q < pieces; q += kThreads) {
-      const int i = q * kV - shift;
-      if (i >= 0 && i + kV <= z.count) {
-        const uint4 v = *reinterpret_cast<const uint4*>(from + i);
-        if (kHold) *reinterpret_cast<uint4*>(held + q * kV) = v;
-        const T* e = reinterpret_cast<const T*>(&v);
+  const int shift = int(reinterpret_cast<uintptr_t>(from) / sizeof(T) % kV);
+  const int pieces = (count + shift + kV - 1) / kV;
+  T* held = reinterpret_cast<T*>(raw + sizeof(Shared));   // with -inf before and behind
+  auto fetch = [&](int q) {
+    alignas(16) T e[kV];
+    const int i = q * kV - shift;
+    if (i >= 0 && i + kV <= count) return *reinterpret_cast<const uint4*>(from + i);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) see(value<T>(e[j]));
-      } else {
-        for (int j = max(i, 0); j < min(i + kV, z.count); ++j) {
-          if (kHold) held[shift + j] = from[j];
-          see(value<T>(from[j]));
-        }
-      }
-    }
+    for (int j = 0; j < kV; ++j) e[j] = i + j >= 0 && i + j < count ? from[i + j] : lowest<T>();
+    return *reinterpret_cast<const uint4*>(e);
+  };
+  auto piece = [&](int q) { return kHold ? reinterpret_cast<const uint4*>(held)[q] : fetch(q); };
+  auto at = [&](int i) { return value<T>(kHold ? held[i + shift] : from[i]); };
+  float most = -INFINITY;
+#pragma unroll 4
+  for (int q = tid; q < pieces; q += kThreads) {
+    const uint4 v = fetch(q);
+    if (kHold) reinterpret_cast<uint4*>(held)[q] = v;
+    most = fmaxf(most, largest<T>(v));
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d)), least = fminf(least, __shfl_xor_sync(~0u, least, d));
-  if (lane == 0) s.found[0][warp] = most, s.found[1][warp] = least;
-  for (int i = tid; i < kBins; i += kThreads) s.mass[0][i] = 0, s.count[0][i] = 0;
+  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+  if (lane == 0) s.warp_top[warp] = most;
+  if (tid < kBins) s.low[0][tid] = s.high[0][tid] = 0;
+  if (tid >= kThreads - kSteps) {
+    const int j = tid - (kThreads - kSteps);
+    s.power[j] = __double2uint_rn(exp2(30.0 - j * (1.0 / kSteps)));
+  }
+  if (tid == 0) s.lowest = 0x7fffffff, s.least[0] = ~0u, s.most[0] = 0, s.listed[0] = 0, s.bin = 0, s.above = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) most = fmaxf(most, s.found[0][w]), least = fminf(least, s.found[1][w]);
-    s.most = most, s.least = least, s.low = 0x7fffffff, s.range[0] = s.range[1] = 0;
+  if (warp == 0) {
+    most = lane < kWarps ? s.warp_top[lane] : -INFINITY;
+#pragma unroll
+    for (int d = kWarps / 2; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (lane == 0) s.top = most;
   }
   cluster.sync();
-  most = -INFINITY, least = INFINITY;
-  for (int c = 0; c < ctas; ++c) {
-    const Shared* o = cluster.map_shared_rank(&s, c);
-    most = fmaxf(most, o->most), least = fminf(least, o->least);
-  }
 
   const float temperature = a.by.temperature_of ? a.by.temperature_of[row] : a.by.temperature;
   const float top_p = a.by.top_p_of ? a.by.top_p_of[row] : a.by.top_p;
   const float min_p = a.by.min_p_of ? a.by.min_p_of[row] : a.by.min_p;
   int top_k = a.by.top_k_of ? a.by.top_k_of[row] : a.by.top_k;
   if (top_k <= 0 || top_k > a.vocab) top_k = a.vocab;
-  float u = a.uniform[row];
-  u = u > 0.f ? fminf(u, 1.f) : 0.f;   // NaN: 0
+  if (warp == 0) {
+    most = lane < ctas ? cluster.map_shared_rank(&s, lane)->top : -INFINITY;
+#pragma unroll
+    for (int d = kMostCtas / 2; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (lane == 0) {
+      s.most_of_row = most;
+      const double r = 1.0 / double(temperature), l = r * 1.4426950408889634;
+      s.wide_rate = r, s.rate = float(l), s.rate_low = float(l - double(float(l)));
+      s.near = temperature > 1e-20f && temperature < 1e20f && fabsf(most) < 1e30f;
+      // the least key that counts: weights below are 0 or below min_p
+      double cut = -28.5;   // 2^40 exp(cut) rounds to 0
+      if (min_p > 0.f) cut = fmax(cut, log(double(min_p)));
+      const float v = most < INFINITY ? __double2float_ru(double(most) + double(temperature) * fmin(cut, 0.0)) : most;
+      s.lo = key_of(fmaxf(v, -3.402823466e38f));
+    }
+  }
+  __syncthreads();
+  most = s.most_of_row;
 
   if (most == -INFINITY) {   // nothing to choose from
     if (rank == 0 && tid == 0) a.tokens[row] = -1;
@@ -168,121 +262,221 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
   if (!(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {   // the largest, the first of them
     int low = 0x7fffffff;
-    for (int i = tid; i < z.count; i += kThreads)
-      if (z.at(i) == most) {
-        low = begin + i;
-        break;
-      }
+    for (int q = tid; q < pieces && low == 0x7fffffff; q += kThreads) {
+      const uint4 v = piece(q);
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int j = kV - 1; j >= 0; --j)
+        if (value<T>(e[j]) == most) low = begin + q * kV - shift + j;
+    }
     low = __reduce_min_sync(~0u, low);
-    if (lane == 0) atomicMin(&s.low, low);
+    if (lane == 0) atomicMin(&s.lowest, low);
     cluster.sync();
     if (rank == 0 && tid == 0) {
-      for (int c = 0; c < ctas; ++c) low = min(low, cluster.map_shared_rank(&s, c)->low);
+      for (int c = 0; c < ctas; ++c) low = min(low, cluster.map_shared_rank(&s, c)->lowest);
       a.tokens[row] = low;
     }
     cluster.sync();
     return;
   }
 
-  // ---- weights
-  const double top = most, rate = 1.0 / double(temperature);
-  auto weight = [&](float v) -> unsigned long long {
-    return v == most ? (unsigned long long)kOne : __double2ull_rn(exp((double(v) - top) * rate) * kOne);
-  };
-  uint32_t lo;   // the least key that counts: weights below are 0 or below min_p
-  {
-    double cut = -28.5;   // 2^40 exp(cut) rounds to 0
-    if (min_p > 0.f) cut = fmax(cut, log(double(min_p)));
-    float v = most < INFINITY ? __double2float_ru(top + double(temperature) * fmin(cut, 0.0)) : most;
-    lo = max(key_of(fmaxf(v, -3.402823466e38f)), key_of(least));
-  }
-  const uint32_t hi = key_of(most);
+  const NearWeights<sizeof(T) == 2> near_weight = {most, s.rate, s.rate_low, s.power};
+  const FarWeights far_weight = {most, s.wide_rate};
+  const bool near = s.near;
+  auto weight = [&](float v) { return near ? near_weight(v) : far_weight(v); };
+  const uint32_t lo = s.lo, hi = key_of(most);
 
   // ---- the border: kept are keys above it, and the first `ties` of its own
+  const int part = (pieces + kWarps - 1) / kWarps;   // of a warp, in pieces
+  const int part_begin = warp * part, part_end = min(part_begin + part, pieces);
+  constexpr int kListed = kListBytes / int(sizeof(T));
   uint32_t border = lo;
   unsigned long long ties = a.vocab;
-  int buffer = 0;
-  // The key at which the sums from the top reach a target; sums of counts, or of weights. `among`: (key, ties) of a border
-  // found before, which limits what is summed.
-  auto descend = [&](bool by_mass, unsigned long long target) {
-    Bins bins;
-    bins.set(lo, hi, true);
-    unsigned long long above = 0;
+  int turn = 0;
+  // A first round of weights leaves the parts' sums over its bins: those before `summed` need no second look.
+  bool binned = false, coarse_even = false;
+  int summed = 0;
+  EvenBins coarse;
+  KeyBins coarse_keys;
+  // Finds the key at which the sums from the top reach a target: of counts, or of weights. The ties of a border found
+  // before are not summed one by one, but by their number.
+  auto descend = [&](const bool by_mass, unsigned long long target) {
+    const bool floored = by_mass && ties < (unsigned long long)a.vocab;
     const uint32_t floor = border;
-    const unsigned long long floor_sum = by_mass && ties < (unsigned long long)a.vocab ? ties * weight(of_key(floor)) : 0;
-    const bool floored = by_mass && ties < (unsigned long long)a.vocab;   // its ties are not summed one by one
+    const unsigned long long floor_weight = floored ? weight(of_key(floor)) : 0, floor_sum = floored ? ties * floor_weight : 0;
+    uint32_t low_key = floored ? min(floor + 1, hi) : lo, high_key = hi;   // hi itself where none is above the border
+    const bool none = floored && floor >= hi;
+    unsigned long long above = 0;
+    int list = -1, listed = 0;   // the list that holds the candidates, or the slice does
     for (int round = 0; round < kMostRounds; ++round) {
-      const bool first = round == 0;
-      for (int i = tid; i < z.count; i += kThreads) {
-        const float v = z.at(i);
-        const uint32_t k = key_of(v);
-        if (k < bins.lo || k > bins.hi || (floored && k <= floor)) continue;
-        const int b = bins.bin(k, v);
-        if (by_mass) atomicAdd(&s.mass[buffer][b], weight(v));
-        else atomicAdd(&s.count[buffer][b], 1u);
+      EvenBins even;
+      KeyBins keys;
+      const int bins = round == 0 && by_mass ? kCoarse : kBins;
+      const float low = of_key(low_key), high = of_key(high_key);
+      const bool by_value = even.set(low, high, bins) && round == 0 && near;
+      keys.set(low_key, high_key, bins);
+      // a 64-bit sum in two halves: whoever makes the lower one overflow carries
+      auto add = [&](uint32_t* lower, uint32_t* upper, unsigned long long w) {
+        const uint32_t l = uint32_t(w), old = atomicAdd(lower, l);
+        const uint32_t h = uint32_t(w >> 32) + (old + l < old);
+        if (h) atomicAdd(upper, h);
+      };
+      if (round == 0 && by_mass) {
+        for (int i = tid; i < kWarps * kCoarse; i += kThreads) (&s.part_low[0][0])[i] = 0, (&s.part_high[0][0])[i] = 0;
+        __syncthreads();
+        binned = true, coarse_even = by_value, coarse = even, coarse_keys = keys;
+        auto sums = [&](const auto& bin, const auto& weight) {
+          for (int q = part_begin + lane; q < part_end; q += 32) {
+            const uint4 p = piece(q);
+            const T* e = reinterpret_cast<const T*>(&p);
+            unsigned long long w[kV];
+            int b[kV];
+#pragma unroll
+            for (int j = 0; j < kV; ++j) w[j] = weight(value<T>(e[j])), b[j] = bin(value<T>(e[j]));
+#pragma unroll
+            for (int j = 0; j < kV; ++j)
+              if (value<T>(e[j]) >= low) add(&s.part_low[warp][b[j]], &s.part_high[warp][b[j]], w[j]);
+          }
+        };
+        if (none) {}
+        else if (by_value) sums(even, near_weight);
+        else if (near) sums(keys, near_weight);
+        else sums(keys, far_weight);
+        __syncthreads();
+        if (tid < kCoarse) {
+          unsigned long long n = 0;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) n += s.part_low[w][tid] + (static_cast<unsigned long long>(s.part_high[w][tid]) << 32);
+          s.low[turn][tid] = uint32_t(n), s.high[turn][tid] = uint32_t(n >> 32);
+        }
+      } else {
+        auto count = [&](float v, const auto& bin) {
+          if (!(v >= low && v <= high)) return;
+          const int b = bin(v);
+          if (by_mass) add(&s.low[turn][b], &s.high[turn][b], weight(v));
+          else atomicAdd(&s.low[turn][b], 1u);
+        };
+        auto counts = [&](const auto& bin) {
+          for (int q = tid; q < pieces; q += kThreads) {
+            const uint4 p = piece(q);
+            const T* e = reinterpret_cast<const T*>(&p);
+#pragma unroll
+            for (int j = 0; j < kV; ++j) count(value<T>(e[j]), bin);
+          }
+        };
+        if (list >= 0)
+          for (int i = tid; i < listed; i += kThreads) count(value<T>(reinterpret_cast<const T*>(s.list[list])[i]), keys);
+        else if (by_value) counts(even);
+        else counts(keys);
       }
       cluster.sync();
-      s.mass[buffer ^ 1][tid] = 0, s.count[buffer ^ 1][tid] = 0;
-      unsigned long long n = 0;
+      if (tid < kBins) s.low[turn ^ 1][tid] = s.high[turn ^ 1][tid] = 0;   // all have read it, before this barrier
+      if (tid == 0) s.least[turn ^ 1] = ~0u, s.most[turn ^ 1] = 0, s.listed[turn ^ 1] = 0;
+      if (warp == 0) {   // neighbouring bins per lane
+        unsigned long long n[kBins / 32], sum = 0;
+        const int each = bins / 32;
+#pragma unroll
+        for (int i = 0; i < kBins / 32; ++i) n[i] = 0;
+        for (int c = 0; c < ctas; ++c) {
+          const Shared* o = cluster.map_shared_rank(&s, c);
+#pragma unroll
+          for (int i = 0; i < kBins / 32; i += 4) {
+            if (i >= each) break;
+            const uint4 l = *reinterpret_cast<const uint4*>(o->low[turn] + lane * each + i);
+            n[i] += l.x, n[i + 1] += l.y, n[i + 2] += l.z, n[i + 3] += l.w;
+            if (by_mass) {
+              const uint4 h = *reinterpret_cast<const uint4*>(o->high[turn] + lane * each + i);
+              n[i] += static_cast<unsigned long long>(h.x) << 32, n[i + 1] += static_cast<unsigned long long>(h.y) << 32;
+              n[i + 2] += static_cast<unsigned long long>(h.z) << 32, n[i + 3] += static_cast<unsigned long long>(h.w) << 32;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kBins / 32; ++i) sum += n[i];
+        const unsigned long long upto = sum_upto(sum, lane), all = __shfl_sync(~0u, upto, 31);
+        if (round == 0 && by_mass) target = min(max((unsigned long long)ceil(double(top_p) * double(all + floor_sum)), 1ull), all + floor_sum);
+        const unsigned long long need = target - above;
+        if (lane == 0) s.all = all, s.target = target, s.outcome = round == 0 && (by_mass ? target > all : target >= all);
+        if (upto >= need && upto - sum < need) {
+          unsigned long long before = upto - sum;
+#pragma unroll
+          for (int i = 0; i < kBins / 32; ++i)
+            if (before < need && before + n[i] >= need) {
+              s.bin = lane * each + i, s.above = above + before;
+              before = need;   // found
+            } else {
+              before += n[i];
+            }
+        }
+      }
+      __syncthreads();
+      target = s.target;
+      if (s.outcome) {   // no border among these
+        if (by_mass) {   // but among the ties of the one there is
+          ties = (target - s.all + floor_weight - 1) / floor_weight;
+          summed = bins;
+        }
+        turn ^= 1;
+        return;
+      }
+      above = s.above;
+      const int found = s.bin;
+      if (round == 0) summed = found;
+      // the bin's candidates, and the range of their keys
+      const int next = turn;
+      uint32_t least = ~0u, greatest = 0;
+      auto see = [&](float v) {
+        const uint32_t k = key_of(v);
+        least = min(least, k), greatest = max(greatest, k);
+      };
+      T* to = reinterpret_cast<T*>(s.list[next]);
+      auto take = [&](const auto& bin) {
+        for (int q = tid; q < pieces; q += kThreads) {
+          const uint4 p = piece(q);
+          const T* e = reinterpret_cast<const T*>(&p);
+          uint32_t mine = 0;
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = value<T>(e[j]);
+            if (v >= low && v <= high && bin(v) == found) mine |= 1u << j;
+          }
+          if (mine) {
+            int i = atomicAdd(&s.listed[next], __popc(mine));
+#pragma unroll
+            for (int j = 0; j < kV; ++j)
+              if (mine >> j & 1) {
+                see(value<T>(e[j]));
+                if (i < kListed) to[i] = e[j];
+                ++i;
+              }
+          }
+        }
+      };
+      if (list >= 0) {
+        for (int i = tid; i < listed; i += kThreads) {
+          const T e = reinterpret_cast<const T*>(s.list[list])[i];
+          const float v = value<T>(e);
+          if (v >= low && v <= high && keys(v) == found) see(v), to[atomicAdd(&s.listed[next], 1)] = e;
+        }
+      } else if (by_value) {
+        take(even);
+      } else {
+        take(keys);
+      }
+      least = __reduce_min_sync(~0u, least), greatest = __reduce_max_sync(~0u, greatest);
+      if (lane == 0 && greatest) atomicMin(&s.least[turn], least), atomicMax(&s.most[turn], greatest);
+      cluster.sync();
       for (int c = 0; c < ctas; ++c) {
         const Shared* o = cluster.map_shared_rank(&s, c);
-        n += by_mass ? o->mass[buffer][tid] : o->count[buffer][tid];
+        least = min(least, o->least[turn]), greatest = max(greatest, o->most[turn]);
       }
-      buffer ^= 1;
-      unsigned long long upto = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long before = __shfl_up_sync(~0u, upto, d);
-        if (lane >= d) upto += before;
-      }
-      if (lane == 31) s.scan[warp] = upto;
-      __syncthreads();
-      unsigned long long all = 0, before = 0;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before = all;
-        all += s.scan[w];
-      }
-      upto += before;
-      if (first && by_mass) {
-        const double part = double(top_p) * double(all + floor_sum);
-        target = min(max((unsigned long long)ceil(part), 1ull), all + floor_sum);
-        if (target > all) {   // among the ties of the border there is
-          ties = (target - all + weight(of_key(floor)) - 1) / weight(of_key(floor));
-          return;
-        }
-      }
-      if (first && !by_mass && target >= all) return;   // all of them
-      const unsigned long long need = target - above;
-      if (upto >= need && upto - n < need) {
-        s.found_above = upto - n;
-        // the bin's keys
-        uint32_t l, h;
-        if (bins.even) {
-          auto first_of = [&](int b) {   // the least key whose bin is b or less
-            uint32_t x = bins.lo, y = bins.hi;
-            while (x < y) {
-              const uint32_t m = x + (y - x) / 2;
-              if (bins.bin(m, of_key(m)) <= b) y = m;
-              else x = m + 1;
-            }
-            return x;
-          };
-          l = first_of(tid);
-          h = tid == 0 ? bins.hi : first_of(tid - 1) - 1;
-        } else {
-          h = bins.hi - (uint32_t(tid) << bins.shift);
-          const uint32_t reach = (1u << bins.shift) - 1;
-          l = h - bins.lo < reach ? bins.lo : h - reach;
-        }
-        s.range[0] = l, s.range[1] = h;
-      }
-      __syncthreads();
-      above += s.found_above;
-      bins.set(s.range[0], s.range[1], false);
-      __syncthreads();
-      if (bins.lo == bins.hi) break;
+      low_key = least, high_key = greatest;
+      listed = s.listed[next];
+      list = listed <= kListed ? next : -1;
+      turn ^= 1;
+      if (least == greatest) break;
     }
-    border = bins.lo;
+    border = low_key;
     if (by_mass) {
       const unsigned long long w = weight(of_key(border));
       ties = w ? (target - above + w - 1) / w : 0;
@@ -294,16 +488,42 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   if (top_p < 1.f) descend(true, 0);
 
   // ---- sums of the kept, per warp's part of the slice
-  const int part = (a.slice + kWarps - 1) / kWarps;
-  const int first = min(warp * part, z.count), end = min(first + part, z.count);
   {
     unsigned long long sum = 0;
     uint32_t equal = 0;
-    for (int i = first + lane; i < end; i += 32) {
-      const float v = z.at(i);
-      const uint32_t k = key_of(v);
-      if (k > border) sum += weight(v);
-      else if (k == border) ++equal;
+    const float last = of_key(border);
+    if (binned) {   // of the bins above the border's, and what of that is above the border
+      for (int b = lane; b < summed; b += 32) sum += s.part_low[warp][b] + (static_cast<unsigned long long>(s.part_high[warp][b]) << 32);
+      auto rest = [&](const auto& bin) {
+        for (int q = part_begin + lane; q < part_end; q += 32) {
+          const uint4 p = piece(q);
+          const T* e = reinterpret_cast<const T*>(&p);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = value<T>(e[j]);
+            equal += v == last;
+            if (v > last && bin(v) >= summed) sum += weight(v);
+          }
+        }
+      };
+      if (coarse_even) rest(coarse);
+      else rest(coarse_keys);
+    } else {
+      auto sums = [&](const auto& weight) {
+        for (int q = part_begin + lane; q < part_end; q += 32) {
+          const uint4 p = piece(q);
+          const T* e = reinterpret_cast<const T*>(&p);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = value<T>(e[j]);
+            const unsigned long long w = weight(v);
+            equal += v == last;
+            sum += v > last ? w : 0;
+          }
+        }
+      };
+      if (near) sums(near_weight);
+      else sums(far_weight);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
@@ -311,86 +531,72 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     if (lane == 0) s.warp_mass[warp] = sum, s.warp_ties[warp] = equal;
   }
   cluster.sync();
-  // Every warp looks where the target falls; the one whose part it is finds the token.
-  const unsigned long long tie = weight(of_key(border));
-  unsigned long long all = 0, before = 0, ties_before = 0, mine = 0;
-  {
-    unsigned long long met = 0;   // ties so far
-    for (int j0 = 0; j0 < ctas * kWarps; j0 += 32) {
-      const int j = j0 + lane;
-      unsigned long long m = 0;
-      uint32_t e = 0;
+  // The part where the target falls: the sums and ties before it, of all CTAs' parts in order.
+  if (warp == 0) {
+    const unsigned long long tie = weight(of_key(border));
+    constexpr int kParts = kMostCtas * kWarps / 32;
+    unsigned long long m[kParts], ahead[kParts], upto[kParts], all = 0, met = 0;
+#pragma unroll
+    for (int b = 0; b < kParts; ++b) {
+      const int j = b * 32 + lane;
+      m[b] = 0;
+      unsigned long long e = 0;
       if (j < ctas * kWarps) {
         const Shared* o = cluster.map_shared_rank(&s, j / kWarps);
-        m = o->warp_mass[j % kWarps], e = o->warp_ties[j % kWarps];
+        m[b] = o->warp_mass[j % kWarps], e = o->warp_ties[j % kWarps];
       }
-      unsigned long long es = e;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long p = __shfl_up_sync(~0u, es, d);
-        if (lane >= d) es += p;
-      }
-      const unsigned long long ahead = met + es - e;
-      m += tie * (ahead < ties ? min((unsigned long long)e, ties - ahead) : 0ull);
-      unsigned long long ms = m;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long p = __shfl_up_sync(~0u, ms, d);
-        if (lane >= d) ms += p;
-      }
-      const int me = rank * kWarps + warp;
-      if (me >= j0 && me < j0 + 32) {
-        before = all + __shfl_sync(~0u, ms - m, me - j0);
-        mine = __shfl_sync(~0u, m, me - j0);
-        ties_before = __shfl_sync(~0u, ahead, me - j0);
-      }
-      all += __shfl_sync(~0u, ms, 31);
+      const unsigned long long es = sum_upto(e, lane);
+      ahead[b] = met + es - e;
+      m[b] += tie * (ahead[b] < ties ? min(e, ties - ahead[b]) : 0ull);
       met += __shfl_sync(~0u, es, 31);
+      upto[b] = all + sum_upto(m[b], lane);
+      all = __shfl_sync(~0u, upto[b], 31);
     }
+    float u = a.uniform[row];
+    u = u > 0.f ? fminf(u, 1.f) : 0.f;   // NaN: 0
+    const unsigned long long target = min((unsigned long long)(double(u) * double(all)), all - 1);
+    if (lane == 0) s.target = target, s.tie = tie;
+#pragma unroll
+    for (int b = 0; b < kParts; ++b)
+      if (upto[b] > target && upto[b] - m[b] <= target) s.chosen = b * 32 + lane, s.before = upto[b] - m[b], s.ties_before = ahead[b];
   }
-  const unsigned long long target = min((unsigned long long)(double(u) * double(all)), all - 1);
-  if (target >= before && target - before < mine) {
-    // lanes take neighbouring elements, then all of them those of the lane whose it is
-    const int each = (end - first + 31) / 32;
-    auto kept = [&](int i, unsigned long long& met) -> unsigned long long {
-      const float v = z.at(i);
+  __syncthreads();
+  const int chosen = s.chosen;
+  const unsigned long long target = s.target, tie = s.tie, before = s.before, ties_before = s.ties_before;
+  if (chosen / kWarps == rank) {   // this CTA's: its threads take the part's neighbouring elements
+    const int w = chosen % kWarps;
+    const int first = max(0, w * part * kV - shift), end = min(count, (w + 1) * part * kV - shift);
+    const int each = (end - first + kThreads - 1) / kThreads;
+    const int x = min(first + tid * each, end), y = min(x + each, end);
+    unsigned long long equal = 0;
+    for (int i = x; i < y; ++i) equal += key_of(at(i)) == border;
+    unsigned long long upto = sum_upto(equal, lane);
+    if (lane == 31) s.scan[0][warp] = upto;
+    __syncthreads();
+    unsigned long long seen = ties_before + upto - equal;
+    for (int v = 0; v < warp; ++v) seen += s.scan[0][v];
+    auto kept = [&](int i, unsigned long long& n) -> unsigned long long {
+      const float v = at(i);
       const uint32_t k = key_of(v);
       if (k > border) return weight(v);
-      if (k == border && met++ < ties) return tie;
-      return 0;
+      return k == border && n++ < ties ? tie : 0;
     };
-    int from = first, to = end, step = each;
-    while (true) {
-      const int x = min(from + lane * step, to), y = min(x + step, to);
-      unsigned long long equal = 0;
-      for (int i = x; i < y; ++i) equal += key_of(z.at(i)) == border;
-      unsigned long long met = equal;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long p = __shfl_up_sync(~0u, met, d);
-        if (lane >= d) met += p;
+    unsigned long long sum = 0, n = seen;
+    for (int i = x; i < y; ++i) sum += kept(i, n);
+    upto = sum_upto(sum, lane);
+    if (lane == 31) s.scan[1][warp] = upto;
+    __syncthreads();
+    unsigned long long running = before + upto - sum;
+    for (int v = 0; v < warp; ++v) running += s.scan[1][v];
+    if (running <= target && target < running + sum) {
+      n = seen;
+      for (int i = x; i < y; ++i) {
+        running += kept(i, n);
+        if (running > target) {
+          a.tokens[row] = begin + i;
+          break;
+        }
       }
-      met += ties_before - equal;
-      const unsigned long long ahead = met;
-      unsigned long long sum = 0;
-      for (int i = x; i < y; ++i) sum += kept(i, met);
-      unsigned long long upto = sum;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long p = __shfl_up_sync(~0u, upto, d);
-        if (lane >= d) upto += p;
-      }
-      upto += before;
-      const uint32_t over = __ballot_sync(~0u, upto > target);
-      const int l = __ffs(over) - 1;   // there is one: the part's sum reaches beyond the target
-      if (step == 1) {
-        if (lane == l) a.tokens[row] = begin + x;
-        break;
-      }
-      from = __shfl_sync(~0u, x, l), to = __shfl_sync(~0u, y, l);
-      before = __shfl_sync(~0u, upto - sum, l);
-      ties_before = __shfl_sync(~0u, ahead, l);
-      step = max(1, (to - from + 31) / 32);
     }
   }
   cluster.sync();   // the others may still read this CTA's numbers
@@ -419,12 +625,12 @@ cudaError_t sample(const void* logits, int64_t stride, int elem, int64_t rows, i
   const int size = elem == 1 ? 4 : 2;
   // CTAs per row: slices of at most 64 KB, so that several CTAs share an SM, and more while rows leave SMs idle
   int ctas = 1;
-  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * 64 * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
+  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * SK * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
   SampleArgs a = {logits, stride, uniform, by, tokens, vocab, 0};
   a.slice = int((int64_t(vocab) + ctas * 64 - 1) / (ctas * 64) * 64);
-  const size_t held = size_t(a.slice) * size + 32;
+  const size_t held = size_t(a.slice) * size + 32;   // and the pieces' overhang
   const bool hold = held <= kHeld;
-  const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + (hold ? held : 0);
+  const size_t smem = sizeof(Shared) + (hold ? held : 0);
   if (elem == 1) return hold ? launch<float, true>(a, rows, ctas, smem, s) : launch<float, false>(a, rows, ctas, smem, s);
   if (elem == 10) return hold ? launch<__half, true>(a, rows, ctas, smem, s) : launch<__half, false>(a, rows, ctas, smem, s);
   return hold ? launch<__nv_bfloat16, true>(a, rows, ctas, smem, s) : launch<__nv_bfloat16, false>(a, rows, ctas, smem, s);

@@ -384,18 +384,21 @@ def _matrix(x, name: str, device: torch.device, dtype: torch.dtype, rows: Option
     _bad(f"{name} must be [{'rows' if rows is None else rows}, {'width' if columns is None else columns}] and contiguous along its rows, got {tuple(x.shape)}")
 
 
-def _vector(x, name: str, device: torch.device, dtypes, n: int):
-    """(address, type) of n contiguous values of one of the types; (None, None) of None."""
+def _vector(x, name: str, device: torch.device, dtypes, n: int) -> int:
+    """The address of n contiguous values of one of the types; 0 of None."""
     if x is None:
-        return None, None
+        return 0
     try:
-        dtype = x.dtype
-        if dtype in dtypes and x.get_device() == device.index and x.shape == (n,) and (x.stride() == (1,) or n == 1) and not _derived(x):
-            return x.data_ptr(), dtype
+        if x.dtype in dtypes and x.get_device() == device.index and x.shape == (n,) and (n == 1 or x.stride() == (1,)) and not _derived(x):
+            return x.data_ptr()
     except AttributeError:
         pass
     _on(x, name, device, getattr(x, "dtype", None) if getattr(x, "dtype", None) in dtypes else dtypes[0], 1)
     _bad(f"{name} must be {n} contiguous values, got {tuple(x.shape)}")
+
+
+_pack_norm = struct.Struct("PPPPPqqqqqPPPPqqiiiifff").pack   # sb_residual_norm_args
+_pack_sampling = struct.Struct("PPPPfffi").pack              # sb_sampling
 
 
 def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Optional[torch.Tensor] = None,
@@ -424,52 +427,55 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
         _bad(f"kind must be 'rms' or 'layer', got {kind!r}")
     rows, xs = _matrix(x, "x", device, dtype, None, None)
     n = x.shape[1]
-    a = _native.ResidualNorm()
-    sum_type, rs = dtype, 0
+    sum_type, rs, rp = dtype, 0, 0
     if residual is not None:
-        sum_type = torch.float32 if getattr(residual, "dtype", None) is torch.float32 else dtype
+        if getattr(residual, "dtype", None) is torch.float32:
+            sum_type = torch.float32
         rs = _matrix(residual, "residual", device, sum_type, rows, n)[1]
-        a.residual = residual.data_ptr()
-    elif residual_out is not None:
-        sum_type = torch.float32 if getattr(residual_out, "dtype", None) is torch.float32 else dtype
-    gs = 0
+        rp = residual.data_ptr()
+    elif residual_out is not None and getattr(residual_out, "dtype", None) is torch.float32:
+        sum_type = torch.float32
+    gp, gs = 0, 0
     if gate is not None:
         if isinstance(gate, torch.Tensor) and gate.dim() == 1:
-            a.gate = _vector(gate, "gate", device, (dtype,), n)[0]
+            gp = _vector(gate, "gate", device, (dtype,), n)
         else:
             gs = _matrix(gate, "gate", device, dtype, rows, n)[1]
-            a.gate = gate.data_ptr()
-    weights = (dtype, torch.float32)
-    kinds = set()
-    for name, v in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        if v is not None:
-            at, t = _vector(v, name, device, weights, n)
-            setattr(a, name, at)
-            kinds.add(t)
-    if len(kinds) > 1:
-        _bad("weights and biases must have the same type")
+            gp = gate.data_ptr()
+    first = weight if weight is not None else post_weight
+    kinds = (dtype,)
+    if first is not None:
+        if getattr(first, "dtype", None) is torch.float32:
+            kinds = (torch.float32,)
+        wp, bp = _vector(weight, "weight", device, kinds, n), _vector(bias, "bias", device, kinds, n)
+        pp, cp = _vector(post_weight, "post_weight", device, kinds, n), _vector(post_bias, "post_bias", device, kinds, n)
+    else:
+        wp = pp = bp = cp = 0
     if weight is None and (bias is not None or out is not None):
         _bad("bias and out need a weight")
     if post_weight is None and post_bias is not None:
         _bad("post_bias needs a post_weight")
-    changed = residual is not None or gate is not None or post_weight is not None or scale != 1.0
-    if weight is None and not changed:
+    h, hp, ss = x, 0, 0
+    if residual is not None or gate is not None or post_weight is not None or scale != 1.0 or residual_out is not None:
+        if residual_out is not None:
+            h = residual_out
+        else:
+            h = torch.empty((rows, n), dtype=sum_type, device=device)
+        ss = _matrix(h, "residual_out", device, sum_type, rows, n)[1]
+        hp = h.data_ptr()
+    elif weight is None:
         _bad("there is nothing to compute")
-    h = x
-    if changed or residual_out is not None:
-        h = residual_out if residual_out is not None else torch.empty((rows, n), dtype=sum_type, device=device)
-        a.sum_row_stride = _matrix(h, "residual_out", device, sum_type, rows, n)[1]
-        a.sum = h.data_ptr()
-    y = None
+    y, yp, ys = None, 0, 0
     if weight is not None:
         y = out if out is not None else torch.empty((rows, n), dtype=dtype, device=device)
-        a.y_row_stride = _matrix(y, "out", device, dtype, rows, n)[1]
-        a.y = y.data_ptr()
-    a.x, a.x_row_stride, a.residual_row_stride, a.gate_row_stride = x.data_ptr(), xs, rs, gs
-    a.rows, a.width, a.elem_type, a.sum_type = rows, n, elem, _ELEM[sum_type]
-    a.weight_type = _ELEM[kinds.pop()] if kinds else elem
-    a.layer_norm, a.scale, a.eps, a.weight_offset = kind == "layer", scale, eps, weight_offset
-    _call("sb_residual_norm", device, C.byref(a))
+        ys = _matrix(y, "out", device, dtype, rows, n)[1]
+        yp = y.data_ptr()
+    try:
+        a = _pack_norm(x.data_ptr(), rp, gp, hp, yp, xs, rs, gs, ss, ys, wp, bp, pp, cp, rows, n, elem, _ELEM[sum_type], _ELEM[kinds[0]],
+                       kind == "layer", scale, eps, weight_offset)
+    except (struct.error, OverflowError) as e:
+        raise B200ArgumentError(f"scale, eps and weight_offset must be numbers of 32 bits: {e}") from None
+    _call("sb_residual_norm", device, a)
     return y, h
 
 
@@ -503,7 +509,7 @@ class MoEWeights:
             _bad(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
         if activation not in ("silu", "gelu"):
             _bad(f"activation must be 'silu' or 'gelu', got {activation!r}")
-        bias = _vector(selection_bias, "selection_bias", device, (torch.float32,), experts)[0]
+        bias = _vector(selection_bias, "selection_bias", device, (torch.float32,), experts)
         self.router, self.gate_up, self.down, self.selection_bias = router, gate_up, down, selection_bias
         self.device, self.dtype, self.experts, self.width, self.inner, self.top_k = device, dtype, experts, width, inner, int(top_k)
         self._c = _native.MoEWeights(router.data_ptr(), gate_up.data_ptr(), down.data_ptr(), bias, router.stride(0), gate_up.stride(0),
@@ -559,25 +565,25 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     if elem is None:
         raise B200NotSupportedError(f"element type {dtype} is not supported")
     rows, stride = _matrix(logits, "logits", device, dtype, None, None)
-    at = _vector(uniform, "uniform", device, (torch.float32,), rows)[0]
-    by = _native.Sampling()
+    at = _vector(uniform, "uniform", device, _FLOAT, rows)
+    tp = pp = mp = kp = 0
     if isinstance(temperature, torch.Tensor):
-        by.temperature_of = _vector(temperature, "temperature", device, (torch.float32,), rows)[0]
-    else:
-        by.temperature = temperature
+        tp, temperature = _vector(temperature, "temperature", device, _FLOAT, rows), 1.0
     if isinstance(top_k, torch.Tensor):
-        by.top_k_of = _vector(top_k, "top_k", device, (torch.int32,), rows)[0]
-    else:
-        by.top_k = min(max(int(top_k), 0), 0x7fffffff)
+        kp, top_k = _vector(top_k, "top_k", device, (torch.int32,), rows), 0
     if isinstance(top_p, torch.Tensor):
-        by.top_p_of = _vector(top_p, "top_p", device, (torch.float32,), rows)[0]
-    else:
-        by.top_p = top_p
+        pp, top_p = _vector(top_p, "top_p", device, _FLOAT, rows), 1.0
     if isinstance(min_p, torch.Tensor):
-        by.min_p_of = _vector(min_p, "min_p", device, (torch.float32,), rows)[0]
-    else:
-        by.min_p = min_p
-    out = torch.empty(rows, dtype=torch.int64, device=device) if out is None else out
-    _call("sb_sample", device, logits.data_ptr(), stride, elem, rows, logits.shape[1], at, C.byref(by),
-          _vector(out, "out", device, (torch.int64,), rows)[0])
+        mp, min_p = _vector(min_p, "min_p", device, _FLOAT, rows), 0.0
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=device)
+    to = _vector(out, "out", device, (torch.int64,), rows)
+    try:
+        by = _pack_sampling(tp, pp, mp, kp, temperature, top_p, min_p, min(max(int(top_k), 0), 0x7fffffff))
+    except (struct.error, OverflowError) as e:
+        raise B200ArgumentError(f"temperature, top_p and min_p must be numbers of 32 bits or tensors: {e}") from None
+    _call("sb_sample", device, logits.data_ptr(), stride, elem, rows, logits.shape[1], at, by, to)
     return out
+
+
+_FLOAT = (torch.float32,)

@@ -132,6 +132,36 @@ def test_residual_norm_forms(width, kind):
     assert h.dtype is FP32
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows,width,pitch", [(4800, 1024, 1024), (1300, 4104, 4112), (1300, 2050, 2050), (2500, 1033, 1033), (640, 11001, 11001),
+                                              (620, 16392, 16392), (900, 5000, 5001), (610, 14001, 14003), (5000, 130, 131)])
+def test_residual_norm_of_many_rows(rows, width, pitch, dtype):
+    """Rows enough for every CTA to take several, from aligned ones to those that begin anywhere, and in place."""
+    gen = torch.Generator().manual_seed(rows + width)
+    x, r, g = (normal(gen, (rows, pitch), dtype)[:, pitch - width:].cuda() for _ in range(3))
+    w, b, p = (normal(gen, (width,), dtype).cuda() for _ in range(3))
+    some = sorted({0, 1, 5, rows // 2, rows - 2, rows - 1})
+    kw = dict(bias=b, post_weight=p, scale=0.3, kind="layer")
+    y, h = decoder.residual_norm(x, w, residual=r, gate=g, **kw)
+    small = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    wy, dy, wh, dh = norm_reference(x[some].cpu(), w.cpu(), residual=r[some].cpu(), gate=g[some].cpu(), **small)
+    within(y[some], wy, rounded(wy, dy, dtype), "y")
+    within(h[some], wh, rounded(wh, dh, dtype), "h")
+    for i in range(0, rows, 97):                      # a few rows at a time, the same results to rounding of sums
+        part = slice(i, min(i + 3, rows))
+        a, c = decoder.residual_norm(x[part], w, residual=r[part], gate=g[part], **kw)
+        scale = float(w.abs().max()) * 8
+        assert (a.float() - y[part].float()).abs().max() <= scale * torch.finfo(dtype).eps + 1e-4
+        assert (c.float() - h[part].float()).abs().max() <= scale * torch.finfo(dtype).eps + 1e-4
+    wide = normal(gen, (rows, width), FP32).cuda()
+    y2, h2 = decoder.residual_norm(x, w, residual=wide, gate=b)
+    wy, dy, wh, dh = norm_reference(x[some].cpu(), w.cpu(), residual=wide[some].cpu(), gate=b.cpu())
+    within(y2[some], wy, rounded(wy, dy, dtype), "y, stream in 32 bits")
+    within(h2[some], wh, rounded(wh, dh, FP32), "h, stream in 32 bits")
+    decoder.residual_norm(x, w, residual=r, gate=g, out=x, residual_out=r, **kw)
+    assert torch.equal(x, y) and torch.equal(r, h)
+
+
 def test_residual_norm_of_a_loud_mean():
     """The variance is taken of differences from the mean: values 1000 off zero keep theirs."""
     gen = torch.Generator().manual_seed(3)
