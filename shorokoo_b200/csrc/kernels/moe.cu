@@ -29,11 +29,14 @@ namespace sb {
 namespace k {
 namespace {
 
+#ifndef MU
+#define MU 4096
+#endif
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlock = 64;          // inputs of a step
 constexpr int kMostExperts = 512;   // of a lane's 16 scores
 
-struct Entry { int expert, row, count, pad; };   // up to 8 NT rows of one expert
+struct Entry { int expert, first, count; };   // up to 8 NT places of the list, of one expert
 
 struct MoEArgs {
   MoEView w;
@@ -41,7 +44,7 @@ struct MoEArgs {
   void* y;
   int64_t xs, ys;
   int tokens, rows;        // rows: tokens * top_k
-  int words, entries;      // mask words of an expert; room for entries
+  int entries;             // room for them
   int splits;              // of the second product's k
   double* logits;          // [tokens][experts]
   int* chosen;             // [rows]
@@ -120,79 +123,91 @@ __device__ __forceinline__ double router_dot(const MoEArgs& a, int t, int e, int
   return sum;
 }
 
-// The experts of a token and their shares, by a warp; equal scores go to the lower expert.
-__device__ __forceinline__ void choose(const MoEArgs& a, int t, int lane, int* chosen, float* share) {
+// The experts of a token and their shares, by a warp; equal scores go to the lower expert. J: scores per lane.
+template <int J>
+__device__ __noinline__ void choose(const MoEArgs& a, int t, int lane, int* chosen, float* share) {
   const MoEView& w = a.w;
   const double* l = a.logits + int64_t(t) * w.experts;
-  uint32_t key[kMostExperts / 32];
-  double top = -INFINITY, all = 0;
-  const bool sums = w.softmax && (w.selection_bias != nullptr || !w.normalize);   // needs the sum over all experts
-  if (w.softmax) {
-    for (int e = lane; e < w.experts; e += 32) top = fmax(top, __ldcg(l + e));
+  double v[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) v[j] = j * 32 + lane < w.experts ? __ldcg(l + j * 32 + lane) : 0.0;
+  uint32_t key[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) key[j] = j * 32 + lane < w.experts ? ordered(float(v[j])) : 0u;
+  double top = 0, all = 0;
+  const bool biased = w.selection_bias != nullptr;
+  if (w.softmax && (biased || !w.normalize)) {   // needs the sum over all experts
+    top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (j * 32 + lane < w.experts) top = fmax(top, v[j]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, d));
-    if (sums) {
-      for (int e = lane; e < w.experts; e += 32) all += exp(__ldcg(l + e) - top);
+#pragma unroll 1
+    for (int e = lane; e < w.experts; e += 32) all += exp(__ldcg(l + e) - top);
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+  }
+  if (biased) {   // the order of score + bias, not that of the logits
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int e = j * 32 + lane;
+      if (e < w.experts) key[j] = ordered(float((w.softmax ? exp(v[j] - top) / all : 1.0 / (1.0 + exp(-v[j]))) + double(w.selection_bias[e])));
     }
   }
-  auto score = [&](double v) { return w.softmax ? exp(v - top) : 1.0 / (1.0 + exp(-v)); };
-#pragma unroll
-  for (int j = 0; j < kMostExperts / 32; ++j) {
-    const int e = j * 32 + lane;
-    key[j] = 0;
-    if (j * 32 < w.experts && e < w.experts) {
-      const double v = __ldcg(l + e);
-      if (w.selection_bias) key[j] = ordered(float((w.softmax ? score(v) / all : score(v)) + double(w.selection_bias[e])));
-      else key[j] = ordered(float(v));
-    }
-  }
-  int mine = 0;   // lane r: the r-th chosen
+  int mine = 0;          // lane r: the r-th chosen
   for (int r = 0; r < w.top_k; ++r) {
-    uint32_t best = 0;
+    uint32_t best = key[0];
 #pragma unroll
-    for (int j = 0; j < kMostExperts / 32; ++j)
-      if (j * 32 < w.experts) best = max(best, key[j]);
+    for (int j = 1; j < J; ++j) best = max(best, key[j]);
     const uint32_t most = __reduce_max_sync(~0u, best);
     uint32_t e = ~0u;
 #pragma unroll
-    for (int j = kMostExperts / 32 - 1; j >= 0; --j)
-      if (j * 32 < w.experts && key[j] == most) e = j * 32 + lane;
+    for (int j = J - 1; j >= 0; --j) e = key[j] == most ? j * 32 + lane : e;
     e = __reduce_min_sync(~0u, e);
+    if ((e & 31) == uint32_t(lane)) {
 #pragma unroll
-    for (int j = 0; j < kMostExperts / 32; ++j)
-      if (e == uint32_t(j * 32 + lane)) key[j] = 0;
+      for (int j = 0; j < J; ++j)
+        if (e >> 5 == uint32_t(j)) key[j] = 0;
+    }
     if (lane == r) mine = int(e);
   }
-  double s = lane < w.top_k ? score(__ldcg(l + mine)) : 0.0;
+  const float z = float(__ldcg(l + mine));
+  float s;
+  if (w.softmax) {
+    const float high = w.normalize ? __shfl_sync(~0u, z, 0) : float(top);   // any shift serves; the first chosen is near the top
+    s = expf(z - high);
+  } else {
+    s = 1.f / (1.f + expf(-z));
+  }
+  if (lane >= w.top_k) s = 0.f;
   if (w.normalize) {
-    double sum = s;
+    float sum = s;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
     s /= sum;
   } else if (w.softmax) {
-    s /= all;
+    s = float(exp(double(z) - top) / all);
   }
   if (lane < w.top_k) {
     chosen[t * w.top_k + lane] = mine;
-    share[t * w.top_k + lane] = float(s * double(w.scale));
+    share[t * w.top_k + lane] = s * w.scale;
   }
 }
 
-// What a CTA knows of the step's rows, in shared memory.
+// What a CTA knows of the step's rows (t * top_k + r: the r-th expert of token t), in shared memory.
 struct Lists {
-  uint32_t* mask;      // [experts][words] tokens of each expert
-  int* base;           // [experts] its first row
   Entry* entry;        // [entries]
-  int* chosen;         // [rows] by token and rank
+  int* base;           // [experts] the first place of an expert's rows in the list
+  int* number;         // [experts] how many they are
+  int* chosen;         // [rows]
   float* share;
-  uint16_t* token;     // [rows] of a row
-  uint16_t* row;       // [rows] of a token and rank
   int* count;          // entries in use
+  uint16_t* row;       // the list: [rows], by expert
+  uint16_t* place;     // [rows] among its expert's
 };
-__host__ __device__ inline size_t lists_bytes(int experts, int words, int entries, int rows) {
-  return size_t(entries) * sizeof(Entry) + size_t(experts) * (words + 1) * 4 + size_t(rows) * 12 + 16;
+__host__ __device__ inline size_t lists_bytes(int experts, int entries, int rows) {
+  return size_t(entries) * sizeof(Entry) + size_t(experts) * 8 + size_t(rows) * 12 + 32;
 }
 
 // The two products. Units: (entry, tile of rows, part of k); a CTA takes every gridDim.x-th.
@@ -291,14 +306,15 @@ struct Product {
       const Unit v = unit(u);
       const Entry en = at.entry[v.entry];
       const int used = (en.count + 7) / 8;   // column tiles
+      const uint16_t* rows = at.row + en.first;
       const uint16_t* column[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int c = n * 8 + g;
         column[n] = nullptr;
         if (c < en.count)
-          column[n] = kFirst ? static_cast<const uint16_t*>(a.x) + at.token[en.row + c] * a.xs
-                             : static_cast<const uint16_t*>(a.hidden) + int64_t(en.row + c) * a.w.inner;
+          column[n] = kFirst ? static_cast<const uint16_t*>(a.x) + rows[c] / a.w.top_k * a.xs
+                             : static_cast<const uint16_t*>(a.hidden) + int64_t(rows[c]) * a.w.inner;
       }
       auto fetch = [&](uint4 (&b)[NT][2], int block) {
 #pragma unroll
@@ -318,10 +334,7 @@ struct Product {
 #pragma unroll
           for (int i = 0; i < 4; ++i) d[n][m][i] = 0.f;
       const int end = end_of(v);
-      uint4 b[NT][2];
-      int block = v.part * blocks + warp;
-      if (block < end) fetch(b, block);
-      for (; block < end; block += kWarps) {
+      auto step = [&](const uint4 (&b)[NT][2]) {
         wait<S - 2>();
         const uint32_t from = ring + stage_out * (MT * 2048) + lane * 16;
         stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
@@ -333,8 +346,6 @@ struct Product {
 #pragma unroll
             for (int h = 0; h < 2; ++h) w[m][r][h] = shared16(from + ((m * 2 + r) * 2 + h) * 512);
         copy_step();   // into the stage read in the step before
-        uint4 ahead[NT][2];
-        if (block + kWarps < end) fetch(ahead, block + kWarps);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if (NT > 1 && n >= used) break;
@@ -346,10 +357,19 @@ struct Product {
               Op<T>::mma(d[n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b[n][h].z, b[n][h].w);
             }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) b[n][h] = ahead[n][h];
+      };
+      // Columns are fetched a step ahead, into registers of their own by turns (a copy between them would wait for them).
+      uint4 even[NT][2], odd[NT][2];
+      int block = v.part * blocks + warp;
+      if (block < end) fetch(even, block);
+      while (block < end) {
+        if (block + kWarps < end) fetch(odd, block + kWarps);
+        step(even);
+        block += kWarps;
+        if (block >= end) break;
+        if (block + kWarps < end) fetch(even, block + kWarps);
+        step(odd);
+        block += kWarps;
       }
       // The warps' sums meet; two buffers in turn, so that one barrier is enough.
       constexpr int kEach = NT * MT * 4 * 32;
@@ -377,14 +397,14 @@ struct Product {
           if (c < en.count && f < out_rows) {
             const float gate = total((nm * 4 + odd) * 32 + l), up = total((nm * 4 + odd + 2) * 32 + l);
             const float act = a.w.gelu ? 0.5f * gate * (1.f + erff(gate * 0.70710678f)) : gate / (1.f + expf(-gate));
-            static_cast<T*>(a.hidden)[int64_t(en.row + c) * a.w.inner + f] = Op<T>::round(act * up);
+            static_cast<T*>(a.hidden)[int64_t(rows[c]) * a.w.inner + f] = Op<T>::round(act * up);
           }
         }
       } else {
         for (int i = threadIdx.x; i < used * MT * 128; i += kThreads) {
           const int l = i & 31, q = i >> 5 & 3, nm = i >> 7, n = nm / MT, m = nm - n * MT;
           const int c = n * 8 + (l & 3) * 2 + (q & 1), r = v.first + m * kApart + (q >> 1) * 8 + (l >> 2);
-          if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + en.row + c) * out_rows + r] = total((nm * 4 + q) * 32 + l);
+          if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + rows[c]) * out_rows + r] = total((nm * 4 + q) * 32 + l);
         }
       }
     }
@@ -392,7 +412,7 @@ struct Product {
 };
 
 template <typename T, int NT, int MT, int S>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const MoEArgs a) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const __grid_constant__ MoEArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   const auto grid = cooperative_groups::this_grid();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -409,59 +429,72 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const Mo
   {
     uint8_t* p = smem + kRing + kSums;
     at.entry = reinterpret_cast<Entry*>(p), p += a.entries * sizeof(Entry);
-    at.mask = reinterpret_cast<uint32_t*>(p), p += size_t(experts) * a.words * 4;
     at.base = reinterpret_cast<int*>(p), p += size_t(experts) * 4;
+    at.number = reinterpret_cast<int*>(p), p += size_t(experts) * 4;
     at.chosen = reinterpret_cast<int*>(p), p += size_t(a.rows) * 4;
     at.share = reinterpret_cast<float*>(p), p += size_t(a.rows) * 4;
-    at.count = reinterpret_cast<int*>(p), p += 16;
-    at.token = reinterpret_cast<uint16_t*>(p), p += size_t(a.rows) * 2;
-    at.row = reinterpret_cast<uint16_t*>(p);
+    at.count = reinterpret_cast<int*>(p), p += 32;   // and the warps' sums
+    at.row = reinterpret_cast<uint16_t*>(p), p += size_t(a.rows) * 2;
+    at.place = reinterpret_cast<uint16_t*>(p);
   }
-  for (int i = tid; i < experts * a.words; i += kThreads) at.mask[i] = 0;
+  for (int i = tid; i < experts; i += kThreads) at.number[i] = 0;
+  auto pick = [&](int t, int* chosen, float* share) {
+    if (experts <= 128) choose<4>(a, t, lane, chosen, share);
+    else choose<kMostExperts / 32>(a, t, lane, chosen, share);
+  };
   if (a.tokens <= 2 * kWarps) {   // every CTA chooses for itself: cheaper than another barrier
-    for (int t = warp; t < a.tokens; t += kWarps) choose(a, t, lane, at.chosen, at.share);
+    for (int t = warp; t < a.tokens; t += kWarps) pick(t, at.chosen, at.share);
+    __syncthreads();
   } else {
-    for (int t = warp * gridDim.x + blockIdx.x; t < a.tokens; t += kWarps * gridDim.x) choose(a, t, lane, a.chosen, a.share);
+    for (int t = warp * gridDim.x + blockIdx.x; t < a.tokens; t += kWarps * gridDim.x) pick(t, a.chosen, a.share);
     grid.sync();
     for (int i = tid; i < a.rows; i += kThreads) at.chosen[i] = __ldcg(a.chosen + i), at.share[i] = __ldcg(a.share + i);
   }
   __syncthreads();
-  for (int i = tid; i < a.rows; i += kThreads) {
-    const int t = i / top_k;
-    atomicOr(at.mask + at.chosen[i] * a.words + (t >> 5), 1u << (t & 31));
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int rows = 0, entries = 0;
-    for (int e0 = 0; e0 < experts; e0 += 32) {
-      const int e = e0 + lane;
-      int n = 0;
-      if (e < experts)
-        for (int i = 0; i < a.words; ++i) n += __popc(at.mask[e * a.words + i]);
-      const int mine = (n + 8 * NT - 1) / (8 * NT);
-      int r = n, m = mine;   // sums up to this lane
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int pr = __shfl_up_sync(~0u, r, d), pm = __shfl_up_sync(~0u, m, d);
-        if (lane >= d) r += pr, m += pm;
+  if (warp == 0) {   // places in the order of the rows: all CTAs have to divide an expert's rows among its entries alike
+    for (int i0 = 0; i0 < a.rows; i0 += 32) {
+      const int i = i0 + lane, e = i < a.rows ? at.chosen[i] : -1 - lane;
+      const uint32_t same = __match_any_sync(~0u, e), lower = same & ((1u << lane) - 1);
+      if (e >= 0) {
+        const int before = at.number[e];
+        at.place[i] = uint16_t(before + __popc(lower));
+        __syncwarp(same);
+        if (lower == 0) at.number[e] = before + __popc(same);
       }
-      const int row = rows + r - n;
-      if (e < experts) at.base[e] = row;
-      for (int i = 0; i < mine; ++i) at.entry[entries + m - mine + i] = {e, row + i * 8 * NT, min(8 * NT, n - i * 8 * NT), 0};
-      rows += __shfl_sync(~0u, r, 31);
-      entries += __shfl_sync(~0u, m, 31);
+      __syncwarp();
     }
-    if (lane == 0) *at.count = entries;
   }
   __syncthreads();
-  for (int i = tid; i < a.rows; i += kThreads) {
-    const int t = i / top_k, e = at.chosen[i];
-    int row = at.base[e];
-    for (int j = 0; j < t >> 5; ++j) row += __popc(at.mask[e * a.words + j]);
-    row += __popc(at.mask[e * a.words + (t >> 5)] & ((1u << (t & 31)) - 1));
-    at.token[row] = uint16_t(t);
-    at.row[i] = uint16_t(row);
+  {   // four experts per thread: where their rows begin, and their entries
+    int n[kMostExperts / kThreads], rows = 0, entries = 0;
+#pragma unroll
+    for (int i = 0; i < kMostExperts / kThreads; ++i) {
+      const int e = tid * (kMostExperts / kThreads) + i;
+      n[i] = e < experts ? at.number[e] : 0;
+      rows += n[i], entries += (n[i] + 8 * NT - 1) / (8 * NT);
+    }
+    int both = rows << 16 | entries;   // each below 2^15
+    const int own = both;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int before = __shfl_up_sync(~0u, both, d);
+      if (lane >= d) both += before;
+    }
+    if (lane == 31) at.count[1 + warp] = both;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) both += at.count[1 + w];
+    if (tid == kThreads - 1) *at.count = both & 0xffff;
+    rows = (both - own) >> 16, entries = (both - own) & 0xffff;
+#pragma unroll
+    for (int i = 0; i < kMostExperts / kThreads; ++i) {
+      const int e = tid * (kMostExperts / kThreads) + i;
+      if (e < experts) at.base[e] = rows;
+      for (int k = 0; k < n[i]; k += 8 * NT) at.entry[entries++] = {e, rows + k, min(8 * NT, n[i] - k)};
+      rows += n[i];
+    }
   }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kThreads) at.row[at.base[at.chosen[i]] + at.place[i]] = uint16_t(i);
   __syncthreads();
 
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S * MT * 2048;
@@ -483,15 +516,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const Mo
   for (int i = blockIdx.x * kThreads + tid; i < a.tokens * quads; i += gridDim.x * kThreads) {
     const int t = i / quads, h = (i - t * quads) * 4;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r < top_k; ++r) {
-      const float s = at.share[t * top_k + r];
-      const float* p = a.partial + int64_t(at.row[t * top_k + r]) * a.w.width + h;
-      float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+    const float* p = a.partial + int64_t(t) * top_k * a.w.width + h;
+    for (int r0 = 0; r0 < top_k; r0 += 4) {   // loads in flight together
+      float4 v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < top_k) v[r] = __ldcg(reinterpret_cast<const float4*>(p + int64_t(r0 + r) * a.w.width));
       for (int j = 1; j < a.splits; ++j) {
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(p + int64_t(j) * a.rows * a.w.width));
-        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        float4 u[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r0 + r < top_k) u[r] = __ldcg(reinterpret_cast<const float4*>(p + (int64_t(j) * a.rows + r0 + r) * a.w.width));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r0 + r < top_k) v[r].x += u[r].x, v[r].y += u[r].y, v[r].z += u[r].z, v[r].w += u[r].w;
       }
-      y.x += s * v.x, y.y += s * v.y, y.z += s * v.z, y.w += s * v.w;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < top_k) {
+          const float s = at.share[t * top_k + r0 + r];
+          y.x += s * v[r].x, y.y += s * v[r].y, y.z += s * v[r].z, y.w += s * v[r].w;
+        }
     }
     alignas(8) T out[4] = {Op<T>::round(y.x), Op<T>::round(y.y), Op<T>::round(y.z), Op<T>::round(y.w)};
     *reinterpret_cast<uint2*>(static_cast<T*>(a.y) + t * a.ys + h) = *reinterpret_cast<const uint2*>(out);
@@ -500,20 +545,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const Mo
 
 // Sizes of one launch over up to `tokens` tokens.
 struct Sizes {
-  int tokens, words, entries, splits, columns;
+  int tokens, entries, splits, columns;
   size_t logits, chosen, hidden, partial, total;
 };
 Sizes sizes(const MoEView& w, int64_t tokens) {
   Sizes z;
   z.tokens = int(std::min<int64_t>(std::max<int64_t>(tokens, 1), std::min(256, 2048 / w.top_k)));
   const int rows = z.tokens * w.top_k;
-  z.columns = z.tokens <= 8 ? 8 : 32;
-  z.words = (z.tokens + 31) / 32;
+  // Columns of a product: 8 where an expert has few tokens on average; an expert that has more is read again (from L2, as
+  // its entries are near each other in time).
+  z.columns = z.tokens <= 8 || rows <= 4 * w.experts ? 8 : 32;
   z.entries = std::min(w.experts, rows) + rows / z.columns;
-  // Parts of the second product's k where (expert, tile) pairs are few, of 256 inputs or more
+  // Parts of the second product's k, of 512 inputs or more, until (expert, tile, part) triples are many for every CTA
   const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + 15) / 16);
   z.splits = 1;
-  while (z.splits < 8 && units * z.splits < 1024 && w.inner / (z.splits * 2) >= 256) z.splits *= 2;
+  while (z.splits < 8 && units * z.splits < MU && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   z.logits = up(size_t(z.tokens) * w.experts * 8);
   z.chosen = up(size_t(rows) * 4);
@@ -525,7 +571,7 @@ Sizes sizes(const MoEView& w, int64_t tokens) {
 
 template <typename T, int NT, int MT, int S>
 cudaError_t launch(MoEArgs a, int sms, cudaStream_t s) {
-  const size_t smem = size_t(kWarps) * S * MT * 2048 + size_t(2) * kWarps * NT * MT * 512 + lists_bytes(a.w.experts, a.words, a.entries, a.rows);
+  const size_t smem = size_t(kWarps) * S * MT * 2048 + size_t(2) * kWarps * NT * MT * 512 + lists_bytes(a.w.experts, a.entries, a.rows);
   const void* kernel = reinterpret_cast<const void*>(moe_kernel<T, NT, MT, S>);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e != cudaSuccess) return e;
@@ -552,7 +598,7 @@ cudaError_t moe(const MoEView& w, const void* x, int64_t xs, void* y, int64_t ys
     MoEArgs a;
     a.w = w;
     a.x = static_cast<const uint16_t*>(x) + t0 * xs, a.y = static_cast<uint16_t*>(y) + t0 * ys, a.xs = xs, a.ys = ys;
-    a.tokens = z.tokens, a.rows = z.tokens * w.top_k, a.words = z.words, a.entries = z.entries, a.splits = z.splits;
+    a.tokens = z.tokens, a.rows = z.tokens * w.top_k, a.entries = z.entries, a.splits = z.splits;
     uint8_t* p = static_cast<uint8_t*>(ws);
     a.logits = reinterpret_cast<double*>(p), p += z.logits;
     a.chosen = reinterpret_cast<int*>(p), p += z.chosen;

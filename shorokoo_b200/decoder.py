@@ -397,7 +397,7 @@ def _vector(x, name: str, device: torch.device, dtypes, n: int) -> int:
     _bad(f"{name} must be {n} contiguous values, got {tuple(x.shape)}")
 
 
-_pack_norm = struct.Struct("PPPPPqqqqqPPPPqqiiiifff").pack   # sb_residual_norm_args
+_pack_norm = struct.Struct("PPPPPqqqqqPPPPqqiiiifff4x").pack   # sb_residual_norm_args
 _pack_sampling = struct.Struct("PPPPfffi").pack              # sb_sampling
 
 
