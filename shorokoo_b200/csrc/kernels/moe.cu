@@ -1,4 +1,4 @@
-// A mixture-of-experts layer for a few tokens, in one cooperative kernel:
+// A mixture-of-experts layer for a few tokens:
 //   l = x R^T,  s = softmax(l) or 1 / (1 + e^-l),  the top_k largest s (+ selection bias), share_e = s_e (/ their sum) scale
 //   y = sum over the chosen e of share_e D_e (act(G_e x) * (U_e x))
 //
@@ -7,13 +7,14 @@
 // as its columns, so that a token more costs next to nothing. Its inputs' order in k does not matter as long as both
 // operands have the same, so a lane takes 8 neighbouring inputs of a row as its part of two products: weights come as
 // they lie in memory, in 16-byte pieces that only the lane that copied them reads (a cp.async ring per warp, without
-// barriers; it runs on over the ends of tiles and is filled for the second product while the grid waits for the first).
+// barriers, that runs on over the ends of tiles).
 // A tile of the first product holds 8 rows of G and the same 8 of U: a lane has gate and input of one feature.
 //
-// The phases, with the grid's barrier between them: the router's dot products; the choice, by every CTA for itself
-// where there are few tokens, and the lists of tokens per expert; the first product over (expert, features), its
-// k split over a CTA's warps; the second over (expert, outputs, part of k) into partial sums; their sum in the order
-// of a token's experts. No atomics decide an order: results repeat.
+// Four kernels in a chain, each launched while the one before it runs: the router's dot products and the choice, a cluster
+// per token; the first product over (expert, features), its k split over a CTA's warps; the second over (expert, outputs,
+// part of k) into partial sums, whose weights are on their way before the first has ended; their sum in the order of a
+// token's experts. No atomics decide an order: results repeat. (All of it in one cooperative launch took 33 us for a
+// token through 8 of 128 experts of 2048 x 768: such a launch and its three barriers cost 8 us, these four kernels 4.)
 // The router sums pieces of 8 products in fp32 and the pieces in fp64: a choice between experts whose scores are next
 // to each other hangs on it. Hidden values are rounded to the weights' type, the second product's operand; the rest
 // stays in fp32.
@@ -29,12 +30,10 @@ namespace sb {
 namespace k {
 namespace {
 
-#ifndef MU
-#define MU 4096
-#endif
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlock = 64;          // inputs of a step
-constexpr int kMostExperts = 512;   // of a lane's 16 scores
+constexpr int kMostExperts = 512;   // a lane has 16 scores
+constexpr int kRouteCtas = 8, kRouteThreads = 512;   // of a token's cluster
 
 struct Entry { int expert, first, count; };   // up to 8 NT places of the list, of one expert
 
@@ -46,7 +45,6 @@ struct MoEArgs {
   int tokens, rows;        // rows: tokens * top_k
   int entries;             // room for them
   int splits;              // of the second product's k
-  double* logits;          // [tokens][experts]
   int* chosen;             // [rows]
   float* share;            // [rows]
   void* hidden;            // [rows][inner]
@@ -123,38 +121,46 @@ __device__ __forceinline__ double router_dot(const MoEArgs& a, int t, int e, int
   return sum;
 }
 
-// The experts of a token and their shares, by a warp; equal scores go to the lower expert. J: scores per lane.
+// What only some layers need, in fp64 (not inline: the choice is a chain that runs once, and waits for its instructions):
+// the largest logit and the sum of e^(l - top) over all experts,
+template <int J> __device__ __noinline__ void sum_scores(const double (&v)[J], int experts, int lane, double& top, double& all) {
+  double t = -INFINITY, a = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (j * 32 + lane < experts) t = fmax(t, v[j]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) t = fmax(t, __shfl_xor_sync(~0u, t, d));
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (j * 32 + lane < experts) a += exp(v[j] - t);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) a += __shfl_xor_sync(~0u, a, d);
+  top = t, all = a;
+}
+// and the order of score + bias.
 template <int J>
-__device__ __noinline__ void choose(const MoEArgs& a, int t, int lane, int* chosen, float* share) {
-  const MoEView& w = a.w;
-  const double* l = a.logits + int64_t(t) * w.experts;
+__device__ __noinline__ void bias_keys(uint32_t (&key)[J], const double (&v)[J], const MoEView& w, int lane, double top, double all) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int e = j * 32 + lane;
+    if (e < w.experts) key[j] = ordered(float((w.softmax ? exp(v[j] - top) / all : 1.0 / (1.0 + exp(-v[j]))) + double(w.selection_bias[e])));
+  }
+}
+
+// The experts of a token and their shares from its logits, by a warp; equal scores go to the lower expert. J: scores per
+// lane.
+template <int J>
+__device__ __forceinline__ void choose(const MoEView& w, const double* l, int lane, int* chosen, float* share) {
   double v[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) v[j] = j * 32 + lane < w.experts ? __ldcg(l + j * 32 + lane) : 0.0;
+  for (int j = 0; j < J; ++j) v[j] = j * 32 + lane < w.experts ? l[j * 32 + lane] : 0.0;
   uint32_t key[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) key[j] = j * 32 + lane < w.experts ? ordered(float(v[j])) : 0u;
   double top = 0, all = 0;
   const bool biased = w.selection_bias != nullptr;
-  if (w.softmax && (biased || !w.normalize)) {   // needs the sum over all experts
-    top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (j * 32 + lane < w.experts) top = fmax(top, v[j]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, d));
-#pragma unroll 1
-    for (int e = lane; e < w.experts; e += 32) all += exp(__ldcg(l + e) - top);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
-  }
-  if (biased) {   // the order of score + bias, not that of the logits
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e = j * 32 + lane;
-      if (e < w.experts) key[j] = ordered(float((w.softmax ? exp(v[j] - top) / all : 1.0 / (1.0 + exp(-v[j]))) + double(w.selection_bias[e])));
-    }
-  }
+  if (w.softmax && (biased || !w.normalize)) sum_scores<J>(v, w.experts, lane, top, all);
+  if (biased) bias_keys<J>(key, v, w, lane, top, all);
   int mine = 0;          // lane r: the r-th chosen
   for (int r = 0; r < w.top_k; ++r) {
     uint32_t best = key[0];
@@ -172,7 +178,7 @@ __device__ __noinline__ void choose(const MoEArgs& a, int t, int lane, int* chos
     }
     if (lane == r) mine = int(e);
   }
-  const float z = float(__ldcg(l + mine));
+  const float z = float(l[mine]);
   float s;
   if (w.softmax) {
     const float high = w.normalize ? __shfl_sync(~0u, z, 0) : float(top);   // any shift serves; the first chosen is near the top
@@ -187,30 +193,129 @@ __device__ __noinline__ void choose(const MoEArgs& a, int t, int lane, int* chos
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
     s /= sum;
   } else if (w.softmax) {
-    s = float(exp(double(z) - top) / all);
+    s /= float(all);
   }
   if (lane < w.top_k) {
-    chosen[t * w.top_k + lane] = mine;
-    share[t * w.top_k + lane] = s * w.scale;
+    chosen[lane] = mine;
+    share[lane] = s * w.scale;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_constant__ MoEArgs a) {
+  __shared__ double logits[kMostExperts];   // of the cluster's first CTA
+  asm volatile("griddepcontrol.launch_dependents;");
+  const auto cluster = cooperative_groups::this_cluster();
+  const int t = blockIdx.x / kRouteCtas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double* to = cluster.map_shared_rank(logits, 0);
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;");   // the first CTA has begun, when the wait below is over
+  bool begun = false;
+  for (int e = warp * kRouteCtas + int(cluster.block_rank()); e < a.w.experts; e += kRouteCtas * (kRouteThreads / 32)) {
+    const double v = router_dot<T>(a, t, e, lane);
+    if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    begun = true;
+    if (lane == 0) to[e] = v;
+  }
+  if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  cluster.sync();
+  if (cluster.block_rank() == 0 && warp == 0) {
+    int* chosen = a.chosen + t * a.w.top_k;
+    float* share = a.share + t * a.w.top_k;
+    if (a.w.experts <= 128) choose<4>(a.w, logits, lane, chosen, share);
+    else choose<kMostExperts / 32>(a.w, logits, lane, chosen, share);
   }
 }
 
 // What a CTA knows of the step's rows (t * top_k + r: the r-th expert of token t), in shared memory.
 struct Lists {
   Entry* entry;        // [entries]
-  int* base;           // [experts] the first place of an expert's rows in the list
-  int* number;         // [experts] how many they are
+  int* number;         // [kWarps][experts] rows of an expert among a warp's quarter of them, then places before those
   int* chosen;         // [rows]
-  float* share;
   int* count;          // entries in use
   uint16_t* row;       // the list: [rows], by expert
-  uint16_t* place;     // [rows] among its expert's
+  uint16_t* place;     // [rows] among its expert's of its quarter
 };
 __host__ __device__ inline size_t lists_bytes(int experts, int entries, int rows) {
-  return size_t(entries) * sizeof(Entry) + size_t(experts) * 8 + size_t(rows) * 12 + 32;
+  return size_t(entries) * sizeof(Entry) + size_t(experts) * kWarps * 4 + size_t(rows) * 8 + 32;
 }
 
-// The two products. Units: (entry, tile of rows, part of k); a CTA takes every gridDim.x-th.
+// The rows by expert, in their order: all CTAs have to divide an expert's rows among its entries alike.
+template <int NT> __device__ __forceinline__ Lists make_lists(const MoEArgs& a, uint8_t* p, int tid) {
+  Lists at;
+  const int experts = a.w.experts, lane = tid & 31, warp = tid >> 5;
+  at.entry = reinterpret_cast<Entry*>(p), p += a.entries * sizeof(Entry);
+  at.number = reinterpret_cast<int*>(p), p += size_t(experts) * kWarps * 4;
+  at.chosen = reinterpret_cast<int*>(p), p += size_t(a.rows) * 4;
+  at.count = reinterpret_cast<int*>(p), p += 32;   // and the warps' sums
+  at.row = reinterpret_cast<uint16_t*>(p), p += size_t(a.rows) * 2;
+  at.place = reinterpret_cast<uint16_t*>(p);
+  if (a.tokens == 1) {   // an entry per row, in any order
+    if (tid < a.rows) at.entry[tid] = {__ldcg(a.chosen + tid), tid, 1}, at.row[tid] = uint16_t(tid);
+    if (tid == 0) *at.count = a.rows;
+    __syncthreads();
+    return at;
+  }
+  for (int i = tid; i < experts * kWarps; i += kThreads) at.number[i] = 0;
+  for (int i = tid; i < a.rows; i += kThreads) at.chosen[i] = __ldcg(a.chosen + i);
+  __syncthreads();
+  const int quarter = (a.rows + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  int* number = at.number + warp * experts;
+  for (int i0 = warp * quarter; i0 < min((warp + 1) * quarter, a.rows); i0 += 32) {
+    const int i = i0 + lane, e = i < a.rows ? at.chosen[i] : -1 - lane;
+    const uint32_t same = __match_any_sync(~0u, e), lower = same & ((1u << lane) - 1);
+    if (e >= 0) {
+      const int before = number[e];
+      at.place[i] = uint16_t(before + __popc(lower));
+      __syncwarp(same);
+      if (lower == 0) number[e] = before + __popc(same);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  // four experts per thread: where their rows begin, and their entries
+  constexpr int kEach = kMostExperts / kThreads;
+  int n[kEach], rows = 0, entries = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = tid * kEach + i;
+    n[i] = 0;
+    if (e < experts)
+      for (int w = 0; w < kWarps; ++w) n[i] += at.number[w * experts + e];
+    rows += n[i], entries += (n[i] + 8 * NT - 1) / (8 * NT);
+  }
+  int both = rows << 16 | entries;   // each below 2^15
+  const int own = both;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int before = __shfl_up_sync(~0u, both, d);
+    if (lane >= d) both += before;
+  }
+  if (lane == 31) at.count[1 + warp] = both;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) both += at.count[1 + w];
+  if (tid == kThreads - 1) *at.count = both & 0xffff;
+  rows = (both - own) >> 16, entries = (both - own) & 0xffff;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = tid * kEach + i;
+    for (int k = 0; k < n[i]; k += 8 * NT) at.entry[entries++] = {e, rows + k, min(8 * NT, n[i] - k)};
+    if (e < experts) {
+      int first = rows;
+      for (int w = 0; w < kWarps; ++w) {
+        const int m = at.number[w * experts + e];
+        at.number[w * experts + e] = first;
+        first += m;
+      }
+    }
+    rows += n[i];
+  }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kThreads) at.row[at.number[i / quarter * experts + at.chosen[i]] + at.place[i]] = uint16_t(i);
+  __syncthreads();
+  return at;
+}
+
+// The two products. Units: (entry, tile of rows, part of k); a CTA takes every ctas-th.
 template <typename T, int NT, int MT, int S, bool kFirst>
 struct Product {
   const MoEArgs& a;
@@ -218,7 +323,7 @@ struct Product {
   const uint32_t ring;   // this warp's
   float* sums;           // [2][kWarps][4 MT NT][32]
   const int lane, warp, g, t;
-  int units, tiles, parts, blocks, depth, out_rows;   // blocks of k in a part; depth: k; out_rows: rows of the weights (of each half)
+  int units, ctas, tiles, parts, blocks, depth, out_rows;   // blocks of k in a part; depth: k; out_rows: rows of the weights (of each half)
   int64_t expert_stride, row_stride, second;          // second: from a row to the one 8 further in the tile
   const uint16_t* weights;
   int copy_unit, copy_block, copy_end;   // the next step to copy
@@ -235,12 +340,15 @@ struct Product {
     blocks = (all + parts - 1) / parts;
     tiles = (out_rows + kTile - 1) / kTile;
     units = *at.count * tiles * parts;
+    ctas = int(gridDim.x);
+    if (units > 0) ctas = (units - 1) / ((units - 1) / ctas + 1) + 1;   // as few as take no longer
+    if (int(blockIdx.x) >= ctas) units = 0;
     expert_stride = kFirst ? a.w.up_expert : a.w.down_expert;
     row_stride = kFirst ? a.w.up_row : a.w.down_row;
     second = (kFirst ? int64_t(a.w.inner) : 8) * row_stride;
     weights = static_cast<const uint16_t*>(kFirst ? a.w.gate_up : a.w.down);
     stage_in = stage_out = 0;
-    copy_unit = blockIdx.x - gridDim.x;
+    copy_unit = int(blockIdx.x) - ctas;
     copy_block = copy_end = 0;
     next_unit();
   }
@@ -262,7 +370,7 @@ struct Product {
 
   __device__ __forceinline__ void next_unit() {   // to the next unit in which this warp has a step
     do {
-      copy_unit += gridDim.x;
+      copy_unit += ctas;
       if (copy_unit >= units) return;
       const Unit v = unit(copy_unit);
       copy_block = v.part * blocks + warp;
@@ -302,7 +410,7 @@ struct Product {
 
   __device__ __forceinline__ void run() {
     int turn = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    for (int u = blockIdx.x; u < units; u += ctas) {
       const Unit v = unit(u);
       const Entry en = at.entry[v.entry];
       const int used = (en.count + 7) / 8;   // column tiles
@@ -411,142 +519,64 @@ struct Product {
   }
 };
 
-template <typename T, int NT, int MT, int S>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) moe_kernel(const __grid_constant__ MoEArgs a) {
+template <typename T, int NT, int MT, int S, bool kFirst>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) product_kernel(const __grid_constant__ MoEArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  const auto grid = cooperative_groups::this_grid();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int experts = a.w.experts, top_k = a.w.top_k;
   constexpr int kRing = kWarps * S * MT * 2048, kSums = 2 * kWarps * NT * MT * 128 * 4;
-
-  for (int i = warp * gridDim.x + blockIdx.x; i < a.tokens * experts; i += kWarps * gridDim.x) {   // spread over the SMs first
-    const double v = router_dot<T>(a, i / experts, i % experts, lane);
-    if (lane == 0) a.logits[i] = v;
-  }
-  grid.sync();
-
-  Lists at;
-  {
-    uint8_t* p = smem + kRing + kSums;
-    at.entry = reinterpret_cast<Entry*>(p), p += a.entries * sizeof(Entry);
-    at.base = reinterpret_cast<int*>(p), p += size_t(experts) * 4;
-    at.number = reinterpret_cast<int*>(p), p += size_t(experts) * 4;
-    at.chosen = reinterpret_cast<int*>(p), p += size_t(a.rows) * 4;
-    at.share = reinterpret_cast<float*>(p), p += size_t(a.rows) * 4;
-    at.count = reinterpret_cast<int*>(p), p += 32;   // and the warps' sums
-    at.row = reinterpret_cast<uint16_t*>(p), p += size_t(a.rows) * 2;
-    at.place = reinterpret_cast<uint16_t*>(p);
-  }
-  for (int i = tid; i < experts; i += kThreads) at.number[i] = 0;
-  auto pick = [&](int t, int* chosen, float* share) {
-    if (experts <= 128) choose<4>(a, t, lane, chosen, share);
-    else choose<kMostExperts / 32>(a, t, lane, chosen, share);
-  };
-  if (a.tokens <= 2 * kWarps) {   // every CTA chooses for itself: cheaper than another barrier
-    for (int t = warp; t < a.tokens; t += kWarps) pick(t, at.chosen, at.share);
-    __syncthreads();
-  } else {
-    for (int t = warp * gridDim.x + blockIdx.x; t < a.tokens; t += kWarps * gridDim.x) pick(t, a.chosen, a.share);
-    grid.sync();
-    for (int i = tid; i < a.rows; i += kThreads) at.chosen[i] = __ldcg(a.chosen + i), at.share[i] = __ldcg(a.share + i);
-  }
-  __syncthreads();
-  if (warp == 0) {   // places in the order of the rows: all CTAs have to divide an expert's rows among its entries alike
-    for (int i0 = 0; i0 < a.rows; i0 += 32) {
-      const int i = i0 + lane, e = i < a.rows ? at.chosen[i] : -1 - lane;
-      const uint32_t same = __match_any_sync(~0u, e), lower = same & ((1u << lane) - 1);
-      if (e >= 0) {
-        const int before = at.number[e];
-        at.place[i] = uint16_t(before + __popc(lower));
-        __syncwarp(same);
-        if (lower == 0) at.number[e] = before + __popc(same);
-      }
-      __syncwarp();
-    }
-  }
-  __syncthreads();
-  {   // four experts per thread: where their rows begin, and their entries
-    int n[kMostExperts / kThreads], rows = 0, entries = 0;
-#pragma unroll
-    for (int i = 0; i < kMostExperts / kThreads; ++i) {
-      const int e = tid * (kMostExperts / kThreads) + i;
-      n[i] = e < experts ? at.number[e] : 0;
-      rows += n[i], entries += (n[i] + 8 * NT - 1) / (8 * NT);
-    }
-    int both = rows << 16 | entries;   // each below 2^15
-    const int own = both;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int before = __shfl_up_sync(~0u, both, d);
-      if (lane >= d) both += before;
-    }
-    if (lane == 31) at.count[1 + warp] = both;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) both += at.count[1 + w];
-    if (tid == kThreads - 1) *at.count = both & 0xffff;
-    rows = (both - own) >> 16, entries = (both - own) & 0xffff;
-#pragma unroll
-    for (int i = 0; i < kMostExperts / kThreads; ++i) {
-      const int e = tid * (kMostExperts / kThreads) + i;
-      if (e < experts) at.base[e] = rows;
-      for (int k = 0; k < n[i]; k += 8 * NT) at.entry[entries++] = {e, rows + k, min(8 * NT, n[i] - k)};
-      rows += n[i];
-    }
-  }
-  __syncthreads();
-  for (int i = tid; i < a.rows; i += kThreads) at.row[at.base[at.chosen[i]] + at.place[i]] = uint16_t(i);
-  __syncthreads();
-
+  // The choice is there: for the first product once the router has ended; the second is launched after that, as the first
+  // lets it begin behind its own wait.
+  if (kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const Lists at = make_lists<NT>(a, smem + kRing + kSums, tid);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S * MT * 2048;
-  float* sums = reinterpret_cast<float*>(smem + kRing);
-  {
-    Product<T, NT, MT, S, true> first(a, at, ring, sums, lane, warp);
-    first.fill();
-    first.run();
-    wait<0>();
-    Product<T, NT, MT, S, false> second(a, at, ring, sums, lane, warp);
-    second.fill();   // weights, while the grid finishes the hidden values
-    grid.sync();
-    second.run();
-    wait<0>();
-  }
-  grid.sync();
+  Product<T, NT, MT, S, kFirst> product(a, at, ring, reinterpret_cast<float*>(smem + kRing), lane, warp);
+  product.fill();   // weights, while the first product finishes the hidden values
+  if (!kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
+  product.run();
+  wait<0>();
+}
 
-  const int quads = a.w.width / 4;
-  for (int i = blockIdx.x * kThreads + tid; i < a.tokens * quads; i += gridDim.x * kThreads) {
-    const int t = i / quads, h = (i - t * quads) * 4;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* p = a.partial + int64_t(t) * top_k * a.w.width + h;
-    for (int r0 = 0; r0 < top_k; r0 += 4) {   // loads in flight together
-      float4 v[4];
+// y of four outputs of a token per thread
+template <typename T>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const __grid_constant__ MoEArgs a) {
+  const int quads = a.w.width / 4, top_k = a.w.top_k;
+  const int i = blockIdx.x * kThreads + threadIdx.x;
+  const int t = i / quads, h = (i - t * quads) * 4;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (t >= a.tokens) return;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* p = a.partial + int64_t(t) * top_k * a.w.width + h;
+  for (int r0 = 0; r0 < top_k; r0 += 4) {   // loads in flight together
+    float4 v[4];
+    float share[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (r0 + r < top_k) v[r] = __ldcg(reinterpret_cast<const float4*>(p + int64_t(r0 + r) * a.w.width));
-      for (int j = 1; j < a.splits; ++j) {
-        float4 u[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r0 + r < top_k) u[r] = __ldcg(reinterpret_cast<const float4*>(p + (int64_t(j) * a.rows + r0 + r) * a.w.width));
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (r0 + r < top_k) v[r].x += u[r].x, v[r].y += u[r].y, v[r].z += u[r].z, v[r].w += u[r].w;
+    for (int r = 0; r < 4; ++r)
+      if (r0 + r < top_k) {
+        v[r] = __ldcg(reinterpret_cast<const float4*>(p + int64_t(r0 + r) * a.w.width));
+        share[r] = __ldcg(a.share + t * top_k + r0 + r);
       }
+    for (int j = 1; j < a.splits; ++j) {
+      float4 u[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (r0 + r < top_k) {
-          const float s = at.share[t * top_k + r0 + r];
-          y.x += s * v[r].x, y.y += s * v[r].y, y.z += s * v[r].z, y.w += s * v[r].w;
-        }
+        if (r0 + r < top_k) u[r] = __ldcg(reinterpret_cast<const float4*>(p + (int64_t(j) * a.rows + r0 + r) * a.w.width));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < top_k) v[r].x += u[r].x, v[r].y += u[r].y, v[r].z += u[r].z, v[r].w += u[r].w;
     }
-    alignas(8) T out[4] = {Op<T>::round(y.x), Op<T>::round(y.y), Op<T>::round(y.z), Op<T>::round(y.w)};
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.y) + t * a.ys + h) = *reinterpret_cast<const uint2*>(out);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r0 + r < top_k) y.x += share[r] * v[r].x, y.y += share[r] * v[r].y, y.z += share[r] * v[r].z, y.w += share[r] * v[r].w;
   }
+  alignas(8) T out[4] = {Op<T>::round(y.x), Op<T>::round(y.y), Op<T>::round(y.z), Op<T>::round(y.w)};
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.y) + t * a.ys + h) = *reinterpret_cast<const uint2*>(out);
 }
 
 // Sizes of one launch over up to `tokens` tokens.
 struct Sizes {
   int tokens, entries, splits, columns;
-  size_t logits, chosen, hidden, partial, total;
+  size_t chosen, hidden, partial, total;
 };
 Sizes sizes(const MoEView& w, int64_t tokens) {
   Sizes z;
@@ -559,28 +589,45 @@ Sizes sizes(const MoEView& w, int64_t tokens) {
   // Parts of the second product's k, of 512 inputs or more, until (expert, tile, part) triples are many for every CTA
   const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + 15) / 16);
   z.splits = 1;
-  while (z.splits < 8 && units * z.splits < MU && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
+  while (z.splits < 8 && units * z.splits < 4096 && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  z.logits = up(size_t(z.tokens) * w.experts * 8);
   z.chosen = up(size_t(rows) * 4);
   z.hidden = up(size_t(rows) * w.inner * 2);
   z.partial = up(size_t(z.splits) * rows * w.width * 4);
-  z.total = z.logits + 2 * z.chosen + z.hidden + z.partial;
+  z.total = 2 * z.chosen + z.hidden + z.partial;
   return z;
 }
 
-template <typename T, int NT, int MT, int S>
-cudaError_t launch(MoEArgs a, int sms, cudaStream_t s) {
+cudaError_t enqueue(void (*kernel)(MoEArgs), const MoEArgs& a, int64_t grid, int threads, size_t smem, int cluster, bool after, cudaStream_t s) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(unsigned(grid)), c.blockDim = dim3(unsigned(threads)), c.dynamicSmemBytes = smem, c.stream = s;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster) at[n].id = cudaLaunchAttributeClusterDimension, at[n].val.clusterDim = {unsigned(cluster), 1, 1}, ++n;
+  if (after) at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[n].val.programmaticStreamSerializationAllowed = 1, ++n;
+  c.attrs = at, c.numAttrs = unsigned(n);
+  return cudaLaunchKernelEx(&c, kernel, a);
+}
+
+template <typename T, int NT, int MT, int S, bool kFirst>
+cudaError_t product(const MoEArgs& a, int sms, cudaStream_t s) {
   const size_t smem = size_t(kWarps) * S * MT * 2048 + size_t(2) * kWarps * NT * MT * 512 + lists_bytes(a.w.experts, a.entries, a.rows);
-  const void* kernel = reinterpret_cast<const void*>(moe_kernel<T, NT, MT, S>);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  const auto kernel = product_kernel<T, NT, MT, S, kFirst>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e != cudaSuccess) return e;
-  int each = 0;
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, kThreads, smem);
+  const int64_t each = std::min<int64_t>(NT == 1 ? 4 : 2, 227 * 1024 / (smem + 1024));
+  const int rows = kFirst ? a.w.inner : a.w.width, tile = kFirst ? 8 * MT : 16 * MT;
+  const int64_t units = int64_t(a.entries) * ((rows + tile - 1) / tile) * (kFirst ? 1 : a.splits);   // at most
+  return enqueue(kernel, a, std::min(units, std::max<int64_t>(each, 1) * sms), kThreads, smem, 0, true, s);
+}
+
+template <typename T>
+cudaError_t launch(const MoEArgs& a, int columns, int sms, cudaStream_t s) {
+  cudaError_t e = enqueue(route_kernel<T>, a, int64_t(a.tokens) * kRouteCtas, kRouteThreads, 0, kRouteCtas, false, s);
+  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, 1, 5, true>(a, sms, s) : product<T, 4, 2, 4, true>(a, sms, s);
+  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, 1, 5, false>(a, sms, s) : product<T, 4, 2, 4, false>(a, sms, s);
   if (e != cudaSuccess) return e;
-  if (each < 1) return cudaErrorInvalidConfiguration;
-  void* args[] = {&a};
-  return cudaLaunchCooperativeKernel(kernel, dim3(unsigned(each * sms)), dim3(kThreads), args, smem, s);
+  return enqueue(combine_kernel<T>, a, (int64_t(a.tokens) * (a.w.width / 4) + kThreads - 1) / kThreads, kThreads, 0, 0, true, s);
 }
 
 }  // namespace
@@ -600,14 +647,11 @@ cudaError_t moe(const MoEView& w, const void* x, int64_t xs, void* y, int64_t ys
     a.x = static_cast<const uint16_t*>(x) + t0 * xs, a.y = static_cast<uint16_t*>(y) + t0 * ys, a.xs = xs, a.ys = ys;
     a.tokens = z.tokens, a.rows = z.tokens * w.top_k, a.entries = z.entries, a.splits = z.splits;
     uint8_t* p = static_cast<uint8_t*>(ws);
-    a.logits = reinterpret_cast<double*>(p), p += z.logits;
     a.chosen = reinterpret_cast<int*>(p), p += z.chosen;
     a.share = reinterpret_cast<float*>(p), p += z.chosen;
     a.hidden = p, p += z.hidden;
     a.partial = reinterpret_cast<float*>(p);
-    cudaError_t e;
-    if (w.elem == 10) e = z.columns == 8 ? launch<__half, 1, 1, 6>(a, sms, s) : launch<__half, 4, 2, 4>(a, sms, s);
-    else e = z.columns == 8 ? launch<__nv_bfloat16, 1, 1, 6>(a, sms, s) : launch<__nv_bfloat16, 4, 2, 4>(a, sms, s);
+    const cudaError_t e = w.elem == 10 ? launch<__half>(a, z.columns, sms, s) : launch<__nv_bfloat16>(a, z.columns, sms, s);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
