@@ -29,17 +29,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-#ifndef ST
-#define ST 256
-#define SB 4
-#define SK 64
-#endif
-constexpr int kThreads = ST, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kMostCtas = 8;            // of a cluster
 constexpr int kHeld = 192 * 1024;       // bytes of a slice that fit shared memory
 constexpr int kCoarse = 128;            // bins of the first round of weights, per warp
-constexpr int kListBytes = 8192;        // of a list of candidates
+constexpr int kListBytes = 4096;       // of a list of candidates
 constexpr int kMostRounds = 6;          // 128 or 256 bins, then at least 128 each of what is left of 2^32 floats
 constexpr int kSteps = 64;              // table of 2^(-j / 64)
 
@@ -84,6 +79,18 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// 2^(30 - j / 64), rounded
+__constant__ uint32_t kPower[kSteps] = {
+    1073741824u, 1062175491u, 1050733751u, 1039415261u, 1028218693u, 1017142735u, 1006186087u, 995347464u,
+    984625594u, 974019220u, 963527098u, 953147997u, 942880699u, 932724001u, 922676710u, 912737649u,
+    902905651u, 893179563u, 883558244u, 874040567u, 864625413u, 855311680u, 846098274u, 836984114u,
+    827968132u, 819049271u, 810226483u, 801498734u, 792865000u, 784324269u, 775875538u, 767517817u,
+    759250125u, 751071493u, 742980960u, 734977579u, 727060411u, 719228525u, 711481005u, 703816941u,
+    696235434u, 688735596u, 681316545u, 673977412u, 666717336u, 659535466u, 652430958u, 645402981u,
+    638450708u, 631573326u, 624770026u, 618040012u, 611382493u, 604796689u, 598281827u, 591837143u,
+    585461881u, 579155293u, 572916640u, 566745190u, 560640218u, 554601009u, 548626854u, 542717053u,
+};
 
 struct alignas(16) Shared {
   // read by the other CTAs of the cluster; what rounds write anew is there twice and used in turn
@@ -181,7 +188,7 @@ __device__ __forceinline__ unsigned long long sum_upto(unsigned long long v, int
 }
 
 template <typename T, bool kHold>
-__global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -217,10 +224,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
   if (lane == 0) s.warp_top[warp] = most;
   if (tid < kBins) s.low[0][tid] = s.high[0][tid] = 0;
-  if (tid >= kThreads - kSteps) {
-    const int j = tid - (kThreads - kSteps);
-    s.power[j] = __double2uint_rn(exp2(30.0 - j * (1.0 / kSteps)));
-  }
+  if (tid < kSteps) s.power[tid] = kPower[tid];
   if (tid == 0) s.lowest = 0x7fffffff, s.least[0] = ~0u, s.most[0] = 0, s.listed[0] = 0, s.bin = 0, s.above = 0;
   __syncthreads();
   if (warp == 0) {
@@ -338,6 +342,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
               if (value<T>(e[j]) >= low) add(&s.part_low[warp][b[j]], &s.part_high[warp][b[j]], w[j]);
           }
         };
+        __syncwarp();
         if (none) {}
         else if (by_value) sums(even, near_weight);
         else if (near) sums(keys, near_weight);
@@ -372,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
       cluster.sync();
       if (tid < kBins) s.low[turn ^ 1][tid] = s.high[turn ^ 1][tid] = 0;   // all have read it, before this barrier
       if (tid == 0) s.least[turn ^ 1] = ~0u, s.most[turn ^ 1] = 0, s.listed[turn ^ 1] = 0;
+      __syncwarp();
       if (warp == 0) {   // neighbouring bins per lane
         unsigned long long n[kBins / 32], sum = 0;
         const int each = bins / 32;
@@ -463,13 +469,18 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
       } else {
         take(keys);
       }
+      __syncwarp();
       least = __reduce_min_sync(~0u, least), greatest = __reduce_max_sync(~0u, greatest);
       if (lane == 0 && greatest) atomicMin(&s.least[turn], least), atomicMax(&s.most[turn], greatest);
       cluster.sync();
-      for (int c = 0; c < ctas; ++c) {
-        const Shared* o = cluster.map_shared_rank(&s, c);
-        least = min(least, o->least[turn]), greatest = max(greatest, o->most[turn]);
+      __syncwarp();
+      if (lane < ctas) {
+        const Shared* o = cluster.map_shared_rank(&s, lane);
+        least = o->least[turn], greatest = o->most[turn];
+      } else {
+        least = ~0u, greatest = 0;
       }
+      least = __reduce_min_sync(~0u, least), greatest = __reduce_max_sync(~0u, greatest);
       low_key = least, high_key = greatest;
       listed = s.listed[next];
       list = listed <= kListed ? next : -1;
@@ -485,7 +496,9 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
     }
   };
   if (top_k < a.vocab) descend(false, top_k);
+  __syncwarp();
   if (top_p < 1.f) descend(true, 0);
+  __syncwarp();
 
   // ---- sums of the kept, per warp's part of the slice
   {
@@ -522,9 +535,24 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
           }
         }
       };
-      if (near) sums(near_weight);
-      else sums(far_weight);
+      if (border != lo || min_p > 0.f) {   // few: their weights alone
+        for (int q = part_begin + lane; q < part_end; q += 32) {
+          const uint4 p = piece(q);
+          const T* e = reinterpret_cast<const T*>(&p);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = value<T>(e[j]);
+            equal += v == last;
+            if (v > last) sum += weight(v);
+          }
+        }
+      } else if (near) {
+        sums(near_weight);
+      } else {
+        sums(far_weight);
+      }
     }
+    __syncwarp();
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
     equal = __reduce_add_sync(~0u, equal);
@@ -532,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
   }
   cluster.sync();
   // The part where the target falls: the sums and ties before it, of all CTAs' parts in order.
+  __syncwarp();
   if (warp == 0) {
     const unsigned long long tie = weight(of_key(border));
     constexpr int kParts = kMostCtas * kWarps / 32;
@@ -570,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
     const int x = min(first + tid * each, end), y = min(x + each, end);
     unsigned long long equal = 0;
     for (int i = x; i < y; ++i) equal += key_of(at(i)) == border;
+    __syncwarp();
     unsigned long long upto = sum_upto(equal, lane);
     if (lane == 31) s.scan[0][warp] = upto;
     __syncthreads();
@@ -583,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, SB) sample_kernel(const SampleArgs a
     };
     unsigned long long sum = 0, n = seen;
     for (int i = x; i < y; ++i) sum += kept(i, n);
+    __syncwarp();
     upto = sum_upto(sum, lane);
     if (lane == 31) s.scan[1][warp] = upto;
     __syncthreads();
@@ -625,7 +656,7 @@ cudaError_t sample(const void* logits, int64_t stride, int elem, int64_t rows, i
   const int size = elem == 1 ? 4 : 2;
   // CTAs per row: slices of at most 64 KB, so that several CTAs share an SM, and more while rows leave SMs idle
   int ctas = 1;
-  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * SK * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
+  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * 64 * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
   SampleArgs a = {logits, stride, uniform, by, tokens, vocab, 0};
   a.slice = int((int64_t(vocab) + ctas * 64 - 1) / (ctas * 64) * 64);
   const size_t held = size_t(a.slice) * size + 32;   // and the pieces' overhang
