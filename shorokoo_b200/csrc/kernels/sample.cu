@@ -51,6 +51,10 @@ template <typename T> __device__ __forceinline__ float value(T x);
 template <> __device__ __forceinline__ float value(float x) { return x; }
 template <> __device__ __forceinline__ float value(__half x) { return __half2float(x); }
 template <> __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T narrow(float x);   // of values that are T's
+template <> __device__ __forceinline__ float narrow(float x) { return x; }
+template <> __device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
 template <typename T> __device__ __forceinline__ T lowest();   // -inf
 template <> __device__ __forceinline__ float lowest() { return -INFINITY; }
 template <> __device__ __forceinline__ __half lowest() { return __ushort_as_half(0xfc00); }
@@ -102,7 +106,7 @@ struct alignas(16) Shared {
   uint32_t warp_ties[kWarps];
   // this CTA's own
   uint32_t power[kSteps];                   // 2^(30 - j / 64)
-  uint32_t part_low[kWarps][kCoarse], part_high[kWarps][kCoarse];   // sums of each warp's part of the slice
+  uint32_t part[3][kWarps][kCoarse];        // sums of each warp's part of the slice, of 16, 16 and 9 bits of the weights
   uint4 list[2][kListBytes / 16];
   int listed[2];
   unsigned long long scan[2][kWarps];
@@ -178,6 +182,15 @@ struct KeyBins {
   __device__ __forceinline__ int operator()(float v) const { return int((hi - key_of(v)) >> shift); }
 };
 
+// a / b rounded up, b > 0: from a quotient of doubles, which is off by little (a division of 64-bit integers takes five
+// times as long)
+__device__ __forceinline__ unsigned long long quotient(unsigned long long a, unsigned long long b) {
+  unsigned long long q = (unsigned long long)(double(a) / double(b));
+  while (q > 0 && q * b >= a) --q;
+  while (q * b < a) ++q;
+  return q;
+}
+
 __device__ __forceinline__ unsigned long long sum_upto(unsigned long long v, int lane) {   // of the lanes up to this one
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -213,6 +226,14 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
   };
   auto piece = [&](int q) { return kHold ? reinterpret_cast<const uint4*>(held)[q] : fetch(q); };
   auto at = [&](int i) { return value<T>(kHold ? held[i + shift] : from[i]); };
+  // The elements of a piece that are wanted, one by one: a warp goes on with as many as its lanes have at most, not with all
+  // that any lane has.
+  auto each_of = [&](int q, uint32_t wanted, auto&& f) {
+    while (wanted) {
+      f(at(q * kV - shift + __ffs(int(wanted)) - 1));
+      wanted &= wanted - 1;
+    }
+  };
   float most = -INFINITY;
 #pragma unroll 4
   for (int q = tid; q < pieces; q += kThreads) {
@@ -302,9 +323,13 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
   int summed = 0;
   EvenBins coarse;
   KeyBins coarse_keys;
+  auto part_sum = [&](int w, int b) {
+    return s.part[0][w][b] + (static_cast<unsigned long long>(s.part[1][w][b]) << 16) + (static_cast<unsigned long long>(s.part[2][w][b]) << 32);
+  };
   // Finds the key at which the sums from the top reach a target: of counts, or of weights. The ties of a border found
   // before are not summed one by one, but by their number.
-  auto descend = [&](const bool by_mass, unsigned long long target) {
+  auto descend = [&](const bool by_mass) {
+    unsigned long long target = top_k;
     const bool floored = by_mass && ties < (unsigned long long)a.vocab;
     const uint32_t floor = border;
     const unsigned long long floor_weight = floored ? weight(of_key(floor)) : 0, floor_sum = floored ? ties * floor_weight : 0;
@@ -325,33 +350,51 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
         const uint32_t h = uint32_t(w >> 32) + (old + l < old);
         if (h) atomicAdd(upper, h);
       };
+      auto add_part = [&](int b, unsigned long long w) {   // without a carry: atomics that return nothing are faster
+        atomicAdd(&s.part[0][warp][b], uint32_t(w) & 0xffffu);
+        const uint32_t m = uint32_t(w) >> 16, h = uint32_t(w >> 32);
+        if (m) atomicAdd(&s.part[1][warp][b], m);
+        if (h) atomicAdd(&s.part[2][warp][b], h);
+      };
       if (round == 0 && by_mass) {
-        for (int i = tid; i < kWarps * kCoarse; i += kThreads) (&s.part_low[0][0])[i] = 0, (&s.part_high[0][0])[i] = 0;
+        for (int i = tid; i < 3 * kWarps * kCoarse; i += kThreads) (&s.part[0][0][0])[i] = 0;
         __syncthreads();
         binned = true, coarse_even = by_value, coarse = even, coarse_keys = keys;
         auto sums = [&](const auto& bin, const auto& weight) {
           for (int q = part_begin + lane; q < part_end; q += 32) {
             const uint4 p = piece(q);
             const T* e = reinterpret_cast<const T*>(&p);
-            unsigned long long w[kV];
-            int b[kV];
 #pragma unroll
-            for (int j = 0; j < kV; ++j) w[j] = weight(value<T>(e[j])), b[j] = bin(value<T>(e[j]));
+            for (int j0 = 0; j0 < kV; j0 += 4) {
+              unsigned long long w[4];
+              int b[4];
 #pragma unroll
-            for (int j = 0; j < kV; ++j)
-              if (value<T>(e[j]) >= low) add(&s.part_low[warp][b[j]], &s.part_high[warp][b[j]], w[j]);
+              for (int j = 0; j < 4; ++j) w[j] = weight(value<T>(e[j0 + j])), b[j] = bin(value<T>(e[j0 + j]));
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (value<T>(e[j0 + j]) >= low) add_part(b[j], w[j]);
+            }
+          }
+        };
+        auto few = [&] {   // the weights of those that count alone
+          for (int q = part_begin + lane; q < part_end; q += 32) {
+            const uint4 p = piece(q);
+            const T* e = reinterpret_cast<const T*>(&p);
+            uint32_t mine = 0;
+#pragma unroll
+            for (int j = 0; j < kV; ++j) mine |= uint32_t(value<T>(e[j]) >= low) << j;
+            each_of(q, mine, [&](float v) { add_part(by_value ? even(v) : keys(v), weight(v)); });
           }
         };
         __syncwarp();
         if (none) {}
-        else if (by_value) sums(even, near_weight);
-        else if (near) sums(keys, near_weight);
-        else sums(keys, far_weight);
+        else if (by_value && !floored && !(min_p > 0.f)) sums(even, near_weight);
+        else few();
         __syncthreads();
         if (tid < kCoarse) {
           unsigned long long n = 0;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) n += s.part_low[w][tid] + (static_cast<unsigned long long>(s.part_high[w][tid]) << 32);
+          for (int w = 0; w < kWarps; ++w) n += part_sum(w, tid);
           s.low[turn][tid] = uint32_t(n), s.high[turn][tid] = uint32_t(n >> 32);
         }
       } else {
@@ -383,18 +426,24 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
         const int each = bins / 32;
 #pragma unroll
         for (int i = 0; i < kBins / 32; ++i) n[i] = 0;
-        for (int c = 0; c < ctas; ++c) {
-          const Shared* o = cluster.map_shared_rank(&s, c);
 #pragma unroll
-          for (int i = 0; i < kBins / 32; i += 4) {
-            if (i >= each) break;
-            const uint4 l = *reinterpret_cast<const uint4*>(o->low[turn] + lane * each + i);
-            n[i] += l.x, n[i + 1] += l.y, n[i + 2] += l.z, n[i + 3] += l.w;
-            if (by_mass) {
-              const uint4 h = *reinterpret_cast<const uint4*>(o->high[turn] + lane * each + i);
-              n[i] += static_cast<unsigned long long>(h.x) << 32, n[i + 1] += static_cast<unsigned long long>(h.y) << 32;
-              n[i + 2] += static_cast<unsigned long long>(h.z) << 32, n[i + 3] += static_cast<unsigned long long>(h.w) << 32;
+        for (int i = 0; i < kBins / 32; i += 4) {
+          if (i >= each) break;
+          const int at = lane * each + i;
+          for (int c0 = 0; c0 < ctas; c0 += 2) {   // loads in flight together
+            uint4 l[2], h[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const Shared* o = cluster.map_shared_rank(&s, min(c0 + c, ctas - 1));
+              l[c] = *reinterpret_cast<const uint4*>(o->low[turn] + at);
+              h[c] = by_mass ? *reinterpret_cast<const uint4*>(o->high[turn] + at) : make_uint4(0, 0, 0, 0);
             }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              if (c0 + c < ctas) {
+                n[i] += l[c].x + (static_cast<unsigned long long>(h[c].x) << 32), n[i + 1] += l[c].y + (static_cast<unsigned long long>(h[c].y) << 32);
+                n[i + 2] += l[c].z + (static_cast<unsigned long long>(h[c].z) << 32), n[i + 3] += l[c].w + (static_cast<unsigned long long>(h[c].w) << 32);
+              }
           }
         }
 #pragma unroll
@@ -419,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
       target = s.target;
       if (s.outcome) {   // no border among these
         if (by_mass) {   // but among the ties of the one there is
-          ties = (target - s.all + floor_weight - 1) / floor_weight;
+          ties = quotient(target - s.all, floor_weight);
           summed = bins;
         }
         turn ^= 1;
@@ -448,13 +497,11 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
           }
           if (mine) {
             int i = atomicAdd(&s.listed[next], __popc(mine));
-#pragma unroll
-            for (int j = 0; j < kV; ++j)
-              if (mine >> j & 1) {
-                see(value<T>(e[j]));
-                if (i < kListed) to[i] = e[j];
-                ++i;
-              }
+            each_of(q, mine, [&](float v) {
+              see(v);
+              if (i < kListed) to[i] = narrow<T>(v);
+              ++i;
+            });
           }
         }
       };
@@ -490,14 +537,16 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
     border = low_key;
     if (by_mass) {
       const unsigned long long w = weight(of_key(border));
-      ties = w ? (target - above + w - 1) / w : 0;
+      ties = w ? quotient(target - above, w) : 0;
     } else {
       ties = target - above;
     }
   };
-  if (top_k < a.vocab) descend(false, top_k);
-  __syncwarp();
-  if (top_p < 1.f) descend(true, 0);
+#pragma unroll 1
+  for (int filter = 0; filter < 2; ++filter) {
+    __syncwarp();
+    if (filter == 0 ? top_k < a.vocab : top_p < 1.f) descend(filter == 1);
+  }
   __syncwarp();
 
   // ---- sums of the kept, per warp's part of the slice
@@ -506,17 +555,19 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
     uint32_t equal = 0;
     const float last = of_key(border);
     if (binned) {   // of the bins above the border's, and what of that is above the border
-      for (int b = lane; b < summed; b += 32) sum += s.part_low[warp][b] + (static_cast<unsigned long long>(s.part_high[warp][b]) << 32);
+      for (int b = lane; b < summed; b += 32) sum += part_sum(warp, b);
       auto rest = [&](const auto& bin) {
         for (int q = part_begin + lane; q < part_end; q += 32) {
           const uint4 p = piece(q);
           const T* e = reinterpret_cast<const T*>(&p);
+          uint32_t mine = 0;
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
             const float v = value<T>(e[j]);
             equal += v == last;
-            if (v > last && bin(v) >= summed) sum += weight(v);
+            mine |= uint32_t(v > last && bin(v) >= summed) << j;
           }
+          each_of(q, mine, [&](float v) { sum += weight(v); });
         }
       };
       if (coarse_even) rest(coarse);
@@ -539,12 +590,14 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
         for (int q = part_begin + lane; q < part_end; q += 32) {
           const uint4 p = piece(q);
           const T* e = reinterpret_cast<const T*>(&p);
+          uint32_t mine = 0;
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
             const float v = value<T>(e[j]);
             equal += v == last;
-            if (v > last) sum += weight(v);
+            mine |= uint32_t(v > last) << j;
           }
+          each_of(q, mine, [&](float v) { sum += weight(v); });
         }
       } else if (near) {
         sums(near_weight);
@@ -592,6 +645,8 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
   __syncthreads();
   const int chosen = s.chosen;
   const unsigned long long target = s.target, tie = s.tie, before = s.before, ties_before = s.ties_before;
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // nothing more is read of the others
   if (chosen / kWarps == rank) {   // this CTA's: its threads take the part's neighbouring elements
     const int w = chosen % kWarps;
     const int first = max(0, w * part * kV - shift), end = min(count, (w + 1) * part * kV - shift);
@@ -630,7 +685,8 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
       }
     }
   }
-  cluster.sync();   // the others may still read this CTA's numbers
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // nor of this CTA
 }
 
 template <typename T, bool kHold>
