@@ -31,9 +31,10 @@ namespace k {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kStages = 5, kWideStages = 4;   // steps of a ring
 constexpr int kBlock = 64;          // inputs of a step
 constexpr int kMostExperts = 512;   // a lane has 16 scores
-constexpr int kRouteCtas = 8, kRouteThreads = 512;   // of a token's cluster
+constexpr int kRouteCtas = 8, kRouteThreads = 512;   // of a token's cluster, at most
 
 struct Entry { int expert, first, count; };   // up to 8 NT places of the list, of one expert
 
@@ -206,11 +207,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const __grid_const
   __shared__ double logits[kMostExperts];   // of the cluster's first CTA
   asm volatile("griddepcontrol.launch_dependents;");
   const auto cluster = cooperative_groups::this_cluster();
-  const int t = blockIdx.x / kRouteCtas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int ctas = int(cluster.num_blocks()), t = blockIdx.x / ctas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double* to = cluster.map_shared_rank(logits, 0);
   asm volatile("barrier.cluster.arrive.relaxed.aligned;");   // the first CTA has begun, when the wait below is over
   bool begun = false;
-  for (int e = warp * kRouteCtas + int(cluster.block_rank()); e < a.w.experts; e += kRouteCtas * (kRouteThreads / 32)) {
+  for (int e = warp * ctas + int(cluster.block_rank()); e < a.w.experts; e += ctas * (kRouteThreads / 32)) {
     const double v = router_dot<T>(a, t, e, lane);
     if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     begun = true;
@@ -315,46 +316,44 @@ template <int NT> __device__ __forceinline__ Lists make_lists(const MoEArgs& a, 
   return at;
 }
 
-// The two products. Units: (entry, tile of rows, part of k); a CTA takes every ctas-th.
-template <typename T, int NT, int MT, int S, bool kFirst>
+__device__ __forceinline__ float activated(int gelu, float gate, float up) {
+  return (gelu ? 0.5f * gate * (1.f + erff(gate * 0.70710678f)) : gate / (1.f + expf(-gate))) * up;
+}
+
+// The two products, for up to 8 rows of an expert. Units: (entry, tile of 8 features or 16 outputs, part of k); a CTA takes
+// every gridDim.x-th, its warps every kWarps-th block of k.
+template <typename T, bool kFirst>
 struct Product {
+  static constexpr int kTile = kFirst ? 8 : 16, kStage = 2048;   // bytes of a step: 16 rows of 64 inputs
   const MoEArgs& a;
   const Lists& at;
   const uint32_t ring;   // this warp's
-  float* sums;           // [2][kWarps][4 MT NT][32]
+  float* sums;           // [2][kWarps][4][32]
   const int lane, warp, g, t;
-  int units, ctas, tiles, parts, blocks, depth, out_rows;   // blocks of k in a part; depth: k; out_rows: rows of the weights (of each half)
-  int64_t expert_stride, row_stride, second;          // second: from a row to the one 8 further in the tile
+  int units, tiles, parts, blocks, depth, out_rows;   // blocks of k in a part; depth: k; out_rows: rows of the weights (of each half)
+  int64_t expert_stride, row_stride, second;          // second: from a row to the one that is 8 further in the tile
   const uint16_t* weights;
   int copy_unit, copy_block, copy_end;   // the next step to copy
   const uint16_t* copy_from;
-  uint32_t copy_there;                   // bit 2 m + r: those rows exist
+  bool copy_second;                      // whether the tile has its second 8 rows
   int stage_in, stage_out;
 
-  __device__ __forceinline__ Product(const MoEArgs& args, const Lists& lists, uint32_t ring_at, float* sums_at, int lane_no, int warp_no)
-      : a(args), at(lists), ring(ring_at), sums(sums_at), lane(lane_no), warp(warp_no), g(lane_no >> 2), t(lane_no & 3) {
+  __device__ __forceinline__ Product(const MoEArgs& args, const Lists& lists, uint32_t ring_at, float* sums_at)
+      : a(args), at(lists), ring(ring_at), sums(sums_at), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
     depth = kFirst ? a.w.width : a.w.inner;
     out_rows = kFirst ? a.w.inner : a.w.width;
     parts = kFirst ? 1 : a.splits;
-    const int all = (depth + kBlock - 1) / kBlock;
-    blocks = (all + parts - 1) / parts;
+    blocks = ((depth + kBlock - 1) / kBlock + parts - 1) / parts;
     tiles = (out_rows + kTile - 1) / kTile;
     units = *at.count * tiles * parts;
-    ctas = int(gridDim.x);
-    if (units > 0) ctas = (units - 1) / ((units - 1) / ctas + 1) + 1;   // as few as take no longer
-    if (int(blockIdx.x) >= ctas) units = 0;
     expert_stride = kFirst ? a.w.up_expert : a.w.down_expert;
     row_stride = kFirst ? a.w.up_row : a.w.down_row;
     second = (kFirst ? int64_t(a.w.inner) : 8) * row_stride;
     weights = static_cast<const uint16_t*>(kFirst ? a.w.gate_up : a.w.down);
     stage_in = stage_out = 0;
-    copy_unit = int(blockIdx.x) - ctas;
-    copy_block = copy_end = 0;
+    copy_unit = int(blockIdx.x) - int(gridDim.x);
     next_unit();
   }
-  static constexpr int kTile = kFirst ? 8 * MT : 16 * MT;   // rows (features) of a unit
-  static constexpr int kApart = kFirst ? 8 : 16;            // between a unit's products
-
   struct Unit { int entry, first, part; };
   __device__ __forceinline__ Unit unit(int u) const {
     Unit v;
@@ -364,111 +363,79 @@ struct Product {
     v.first = (e - v.entry * tiles) * kTile;
     return v;
   }
-  __device__ __forceinline__ int end_of(const Unit& v) const {
-    return min((v.part + 1) * blocks, (depth + kBlock - 1) / kBlock);
-  }
+  __device__ __forceinline__ int end_of(const Unit& v) const { return min((v.part + 1) * blocks, (depth + kBlock - 1) / kBlock); }
 
   __device__ __forceinline__ void next_unit() {   // to the next unit in which this warp has a step
     do {
-      copy_unit += ctas;
+      copy_unit += int(gridDim.x);
       if (copy_unit >= units) return;
       const Unit v = unit(copy_unit);
       copy_block = v.part * blocks + warp;
       copy_end = end_of(v);
       copy_from = weights + at.entry[v.entry].expert * expert_stride + (v.first + g) * row_stride + 8 * t;
-      copy_there = 0;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (v.first + m * kApart + g < out_rows) copy_there |= 1u << (2 * m);
-        if (v.first + m * kApart + g + (kFirst ? 0 : 8) < out_rows) copy_there |= 2u << (2 * m);
-      }
+      copy_second = kFirst || v.first + 8 < out_rows;   // (features and outputs come in eights)
     } while (copy_block >= copy_end);
   }
   __device__ __forceinline__ void copy_step() {
     if (copy_unit < units) {
-      const uint32_t to = ring + stage_in * (MT * 2048) + lane * 16;
+      const uint32_t to = ring + stage_in * kStage + lane * 16;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = copy_block * kBlock + h * 32;
-            const bool there = (copy_there >> (2 * m + r) & 1) && k + 8 * t < depth;
-            copy16(to + ((m * 2 + r) * 2 + h) * 512, there ? copy_from + m * kApart * row_stride + r * second + k : weights, there);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int k = copy_block * kBlock + h * 32;
+          const bool there = (r == 0 || copy_second) && k + 8 * t < depth;
+          copy16(to + (r * 2 + h) * 512, there ? copy_from + r * second + k : weights, there);
+        }
       copy_block += kWarps;
       if (copy_block >= copy_end) next_unit();
     }
     commit();
-    stage_in = stage_in + 1 == S ? 0 : stage_in + 1;
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
   }
   __device__ __forceinline__ void fill() {
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) copy_step();
+    for (int i = 0; i < kStages - 1; ++i) copy_step();
   }
 
   __device__ __forceinline__ void run() {
     int turn = 0;
-    for (int u = blockIdx.x; u < units; u += ctas) {
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit v = unit(u);
       const Entry en = at.entry[v.entry];
-      const int used = (en.count + 7) / 8;   // column tiles
       const uint16_t* rows = at.row + en.first;
-      const uint16_t* column[NT];
+      const uint16_t* column = nullptr;   // of the lane's token
+      if (g < en.count)
+        column = kFirst ? static_cast<const uint16_t*>(a.x) + rows[g] / a.w.top_k * a.xs : static_cast<const uint16_t*>(a.hidden) + int64_t(rows[g]) * a.w.inner;
+      auto fetch = [&](uint4 (&b)[2], int block) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int c = n * 8 + g;
-        column[n] = nullptr;
-        if (c < en.count)
-          column[n] = kFirst ? static_cast<const uint16_t*>(a.x) + rows[c] / a.w.top_k * a.xs
-                             : static_cast<const uint16_t*>(a.hidden) + int64_t(rows[c]) * a.w.inner;
-      }
-      auto fetch = [&](uint4 (&b)[NT][2], int block) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = block * kBlock + h * 32 + 8 * t;
-            b[n][h] = make_uint4(0, 0, 0, 0);
-            if (column[n] != nullptr && k < depth) b[n][h] = *reinterpret_cast<const uint4*>(column[n] + k);
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int k = block * kBlock + h * 32 + 8 * t;
+          b[h] = make_uint4(0, 0, 0, 0);
+          if (column != nullptr && k < depth) b[h] = *reinterpret_cast<const uint4*>(column + k);
+        }
       };
-      float d[NT][MT][4];
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      auto step = [&](const uint4 (&b)[2]) {
+        wait<kStages - 2>();
+        const uint32_t from = ring + stage_out * kStage + lane * 16;
+        stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
+        uint4 w[2][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[n][m][i] = 0.f;
-      const int end = end_of(v);
-      auto step = [&](const uint4 (&b)[NT][2]) {
-        wait<S - 2>();
-        const uint32_t from = ring + stage_out * (MT * 2048) + lane * 16;
-        stage_out = stage_out + 1 == S ? 0 : stage_out + 1;
-        uint4 w[MT][2][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[m][r][h] = shared16(from + ((m * 2 + r) * 2 + h) * 512);
+          for (int h = 0; h < 2; ++h) w[r][h] = shared16(from + (r * 2 + h) * 512);
         copy_step();   // into the stage read in the step before
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (NT > 1 && n >= used) break;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              Op<T>::mma(d[n][m], w[m][0][h].x, w[m][1][h].x, w[m][0][h].y, w[m][1][h].y, b[n][h].x, b[n][h].y);
-              Op<T>::mma(d[n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b[n][h].z, b[n][h].w);
-            }
+        for (int h = 0; h < 2; ++h) {
+          Op<T>::mma(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, b[h].x, b[h].y);
+          Op<T>::mma(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, b[h].z, b[h].w);
         }
       };
       // Columns are fetched a step ahead, into registers of their own by turns (a copy between them would wait for them).
-      uint4 even[NT][2], odd[NT][2];
+      const int end = end_of(v);
       int block = v.part * blocks + warp;
+      uint4 even[2], odd[2];
       if (block < end) fetch(even, block);
       while (block < end) {
         if (block + kWarps < end) fetch(odd, block + kWarps);
@@ -480,61 +447,212 @@ struct Product {
         block += kWarps;
       }
       // The warps' sums meet; two buffers in turn, so that one barrier is enough.
-      constexpr int kEach = NT * MT * 4 * 32;
-      float* all = sums + turn * kWarps * kEach;
+      float* all = sums + turn * kWarps * 128;
       turn ^= 1;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (NT > 1 && n >= used) break;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) all[warp * kEach + ((n * MT + m) * 4 + i) * 32 + lane] = d[n][m][i];
-      }
+      for (int i = 0; i < 4; ++i) all[warp * 128 + i * 32 + lane] = d[i];
       __syncthreads();
-      auto total = [&](int q) {
-        float s = all[q];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) s += all[w * kEach + q];
-        return s;
-      };
+      auto total = [&](int q) { return all[q] + all[128 + q] + all[256 + q] + all[384 + q]; };
+      static_assert(kWarps == 4, "the sum above");
+      const int l = threadIdx.x & 31, q = threadIdx.x >> 5;   // a value of the tile per thread, or a pair of them
+      const int c = (l & 3) * 2 + (q & 1);
       if (kFirst) {
-        for (int i = threadIdx.x; i < used * MT * 64; i += kThreads) {
-          const int l = i & 31, odd = i >> 5 & 1, nm = i >> 6, n = nm / MT, m = nm - n * MT;
-          const int c = n * 8 + (l & 3) * 2 + odd, f = v.first + m * kApart + (l >> 2);
-          if (c < en.count && f < out_rows) {
-            const float gate = total((nm * 4 + odd) * 32 + l), up = total((nm * 4 + odd + 2) * 32 + l);
-            const float act = a.w.gelu ? 0.5f * gate * (1.f + erff(gate * 0.70710678f)) : gate / (1.f + expf(-gate));
-            static_cast<T*>(a.hidden)[int64_t(rows[c]) * a.w.inner + f] = Op<T>::round(act * up);
-          }
-        }
+        if (q < 2 && c < en.count)
+          static_cast<T*>(a.hidden)[int64_t(rows[c]) * a.w.inner + v.first + (l >> 2)] = Op<T>::round(activated(a.w.gelu, total(q * 32 + l), total((q + 2) * 32 + l)));
       } else {
-        for (int i = threadIdx.x; i < used * MT * 128; i += kThreads) {
-          const int l = i & 31, q = i >> 5 & 3, nm = i >> 7, n = nm / MT, m = nm - n * MT;
-          const int c = n * 8 + (l & 3) * 2 + (q & 1), r = v.first + m * kApart + (q >> 1) * 8 + (l >> 2);
-          if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + rows[c]) * out_rows + r] = total((nm * 4 + q) * 32 + l);
-        }
+        const int r = v.first + (q >> 1) * 8 + (l >> 2);
+        if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + rows[c]) * out_rows + r] = total(q * 32 + l);
       }
     }
   }
 };
 
-template <typename T, int NT, int MT, int S, bool kFirst>
+// The same for experts of many tokens, 32 at a time: there the columns weigh as much as the weights, so a CTA's warps share
+// them (in shared memory, swizzled by 16-byte pieces) and have rows of their own, over all of k.
+template <typename T, bool kFirst>
+struct WideProduct {
+  static constexpr int NT = 4, MT = 2;
+  static constexpr int kWarpRows = kFirst ? 8 * MT : 16 * MT, kTile = kWarps * kWarpRows, kApart = kFirst ? 8 : 16;
+  static constexpr int kStage = kWarps * MT * 2048 + NT * 8 * 128;
+  const MoEArgs& a;
+  const Lists& at;
+  const uint32_t ring;
+  const int tid, lane, warp, g, t;
+  int units, tiles, parts, blocks, depth, out_rows;
+  int64_t expert_stride, row_stride, second;
+  const uint16_t* weights;
+  int copy_unit, copy_block, copy_end;
+  const uint16_t* copy_from;
+  const uint16_t* copy_column;   // of the token that this thread copies, or null
+  uint32_t copy_there;
+  int stage_in, stage_out;
+
+  __device__ __forceinline__ WideProduct(const MoEArgs& args, const Lists& lists, uint32_t ring_at)
+      : a(args), at(lists), ring(ring_at), tid(threadIdx.x), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g(lane >> 2), t(lane & 3) {
+    depth = kFirst ? a.w.width : a.w.inner;
+    out_rows = kFirst ? a.w.inner : a.w.width;
+    parts = kFirst ? 1 : a.splits;
+    blocks = ((depth + kBlock - 1) / kBlock + parts - 1) / parts;
+    tiles = (out_rows + kTile - 1) / kTile;
+    units = *at.count * tiles * parts;
+    expert_stride = kFirst ? a.w.up_expert : a.w.down_expert;
+    row_stride = kFirst ? a.w.up_row : a.w.down_row;
+    second = (kFirst ? int64_t(a.w.inner) : 8) * row_stride;
+    weights = static_cast<const uint16_t*>(kFirst ? a.w.gate_up : a.w.down);
+    stage_in = stage_out = 0;
+    copy_unit = int(blockIdx.x) - int(gridDim.x);
+    next_unit();
+  }
+  struct Unit { int entry, first, part, begin, end; };
+  __device__ __forceinline__ Unit unit(int u) const {   // entries innermost: those of one expert read its weights together
+    Unit v;
+    const int e = u / *at.count;
+    v.entry = u - e * *at.count;
+    v.part = e % parts;
+    v.first = e / parts * kTile;
+    v.begin = v.part * blocks;
+    v.end = min(v.begin + blocks, (depth + kBlock - 1) / kBlock);
+    return v;
+  }
+  __device__ __forceinline__ void next_unit() {
+    do {
+      copy_unit += int(gridDim.x);
+      if (copy_unit >= units) return;
+      const Unit v = unit(copy_unit);
+      const Entry en = at.entry[v.entry];
+      copy_block = v.begin, copy_end = v.end;
+      copy_from = weights + en.expert * expert_stride + (v.first + warp * kWarpRows + g) * row_stride + 8 * t;
+      copy_there = 0;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int r = v.first + warp * kWarpRows + m * kApart + g;
+        if (r < out_rows) copy_there |= 1u << (2 * m);
+        if (r + (kFirst ? 0 : 8) < out_rows) copy_there |= 2u << (2 * m);
+      }
+      copy_column = nullptr;
+      if (tid / 4 < en.count) {
+        const int row = at.row[en.first + tid / 4];
+        copy_column = kFirst ? static_cast<const uint16_t*>(a.x) + row / a.w.top_k * a.xs : static_cast<const uint16_t*>(a.hidden) + int64_t(row) * a.w.inner;
+      }
+    } while (copy_block >= copy_end);
+  }
+  __device__ __forceinline__ void copy_step() {
+    if (copy_unit < units) {
+      const uint32_t stage = ring + stage_in * kStage, to = stage + warp * (MT * 2048) + lane * 16;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = copy_block * kBlock + h * 32;
+            const bool there = (copy_there >> (2 * m + r) & 1) && k + 8 * t < depth;
+            copy16(to + ((m * 2 + r) * 2 + h) * 512, there ? copy_from + m * kApart * row_stride + r * second + k : weights, there);
+          }
+      const int token = tid / 4;   // two of its 8 pieces
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = (tid % 4) * 2 + i, k = copy_block * kBlock + c * 8;
+        const bool there = copy_column != nullptr && k < depth;
+        copy16(stage + kWarps * MT * 2048 + token * 128 + ((c ^ (token & 7)) * 16), there ? copy_column + k : weights, there);
+      }
+      if (++copy_block >= copy_end) next_unit();
+    }
+    commit();
+    stage_in = stage_in + 1 == kWideStages ? 0 : stage_in + 1;
+  }
+  __device__ __forceinline__ void run() {
+#pragma unroll
+    for (int i = 0; i < kWideStages - 1; ++i) copy_step();
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const Unit v = unit(u);
+      const Entry en = at.entry[v.entry];
+      const int used = (en.count + 7) / 8;
+      float d[NT][MT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[n][m][i] = 0.f;
+      for (int block = v.begin; block < v.end; ++block) {
+        wait<kWideStages - 2>();
+        __syncthreads();   // all copies of this step are there, and all have read the step before
+        const uint32_t stage = ring + stage_out * kStage, from = stage + warp * (MT * 2048) + lane * 16;
+        stage_out = stage_out + 1 == kWideStages ? 0 : stage_out + 1;
+        uint4 w[MT][2][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[m][r][h] = shared16(from + ((m * 2 + r) * 2 + h) * 512);
+        copy_step();   // into the stage read in the step before
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (n >= used) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 b = shared16(stage + kWarps * MT * 2048 + (n * 8 + g) * 128 + (((h * 4 + t) ^ g) * 16));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              Op<T>::mma(d[n][m], w[m][0][h].x, w[m][1][h].x, w[m][0][h].y, w[m][1][h].y, b.x, b.y);
+              Op<T>::mma(d[n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b.z, b.w);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (n >= used) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = n * 8 + t * 2 + i;
+          if (c >= en.count) continue;
+          const int row = at.row[en.first + c];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const int r = v.first + warp * kWarpRows + m * kApart + g;
+            if (kFirst) {
+              if (r < out_rows) static_cast<T*>(a.hidden)[int64_t(row) * a.w.inner + r] = Op<T>::round(activated(a.w.gelu, d[n][m][i], d[n][m][i + 2]));
+            } else {
+              float* to = a.partial + (int64_t(v.part) * a.rows + row) * out_rows + r;
+              if (r < out_rows) to[0] = d[n][m][i];
+              if (r + 8 < out_rows) to[8] = d[n][m][i + 2];
+            }
+          }
+        }
+      }
+    }
+    wait<0>();
+  }
+};
+
+constexpr int kSums = 2 * kWarps * 128 * 4;   // of the warps, twice
+__host__ __device__ constexpr int ring_bytes(int columns) {
+  return columns == 1 ? kWarps * kStages * 2048 : kWideStages * (kWarps * 2 * 2048 + 4096);
+}
+template <typename T, int NT, bool kFirst>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) product_kernel(const __grid_constant__ MoEArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kRing = kWarps * S * MT * 2048, kSums = 2 * kWarps * NT * MT * 128 * 4;
+  constexpr int kHeld = ring_bytes(NT) + (NT == 1 ? kSums : 0);
   // The choice is there: for the first product once the router has ended; the second is launched after that, as the first
   // lets it begin behind its own wait.
   if (kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  const Lists at = make_lists<NT>(a, smem + kRing + kSums, tid);
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S * MT * 2048;
-  Product<T, NT, MT, S, kFirst> product(a, at, ring, reinterpret_cast<float*>(smem + kRing), lane, warp);
-  product.fill();   // weights, while the first product finishes the hidden values
-  if (!kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
-  product.run();
-  wait<0>();
+  const Lists at = make_lists<NT>(a, smem + kHeld, threadIdx.x);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  if constexpr (NT == 1) {
+    Product<T, kFirst> product(a, at, ring + (threadIdx.x >> 5) * kStages * 2048, reinterpret_cast<float*>(smem + ring_bytes(NT)));
+    product.fill();   // weights, while the first product finishes the hidden values
+    if (!kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
+    product.run();
+    wait<0>();
+  } else {
+    WideProduct<T, kFirst> product(a, at, ring);
+    if (!kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
+    product.run();
+  }
 }
 
 // y of four outputs of a token per thread
@@ -587,9 +705,10 @@ Sizes sizes(const MoEView& w, int64_t tokens) {
   z.columns = z.tokens <= 8 || rows <= 4 * w.experts ? 8 : 32;
   z.entries = std::min(w.experts, rows) + rows / z.columns;
   // Parts of the second product's k, of 512 inputs or more, until (expert, tile, part) triples are many for every CTA
-  const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + 15) / 16);
+  const int tile = z.columns == 8 ? 16 : 32 * kWarps;
+  const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + tile - 1) / tile), enough = z.columns == 8 ? 4096 : 1024;
   z.splits = 1;
-  while (z.splits < 8 && units * z.splits < 4096 && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
+  while (z.splits < 8 && units * z.splits < enough && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   z.chosen = up(size_t(rows) * 4);
   z.hidden = up(size_t(rows) * w.inner * 2);
@@ -609,23 +728,25 @@ cudaError_t enqueue(void (*kernel)(MoEArgs), const MoEArgs& a, int64_t grid, int
   return cudaLaunchKernelEx(&c, kernel, a);
 }
 
-template <typename T, int NT, int MT, int S, bool kFirst>
+template <typename T, int NT, bool kFirst>
 cudaError_t product(const MoEArgs& a, int sms, cudaStream_t s) {
-  const size_t smem = size_t(kWarps) * S * MT * 2048 + size_t(2) * kWarps * NT * MT * 512 + lists_bytes(a.w.experts, a.entries, a.rows);
-  const auto kernel = product_kernel<T, NT, MT, S, kFirst>;
+  const size_t smem = size_t(ring_bytes(NT)) + (NT == 1 ? kSums : 0) + lists_bytes(a.w.experts, a.entries, a.rows);
+  const auto kernel = product_kernel<T, NT, kFirst>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e != cudaSuccess) return e;
   const int64_t each = std::min<int64_t>(NT == 1 ? 4 : 2, 227 * 1024 / (smem + 1024));
-  const int rows = kFirst ? a.w.inner : a.w.width, tile = kFirst ? 8 * MT : 16 * MT;
+  const int rows = kFirst ? a.w.inner : a.w.width, tile = (kFirst ? 8 : 16) * (NT == 1 ? 1 : 2 * kWarps);
   const int64_t units = int64_t(a.entries) * ((rows + tile - 1) / tile) * (kFirst ? 1 : a.splits);   // at most
   return enqueue(kernel, a, std::min(units, std::max<int64_t>(each, 1) * sms), kThreads, smem, 0, true, s);
 }
 
 template <typename T>
 cudaError_t launch(const MoEArgs& a, int columns, int sms, cudaStream_t s) {
-  cudaError_t e = enqueue(route_kernel<T>, a, int64_t(a.tokens) * kRouteCtas, kRouteThreads, 0, kRouteCtas, false, s);
-  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, 1, 5, true>(a, sms, s) : product<T, 4, 2, 4, true>(a, sms, s);
-  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, 1, 5, false>(a, sms, s) : product<T, 4, 2, 4, false>(a, sms, s);
+  int ctas = 1;   // a warp per expert while that fits the card (200 tokens of 32 experts by 8 CTAs each: 20 us)
+  while (ctas < kRouteCtas && ctas * (kRouteThreads / 32) < a.w.experts && int64_t(a.tokens) * ctas <= 2 * sms) ctas *= 2;
+  cudaError_t e = enqueue(route_kernel<T>, a, int64_t(a.tokens) * ctas, kRouteThreads, 0, ctas, false, s);
+  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, true>(a, sms, s) : product<T, 4, true>(a, sms, s);
+  if (e == cudaSuccess) e = columns == 8 ? product<T, 1, false>(a, sms, s) : product<T, 4, false>(a, sms, s);
   if (e != cudaSuccess) return e;
   return enqueue(combine_kernel<T>, a, (int64_t(a.tokens) * (a.w.width / 4) + kThreads - 1) / kThreads, kThreads, 0, 0, true, s);
 }

@@ -107,13 +107,14 @@ template <typename T, int V, bool kEdges> __device__ __forceinline__ void store(
 
 // A piece of weights, which are aligned as a whole, from any element: `skip` elements into the 16 from the boundary
 // before it. (Read-only loads: they need not wait for the stores before them.)
-template <typename W> __device__ __forceinline__ Piece<W, 8> shifted(const W* p, int skip) {
+template <typename W, bool kStaged> __device__ __forceinline__ Piece<W, 8> shifted(const W* p, int skip) {
   Piece<W, 8> v;
   uint32_t* w = reinterpret_cast<uint32_t*>(v.e);
   auto words = [](uint32_t* to, const W* from, int n) {
 #pragma unroll
     for (int i = 0; i < n; i += 4) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(from) + i / 4);
+      const uint4* at = reinterpret_cast<const uint4*>(from) + i / 4;
+      const uint4 q = kStaged ? *at : __ldg(at);
       to[i] = q.x, to[i + 1] = q.y, to[i + 2] = q.z, to[i + 3] = q.w;
     }
   };
@@ -144,15 +145,20 @@ template <typename W> __device__ __forceinline__ Piece<W, 8> shifted(const W* p,
   }
   return v;
 }
-template <typename W, int V, bool kEdges> __device__ __forceinline__ void weights(float (&to)[V], const void* p, int at, int width) {
+// kStaged: from a copy in shared memory, laid out as the rows' pieces are, with zeros before and behind.
+constexpr int kPad = 16;   // of them, at least, on either side
+template <typename W, int V, bool kEdges, bool kStaged>
+__device__ __forceinline__ void weights(float (&to)[V], const void* p, int at, int width) {
   const W* w = static_cast<const W*>(p);
-  if constexpr (V == 1) {
+  if constexpr (kStaged) {
+    shifted<W, true>(w + at, 0).widened(to);
+  } else if constexpr (V == 1) {
     to[0] = widen<W>(__ldg(w + at));
   } else if constexpr (!kEdges) {
-    shifted<W>(w + at, 0).widened(to);
+    shifted<W, false>(w + at, 0).widened(to);
   } else {
     const int skip = at & 7;
-    if (at >= skip && at + (skip ? 16 - skip : 8) <= width) shifted<W>(w + at, skip).widened(to);
+    if (at >= skip && at + (skip ? 16 - skip : 8) <= width) shifted<W, false>(w + at, skip).widened(to);
     else load_part<W>(w, at, width).widened(to);
   }
 }
@@ -212,15 +218,15 @@ __device__ __forceinline__ float2 moments(const float (&z)[P][V], const Residual
 }
 
 // z becomes (z - mean) factor w + b; elements outside the row stay 0.
-template <typename W, int V, int P, bool kEdges>
+template <typename W, int V, int P, bool kEdges, bool kStaged>
 __device__ __forceinline__ void apply(float (&z)[P][V], float2 c, const void* w, const void* b, const ResidualNormArgs& a, int first, int stride) {
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int at = first + p * stride;
     if (at >= a.width) continue;
     float f[V], g[V];
-    weights<W, V, kEdges>(f, w, at, a.width);
-    if (b) weights<W, V, kEdges>(g, b, at, a.width);
+    weights<W, V, kEdges, kStaged>(f, w, at, a.width);
+    if (b) weights<W, V, kEdges, kStaged>(g, b, at, a.width);
     if (a.layer) {
 #pragma unroll
       for (int e = 0; e < V; ++e) z[p][e] -= c.x;
@@ -239,10 +245,15 @@ __device__ __forceinline__ void apply(float (&z)[P][V], float2 c, const void* w,
   }
 }
 
+struct Vectors {   // the arguments' or copies of them
+  const void *weight, *bias, *post_weight, *post_bias, *gate;
+};
+
 // A row from its x in z on; residual and gate come by r(p, at) and g(p, at).
-template <typename T, typename S, typename W, int V, int P, bool kEdges, bool kWarp, typename R, typename G>
-__device__ __forceinline__ void finish(float (&z)[P][V], const ResidualNormArgs& a, int64_t m, Row<kWarp>& row, int first, int stride, R&& r, G&& g) {
-  if (a.post_weight) apply<W, V, P, kEdges>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), a.post_weight, a.post_bias, a, first, stride);
+template <typename T, typename S, typename W, int V, int P, bool kEdges, bool kStaged, bool kWarp, typename R, typename G>
+__device__ __forceinline__ void finish(float (&z)[P][V], const ResidualNormArgs& a, const Vectors& w, int64_t m, Row<kWarp>& row, int first,
+                                       int stride, R&& r, G&& g) {
+  if (a.post_weight) apply<W, V, P, kEdges, kStaged>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), w.post_weight, w.post_bias, a, first, stride);
   S* sum = static_cast<S*>(a.sum) + m * a.ss;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -254,7 +265,7 @@ __device__ __forceinline__ void finish(float (&z)[P][V], const ResidualNormArgs&
     }
     float f[V];
     if (a.gate) {
-      if (a.gs == 0) weights<T, V, kEdges>(f, a.gate, at, a.width);
+      if (a.gs == 0) weights<T, V, kEdges, kStaged>(f, w.gate, at, a.width);
       else g(p, at).widened(f);
 #pragma unroll
       for (int e = 0; e < V; ++e) z[p][e] *= f[e];
@@ -264,10 +275,15 @@ __device__ __forceinline__ void finish(float (&z)[P][V], const ResidualNormArgs&
 #pragma unroll
       for (int e = 0; e < V; ++e) z[p][e] += f[e];
     }
+    if (!whole<V, kEdges>(at, a.width)) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (!inside(at + e, a.width)) z[p][e] = 0.f;
+    }
     if (a.sum) store<S, V, kEdges>(sum, at, a.width, z[p]);
   }
   if (!a.y) return;
-  apply<W, V, P, kEdges>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), a.weight, a.bias, a, first, stride);
+  apply<W, V, P, kEdges, kStaged>(z, moments<V, P, kEdges, kWarp>(z, a, row, first, stride), w.weight, w.bias, a, first, stride);
   T* y = static_cast<T*>(a.y) + m * a.ys;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -316,7 +332,8 @@ __global__ void __launch_bounds__(kMost == 32 ? 128 : kMost) residual_norm_kerne
       }
     }
   }
-  finish<T, S, W, V, P, kEdges, kWarp>(z, a, m, row, first, stride, [&](int p, int) { return r[p]; }, [&](int p, int) { return g[p]; });
+  const Vectors w = {a.weight, a.bias, a.post_weight, a.post_bias, a.gate};
+  finish<T, S, W, V, P, kEdges, false, kWarp>(z, a, w, m, row, first, stride, [&](int p, int) { return r[p]; }, [&](int p, int) { return g[p]; });
 }
 
 // Many rows: CTAs that stay and take every gridDim.x-th row, whose inputs arrive in shared memory (cp.async, a ring of
@@ -333,6 +350,7 @@ __device__ __forceinline__ void copy_row(uint8_t* to, const uint8_t* from, int b
 
 struct RowRing {
   int stages, r, g, bytes;   // offsets of residual and gate in a stage, and a stage's bytes
+  int vectors;               // with edges: where the copies of the weights begin
 };
 
 template <typename T, typename S, typename W, int P, bool kEdges, int kMost, int kCtas>
@@ -353,6 +371,21 @@ __global__ void __launch_bounds__(kMost, kCtas) residual_norm_stream(const Resid
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  Vectors w = {a.weight, a.bias, a.post_weight, a.post_bias, a.gs == 0 ? a.gate : nullptr};
+  if constexpr (kEdges) {   // all rows of a CTA begin alike: gridDim.x is a multiple of 8
+    uint8_t* to = held + ring.vectors;
+    const int before = kPad + overhang<T, kEdges>(a, blockIdx.x);
+    auto stage = [&](const void*& p, auto one) {
+      using E = decltype(one);
+      if (p == nullptr) return;
+      E* v = reinterpret_cast<E*>(to);
+      for (int i = tid; i < a.width + 3 * kPad; i += blockDim.x)
+        v[i] = inside(i - before, a.width) ? static_cast<const E*>(p)[i - before] : narrow<E>(0.f);
+      p = v + before;
+      to += ((a.width + 3 * kPad) * int(sizeof(E)) + 15) / 16 * 16;
+    };
+    stage(w.weight, W()), stage(w.bias, W()), stage(w.post_weight, W()), stage(w.post_bias, W()), stage(w.gate, T());
+  }
   for (int i = 0; i < ring.stages - 1; ++i) copy(blockIdx.x + int64_t(i) * gridDim.x, i);
   int in = ring.stages - 1, out = 0;
   for (int64_t m = blockIdx.x; m < a.rows; m += gridDim.x) {
@@ -374,24 +407,30 @@ __global__ void __launch_bounds__(kMost, kCtas) residual_norm_stream(const Resid
     for (int p = 0; p < P; ++p) {
       const int at = first + p * stride;
       if (at < a.width) {
-        load<T, V, kEdges>(x, at, a.width).widened(z[p]);
+        load<T, V, false>(x, at, a.width).widened(z[p]);
+        if (!whole<V, kEdges>(at, a.width)) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (!inside(at + e, a.width)) z[p][e] = 0.f;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) z[p][e] = 0.f;
       }
     }
-    finish<T, S, W, V, P, kEdges, false>(z, a, m, row, first, stride, [&](int, int at) { return load<S, V, kEdges>(r, at, a.width); },
-                                         [&](int, int at) { return load<T, V, kEdges>(g, at, a.width); });
+    finish<T, S, W, V, P, kEdges, kEdges, false>(z, a, w, m, row, first, stride, [&](int, int at) { return load<S, V, false>(r, at, a.width); },
+                                                 [&](int, int at) { return load<T, V, false>(g, at, a.width); });
   }
 }
 
 template <typename T, typename S, typename W, int P, bool kEdges, int kMost, int kCtas>
-cudaError_t stream(const ResidualNormArgs& a, RowRing ring, int threads, int ctas, int sms, cudaStream_t s) {
+cudaError_t stream(const ResidualNormArgs& a, RowRing ring, size_t smem, int threads, int ctas, int sms, cudaStream_t s) {
   const auto kernel = residual_norm_stream<T, S, W, P, kEdges, kMost, kCtas>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
   if (e != cudaSuccess) return e;
-  const int64_t grid = std::min<int64_t>(a.rows, int64_t(ctas) * sms);
-  kernel<<<unsigned(grid), threads, size_t(ring.stages) * ring.bytes, s>>>(a, ring);
+  int64_t grid = std::min<int64_t>(a.rows, int64_t(ctas) * sms);
+  if (kEdges && grid >= 8) grid -= grid % 8;
+  kernel<<<unsigned(grid), threads, smem, s>>>(a, ring);
   return cudaGetLastError();
 }
 
@@ -416,19 +455,27 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   // one piece 45, four 47; without the ring 97). Shorter rows go a warp each without it (12608 of 768 in fp32: 36 us, 39 with).
   constexpr int kEach = 2;
   RowRing ring;
-  const int pad = kEdges ? 32 : 0;   // a row that begins and ends inside a piece
+  const int pad = kEdges ? 48 : 0;   // a row that begins and ends inside a piece: what such pieces hold besides
   auto up = [](int n) { return (n + 15) / 16 * 16; };
   ring.r = up(a.width * int(sizeof(T))) + pad;
   ring.g = ring.r + (a.residual ? up(a.width * int(sizeof(S))) + pad : 0);
   ring.bytes = ring.g + (a.gate && a.gs != 0 ? up(a.width * int(sizeof(T))) + pad : 0);
   int threads = 128;
   while (threads * kEach < pieces) threads *= 2;
-  const int kRing = 216 * 1024;
-  const int ctas = std::min(1024 / threads, kRing / (2 * ring.bytes));
+  const int room = 216 * 1024;
+  int staged = 0;   // copies of the weights
+  if (kEdges) {
+    for (const void* p : {a.weight, a.bias, a.post_weight, a.post_bias})
+      if (p) staged += up((a.width + 3 * kPad) * int(sizeof(W)));
+    if (a.gate && a.gs == 0) staged += up((a.width + 3 * kPad) * int(sizeof(T)));
+  }
+  const int ctas = std::min(threads <= 256 ? 5 * (256 / threads) : 1024 / threads, room / (2 * ring.bytes + staged));
   if (pieces >= 128 && threads <= 1024 && ctas > 0 && a.rows >= 2 * int64_t(ctas) * sms) {
-    ring.stages = std::min(4, kRing / (ctas * ring.bytes));
-    if (threads <= 256) return stream<T, S, W, kEach, kEdges, 256, 4>(a, ring, threads, ctas, sms, s);
-    return stream<T, S, W, kEach, kEdges, 1024, 1>(a, ring, threads, ctas, sms, s);
+    ring.stages = std::min(4, (room / ctas - staged) / ring.bytes);
+    ring.vectors = ring.stages * ring.bytes;
+    const size_t smem = size_t(ring.vectors) + staged;
+    if (threads <= 256) return stream<T, S, W, kEach, kEdges, 256, 5>(a, ring, smem, threads, ctas, sms, s);
+    return stream<T, S, W, kEach, kEdges, 1024, 1>(a, ring, smem, threads, ctas, sms, s);
   }
   // Pieces per thread: with rows for every SM four, so that a row takes few warps; otherwise one, so that it takes many.
   int each = a.rows >= 2 * int64_t(sms) || pieces > 1024 ? 4 : 1;
