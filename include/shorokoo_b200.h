@@ -356,7 +356,7 @@ typedef struct sb_moe_weights {
 } sb_moe_weights;
 SB_API int32_t sb_moe_workspace(const sb_moe_weights* weights, int64_t tokens, size_t* bytes);
 /* x, y [tokens][width] of elem_type; y may be x itself. workspace: 256-byte aligned, at least
- * sb_moe_workspace bytes, not shared with a call that may overlap. A cooperative launch. */
+ * sb_moe_workspace bytes, not shared with a call that may overlap. */
 SB_API int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_row_stride, void* y, int64_t y_row_stride,
                       int64_t tokens, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -366,7 +366,7 @@ SB_API int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_ro
  * which the running sum of the kept w, in order of the index, exceeds uniform[row] (float32, [0, 1)) times their sum.
  * Settings of each row (device arrays) or, where the array is NULL, of all. temperature 0 (or less, or NaN): the first
  * of the largest. top_k 0 (or less): any number. top_p 1 (or more, or NaN) and min_p 0 (or less, or NaN): no filter;
- * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0. */
+ * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0. vocab: at most 2^21. */
 typedef struct sb_sampling {
   const float *temperature_of, *top_p_of, *min_p_of;
   const int32_t* top_k_of;

@@ -447,8 +447,10 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
     if first is not None:
         if getattr(first, "dtype", None) is torch.float32:
             kinds = (torch.float32,)
-        wp, bp = _vector(weight, "weight", device, kinds, n), _vector(bias, "bias", device, kinds, n)
-        pp, cp = _vector(post_weight, "post_weight", device, kinds, n), _vector(post_bias, "post_bias", device, kinds, n)
+        wp = _vector(weight, "weight", device, kinds, n)
+        bp = _vector(bias, "bias", device, kinds, n) if bias is not None else 0
+        pp = _vector(post_weight, "post_weight", device, kinds, n) if post_weight is not None else 0
+        cp = _vector(post_bias, "post_bias", device, kinds, n) if post_bias is not None else 0
     else:
         wp = pp = bp = cp = 0
     if weight is None and (bias is not None or out is not None):
@@ -457,18 +459,19 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
         _bad("post_bias needs a post_weight")
     h, hp, ss = x, 0, 0
     if residual is not None or gate is not None or post_weight is not None or scale != 1.0 or residual_out is not None:
-        if residual_out is not None:
-            h = residual_out
+        if residual_out is None:
+            h, ss = x.new_empty((rows, n), dtype=sum_type), n
         else:
-            h = torch.empty((rows, n), dtype=sum_type, device=device)
-        ss = _matrix(h, "residual_out", device, sum_type, rows, n)[1]
+            h, ss = residual_out, _matrix(residual_out, "residual_out", device, sum_type, rows, n)[1]
         hp = h.data_ptr()
     elif weight is None:
         _bad("there is nothing to compute")
     y, yp, ys = None, 0, 0
     if weight is not None:
-        y = out if out is not None else torch.empty((rows, n), dtype=dtype, device=device)
-        ys = _matrix(y, "out", device, dtype, rows, n)[1]
+        if out is None:
+            y, ys = x.new_empty((rows, n)), n
+        else:
+            y, ys = out, _matrix(out, "out", device, dtype, rows, n)[1]
         yp = y.data_ptr()
     try:
         a = _pack_norm(x.data_ptr(), rp, gp, hp, yp, xs, rs, gs, ss, ys, wp, bp, pp, cp, rows, n, elem, _ELEM[sum_type], _ELEM[kinds[0]],
@@ -534,7 +537,7 @@ class MoEWeights:
 def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The mixture-of-experts layer of x [tokens, width], of the weights' type: for each token the sum over its
     experts of share * down (act(gate x) * (up x)). Meant for few tokens: an expert's weights are read once for every
-    32 of its tokens. Hidden values are rounded to the weights' type. ``out`` may be x itself. A cooperative launch."""
+    32 of its tokens. Hidden values are rounded to the weights' type. ``out`` may be x itself."""
     if not isinstance(weights, MoEWeights):
         _bad("weights must be MoEWeights")
     for name in ("router", "gate_up", "down"):   # since the object was made, or made without recording
@@ -542,8 +545,10 @@ def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None
             raise B200NotSupportedError(f"{name} requires a gradient or has a tangent, which these operators do not record")
     device, dtype = weights.device, weights.dtype
     tokens, xs = _matrix(x, "x", device, dtype, None, weights.width)
-    out = torch.empty((tokens, weights.width), dtype=dtype, device=device) if out is None else out
-    ys = _matrix(out, "out", device, dtype, tokens, weights.width)[1]
+    if out is None:
+        out, ys = x.new_empty((tokens, weights.width)), weights.width
+    else:
+        ys = _matrix(out, "out", device, dtype, tokens, weights.width)[1]
     n = weights._workspace(tokens)
     space = torch.empty(n, dtype=torch.uint8, device=device)
     _call("sb_moe", device, weights._ref, x.data_ptr(), xs, out.data_ptr(), ys, tokens, space.data_ptr(), n)
@@ -576,8 +581,10 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     if isinstance(min_p, torch.Tensor):
         mp, min_p = _vector(min_p, "min_p", device, _FLOAT, rows), 0.0
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=device)
-    to = _vector(out, "out", device, (torch.int64,), rows)
+        out = logits.new_empty((rows,), dtype=torch.int64)
+        to = out.data_ptr()
+    else:
+        to = _vector(out, "out", device, (torch.int64,), rows)
     try:
         by = _pack_sampling(tp, pp, mp, kp, temperature, top_p, min_p, min(max(int(top_k), 0), 0x7fffffff))
     except (struct.error, OverflowError) as e:

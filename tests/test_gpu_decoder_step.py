@@ -303,6 +303,7 @@ def check_moe(x, weights, **kw):
     (1, 1, 1, 8, 8), (1, 8, 2, 64, 24), (2, 5, 5, 72, 40), (3, 16, 4, 256, 136), (8, 33, 7, 128, 64), (9, 33, 7, 128, 64), (1, 128, 8, 512, 96),
     (13, 60, 6, 264, 200), (17, 4, 1, 2048, 16), (33, 8, 2, 64, 520), (40, 2, 2, 200, 72), (1, 512, 32, 64, 32), (7, 512, 32, 64, 32),
     (70, 512, 32, 64, 32), (257, 6, 3, 64, 48), (600, 3, 1, 72, 64), (130, 40, 20, 64, 24), (4, 4, 2, 4096, 1032), (1, 2, 1, 1024, 4096),
+    (40, 4, 2, 200, 2056), (260, 32, 4, 136, 1544), (50, 5, 1, 1032, 64),   # columns shared by a CTA, parts of k, ragged tiles
 ])
 def test_moe_sizes(tokens, experts, top_k, width, inner, dtype):
     gen = torch.Generator().manual_seed(tokens * 1009 + experts * 31 + width)
@@ -499,6 +500,15 @@ def test_sample_equal_logits(dtype):
     for kw in (dict(), dict(top_k=1), dict(top_k=700), dict(top_k=3000), dict(top_p=0.3), dict(top_p=0.77), dict(top_k=4000, top_p=0.4), dict(min_p=0.2),
                dict(temperature=0.0), dict(top_k=8999), dict(top_p=0.99999)):
         check_sample(logits, u, **kw)
+
+
+def test_sample_of_the_widest_rows():
+    """2^21 equal logits (their weights sum to 2^61), and few above the others."""
+    logits = torch.zeros((3, 1 << 21), dtype=BF16)
+    logits[1, 1234567] = 9.0
+    logits[2, ::4097] = 3.5
+    for kw in (dict(), dict(top_p=0.5), dict(top_k=100000)):
+        check_sample(logits, torch.tensor([0.75, 0.999, 0.5]), **kw)
 
 
 def test_sample_every_part_of_the_unit_interval():
