@@ -34,12 +34,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 384, kWarps = kThreads / 32;
 constexpr int kBins = 256;
 constexpr int kMostCtas = 8;            // of a cluster
 constexpr int kHeld = 192 * 1024;       // bytes of a slice that fit shared memory
 constexpr int kCoarse = 128;            // bins of the first round of weights, per warp
-constexpr int kListBytes = 4096;        // of a list of candidates
+constexpr int kListBytes = 6144;        // of a list of candidates
 constexpr int kMostRounds = 6;          // 128 or 256 bins, then at least 128 each of what is left of 2^32 floats
 constexpr int kSteps = 64;              // table of 2^(-j / 64)
 
@@ -206,7 +206,7 @@ __device__ __forceinline__ unsigned long long sum_upto(unsigned long long v, int
 }
 
 template <typename T, bool kHold>
-__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& s = *reinterpret_cast<Shared*>(raw);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const SampleArgs a)
   if (warp == 0) {
     most = lane < kWarps ? s.warp_top[lane] : -INFINITY;
 #pragma unroll
-    for (int d = kWarps / 2; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
     if (lane == 0) s.top = most;
   }
   cluster.sync();
@@ -715,9 +715,10 @@ cudaError_t launch(const SampleArgs& a, int64_t rows, int ctas, size_t smem, cud
 cudaError_t sample(const void* logits, int64_t stride, int elem, int64_t rows, int vocab, const float* uniform, const SamplingView& by,
                    int64_t* tokens, int sms, cudaStream_t s) {
   const int size = elem == 1 ? 4 : 2;
-  // CTAs per row: slices of at most 64 KB, so that several CTAs share an SM, and more while rows leave SMs idle
+  // CTAs per row: slices of at most 128 KB, so that two CTAs mostly share an SM (256 rows of 300 KB: 187 us; 64 KB, three of
+  // 256 threads: 209), and more while rows leave SMs idle
   int ctas = 1;
-  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * 64 * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
+  while (ctas < kMostCtas && (int64_t(vocab) * size > int64_t(ctas) * 128 * 1024 || (rows * ctas * 2 <= sms && vocab > ctas * 2048))) ctas *= 2;
   SampleArgs a = {logits, stride, uniform, by, tokens, vocab, 0};
   a.slice = int((int64_t(vocab) + ctas * 64 - 1) / (ctas * 64) * 64);
   const size_t held = size_t(a.slice) * size + 32;   // and the pieces' overhang

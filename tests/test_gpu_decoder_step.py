@@ -13,6 +13,7 @@ u = 2^-23 (tensor-core sums may truncate):
                  with a chance of about 10^-8 a row.
 """
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -449,8 +450,18 @@ def chosen(row, u, temperature, top_k, top_p, min_p):
         mass = np.cumsum(w[order])
         order = order[: max(1, int((mass < top_p * mass[-1]).sum()) + 1)]
     order = np.sort(order)
-    mass = np.cumsum(w[order])
-    return int(order[min(int((mass <= min(max(u, 0.0), 1.0) * mass[-1]).sum()), order.size - 1)])
+    mass, u = np.cumsum(w[order]), min(max(u, 0.0), 1.0)
+    at = min(int((mass <= u * mass[-1]).sum()), order.size - 1)
+    kinds = np.unique(w[order])
+    if kinds.size <= 4:   # sums of few different weights may equal u times theirs, which rounded sums do not show: exact ones
+        counts = [np.cumsum(w[order] == v) for v in kinds]
+        upto = lambda i: sum(Fraction(float(v)) * int(c[i]) for v, c in zip(kinds, counts)) if i >= 0 else 0
+        target = Fraction(u) * upto(order.size - 1)
+        while at > 0 and upto(at - 1) > target:
+            at -= 1
+        while at < order.size - 1 and upto(at) <= target:
+            at += 1
+    return int(order[at])
 
 
 def check_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
