@@ -39,7 +39,8 @@ constexpr int kBins = 256;
 constexpr int kMostCtas = 8;            // of a cluster
 constexpr int kHeld = 192 * 1024;       // bytes of a slice that fit shared memory
 constexpr int kCoarse = 128;            // bins of the first round of weights, per warp
-constexpr int kListBytes = 6144;        // of a list of candidates
+constexpr int kListBytes = 4096;        // of a list of candidates
+constexpr int kSettled = 256;           // candidates of a row that are ranked one against another
 constexpr int kMostRounds = 6;          // 128 or 256 bins, then at least 128 each of what is left of 2^32 floats
 constexpr int kSteps = 64;              // table of 2^(-j / 64)
 
@@ -114,13 +115,16 @@ struct alignas(16) Shared {
   uint32_t part[3][kWarps][kCoarse];        // sums of each warp's part of the slice, of 16, 16 and 9 bits of the weights
   uint4 list[2][kListBytes / 16];
   int listed[2];
+  float rank_value[kSettled];
+  unsigned long long rank_weight[kSettled];
   unsigned long long scan[2][kWarps];
   float warp_top[kWarps];
   // what its first warp found out
   unsigned long long all, target, above, before, ties_before, tie;
   double wide_rate;
   float most_of_row, rate, rate_low;
-  uint32_t lo;
+  unsigned long long ties;
+  uint32_t lo, border;
   int near, outcome, bin, chosen;
 };
 
@@ -331,6 +335,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   auto part_sum = [&](int w, int b) {
     return s.part[0][w][b] + (static_cast<unsigned long long>(s.part[1][w][b]) << 16) + (static_cast<unsigned long long>(s.part[2][w][b]) << 32);
   };
+  // The candidates that the CTAs have listed (each lane: how many of its CTA, and how many before them): the one at which
+  // the sums from the top reach need(their sum), by ranking all against all. Whether there is one.
+  auto settle = [&](const bool by_mass, int number, int before, int total, auto&& need_of) {
+    float v = 0.f;
+    for (int c = 0; c < ctas; ++c) {
+      const int i = tid - __shfl_sync(~0u, before, c), n = __shfl_sync(~0u, number, c);
+      if (i >= 0 && i < n) v = value<T>(reinterpret_cast<const T*>(cluster.map_shared_rank(&s, c)->list[turn])[i]);
+    }
+    const unsigned long long own = by_mass && tid < total ? weight(v) : 1ull;
+    if (tid < total) s.rank_value[tid] = v, s.rank_weight[tid] = own;
+    if (tid == 0) s.outcome = 0;
+    __syncthreads();
+    unsigned long long all = 0;
+    for (int j = lane; j < total; j += 32) all += s.rank_weight[j];
+    __syncwarp();
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+    const unsigned long long need = need_of(all);
+    if (tid < total) {
+      unsigned long long greater = 0, equal = 0;
+      for (int j = 0; j < total; ++j) {
+        const float x = s.rank_value[j];
+        const unsigned long long w = s.rank_weight[j];
+        greater += x > v ? w : 0;
+        equal += x == v ? w : 0;
+      }
+      if (greater < need && need <= greater + equal) s.border = key_of(v), s.ties = quotient(need - greater, own), s.outcome = 1;
+    }
+    __syncthreads();
+    turn ^= 1;
+    if (s.outcome) border = s.border, ties = s.ties;
+    return s.outcome != 0;
+  };
+  // How many the CTAs have listed, each lane its CTA's; before them; in all, or more than can be settled.
+  auto numbers = [&](int& number, int& before) {
+    number = lane < ctas ? cluster.map_shared_rank(&s, lane)->listed[turn] : 0;
+    int upto = number;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int p = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += p;
+    }
+    before = upto - number;
+    const bool fits = __all_sync(~0u, number <= kListed);
+    const int total = __shfl_sync(~0u, upto, 31);
+    return fits ? total : kSettled + 1;
+  };
   // Finds the key at which the sums from the top reach a target: of counts, or of weights. The ties of a border found
   // before are not summed one by one, but by their number.
   auto descend = [&](const bool by_mass) {
@@ -338,6 +389,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const bool floored = by_mass && ties < (unsigned long long)a.vocab;
     const uint32_t floor = border;
     const unsigned long long floor_weight = floored ? weight(of_key(floor)) : 0, floor_sum = floored ? ties * floor_weight : 0;
+    const auto part_of = [&](unsigned long long all) {
+      return min(max((unsigned long long)ceil(double(top_p) * double(all + floor_sum)), 1ull), all + floor_sum);
+    };
+    if (floored && top_k <= kSettled) {   // all that are above the border there is
+      const float last = of_key(floor);
+      T* to = reinterpret_cast<T*>(s.list[turn]);
+      for (int q = tid; q < pieces; q += kThreads) {
+        const uint4 p = piece(q);
+        const T* e = reinterpret_cast<const T*>(&p);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < kV; ++j) mine |= uint32_t(value<T>(e[j]) > last) << j;
+        if (mine) {
+          int i = atomicAdd(&s.listed[turn], __popc(mine));
+          each_of(q, mine, [&](float v) { to[i++] = narrow<T>(v); });   // less than top_k
+        }
+      }
+      cluster.sync();
+      __syncwarp();
+      int number, before;
+      const int total = numbers(number, before);
+      unsigned long long target = 0, sum = 0;
+      if (!settle(true, number, before, total, [&](unsigned long long all) { return sum = all, target = part_of(all); }))
+        ties = quotient(target - sum, floor_weight);   // among the border's ties
+      return;
+    }
     uint32_t low_key = floored ? min(floor + 1, hi) : lo, high_key = hi;   // hi itself where none is above the border
     const bool none = floored && floor >= hi;
     unsigned long long above = 0;
@@ -454,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 #pragma unroll
         for (int i = 0; i < kBins / 32; ++i) sum += n[i];
         const unsigned long long upto = sum_upto(sum, lane), all = __shfl_sync(~0u, upto, 31);
-        if (round == 0 && by_mass) target = min(max((unsigned long long)ceil(double(top_p) * double(all + floor_sum)), 1ull), all + floor_sum);
+        if (round == 0 && by_mass) target = part_of(all);
         const unsigned long long need = target - above;
         if (lane == 0) s.all = all, s.target = target, s.outcome = round == 0 && (by_mass ? target > all : target >= all);
         if (upto >= need && upto - sum < need) {
@@ -534,6 +611,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
       least = __reduce_min_sync(~0u, least), greatest = __reduce_max_sync(~0u, greatest);
       low_key = least, high_key = greatest;
+      if (least != greatest) {
+        int number, before;
+        const int total = numbers(number, before);
+        if (total <= kSettled) {
+          settle(by_mass, number, before, total, [&](unsigned long long) { return target - above; });
+          return;
+        }
+      }
       listed = s.listed[next];
       list = listed <= kListed ? next : -1;
       turn ^= 1;
