@@ -17,9 +17,9 @@
 // order needs the weights of the border's bin only, and then of the part that the draw falls in.
 //
 // The weights' arithmetic (about 25 instructions each) and the cluster's barriers bound it, not the logits' bytes (12 us):
-// 256 rows of 150001 in bf16 take 37 us for the largest alone, 101 us without a filter, 143 us with top_k 50, 209 us with
-// top_p 0.9 (barriers are 40% of a warp's cycles; three CTAs per SM hide part of them). One row of 32000: 14.5 us, a chain
-// of seven barriers. Exponentials in fp64 and 64-bit atomics in place of the table and the halves: 584 us for the 209.
+// 256 rows of 150001 in bf16 take 30 us for the largest alone, 96 us without a filter, 107 us with top_k 50, 187 us with
+// top_p 0.9 (two CTAs per SM hide part of the barriers). One row of 32000: 16 us, a chain of seven barriers. Exponentials
+// in fp64 and 64-bit atomics in place of the table and the halves: 584 us for the 187.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

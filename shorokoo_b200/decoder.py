@@ -540,8 +540,9 @@ def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None
     32 of its tokens. Hidden values are rounded to the weights' type. ``out`` may be x itself."""
     if not isinstance(weights, MoEWeights):
         _bad("weights must be MoEWeights")
-    for name in ("router", "gate_up", "down"):   # since the object was made, or made without recording
-        if _derived(getattr(weights, name)):
+    for name in ("router", "gate_up", "down", "selection_bias"):   # since the object was made, or made without recording
+        t = getattr(weights, name)
+        if t is not None and _derived(t):
             raise B200NotSupportedError(f"{name} requires a gradient or has a tangent, which these operators do not record")
     device, dtype = weights.device, weights.dtype
     tokens, xs = _matrix(x, "x", device, dtype, None, weights.width)
