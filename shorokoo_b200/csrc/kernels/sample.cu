@@ -130,6 +130,8 @@ struct alignas(16) Shared {
 
 constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: sums with it are rounded to integers, in their low bits
 
+static_assert(sizeof(Shared) + kHeld <= 227 * 1024, "a slice beside what a CTA keeps");
+
 // exp((v - top) / T) in units of 2^-40 for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
 // floats, k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms
 // of its series (the next is 2^-34), in integers: off by about 2^-30 of itself, where expf would be off by up to 2^-21
@@ -191,9 +193,10 @@ struct KeyBins {
   __device__ __forceinline__ int operator()(float v) const { return int((hi - key_of(v)) >> shift); }
 };
 
-// a / b rounded up, b > 0: from a quotient of doubles, which is off by little (a division of 64-bit integers takes five
+// a / b rounded up (0 for b = 0): from a quotient of doubles, which is off by little (a division of 64-bit integers takes five
 // times as long)
 __device__ __forceinline__ unsigned long long quotient(unsigned long long a, unsigned long long b) {
+  if (b == 0) return 0;
   unsigned long long q = (unsigned long long)(double(a) / double(b));
   while (q > 0 && q * b >= a) --q;
   while (q * b < a) ++q;

@@ -159,6 +159,15 @@ def test_residual_norm_of_many_rows(rows, width, pitch, dtype):
     wy, dy, wh, dh = norm_reference(x[some].cpu(), w.cpu(), residual=wide[some].cpu(), gate=b.cpu())
     within(y2[some], wy, rounded(wy, dy, dtype), "y, stream in 32 bits")
     within(h2[some], wh, rounded(wh, dh, FP32), "h, stream in 32 bits")
+    some_of = lambda t: t[some].cpu()
+    for more in (dict(residual=r, gate=g), dict(gate=g), dict(residual=r), dict(residual=wide, gate=g, scale=-0.5)):   # h alone
+        none, h3 = decoder.residual_norm(x, None, **more)
+        _, _, wh, dh = norm_reference(some_of(x), None, **{k: some_of(v) if isinstance(v, torch.Tensor) else v for k, v in more.items()})
+        assert none is None
+        within(h3[some], wh, rounded(wh, dh, h3.dtype), "h alone")
+    y4, h4 = decoder.residual_norm(x, w.float(), bias=b.float(), weight_offset=1.0)
+    wy, dy, _, _ = norm_reference(some_of(x), w.float().cpu(), bias=b.float().cpu(), weight_offset=1.0)
+    within(y4[some], wy, rounded(wy, dy, dtype), "weights in 32 bits")
     decoder.residual_norm(x, w, residual=r, gate=g, out=x, residual_out=r, **kw)
     assert torch.equal(x, y) and torch.equal(r, h)
 
@@ -488,7 +497,7 @@ def test_sample(rows, vocab, dtype):
         check_sample(logits, torch.rand(rows, generator=gen), **kw)
 
 
-@pytest.mark.parametrize("vocab,dtype", [(262144, FP32), (500001, FP32), (900013, BF16)])
+@pytest.mark.parametrize("vocab,dtype", [(262144, FP32), (380001, FP32), (500001, FP32), (900013, BF16)])
 def test_sample_wide(vocab, dtype):
     """Slices beyond shared memory (the last two) and near its limit."""
     gen = torch.Generator().manual_seed(vocab)
