@@ -463,8 +463,7 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   ring.r = up(a.width * int(sizeof(T))) + pad;
   ring.g = ring.r + (a.residual ? up(a.width * int(sizeof(S))) + pad : 0);
   ring.bytes = ring.g + (a.gate && a.gs != 0 ? up(a.width * int(sizeof(T))) + pad : 0);
-  int threads = 128;
-  while (threads * kEach < pieces) threads *= 2;
+  int threads = std::max(128, (pieces + 32 * kEach - 1) / (32 * kEach) * 32);
   const int room = 216 * 1024;
   int staged = 0;   // copies of the weights
   if (kEdges) {
@@ -472,7 +471,8 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
       if (p) staged += up((a.width + 3 * kPad) * int(sizeof(W)));
     if (a.gate && a.gs == 0) staged += up((a.width + 3 * kPad) * int(sizeof(T)));
   }
-  const int ctas = std::min(threads <= 256 ? 5 * (256 / threads) : 1024 / threads, room / (2 * ring.bytes + staged));
+  const int ctas = std::min(threads <= 256 ? 1280 / threads : 1024 / threads, room / (2 * ring.bytes + staged));
+  if (ctas == 1) threads = 1024;   // one row at a time: more warps hide more of its chain (777 of 11001: 53 us, 704 threads 59)
   if (pieces >= 128 && threads <= 1024 && ctas > 0 && a.rows >= 2 * int64_t(ctas) * sms && int64_t(ctas) * sms >= 8) {
     ring.stages = std::min(4, (room / ctas - staged) / ring.bytes);
     ring.vectors = ring.stages * ring.bytes;
