@@ -463,7 +463,7 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   ring.r = up(a.width * int(sizeof(T))) + pad;
   ring.g = ring.r + (a.residual ? up(a.width * int(sizeof(S))) + pad : 0);
   ring.bytes = ring.g + (a.gate && a.gs != 0 ? up(a.width * int(sizeof(T))) + pad : 0);
-  int threads = std::max(128, (pieces + 32 * kEach - 1) / (32 * kEach) * 32);
+  int threads = std::max(64, (pieces + 32 * kEach - 1) / (32 * kEach) * 32);
   const int room = 216 * 1024;
   int staged = 0;   // copies of the weights
   if (kEdges) {
