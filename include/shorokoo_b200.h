@@ -341,7 +341,8 @@ SB_API int32_t sb_residual_norm(const sb_residual_norm_args* args, void* stream)
  * [experts][2 * inner][width], down [experts][width][inner] (elem_type: float16 or bfloat16), rows contiguous and the
  * other strides in elements; selection_bias float32. Meant for few tokens: an expert's weights are read once for every
  * 32 of its tokens. experts: at most 512; top_k: at most 32; width and inner: multiples of 8; pointers
- * 16-byte aligned and strides multiples of 8 elements. Hidden values are rounded to elem_type. */
+ * 16-byte aligned and strides multiples of 8 elements. Hidden values are held as two numbers
+ * of elem_type (16 bits in bfloat16, 22 in float16, where they overflow beyond 65504). */
 #define SB_MOE_SOFTMAX 0
 #define SB_MOE_SIGMOID 1
 #define SB_MOE_SILU 0

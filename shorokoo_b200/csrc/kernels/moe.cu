@@ -19,8 +19,8 @@
 // of which the router and the choice take 4.5, the lists 1, the products 18; 200 tokens of 32 experts (0.4 GB) 118 us.
 //
 // The router sums pieces of 8 products in fp32 and the pieces in fp64: a choice between experts whose scores are next
-// to each other hangs on it. Hidden values are rounded to the weights' type, the second product's operand; the rest
-// stays in fp32.
+// to each other hangs on it. Hidden values are two numbers of the weights' type, the second product's operands (see below);
+// all else stays in fp32.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,7 +34,7 @@ namespace k {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStages = 5, kWideStages = 4;   // steps of a ring
+constexpr int kStages = 5;          // steps of a ring
 constexpr int kBlock = 64;          // inputs of a step
 constexpr int kMostExperts = 512;   // a lane has 16 scores
 constexpr int kRouteCtas = 8, kRouteThreads = 512;   // of a token's cluster, at most
@@ -51,14 +51,16 @@ struct MoEArgs {
   int splits;              // of the second product's k
   int* chosen;             // [rows]
   float* share;            // [rows]
-  void* hidden;            // [rows][inner]
+  void* hidden;            // [2][rows][inner]: values in the weights' type, and kRest times what they lost
   float* partial;          // [splits][rows][width]
 };
 
 template <typename T> struct Op;
 template <> struct Op<__half> {
   static __device__ __forceinline__ float2 both(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+  static constexpr float kMost = 65504.f, kRest = 2048.f;
   static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -67,7 +69,9 @@ template <> struct Op<__half> {
 };
 template <> struct Op<__nv_bfloat16> {
   static __device__ __forceinline__ float2 both(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+  static constexpr float kMost = 3.38953139e38f, kRest = 256.f;
   static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -323,11 +327,23 @@ __device__ __forceinline__ float activated(int gelu, float gate, float up) {
   return (gelu ? 0.5f * gate * (1.f + erff(gate * 0.70710678f)) : gate / (1.f + expf(-gate))) * up;
 }
 
+// A hidden value goes to the second product as two operands: rounded to the type, and kRest times the rest of it, which keeps
+// fp16's rests normal numbers. Together they have the bits that the second product's fp32 sums can make use of, 16 in bf16
+// and 22 in fp16; rounded once, they added half as much again to the error of the results. (Beyond the type's largest
+// number the rest is infinite, and so is the result.)
+template <typename T> __device__ __forceinline__ void store_hidden(const MoEArgs& a, int row, int feature, float v) {
+  T* to = static_cast<T*>(a.hidden) + int64_t(row) * a.w.inner + feature;
+  const T whole = Op<T>::round(fminf(fmaxf(v, -Op<T>::kMost), Op<T>::kMost));
+  to[0] = whole;
+  to[int64_t(a.rows) * a.w.inner] = Op<T>::round((v - Op<T>::widen(whole)) * Op<T>::kRest);
+}
+
 // The two products, for up to 8 rows of an expert. Units: (entry, tile of 8 features or 16 outputs, part of k); a CTA takes
 // every gridDim.x-th, its warps every kWarps-th block of k.
 template <typename T, bool kFirst>
 struct Product {
   static constexpr int kTile = kFirst ? 8 : 16, kStage = 2048;   // bytes of a step: 16 rows of 64 inputs
+  static constexpr int kSets = kFirst ? 1 : 2;                   // of columns: hidden values and their rests
   const MoEArgs& a;
   const Lists& at;
   const uint32_t ring;   // this warp's
@@ -410,16 +426,18 @@ struct Product {
       const uint16_t* column = nullptr;   // of the lane's token
       if (g < en.count)
         column = kFirst ? static_cast<const uint16_t*>(a.x) + rows[g] / a.w.top_k * a.xs : static_cast<const uint16_t*>(a.hidden) + int64_t(rows[g]) * a.w.inner;
-      auto fetch = [&](uint4 (&b)[2], int block) {
+      auto fetch = [&](uint4 (&b)[kSets][2], int block) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = block * kBlock + h * 32 + 8 * t;
-          b[h] = make_uint4(0, 0, 0, 0);
-          if (column != nullptr && k < depth) b[h] = *reinterpret_cast<const uint4*>(column + k);
-        }
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k = block * kBlock + h * 32 + 8 * t;
+            b[s][h] = make_uint4(0, 0, 0, 0);
+            if (column != nullptr && k < depth) b[s][h] = *reinterpret_cast<const uint4*>(column + s * (int64_t(a.rows) * a.w.inner) + k);
+          }
       };
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-      auto step = [&](const uint4 (&b)[2]) {
+      float d[kSets][4] = {};
+      auto step = [&](const uint4 (&b)[kSets][2]) {
         wait<kStages - 2>();
         const uint32_t from = ring + stage_out * kStage + lane * 16;
         stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
@@ -430,15 +448,17 @@ struct Product {
           for (int h = 0; h < 2; ++h) w[r][h] = shared16(from + (r * 2 + h) * 512);
         copy_step();   // into the stage read in the step before
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          Op<T>::mma(d, w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, b[h].x, b[h].y);
-          Op<T>::mma(d, w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, b[h].z, b[h].w);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int s = 0; s < kSets; ++s) {
+            Op<T>::mma(d[s], w[0][h].x, w[1][h].x, w[0][h].y, w[1][h].y, b[s][h].x, b[s][h].y);
+            Op<T>::mma(d[s], w[0][h].z, w[1][h].z, w[0][h].w, w[1][h].w, b[s][h].z, b[s][h].w);
+          }
       };
       // Columns are fetched a step ahead, into registers of their own by turns (a copy between them would wait for them).
       const int end = end_of(v);
       int block = v.part * blocks + warp;
-      uint4 even[2], odd[2];
+      uint4 even[kSets][2], odd[kSets][2];
       if (block < end) fetch(even, block);
       while (block < end) {
         if (block + kWarps < end) fetch(odd, block + kWarps);
@@ -453,15 +473,14 @@ struct Product {
       float* all = sums + turn * kWarps * 128;
       turn ^= 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) all[warp * 128 + i * 32 + lane] = d[i];
+      for (int i = 0; i < 4; ++i) all[warp * 128 + i * 32 + lane] = kFirst ? d[0][i] : fmaf(d[kSets - 1][i], 1.f / Op<T>::kRest, d[0][i]);
       __syncthreads();
       auto total = [&](int q) { return all[q] + all[128 + q] + all[256 + q] + all[384 + q]; };
       static_assert(kWarps == 4, "the sum above");
       const int l = threadIdx.x & 31, q = threadIdx.x >> 5;   // a value of the tile per thread, or a pair of them
       const int c = (l & 3) * 2 + (q & 1);
       if (kFirst) {
-        if (q < 2 && c < en.count)
-          static_cast<T*>(a.hidden)[int64_t(rows[c]) * a.w.inner + v.first + (l >> 2)] = Op<T>::round(activated(a.w.gelu, total(q * 32 + l), total((q + 2) * 32 + l)));
+        if (q < 2 && c < en.count) store_hidden<T>(a, rows[c], v.first + (l >> 2), activated(a.w.gelu, total(q * 32 + l), total((q + 2) * 32 + l)));
       } else {
         const int r = v.first + (q >> 1) * 8 + (l >> 2);
         if (c < en.count && r < out_rows) a.partial[(int64_t(v.part) * a.rows + rows[c]) * out_rows + r] = total(q * 32 + l);
@@ -474,9 +493,12 @@ struct Product {
 // them (in shared memory, swizzled by 16-byte pieces) and have rows of their own, over all of k.
 template <typename T, bool kFirst>
 struct WideProduct {
-  static constexpr int NT = 4, MT = 2;
+  // kRing: steps of the ring. With twice the columns the second product's is shorter, so that two CTAs share an SM beside their
+  // lists (256 tokens through 8 of 64 experts of 1024 x 512: 118 us, 131 with four steps; 200 of 32 experts 129 and 133).
+  static constexpr int NT = 4, MT = 2, kRing = kFirst ? 4 : 3;
   static constexpr int kWarpRows = kFirst ? 8 * MT : 16 * MT, kTile = kWarps * kWarpRows, kApart = kFirst ? 8 : 16;
-  static constexpr int kStage = kWarps * MT * 2048 + NT * 8 * 128;
+  static constexpr int kSets = kFirst ? 1 : 2, kColumns = NT * 8 * 128;   // of columns; bytes of a set
+  static constexpr int kStage = kWarps * MT * 2048 + kSets * kColumns;
   const MoEArgs& a;
   const Lists& at;
   const uint32_t ring;
@@ -557,32 +579,29 @@ struct WideProduct {
       for (int i = 0; i < 2; ++i) {
         const int c = (tid % 4) * 2 + i, k = copy_block * kBlock + c * 8;
         const bool there = copy_column != nullptr && k < depth;
-        copy16(stage + kWarps * MT * 2048 + token * 128 + ((c ^ (token & 7)) * 16), there ? copy_column + k : weights, there);
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+          copy16(stage + kWarps * MT * 2048 + s * kColumns + token * 128 + ((c ^ (token & 7)) * 16),
+                 there ? copy_column + s * (int64_t(a.rows) * a.w.inner) + k : weights, there);
       }
       if (++copy_block >= copy_end) next_unit();
     }
     commit();
-    stage_in = stage_in + 1 == kWideStages ? 0 : stage_in + 1;
+    stage_in = stage_in + 1 == kRing ? 0 : stage_in + 1;
   }
   __device__ __forceinline__ void run() {
 #pragma unroll
-    for (int i = 0; i < kWideStages - 1; ++i) copy_step();
+    for (int i = 0; i < kRing - 1; ++i) copy_step();
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Unit v = unit(u);
       const Entry en = at.entry[v.entry];
       const int used = (en.count + 7) / 8;
-      float d[NT][MT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[n][m][i] = 0.f;
+      float d[kSets][NT][MT][4] = {};
       for (int block = v.begin; block < v.end; ++block) {
-        wait<kWideStages - 2>();
+        wait<kRing - 2>();
         __syncthreads();   // all copies of this step are there, and all have read the step before
         const uint32_t stage = ring + stage_out * kStage, from = stage + warp * (MT * 2048) + lane * 16;
-        stage_out = stage_out + 1 == kWideStages ? 0 : stage_out + 1;
+        stage_out = stage_out + 1 == kRing ? 0 : stage_out + 1;
         uint4 w[MT][2][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -596,11 +615,14 @@ struct WideProduct {
           if (n >= used) break;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint4 b = shared16(stage + kWarps * MT * 2048 + (n * 8 + g) * 128 + (((h * 4 + t) ^ g) * 16));
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              Op<T>::mma(d[n][m], w[m][0][h].x, w[m][1][h].x, w[m][0][h].y, w[m][1][h].y, b.x, b.y);
-              Op<T>::mma(d[n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b.z, b.w);
+            for (int s = 0; s < kSets; ++s) {
+              const uint4 b = shared16(stage + kWarps * MT * 2048 + s * kColumns + (n * 8 + g) * 128 + (((h * 4 + t) ^ g) * 16));
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                Op<T>::mma(d[s][n][m], w[m][0][h].x, w[m][1][h].x, w[m][0][h].y, w[m][1][h].y, b.x, b.y);
+                Op<T>::mma(d[s][n][m], w[m][0][h].z, w[m][1][h].z, w[m][0][h].w, w[m][1][h].w, b.z, b.w);
+              }
             }
           }
         }
@@ -617,11 +639,12 @@ struct WideProduct {
           for (int m = 0; m < MT; ++m) {
             const int r = v.first + warp * kWarpRows + m * kApart + g;
             if (kFirst) {
-              if (r < out_rows) static_cast<T*>(a.hidden)[int64_t(row) * a.w.inner + r] = Op<T>::round(activated(a.w.gelu, d[n][m][i], d[n][m][i + 2]));
+              if (r < out_rows) store_hidden<T>(a, row, r, activated(a.w.gelu, d[0][n][m][i], d[0][n][m][i + 2]));
             } else {
               float* to = a.partial + (int64_t(v.part) * a.rows + row) * out_rows + r;
-              if (r < out_rows) to[0] = d[n][m][i];
-              if (r + 8 < out_rows) to[8] = d[n][m][i + 2];
+              auto both = [&](int j) { return fmaf(d[kSets - 1][n][m][j], 1.f / Op<T>::kRest, d[0][n][m][j]); };
+              if (r < out_rows) to[0] = both(i);
+              if (r + 8 < out_rows) to[8] = both(i + 2);
             }
           }
         }
@@ -632,13 +655,14 @@ struct WideProduct {
 };
 
 constexpr int kSums = 2 * kWarps * 128 * 4;   // of the warps, twice
-__host__ __device__ constexpr int ring_bytes(int columns) {
-  return columns == 1 ? kWarps * kStages * 2048 : kWideStages * (kWarps * 2 * 2048 + 4096);
+template <typename T, int NT, bool kFirst> constexpr int ring_bytes() {
+  if constexpr (NT == 1) return kWarps * kStages * 2048;
+  else return WideProduct<T, kFirst>::kRing * WideProduct<T, kFirst>::kStage;
 }
 template <typename T, int NT, bool kFirst>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) product_kernel(const __grid_constant__ MoEArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int kHeld = ring_bytes(NT) + (NT == 1 ? kSums : 0);
+  constexpr int kHeld = ring_bytes<T, NT, kFirst>() + (NT == 1 ? kSums : 0);
   // The choice is there: for the first product once the router has ended; the second is launched after that, as the first
   // lets it begin behind its own wait.
   if (kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -646,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) product_kernel(cons
   const Lists at = make_lists<NT>(a, smem + kHeld, threadIdx.x);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
   if constexpr (NT == 1) {
-    Product<T, kFirst> product(a, at, ring + (threadIdx.x >> 5) * kStages * 2048, reinterpret_cast<float*>(smem + ring_bytes(NT)));
+    Product<T, kFirst> product(a, at, ring + (threadIdx.x >> 5) * kStages * 2048, reinterpret_cast<float*>(smem + ring_bytes<T, NT, kFirst>()));
     product.fill();   // weights, while the first product finishes the hidden values
     if (!kFirst) asm volatile("griddepcontrol.wait;" ::: "memory");
     product.run();
@@ -714,7 +738,7 @@ Sizes sizes(const MoEView& w, int64_t tokens) {
   while (z.splits < 8 && units * z.splits < enough && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   z.chosen = up(size_t(rows) * 4);
-  z.hidden = up(size_t(rows) * w.inner * 2);
+  z.hidden = up(size_t(rows) * w.inner * 4);
   z.partial = up(size_t(z.splits) * rows * w.width * 4);
   z.total = 2 * z.chosen + z.hidden + z.partial;
   return z;
@@ -733,7 +757,7 @@ cudaError_t enqueue(void (*kernel)(MoEArgs), const MoEArgs& a, int64_t grid, int
 
 template <typename T, int NT, bool kFirst>
 cudaError_t product(const MoEArgs& a, int sms, cudaStream_t s) {
-  const size_t smem = size_t(ring_bytes(NT)) + (NT == 1 ? kSums : 0) + lists_bytes(a.w.experts, a.entries, a.rows);
+  const size_t smem = size_t(ring_bytes<T, NT, kFirst>()) + (NT == 1 ? kSums : 0) + lists_bytes(a.w.experts, a.entries, a.rows);
   const auto kernel = product_kernel<T, NT, kFirst>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e != cudaSuccess) return e;

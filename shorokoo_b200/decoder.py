@@ -537,7 +537,8 @@ class MoEWeights:
 def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The mixture-of-experts layer of x [tokens, width], of the weights' type: for each token the sum over its
     experts of share * down (act(gate x) * (up x)). Meant for few tokens: an expert's weights are read once for every
-    32 of its tokens. Hidden values are rounded to the weights' type. ``out`` may be x itself."""
+    32 of its tokens. Hidden values are held as two numbers of the weights' type (16 bits in bfloat16, 22 in
+    float16, where they overflow beyond 65504). ``out`` may be x itself."""
     if not isinstance(weights, MoEWeights):
         _bad("weights must be MoEWeights")
     for name in ("router", "gate_up", "down", "selection_bias"):   # since the object was made, or made without recording

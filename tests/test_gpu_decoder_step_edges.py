@@ -1,0 +1,59 @@
+"""More GPU tests of the residual norms, mixture-of-experts layers and sampling: routers with logits far apart, scores
+next to each other, hidden values that cancel, draws in a row's flat tail, the streaming forms of the norms. Tolerances
+as in the tests beside these (h, v, u there), and with what each test says.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from shorokoo_b200 import B200ArgumentError, B200NotSupportedError, decoder
+from test_gpu_decoder_step import BF16, FP16, FP32, U, V, check_moe, half, layer, moe_reference, norm_reference, normal, rounded, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- mixture of experts ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens,experts,top_k,width,inner", [(1, 4, 2, 16, 64), (3, 4, 2, 16, 64), (40, 2, 1, 16, 64), (90, 5, 3, 24, 72),
+                                                              (2, 3, 2, 16, 1032), (50, 2, 2, 16, 1032)])
+def test_moe_keeps_hidden_values_that_cancel(tokens, experts, top_k, width, inner, dtype):
+    """Pairs of features with nearly the same hidden value and opposite weights behind them. What a rounding of hidden values to the
+    type would lose (h of each) is many times what is left of a pair; two values of the type hold them to h^2 (fp16: of values
+    and remainders that are normal numbers; the remainders are held 2^11 times as large, so 2^-36 and h 2^-25 below that)."""
+    gen = torch.Generator().manual_seed(tokens * 31 + inner)
+    router, gate_up, down = layer(gen, experts, width, inner, dtype)
+    gate_up[:, 1:inner:2] = gate_up[:, 0:inner:2]
+    gate_up[:, inner + 1::2] = (gate_up[:, inner::2].float() * (1 + 0.1 * torch.randn((experts, inner // 2, 1), generator=gen))).to(dtype)
+    down[:, :, 1::2] = -down[:, :, 0::2]
+    x = normal(gen, (tokens, width), dtype)
+    xd = x.double()
+    share, chosen = torch.softmax(xd @ router.double().t(), 1).topk(top_k, dim=1)
+    share = share / share.sum(1, keepdim=True)
+    want, slack = torch.zeros_like(xd), torch.zeros_like(xd)
+    for t in range(tokens):
+        for s, e in zip(share[t], chosen[t]):
+            w, d = gate_up[e].double(), down[e].double()
+            both, size = w @ xd[t], (width / 16 + 8) * U * (w.abs() @ xd[t].abs())
+            act, up = both[:inner] * torch.sigmoid(both[:inner]), both[inner:]
+            hidden = act * up
+            dact = 1.13 * size[:inner] + 6 * V * act.abs()
+            dh = up.abs() * dact + act.abs() * size[inner:] + dact * size[inner:] + 3 * V * hidden.abs()
+            dh = dh + half(dtype) ** 2 * (hidden.abs() + dh) + (half(dtype) * 2.0 ** -25 + 2.0 ** -36 if dtype is FP16 else 0.0)
+            want[t] += s * (d @ hidden)
+            slack[t] += s * (d.abs() @ dh + ((inner / 16 + 16) * U + 8 * V) * (d.abs() @ hidden.abs()))
+    w = decoder.MoEWeights(router.cuda(), gate_up.cuda(), down.cuda(), top_k=top_k)
+    within(decoder.moe(x.cuda(), w), want, rounded(want, slack, dtype), "moe")
+
+
+def by_logits(gen, logits, tokens, dtype, width=32, inner=40, router_type=None):
+    """x and a layer whose experts have these logits for every token, from the first input alone; the others are the tokens' own."""
+    router, gate_up, down = layer(gen, len(logits), width, inner, dtype, router_type)
+    router[:] = 0
+    router[:, 0] = torch.tensor(logits)
+    x = normal(gen, (tokens, width), dtype)
+    x[:, 0] = 1.0
+    return x, (router, gate_up, down)
