@@ -186,13 +186,23 @@ __device__ __forceinline__ void choose(const MoEView& w, const double* l, int la
     }
     if (lane == r) mine = int(e);
   }
-  const float z = float(l[mine]);
+  const double z = l[mine];
   float s;
   if (w.softmax) {
-    const float high = w.normalize ? __shfl_sync(~0u, z, 0) : float(top);   // any shift serves; the first chosen is near the top
-    s = expf(z - high);
+    // Shares are quotients, whatever the logits are shifted by; the largest of the chosen keeps them within fp32's range.
+    // That is the first chosen's, but where a bias has chosen.
+    double high = top;
+    if (w.normalize) {
+      high = biased && lane >= w.top_k ? -INFINITY : z;
+      if (biased) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) high = fmax(high, __shfl_xor_sync(~0u, high, d));
+      }
+      high = __shfl_sync(~0u, high, 0);
+    }
+    s = expf(float(z - high));
   } else {
-    s = 1.f / (1.f + expf(-z));
+    s = 1.f / (1.f + expf(float(-z)));
   }
   if (lane >= w.top_k) s = 0.f;
   if (w.normalize) {

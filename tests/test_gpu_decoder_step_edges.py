@@ -57,3 +57,15 @@ def by_logits(gen, logits, tokens, dtype, width=32, inner=40, router_type=None):
     x = normal(gen, (tokens, width), dtype)
     x[:, 0] = 1.0
     return x, (router, gate_up, down)
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+@pytest.mark.parametrize("logits,bias,top_k", [
+    ((-100.0, 0.0), (2.0, 0.0), 2), ((45.0, -50.0, 1.0, 2.0), (0.0, 10.0, 0.0, 0.0), 2), ((-300.0, -200.0, 0.0, -1.0, 5.0), (9.0, 8.0, 0.0, 0.0, 7.0), 3),
+    ((-300.0, -200.0, 0.0, -1.0, 5.0), (9.0, 8.0, 0.0, 0.0, 7.0), 5), ((0.0, -200.0, -201.0), (0.0, 5.0, 4.0), 2)])
+def test_moe_softmax_shares_of_experts_chosen_by_their_bias(logits, bias, top_k, tokens):
+    """The first chosen has a logit far below another's, or all chosen are far below the rest."""
+    gen = torch.Generator().manual_seed(tokens + len(logits))
+    for dtype in (BF16, FP16):
+        x, weights = by_logits(gen, logits, tokens, dtype)
+        check_moe(x, weights, top_k=top_k, selection_bias=torch.tensor(bias))
