@@ -187,22 +187,23 @@ __device__ __forceinline__ void choose(const MoEView& w, const double* l, int la
     if (lane == r) mine = int(e);
   }
   const double z = l[mine];
+  // Shares that are normalized are quotients, whatever the scores are multiplied by: a factor that brings the largest of the
+  // chosen near 1 keeps them within fp32's range. Its logit is the first chosen's, but where a bias has chosen.
+  double high = top;
+  if (w.normalize) {
+    high = biased && lane >= w.top_k ? -INFINITY : z;
+    if (biased) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) high = fmax(high, __shfl_xor_sync(~0u, high, d));
+    }
+    high = __shfl_sync(~0u, high, 0);
+  }
   float s;
   if (w.softmax) {
-    // Shares are quotients, whatever the logits are shifted by; the largest of the chosen keeps them within fp32's range.
-    // That is the first chosen's, but where a bias has chosen.
-    double high = top;
-    if (w.normalize) {
-      high = biased && lane >= w.top_k ? -INFINITY : z;
-      if (biased) {
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) high = fmax(high, __shfl_xor_sync(~0u, high, d));
-      }
-      high = __shfl_sync(~0u, high, 0);
-    }
     s = expf(float(z - high));
-  } else {
-    s = 1.f / (1.f + expf(float(-z)));
+  } else {   // e^-c / (1 + e^-z), with c the largest logit where that is below 0
+    const double c = w.normalize ? fmin(high, 0.0) : 0.0;
+    s = 1.f / (expf(float(c)) + expf(float(c - z)));
   }
   if (lane >= w.top_k) s = 0.f;
   if (w.normalize) {

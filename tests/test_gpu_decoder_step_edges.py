@@ -69,3 +69,26 @@ def test_moe_softmax_shares_of_experts_chosen_by_their_bias(logits, bias, top_k,
     for dtype in (BF16, FP16):
         x, weights = by_logits(gen, logits, tokens, dtype)
         check_moe(x, weights, top_k=top_k, selection_bias=torch.tensor(bias))
+
+
+@pytest.mark.parametrize("tokens", [1, 30])
+@pytest.mark.parametrize("logits,bias,top_k", [
+    ((-91.0, -92.0, -95.0), None, 2), ((-91.0,), None, 1), ((-300.0, -120.0, -119.0, -118.0), None, 3), ((-300.0, -120.0, -119.0, 3.0), None, 3),
+    ((-100.0, -101.0, 60.0, 61.0), (5.0, 4.0, 0.0, 0.0), 2), ((-100.0, -101.0, 60.0, 61.0), (5.0, 4.0, 0.0, 3.5), 3)])
+def test_moe_sigmoid_shares_of_scores_next_to_nothing(logits, bias, top_k, tokens):
+    """Scores of 10^-40 and less have their ratios all the same."""
+    gen = torch.Generator().manual_seed(tokens + len(logits))
+    for dtype in (BF16, FP16):
+        x, weights = by_logits(gen, logits, tokens, dtype)
+        check_moe(x, weights, top_k=top_k, scoring="sigmoid", selection_bias=None if bias is None else torch.tensor(bias))
+
+
+def test_moe_sigmoid_share_of_a_single_expert():
+    """All of it, at any score, also at those that are none in 64 bits."""
+    gen = torch.Generator().manual_seed(1)
+    x, (router, gate_up, down) = by_logits(gen, (0.0, -1.0), 3, BF16)
+    run = lambda: decoder.moe(x.cuda(), decoder.MoEWeights(router.cuda(), gate_up.cuda(), down.cuda(), top_k=1, scoring="sigmoid"))
+    want = run()
+    for logit in (-50.0, -1000.0, -1e30, 1000.0):
+        router[:, 0] = torch.tensor([logit, 2 * logit if logit < 0 else -logit])
+        assert torch.equal(run(), want)
