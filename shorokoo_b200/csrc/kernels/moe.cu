@@ -90,11 +90,12 @@ __device__ __forceinline__ uint4 shared16(uint32_t at) {
   return v;
 }
 
-// A score as an integer of the same order, NaN below all and 0 for none
-__device__ __forceinline__ uint32_t ordered(float v) {
-  if (v != v) return 1u;
-  const uint32_t b = __float_as_uint(v);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// A score as an integer of the same order, NaN below all and 0 for none. In 64 bits: scores that fp32 does not tell apart, more
+// of them beside a large bias, would go by the expert's number.
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  if (v != v) return 1ull;
+  const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
+  return b >> 63 ? ~b : b | 1ull << 63;
 }
 
 // One dot product of the router, by a warp.
@@ -147,11 +148,11 @@ template <int J> __device__ __noinline__ void sum_scores(const double (&v)[J], i
 }
 // and the order of score + bias.
 template <int J>
-__device__ __noinline__ void bias_keys(uint32_t (&key)[J], const double (&v)[J], const MoEView& w, int lane, double top, double all) {
+__device__ __noinline__ void bias_keys(unsigned long long (&key)[J], const double (&v)[J], const MoEView& w, int lane, double top, double all) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int e = j * 32 + lane;
-    if (e < w.experts) key[j] = ordered(float((w.softmax ? exp(v[j] - top) / all : 1.0 / (1.0 + exp(-v[j]))) + double(w.selection_bias[e])));
+    if (e < w.experts) key[j] = ordered((w.softmax ? exp(v[j] - top) / all : 1.0 / (1.0 + exp(-v[j]))) + double(w.selection_bias[e]));
   }
 }
 
@@ -162,23 +163,24 @@ __device__ __forceinline__ void choose(const MoEView& w, const double* l, int la
   double v[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) v[j] = j * 32 + lane < w.experts ? l[j * 32 + lane] : 0.0;
-  uint32_t key[J];
+  unsigned long long key[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) key[j] = j * 32 + lane < w.experts ? ordered(float(v[j])) : 0u;
+  for (int j = 0; j < J; ++j) key[j] = j * 32 + lane < w.experts ? ordered(v[j]) : 0ull;
   double top = 0, all = 0;
   const bool biased = w.selection_bias != nullptr;
   if (w.softmax && (biased || !w.normalize)) sum_scores<J>(v, w.experts, lane, top, all);
   if (biased) bias_keys<J>(key, v, w, lane, top, all);
   int mine = 0;          // lane r: the r-th chosen
   for (int r = 0; r < w.top_k; ++r) {
-    uint32_t best = key[0];
+    unsigned long long best = key[0];
+    int at = 0;
 #pragma unroll
-    for (int j = 1; j < J; ++j) best = max(best, key[j]);
-    const uint32_t most = __reduce_max_sync(~0u, best);
-    uint32_t e = ~0u;
-#pragma unroll
-    for (int j = J - 1; j >= 0; --j) e = key[j] == most ? j * 32 + lane : e;
-    e = __reduce_min_sync(~0u, e);
+    for (int j = 1; j < J; ++j)
+      if (key[j] > best) best = key[j], at = j;
+    const uint32_t upper = uint32_t(best >> 32), lower = uint32_t(best);
+    const bool first = upper == __reduce_max_sync(~0u, upper);
+    const uint32_t rest = __reduce_max_sync(~0u, first ? lower : 0u);
+    const uint32_t e = __reduce_min_sync(~0u, first && lower == rest ? at * 32 + lane : ~0u);
     if ((e & 31) == uint32_t(lane)) {
 #pragma unroll
       for (int j = 0; j < J; ++j)

@@ -92,3 +92,24 @@ def test_moe_sigmoid_share_of_a_single_expert():
     for logit in (-50.0, -1000.0, -1e30, 1000.0):
         router[:, 0] = torch.tensor([logit, 2 * logit if logit < 0 else -logit])
         assert torch.equal(run(), want)
+
+
+@pytest.mark.parametrize("experts", [6, 300])
+@pytest.mark.parametrize("kw", [dict(), dict(scoring="sigmoid"), dict(selection_bias=0.0), dict(selection_bias=1000.0),
+                                dict(selection_bias=-3.0, scoring="sigmoid"), dict(normalize=False)])
+def test_moe_orders_experts_by_scores_in_64_bits(kw, experts):
+    """Two logits 2^-30 apart (with a bias of 1000 2^-20, where fp32 has steps of 2^-14): the larger is chosen, not the lower expert."""
+    gen = torch.Generator().manual_seed(experts)
+    for tokens in (1, 20):
+        x, weights = by_logits(gen, [0.0] * experts, tokens, BF16, router_type=FP32)
+        bias = kw.get("selection_bias")
+        x[:, 8] = 2.0 ** -10 if bias == 1000.0 else 2.0 ** -15
+        weights[0][[1, 4], 0] = 1.0
+        weights[0][4, 8] = x[0, 8].float()
+        given = dict(kw)
+        if bias is not None:
+            given["selection_bias"] = torch.zeros(experts)
+            given["selection_bias"][[1, 4]] = bias if bias > 0 else 0.0
+            if bias < 0:
+                given["selection_bias"] += bias
+        check_moe(x, weights, top_k=1, gap=0.0, **given)
