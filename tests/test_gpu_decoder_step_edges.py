@@ -113,3 +113,18 @@ def test_moe_orders_experts_by_scores_in_64_bits(kw, experts):
             if bias < 0:
                 given["selection_bias"] += bias
         check_moe(x, weights, top_k=1, gap=0.0, **given)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens", [1, 20])
+def test_moe_sums_a_16_bit_router_in_64_bits(tokens, dtype):
+    """Products of one piece of eight inputs, of 1 and of 2^-26, and such as cancel: 32 bits would lose the small ones."""
+    gen = torch.Generator().manual_seed(tokens)
+    x, weights = by_logits(gen, [0.0] * 5, tokens, dtype)
+    x[:, 1], x[:, 2] = 2.0 ** -13, -1.0
+    weights[0][[1, 4], 0] = 1.0
+    weights[0][4, 1] = 2.0 ** -13
+    check_moe(x, weights, top_k=1, gap=0.0)
+    weights[0][:, 2] = 1.0 - 2.0 ** -6          # 0 in place of 1, 2^-6 in place of 0
+    weights[0][[1, 4], 2] = 1.0 - 2.0 ** -5
+    check_moe(x, weights, top_k=1, gap=0.0)
