@@ -367,7 +367,7 @@ SB_API int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_ro
  * which the running sum of the kept w, in order of the index, exceeds uniform[row] (float32, [0, 1)) times their sum.
  * Settings of each row (device arrays) or, where the array is NULL, of all. temperature 0 (or less, or NaN): the first
  * of the largest. top_k 0 (or less): any number. top_p 1 (or more, or NaN) and min_p 0 (or less, or NaN): no filter;
- * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0. vocab: at most 2^21. */
+ * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-43 count as 0. vocab: at most 2^21. */
 typedef struct sb_sampling {
   const float *temperature_of, *top_p_of, *min_p_of;
   const int32_t* top_k_of;

@@ -6,9 +6,11 @@
 // A row belongs to a cluster of up to 8 CTAs that hold its slices in shared memory: the logits are read from memory
 // once, whatever the passes, and a few rows still spread over the card.
 //
-// Weights are integers, exp(.) in units of 2^-40 in 64 bits: their sums do not depend on an order, so that results repeat and
-// all CTAs of a cluster come to the same decisions. They are off by about 2^-30 of themselves; from fp32 arithmetic the
-// sums of a flat row of 10^5 tokens would be off by 10^-4 to 10^-3 of a token, and so would the choice.
+// Weights are integers, exp(.) in units of 2^-42 in 64 bits (2^21 of them sum to less than 2^64): their sums do not depend
+// on an order, so that results repeat and all CTAs of a cluster come to the same decisions. They are off by at most 2^-28.8 of
+// themselves and half a unit, either way: cut off instead of rounded, and to units of 2^-40, they drew another token in one of
+// some hundred rows with a peak and a tail of 10^5 tokens. From fp32 arithmetic the sums of a flat row of 10^5 tokens would
+// be off by 10^-4 to 10^-3 of a token, and so would the choice.
 //
 // The filters keep what lies above a border in (logit, index). It is found without sorting: a histogram over the range that
 // holds it, of counts for top_k and of weights for top_p, then over the border's bin alone, whose candidates are listed, until
@@ -43,6 +45,7 @@ constexpr int kListBytes = 4096;        // of a list of candidates
 constexpr int kSettled = 256;           // candidates of a row that are ranked one against another
 constexpr int kMostRounds = 6;          // 128 or 256 bins, then at least 128 each of what is left of 2^32 floats
 constexpr int kSteps = 64;              // table of 2^(-j / 64)
+constexpr int kUnit = 42;               // bits of the largest weight
 
 struct SampleArgs {
   const void* logits;
@@ -112,7 +115,7 @@ struct alignas(16) Shared {
   uint32_t warp_ties[kWarps];
   // this CTA's own
   uint32_t power[kSteps];                   // 2^(30 - j / 64)
-  uint32_t part[3][kWarps][kCoarse];        // sums of each warp's part of the slice, of 16, 16 and 9 bits of the weights
+  uint32_t part[3][kWarps][kCoarse];        // sums of each warp's part of the slice, of 16, 16 and 11 bits of the weights
   uint4 list[2][kListBytes / 16];
   int listed[2];
   float rank_value[kSettled];
@@ -132,12 +135,12 @@ constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: sums with it are rounded t
 
 static_assert(sizeof(Shared) + kHeld <= 227 * 1024, "a slice beside what a CTA keeps");
 
-// exp((v - top) / T) in units of 2^-40 for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
+// exp((v - top) / T) in units of 2^-kUnit for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
 // floats, k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms
-// of its series (the next is 2^-34), in integers: off by about 2^-30 of itself, where expf would be off by up to 2^-21
+// of its series (the next is 2^-34), in integers: off by up to 2^-28.8 of itself, where expf would be off by up to 2^-21
 // (the difference top - v alone by 2^-20) and exp in fp64 takes three times as long.
 __device__ __noinline__ unsigned long long wide_exp(double d, double rate) {   // any finite d and temperature
-  return __double2ull_rn(exp(d * rate) * 1099511627776.0);
+  return __double2ull_rn(exp(d * rate) * double(1ull << kUnit));
 }
 // kShort: v and top have 16 bits, and top - v is as good as exact: what it loses (of logits below 2^-7) is 2^-25 of it.
 template <bool kShort> struct NearWeights {   // temperatures and logits that are floats like others
@@ -158,14 +161,14 @@ template <bool kShort> struct NearWeights {   // temperatures and logits that ar
     const int zi = int(__float_as_uint(fmaf(z, 536870912.f, kMagic)) - 0x4b400000u);   // in units of 2^-29
     const uint32_t p = power[k % kSteps];
     const uint32_t w = p - uint32_t(__mulhi(int(p), zi * 8));
-    return (static_cast<unsigned long long>(w) << 10) >> (k / kSteps & 63);
+    return (((static_cast<unsigned long long>(w) << (kUnit - 30 + 1)) >> (k / kSteps & 63)) + 1) >> 1;   // rounded
   }
 };
 struct FarWeights {   // any others
   float top;
   double rate;   // 1 / T
   __device__ __forceinline__ unsigned long long operator()(float v) const {
-    return v == top ? 1ull << 40 : wide_exp(double(v) - double(top), rate);
+    return v == top ? 1ull << kUnit : wide_exp(double(v) - double(top), rate);
   }
 };
 
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       s.wide_rate = r, s.rate = float(l), s.rate_low = float(l - double(float(l)));
       s.near = temperature > 1e-20f && temperature < 1e20f && fabsf(most) < 1e30f;
       // the least key that counts: weights below are 0 or below min_p
-      double cut = -28.5;   // 2^40 exp(cut) rounds to 0
+      double cut = -29.9;   // 2^kUnit exp(cut) rounds to 0
       if (min_p > 0.f) cut = fmax(cut, log(double(min_p)));
       const float v = most < INFINITY ? __double2float_ru(double(most) + double(temperature) * fmin(cut, 0.0)) : most;
       s.lo = key_of(fmaxf(v, -3.402823466e38f));

@@ -565,7 +565,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     (equal logits: the lower index first); the token is the first index at which the running sum of the kept w, in order
     of the index, exceeds uniform times their sum. Each setting is a number or a tensor of one per row (float32, top_k
     int32). Temperature 0 (or less): the first of the largest; top_k 0 (or less), top_p 1 (or more) and min_p 0 (or
-    less) filter nothing. A row without a logit above -inf gives -1. Weights below 2^-41 count as 0."""
+    less) filter nothing. A row without a logit above -inf gives -1. Weights below 2^-43 count as 0."""
     device = _cuda(logits, "logits")
     dtype = logits.dtype
     elem = _ELEM.get(dtype)

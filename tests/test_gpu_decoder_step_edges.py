@@ -128,3 +128,37 @@ def test_moe_sums_a_16_bit_router_in_64_bits(tokens, dtype):
     weights[0][:, 2] = 1.0 - 2.0 ** -6          # 0 in place of 1, 2^-6 in place of 0
     weights[0][[1, 4], 2] = 1.0 - 2.0 ** -5
     check_moe(x, weights, top_k=1, gap=0.0)
+
+
+# ---- sampling --------------------------------------------------------------------------------
+
+def check_draws(row, u, temperature=1.0):
+    """The tokens of one row for many u, against sums in long double. Weights are off by half a unit of 2^-42 of the largest and
+    2^-28.8 of themselves, so that a running sum and u times all of them differ by at most n units and 2^-27.8 of all from
+    what they are; a token whose border is nearer than that to the target may be its neighbour."""
+    row = row.double().numpy().astype(np.longdouble)
+    w = np.exp((row - row.max()) / np.longdouble(np.float32(temperature)))
+    mass = np.concatenate((np.zeros(1, np.longdouble), np.cumsum(w)))
+    off = row.size * np.longdouble(2) ** -42 + np.longdouble(2) ** np.longdouble(-27.8) * mass[-1] + np.longdouble(2) ** -41
+    target = u.numpy().astype(np.longdouble) * mass[-1]
+    def check(got):
+        got = got.cpu().numpy()
+        wrong = (target < mass[got] - off) | (target >= mass[got + 1] + off)
+        assert not wrong.any(), f"{int(wrong.sum())} of {wrong.size} draws are off"
+    return check
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("vocab", [150001, 200000])
+def test_sample_in_the_tail_of_a_peaked_row(vocab, dtype):
+    """One token with nearly all the mass and a tail of weights of some 10^-9, where nearly all the u of this test point: roundings of the
+    weights that go one way add up along it."""
+    gen = torch.Generator().manual_seed(vocab)
+    row = (0.3 * torch.randn(vocab, generator=gen)).to(dtype)
+    row[100] = 19.0
+    tail = float(torch.exp(row.double() - 19.0).sum()) - 1.0
+    u = torch.cat((torch.rand(100, generator=gen), 1 - tail / (1 + tail) * torch.rand(3000, generator=gen).double())).float().clamp(max=1 - 2.0 ** -24)
+    check = check_draws(row, u)
+    logits = row.cuda().expand(u.numel(), vocab)
+    check(decoder.sample(logits, u.cuda()))
+    check(torch.cat([decoder.sample(logits[i: i + 10], u[i: i + 10].cuda()) for i in range(0, 400, 10)] + [decoder.sample(logits[400:], u[400:].cuda())]))
