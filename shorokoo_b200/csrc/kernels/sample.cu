@@ -7,7 +7,7 @@
 // once, whatever the passes, and a few rows still spread over the card.
 //
 // Weights are integers, exp(.) in units of 2^-42 in 64 bits (2^21 of them sum to less than 2^64): their sums do not depend
-// on an order, so that results repeat and all CTAs of a cluster come to the same decisions. They are off by at most 2^-28.8 of
+// on an order, so that results repeat and all CTAs of a cluster come to the same decisions. They are off by at most 2^-28 of
 // themselves and half a unit, either way: cut off instead of rounded, and to units of 2^-40, they drew another token in one of
 // some hundred rows with a peak and a tail of 10^5 tokens. From fp32 arithmetic the sums of a flat row of 10^5 tokens would
 // be off by 10^-4 to 10^-3 of a token, and so would the choice.
@@ -137,7 +137,8 @@ static_assert(sizeof(Shared) + kHeld <= 227 * 1024, "a slice beside what a CTA k
 
 // exp((v - top) / T) in units of 2^-kUnit for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
 // floats, k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms
-// of its series (the next is 2^-34), in integers: off by up to 2^-28.8 of itself, where expf would be off by up to 2^-21
+// of its series (the next is 2^-34), in integers: off by up to 2^-28 of itself (a quarter each from the table and from z, half from the
+// product, which is cut off), where expf would be off by up to 2^-21
 // (the difference top - v alone by 2^-20) and exp in fp64 takes three times as long.
 __device__ __noinline__ unsigned long long wide_exp(double d, double rate) {   // any finite d and temperature
   return __double2ull_rn(exp(d * rate) * double(1ull << kUnit));

@@ -134,12 +134,13 @@ def test_moe_sums_a_16_bit_router_in_64_bits(tokens, dtype):
 
 def check_draws(row, u, temperature=1.0):
     """The tokens of one row for many u, against sums in long double. Weights are off by half a unit of 2^-42 of the largest and
-    2^-28.8 of themselves, so that a running sum and u times all of them differ by at most n units and 2^-27.8 of all from
-    what they are; a token whose border is nearer than that to the target may be its neighbour."""
+    by 2^-28 of themselves (a number of 2^29 to 2^30, off by half from a table, times one off by 2^-30, the product cut off to a whole
+    number: 2^-30 + 2^-30 + 2^-29), so that a running sum and u times all of them differ by at most n units and 2^-27 of
+    all from what they are; a token whose border is nearer than that to the target may be its neighbour."""
     row = row.double().numpy().astype(np.longdouble)
     w = np.exp((row - row.max()) / np.longdouble(np.float32(temperature)))
     mass = np.concatenate((np.zeros(1, np.longdouble), np.cumsum(w)))
-    off = row.size * np.longdouble(2) ** -42 + np.longdouble(2) ** np.longdouble(-27.8) * mass[-1] + np.longdouble(2) ** -41
+    off = row.size * np.longdouble(2) ** -42 + np.longdouble(2) ** -27 * mass[-1] + np.longdouble(2) ** -41
     target = u.numpy().astype(np.longdouble) * mass[-1]
     def check(got):
         got = got.cpu().numpy()
