@@ -7,7 +7,7 @@
 // once, whatever the passes, and a few rows still spread over the card.
 //
 // Weights are integers, exp(.) in units of 2^-42 in 64 bits (2^21 of them sum to less than 2^64): their sums do not depend
-// on an order, so that results repeat and all CTAs of a cluster come to the same decisions. They are off by at most 2^-28 of
+// on an order, so that results repeat and all CTAs of a cluster come to the same decisions. They are off by at most 2^-27.9 of
 // themselves and half a unit, either way: cut off instead of rounded, and to units of 2^-40, they drew another token in one of
 // some hundred rows with a peak and a tail of 10^5 tokens. From fp32 arithmetic the sums of a flat row of 10^5 tokens would
 // be off by 10^-4 to 10^-3 of a token, and so would the choice.
@@ -125,7 +125,7 @@ struct alignas(16) Shared {
   // what its first warp found out
   unsigned long long all, target, above, before, ties_before, tie;
   double wide_rate;
-  float most_of_row, rate, rate_low;
+  float most_of_row, start, start_low, rate, rate_low;
   unsigned long long ties;
   uint32_t lo, border;
   int near, outcome, bin, chosen;
@@ -135,29 +135,24 @@ constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: sums with it are rounded t
 
 static_assert(sizeof(Shared) + kHeld <= 227 * 1024, "a slice beside what a CTA keeps");
 
-// exp((v - top) / T) in units of 2^-kUnit for v from top down to where it is nothing. With y = (top - v) log2(e) / T in two
-// floats, k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms
-// of its series (the next is 2^-34), in integers: off by up to 2^-28 of itself (a quarter each from the table and from z, half from the
-// product, which is cut off), where expf would be off by up to 2^-21
-// (the difference top - v alone by 2^-20) and exp in fp64 takes three times as long.
+// exp((v - top) / T) in units of 2^-kUnit for v from top down to where it is nothing: 2^-y with y = (top - v) log2(e) / T. With
+// k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms of its
+// series (the next is 2^-33), in integers: off by up to 2^-27.9 of itself (a quarter each from the table and from z, half from
+// the product, which is cut off), where expf would be off by up to 2^-21 and exp in fp64 takes three times as long. g is taken as
+// (top log2(e) / T - k / 64) - v log2(e) / T, the former without rounding (top's part is split at 2^-8), the latter and the
+// difference with one: top - v would lose what small v have, in 16 bits too (up to 2^-21 of a weight below a top of 10).
 __device__ __noinline__ unsigned long long wide_exp(double d, double rate) {   // any finite d and temperature
   return __double2ull_rn(exp(d * rate) * double(1ull << kUnit));
 }
-// kShort: v and top have 16 bits, and top - v is as good as exact: what it loses (of logits below 2^-7) is 2^-25 of it.
-template <bool kShort> struct NearWeights {   // temperatures and logits that are floats like others
-  float top, rate, rate_low;   // log2(e) / T
+constexpr float kNearTop = 65536.f;   // multiples of 2^-8 below it are floats
+struct NearWeights {   // temperatures and logits that are floats like others, top log2(e) / T below kNearTop
+  float start, start_low;   // top log2(e) / T in multiples of 2^-8, and the rest
+  float rate, rate_low;     // log2(e) / T
   const uint32_t* power;
   __device__ __forceinline__ unsigned long long operator()(float v) const {
-    const float d = top - v;
-    const float y = d * rate;
-    float y_low = fmaf(d, rate_low, fmaf(d, rate, -y));
-    if (!kShort) {
-      const float b = d - top;
-      y_low = fmaf((top - (d - b)) - (v + b), rate, y_low);   // what d lost
-    }
-    const float shifted = fmaf(y, float(kSteps), kMagic);
+    const float shifted = fmaf(fmaf(-v, rate, start), float(kSteps), kMagic);
     const uint32_t k = __float_as_uint(shifted);
-    const float g = fmaf(shifted - kMagic, -1.f / kSteps, y) + y_low;
+    const float g = fmaf(-v, rate, fmaf(shifted - kMagic, -1.f / kSteps, start)) + fmaf(-v, rate_low, start_low);
     const float z = g * fmaf(-g, fmaf(-g, 0.0555041087f, 0.240226507f), 0.693147181f);
     const int zi = int(__float_as_uint(fmaf(z, 536870912.f, kMagic)) - 0x4b400000u);   // in units of 2^-29
     const uint32_t p = power[k % kSteps];
@@ -285,7 +280,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       s.most_of_row = most;
       const double r = 1.0 / double(temperature), l = r * 1.4426950408889634;
       s.wide_rate = r, s.rate = float(l), s.rate_low = float(l - double(float(l)));
-      s.near = temperature > 1e-20f && temperature < 1e20f && fabsf(most) < 1e30f;
+      const double at = double(most) * l;
+      s.start = float(rint(at * 256.0) / 256.0), s.start_low = float(at - double(s.start));
+      s.near = temperature > 1e-20f && temperature < 1e20f && fabs(at) < kNearTop;
       // the least key that counts: weights below are 0 or below min_p
       double cut = -29.9;   // 2^kUnit exp(cut) rounds to 0
       if (min_p > 0.f) cut = fmax(cut, log(double(min_p)));
@@ -321,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     return;
   }
 
-  const NearWeights<sizeof(T) == 2> near_weight = {most, s.rate, s.rate_low, s.power};
+  const NearWeights near_weight = {s.start, s.start_low, s.rate, s.rate_low, s.power};
   const FarWeights far_weight = {most, s.wide_rate};
   const bool near = s.near;
   auto weight = [&](float v) { return near ? near_weight(v) : far_weight(v); };

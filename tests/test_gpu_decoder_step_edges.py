@@ -134,13 +134,14 @@ def test_moe_sums_a_16_bit_router_in_64_bits(tokens, dtype):
 
 def check_draws(row, u, temperature=1.0):
     """The tokens of one row for many u, against sums in long double. Weights are off by half a unit of 2^-42 of the largest and
-    by 2^-28 of themselves (a number of 2^29 to 2^30, off by half from a table, times one off by 2^-30, the product cut off to a whole
-    number: 2^-30 + 2^-30 + 2^-29), so that a running sum and u times all of them differ by at most n units and 2^-27 of
-    all from what they are; a token whose border is nearer than that to the target may be its neighbour."""
+    by 2^-27.9 of themselves (a number of 2^29 to 2^30, off by half from a table, times one off by 2^-30, the product cut off to a
+    whole number: 2^-30 + 2^-30 + 2^-29, and 2^-32 of what is rounded before), so that a running sum and u times all of
+    them differ by at most n units and 2^-26.9 of all from what they are; a token whose border is nearer than that to the target
+    may be its neighbour."""
     row = row.double().numpy().astype(np.longdouble)
     w = np.exp((row - row.max()) / np.longdouble(np.float32(temperature)))
     mass = np.concatenate((np.zeros(1, np.longdouble), np.cumsum(w)))
-    off = row.size * np.longdouble(2) ** -42 + np.longdouble(2) ** -27 * mass[-1] + np.longdouble(2) ** -41
+    off = row.size * np.longdouble(2) ** -42 + np.longdouble(2) ** np.longdouble(-26.9) * mass[-1] + np.longdouble(2) ** -41
     target = u.numpy().astype(np.longdouble) * mass[-1]
     def check(got):
         got = got.cpu().numpy()
@@ -163,3 +164,24 @@ def test_sample_in_the_tail_of_a_peaked_row(vocab, dtype):
     logits = row.cuda().expand(u.numel(), vocab)
     check(decoder.sample(logits, u.cuda()))
     check(torch.cat([decoder.sample(logits[i: i + 10], u[i: i + 10].cuda()) for i in range(0, 400, 10)] + [decoder.sample(logits[400:], u[400:].cuda())]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_sample_of_tiny_logits_below_a_large_one(dtype):
+    """What the difference from the largest loses in fp32 is the same for all of them, and as much as some tokens weigh."""
+    gen = torch.Generator().manual_seed(5)
+    row = torch.full((150001,), 7 * 2.0 ** -24).to(dtype)
+    row[::1000] = torch.randn(151, generator=gen).to(dtype)
+    row[100000] = 10.0
+    u = torch.rand(20000, generator=gen)
+    check_draws(row, u)(decoder.sample(row.cuda().expand(u.numel(), row.numel()), u.cuda()))
+
+
+@pytest.mark.parametrize("temperature", [1e-2, 1e-3, 1e-4, 1e-6])
+def test_sample_at_low_temperatures(temperature):
+    """Quotients of logit and temperature from thousands to millions, and tokens near enough to count all the same."""
+    gen = torch.Generator().manual_seed(6)
+    for top in (30.0, -50.0, 1000.0):
+        row = top - 10 * max(temperature, abs(top) * 2.0 ** -22) * torch.rand(50001, generator=gen)
+        u = torch.rand(4000, generator=gen)
+        check_draws(row, u, temperature)(decoder.sample(row.cuda().expand(u.numel(), row.numel()), u.cuda(), temperature=temperature))
