@@ -415,9 +415,9 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
     as (y, h). norm(z) is z / sqrt(mean(z^2) + eps) or, with kind "layer", the same of z less its mean.
     ``residual`` [rows, width] has x's type or float32, and so has h; ``gate`` is [width] or [rows, width] of x's
     type; weights and biases [width] have x's type or float32, all of them the same one; ``weight_offset`` is added
-    to both weights. Without residual, gate, post_weight and scale h is x itself; without a weight y is None. y is
-    taken of h before h is rounded. ``out`` may be x, and ``residual_out`` x or residual; they may not overlap an
-    input otherwise."""
+    to both weights. Without residual, gate, post_weight and scale h is x itself, or a copy where ``out`` is x; without a
+    weight y is None. y is taken of h before h is rounded. ``out`` may be x, and ``residual_out`` x or residual; they may
+    not overlap an input otherwise."""
     device = _cuda(x, "x")
     dtype = x.dtype
     elem = _ELEM.get(dtype)
@@ -458,7 +458,8 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
     if post_weight is None and post_bias is not None:
         _bad("post_bias needs a post_weight")
     h, hp, ss = x, 0, 0
-    if residual is not None or gate is not None or post_weight is not None or scale != 1.0 or residual_out is not None:
+    over = weight is not None and out is not None and isinstance(out, torch.Tensor) and out.data_ptr() == x.data_ptr()
+    if residual is not None or gate is not None or post_weight is not None or scale != 1.0 or residual_out is not None or over:
         if residual_out is None:
             h, ss = x.new_empty((rows, n), dtype=sum_type), n
         else:

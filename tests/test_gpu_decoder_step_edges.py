@@ -185,3 +185,20 @@ def test_sample_at_low_temperatures(temperature):
         row = top - 10 * max(temperature, abs(top) * 2.0 ** -22) * torch.rand(50001, generator=gen)
         u = torch.rand(4000, generator=gen)
         check_draws(row, u, temperature)(decoder.sample(row.cuda().expand(u.numel(), row.numel()), u.cuda(), temperature=temperature))
+
+
+# ---- residual norms --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,width,dtype", [(3, 64, BF16), (700, 4096, BF16), (5, 75, FP32)])
+def test_residual_norm_over_x_leaves_h(rows, width, dtype):
+    """Where h is x itself and y goes over x, h is a tensor of its own."""
+    gen = torch.Generator().manual_seed(rows)
+    x, w = normal(gen, (rows, width), dtype).cuda(), normal(gen, (width,), dtype).cuda()
+    before = x.clone()
+    want, h = decoder.residual_norm(x, w)
+    assert h is x and torch.equal(x, before)
+    y, h = decoder.residual_norm(x, w, out=x)
+    assert y is x and torch.equal(y, want) and torch.equal(h, before)
+    x = before.clone()
+    y, h = decoder.residual_norm(x, w, out=x.view(rows, width))          # the same memory by another name
+    assert torch.equal(x, want) and torch.equal(h, before)
