@@ -667,20 +667,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       if (coarse_even) rest(coarse);
       else rest(coarse_keys);
     } else {
-      auto sums = [&](const auto& weight) {
-        for (int q = part_begin + lane; q < part_end; q += 32) {
-          const uint4 p = piece(q);
-          const T* e = reinterpret_cast<const T*>(&p);
-#pragma unroll
-          for (int j = 0; j < kV; ++j) {
-            const float v = value<T>(e[j]);
-            const unsigned long long w = weight(v);
-            equal += v == last;
-            sum += v > last ? w : 0;
-          }
-        }
-      };
-      if (border != lo || min_p > 0.f) {   // few: their weights alone
+      if (border != lo || min_p > 0.f || !near) {   // few (at low temperatures too): their weights alone
         for (int q = part_begin + lane; q < part_end; q += 32) {
           const uint4 p = piece(q);
           const T* e = reinterpret_cast<const T*>(&p);
@@ -693,10 +680,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
           }
           each_of(q, mine, [&](float v) { sum += weight(v); });
         }
-      } else if (near) {
-        sums(near_weight);
       } else {
-        sums(far_weight);
+        for (int q = part_begin + lane; q < part_end; q += 32) {
+          const uint4 p = piece(q);
+          const T* e = reinterpret_cast<const T*>(&p);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = value<T>(e[j]);
+            const unsigned long long w = near_weight(v);
+            equal += v == last;
+            sum += v > last ? w : 0;
+          }
+        }
       }
     }
     __syncwarp();
