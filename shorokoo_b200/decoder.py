@@ -513,13 +513,19 @@ class MoEWeights:
             _bad(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
         if activation not in ("silu", "gelu"):
             _bad(f"activation must be 'silu' or 'gelu', got {activation!r}")
+        try:
+            top_k, scale = int(top_k), float(scale)
+        except (TypeError, ValueError, OverflowError) as e:
+            raise B200ArgumentError(f"top_k and scale must be numbers: {e}") from None
+        if not 0 < top_k <= experts:   # (the C structure would keep 32 bits of it)
+            _bad(f"top_k {top_k} of {experts} experts")
         bias = _vector(selection_bias, "selection_bias", device, (torch.float32,), experts)
         self.router, self.gate_up, self.down, self.selection_bias = router, gate_up, down, selection_bias
-        self.device, self.dtype, self.experts, self.width, self.inner, self.top_k = device, dtype, experts, width, inner, int(top_k)
+        self.device, self.dtype, self.experts, self.width, self.inner, self.top_k = device, dtype, experts, width, inner, top_k
         self._c = _native.MoEWeights(router.data_ptr(), gate_up.data_ptr(), down.data_ptr(), bias, router.stride(0), gate_up.stride(0),
                                      gate_up.stride(1), down.stride(0), down.stride(1), experts, width, inner, _ELEM[dtype],
                                      _ELEM[router.dtype], self.top_k, int(scoring == "sigmoid"), int(bool(normalize)),
-                                     int(activation == "gelu"), float(scale))
+                                     int(activation == "gelu"), scale)
         self._ref = C.byref(self._c)
         self._space = {}
         self._workspace(1)   # refuses what the layer does not support
@@ -590,8 +596,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
         to = _vector(out, "out", device, (torch.int64,), rows)
     try:
         by = _pack_sampling(tp, pp, mp, kp, temperature, top_p, min_p, min(max(int(top_k), 0), 0x7fffffff))
-    except (struct.error, OverflowError) as e:
-        raise B200ArgumentError(f"temperature, top_p and min_p must be numbers of 32 bits or tensors: {e}") from None
+    except (struct.error, TypeError, ValueError, OverflowError) as e:
+        raise B200ArgumentError(f"temperature, top_k, top_p and min_p must be numbers of 32 bits or tensors: {e}") from None
     _call("sb_sample", device, logits.data_ptr(), stride, elem, rows, logits.shape[1], at, by, to)
     return out
 

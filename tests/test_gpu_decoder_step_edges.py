@@ -202,3 +202,18 @@ def test_residual_norm_over_x_leaves_h(rows, width, dtype):
     x = before.clone()
     y, h = decoder.residual_norm(x, w, out=x.view(rows, width))          # the same memory by another name
     assert torch.equal(x, want) and torch.equal(h, before)
+
+
+def test_settings_that_are_no_numbers_of_their_type_are_refused():
+    gen = torch.Generator().manual_seed(1)
+    r, g, d = (t.cuda() for t in layer(gen, 4, 64, 32, BF16))
+    for top_k in (2 ** 32 + 2, -2 ** 32 + 2, 2 ** 31, math.nan, math.inf, None, "two"):
+        with pytest.raises(B200ArgumentError):
+            decoder.MoEWeights(r, g, d, top_k=top_k)
+    with pytest.raises(B200ArgumentError):
+        decoder.MoEWeights(r, g, d, top_k=2, scale="one")
+    x, u = torch.zeros(3, 50, device="cuda"), torch.zeros(3, device="cuda")
+    for kw in (dict(top_k=math.nan), dict(top_k=None), dict(top_k="two"), dict(top_p=None), dict(temperature="hot"), dict(top_k=math.inf)):
+        with pytest.raises(B200ArgumentError):
+            decoder.sample(x, u, **kw)
+    assert decoder.sample(x, u, top_k=2 ** 40).tolist() == [0, 0, 0]     # more than there are
