@@ -407,8 +407,7 @@ int32_t sb_sample(const void* logits, int64_t logits_row_stride, int32_t elem_ty
               std::string("element type ") + dtype_name(elem_type));
     need(by != nullptr, "by is null");
     need(rows >= 0 && rows <= (int64_t(1) << 26) && vocab > 0, "sizes out of range");
-    // the kernel's halves of a part's sums hold 65536 weights, an eighth of a slice of an eighth of a row
-    supported(vocab <= (1 << 21), "vocab " + std::to_string(vocab) + " (at most 2^21)");
+    supported(vocab <= k::kMostVocab, "vocab " + std::to_string(vocab) + " (at most 2^21)");
     need(by->temperature_of != nullptr || !std::isnan(by->temperature), "temperature is NaN");
     need(by->top_p_of != nullptr || !std::isnan(by->top_p), "top_p is NaN");
     need(by->min_p_of != nullptr || !std::isnan(by->min_p), "min_p is NaN");

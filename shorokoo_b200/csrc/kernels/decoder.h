@@ -83,6 +83,8 @@ struct MoEView {
 size_t moe_workspace(const MoEView& w, int64_t tokens);
 cudaError_t moe(const MoEView& w, const void* x, int64_t xs, void* y, int64_t ys, int64_t tokens, void* ws, int sms, cudaStream_t s);
 
+constexpr int kMostVocab = 1 << 21;   // logits of a row that sample takes
+
 // Settings of all rows, or (not null) of each.
 struct SamplingView {
   const float *temperature_of, *top_p_of, *min_p_of;

@@ -134,6 +134,10 @@ struct alignas(16) Shared {
 constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: sums with it are rounded to integers, in their low bits
 
 static_assert(sizeof(Shared) + kHeld <= 227 * 1024, "a slice beside what a CTA keeps");
+// The widest row's sums: all of it in 64 bits, a warp's part of a slice (a slice rounded up to 64, a part to pieces) in words of
+// 16, 16 and kUnit - 31 bits of each weight.
+constexpr int kMostPart = (kMostVocab / kMostCtas + 64) / kWarps + 2 * 8;
+static_assert(kMostVocab <= 1 << (63 - kUnit) && kMostPart <= 1 << 16 && kMostPart <= 1 << (32 - (kUnit - 31)), "sums of weights");
 
 // exp((v - top) / T) in units of 2^-kUnit for v from top down to where it is nothing: 2^-y with y = (top - v) log2(e) / T. With
 // k = y rounded to 64ths and g what is left of it, it is 2^(-k / 64) from a table, times 1 - z, z = 1 - 2^-g by three terms of its
