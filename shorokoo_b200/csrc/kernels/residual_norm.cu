@@ -437,9 +437,12 @@ cudaError_t stream(const ResidualNormArgs& a, RowRing ring, size_t smem, int thr
   return cudaGetLastError();
 }
 
-template <typename T, typename S, typename W, int V, int P, bool kEdges>
+// kLong: rows that take all of 1024 threads
+template <typename T, typename S, typename W, int V, int P, bool kEdges, bool kLong = false>
 cudaError_t start(const ResidualNormArgs& a, int threads, cudaStream_t s) {
-  if (threads == 32) {
+  if constexpr (kLong) {
+    residual_norm_kernel<T, S, W, V, P, kEdges, 1024><<<unsigned(a.rows), 1024, 0, s>>>(a);
+  } else if (threads == 32) {
     constexpr int kRows = 4;   // of a CTA
     residual_norm_kernel<T, S, W, V, P, kEdges, 32><<<unsigned((a.rows + kRows - 1) / kRows), 32 * kRows, 0, s>>>(a);
   } else if (threads <= 256) {
@@ -485,7 +488,8 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   threads = 32;
   while (threads < 1024 && threads * each < pieces) threads *= 2;
   if (each == 1) return start<T, S, W, 8, 1, kEdges>(a, threads, s);
-  if (kEdges && pieces > 4096) return start<T, S, W, 8, 5, kEdges>(a, threads, s);   // 32768 elements and an overhang
+  if constexpr (kEdges)
+    if (pieces > 4096) return start<T, S, W, 8, 5, kEdges, true>(a, threads, s);   // 32768 elements and an overhang
   return start<T, S, W, 8, 4, kEdges>(a, threads, s);
 }
 
@@ -496,7 +500,7 @@ cudaError_t launch_single(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   while (threads < 1024 && threads * each < a.width) threads *= 2;
   if (each == 4) return start<T, S, W, 1, 4, false>(a, threads, s);
   if (each == 16) return start<T, S, W, 1, 16, false>(a, threads, s);
-  return start<T, S, W, 1, 32, false>(a, threads, s);
+  return start<T, S, W, 1, 32, false, true>(a, threads, s);
 }
 
 enum Form { kSingle, kPieces, kWithEdges };
