@@ -217,3 +217,66 @@ def test_settings_that_are_no_numbers_of_their_type_are_refused():
         with pytest.raises(B200ArgumentError):
             decoder.sample(x, u, **kw)
     assert decoder.sample(x, u, top_k=2 ** 40).tolist() == [0, 0, 0]     # more than there are
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows,width,pitch", [(6100, 1024, 1024), (6100, 1033, 1033), (6000, 1500, 1501), (3100, 2048, 2056), (3100, 2050, 2050), (1600, 4096, 4096),
+                                              (1600, 4099, 4099), (1600, 4095, 4100), (950, 5003, 5003), (950, 6000, 6000), (620, 11001, 11001)])
+def test_residual_norm_of_rows_that_stream(rows, width, pitch, dtype):
+    """More than two rows for each of as many CTAs as 148 multiprocessors hold (20 of the shortest rows here), in every type, aligned or not;
+    rows spread over all of them against the formula, in the forms that differ in what streams beside x."""
+    gen = torch.Generator(device="cuda").manual_seed(rows + width)
+    rand = lambda *shape, kind=dtype: torch.randn(shape, device="cuda", generator=gen).to(kind)
+    x, r, g = (rand(rows, pitch)[:, pitch - width:] for _ in range(3))
+    wide = rand(rows, pitch, kind=FP32)[:, pitch - width:]
+    w, b, p, c, v = (rand(width) for _ in range(5))
+    f = lambda t: t.float() * 1.001
+    room = lambda kind: torch.empty((rows, pitch), dtype=kind, device="cuda")[:, pitch - width:]     # rows that begin as x's do
+    some = sorted({i * (rows - 1) // 60 for i in range(61)} | {i for i in (1, 2, 147, 148, 739, 740, rows - 2) if i < rows})
+    host = lambda t: t if not isinstance(t, torch.Tensor) else t[some].cpu() if t.dim() == 2 else t.cpu()
+    for given in (dict(residual=r), dict(bias=b, residual=r, post_weight=p, post_bias=c, gate=g, scale=0.3, kind="layer"),
+                  dict(residual=wide, gate=v, kind="layer", eps=1e-5), dict(residual=wide, post_weight=p, gate=g, weight_offset=1.0), dict(gate=g, bias=b)):
+        for weight in (w, f(w)):
+            if weight.dtype is FP32:
+                given = {k: f(t) if k in ("bias", "post_weight", "post_bias") else t for k, t in given.items()}
+            stream = given["residual"].dtype if "residual" in given else dtype
+            y, h = decoder.residual_norm(x, weight, out=room(dtype), residual_out=room(stream), **given)
+            wy, dy, wh, dh = norm_reference(host(x), weight.cpu(), **{k: host(t) for k, t in given.items()})
+            within(y[some], wy, rounded(wy, dy, dtype), "y")
+            within(h[some], wh, rounded(wh, dh, h.dtype), "h")
+    given = dict(gate=g, post_weight=p)
+    a, d = room(dtype).copy_(x), room(FP32).copy_(wide)
+    y, h = decoder.residual_norm(x, w, residual=wide, out=room(dtype), residual_out=room(FP32), **given)
+    decoder.residual_norm(a, w, residual=d, out=a, residual_out=d, **given)
+    assert torch.equal(a, y) and torch.equal(d, h)
+
+
+# ---- what is refused -------------------------------------------------------------------------
+
+def test_tensors_with_a_gradient_or_a_tangent_are_refused():
+    gen = torch.Generator().manual_seed(1)
+    r, g, d = (t.cuda() for t in layer(gen, 4, 64, 32, BF16))
+    x, w, bias = normal(gen, (3, 64), BF16).cuda(), torch.ones(64, dtype=BF16, device="cuda"), torch.zeros(4, device="cuda")
+    logits, u, k = torch.zeros(3, 50, device="cuda"), torch.zeros(3, device="cuda"), torch.ones(3, device="cuda")
+    experts = decoder.MoEWeights(r, g, d, top_k=2)
+    norm = lambda **t: decoder.residual_norm(**dict(dict(x=x, weight=w, bias=w, residual=x, post_weight=w, post_bias=w, gate=x), **t))
+    calls = [(lambda t, n=n: norm(**{n: t}), s) for n, s in (("x", x), ("weight", w), ("bias", w), ("residual", x), ("post_weight", w), ("post_bias", w), ("gate", x),
+                                                             ("gate", w), ("out", x), ("residual_out", x))]
+    calls += [(lambda t: decoder.moe(t, experts), x), (lambda t: decoder.moe(x, experts, out=t), x), (lambda t: decoder.MoEWeights(r, g, d, top_k=2, selection_bias=t), bias),
+              (lambda t: decoder.MoEWeights(t, g, d, top_k=2), r), (lambda t: decoder.MoEWeights(r, t, d, top_k=2), g), (lambda t: decoder.MoEWeights(r, g, t, top_k=2), d)]
+    calls += [(lambda t: decoder.sample(t, u), logits), (lambda t: decoder.sample(logits, t), u)]
+    calls += [(lambda t, n=n: decoder.sample(logits, u, **{n: t}), k) for n in ("temperature", "top_p", "min_p")]
+    for i, (call, t) in enumerate(calls):
+        call(t.clone())
+        with pytest.raises(B200NotSupportedError, match="gradient"):
+            call(t.clone().requires_grad_())
+            pytest.fail(f"call {i} was accepted")
+        with torch.no_grad():
+            call(t.clone().requires_grad_())
+        with forward_ad.dual_level(), pytest.raises(B200NotSupportedError, match="tangent"):
+            call(forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+            pytest.fail(f"call {i} was accepted")
+    with torch.no_grad():
+        late = decoder.MoEWeights(r, g, d, top_k=2, selection_bias=bias.clone().requires_grad_())
+    with pytest.raises(B200NotSupportedError, match="gradient"):
+        decoder.moe(x, late)
