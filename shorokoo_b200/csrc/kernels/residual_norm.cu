@@ -196,7 +196,11 @@ __device__ __forceinline__ float2 moments(const float (&z)[P][V], const Residual
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int e = 0; e < V; ++e) s += z[p][e];
-    mean = row.sum(s) * a.per_width;
+    // The product with the rounded 1 / width, and what that leaves of the sum: without the latter equal values would be off
+    // their mean, by as much as a row's spread may be. (A division there: 777 rows of 11001 55 us, not 54.)
+    s = row.sum(s);
+    mean = s * a.per_width;
+    mean = fmaf(fmaf(-mean, float(a.width), s), a.per_width, mean);
     s = 0.f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {

@@ -250,6 +250,17 @@ def test_residual_norm_of_rows_that_stream(rows, width, pitch, dtype):
     decoder.residual_norm(a, w, residual=d, out=a, residual_out=d, **given)
     assert torch.equal(a, y) and torch.equal(d, h)
 
+@pytest.mark.parametrize("rows,width", [(3, 3), (5, 48), (2, 768), (700, 768), (400, 1001), (1300, 4100), (2, 6000), (300, 11001), (2, 20000)])
+def test_residual_norm_of_equal_values(rows, width):
+    """A layer norm of equal values of 8 bits: their sums and mean are exact, so nothing is left but the bias."""
+    gen = torch.Generator().manual_seed(width)
+    w, b = normal(gen, (width,), FP32).cuda(), normal(gen, (width,), FP32).cuda()
+    value = torch.tensor([1000.0, -3.5, 1.0078125, 253.0, 30000.0, 1e-3, 0.0, 44032.0]).bfloat16().float()
+    x = value[torch.arange(rows) % 8][:, None].expand(rows, width).cuda()
+    for kind in (BF16, FP32):
+        y, h = decoder.residual_norm(x.to(kind), w.to(kind), bias=b.to(kind), kind="layer", residual=torch.zeros_like(x, dtype=kind))
+        assert torch.equal(h, x.to(kind)) and torch.equal(y, b.to(kind).expand(rows, width))
+
 
 # ---- what is refused -------------------------------------------------------------------------
 
