@@ -741,14 +741,17 @@ Sizes sizes(const MoEView& w, int64_t tokens) {
   z.tokens = int(std::min<int64_t>(std::max<int64_t>(tokens, 1), std::min(256, 2048 / w.top_k)));
   const int rows = z.tokens * w.top_k;
   // Columns of a product: 8 where an expert has few tokens on average; an expert that has more is read again (from L2, as
-  // its entries are near each other in time).
-  z.columns = z.tokens <= 8 || rows <= 4 * w.experts ? 8 : 32;
+  // its entries are near each other in time). 8 of 128 experts of 2048 x 768, 4 tokens each on average: 219 us with 8
+  // columns, 240 with 32; 6 tokens 250 and 255, 8 tokens 306 and 262. (6 of 64: 9 tokens 156 and 149.)
+  z.columns = z.tokens <= 8 || rows <= 6 * w.experts ? 8 : 32;
   z.entries = std::min(w.experts, rows) + rows / z.columns;
-  // Parts of the second product's k, of 512 inputs or more, until (expert, tile, part) triples are many for every CTA
+  // Parts of the second product's k, of 1024 inputs or more, until (expert, tile, part) triples are many for every CTA (64
+  // tokens through 2 of 8 experts of 1024 x 4096 75 us, in one part 138, in parts of 512 79; half or twice as many
+  // triples: within 2 in 100)
   const int tile = z.columns == 8 ? 16 : 32 * kWarps;
   const int64_t units = int64_t(std::min(w.experts, rows)) * ((w.width + tile - 1) / tile), enough = z.columns == 8 ? 4096 : 1024;
   z.splits = 1;
-  while (z.splits < 8 && units * z.splits < enough && w.inner / (z.splits * 2) >= 512) z.splits *= 2;
+  while (z.splits < 8 && units * z.splits < enough && w.inner / (z.splits * 2) >= 1024) z.splits *= 2;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   z.chosen = up(size_t(rows) * 4);
   z.hidden = up(size_t(rows) * w.inner * 4);

@@ -462,7 +462,9 @@ template <typename T, typename S, typename W, bool kEdges>
 cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   const int pieces = (a.width + 7) / 8 + (kEdges ? 1 : 0);
   // Many rows of 1024 elements or more: two pieces per thread (4099 rows of 4096 in bf16 with both norms and a gate: 39 us,
-  // one piece 45, four 46; without the ring 97). Shorter rows go a warp each without it (12608 of 768 in fp32: 36 us, 39 with).
+  // one piece 45, four 46; without the ring 97). Shorter rows go a warp each without it (12608 of 768 in fp32: 36 us, 39 with;
+  // 12000 of 768 in bf16 with both norms 25 and 29, of 1280 45 and 41). Many: enough for every CTA (1200 of 4096 16 us, 21
+  // without), with edges, whose weights have to be staged first, for every CTA to take two (900 of 4099 26 us without, 32 with).
   constexpr int kEach = 2;
   RowRing ring;
   const int pad = kEdges ? 48 : 0;   // a row that begins and ends inside a piece: what such pieces hold besides
@@ -480,7 +482,7 @@ cudaError_t launch_wide(const ResidualNormArgs& a, int sms, cudaStream_t s) {
   }
   const int ctas = std::min(threads <= 256 ? 1280 / threads : 1024 / threads, room / (2 * ring.bytes + staged));
   if (ctas == 1) threads = 1024;   // one row at a time: more warps hide more of its chain (777 of 11001: 53 us, 704 threads 59)
-  if (pieces >= 128 && threads <= 1024 && ctas > 0 && a.rows >= 2 * int64_t(ctas) * sms && int64_t(ctas) * sms >= 8) {
+  if (pieces >= 128 && threads <= 1024 && ctas > 0 && a.rows >= (kEdges ? 2 : 1) * int64_t(ctas) * sms && int64_t(ctas) * sms >= 8) {
     ring.stages = std::min(4, (room / ctas - staged) / ring.bytes);
     ring.vectors = ring.stages * ring.bytes;
     const size_t smem = size_t(ring.vectors) + staged;

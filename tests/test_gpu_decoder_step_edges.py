@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("tokens,experts,top_k,width,inner", [(1, 4, 2, 16, 64), (3, 4, 2, 16, 64), (40, 2, 1, 16, 64), (90, 5, 3, 24, 72),
-                                                              (2, 3, 2, 16, 1032), (50, 2, 2, 16, 1032)])
+                                                              (2, 3, 2, 16, 1032), (50, 2, 2, 16, 1032), (2, 3, 2, 16, 2056), (50, 2, 2, 16, 2056)])
 def test_moe_keeps_hidden_values_that_cancel(tokens, experts, top_k, width, inner, dtype):
     """Pairs of features with nearly the same hidden value and opposite weights behind them. What a rounding of hidden values to the
     type would lose (h of each) is many times what is left of a pair; two values of the type hold them to h^2 (fp16: of values
