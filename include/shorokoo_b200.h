@@ -321,7 +321,8 @@ SB_API int32_t sb_linear_w4(const sb_w4_weights* weights, const void* x, int64_t
  * bfloat16), residual and sum (where h goes; NULL: nowhere) elem_type or float32, weights and biases elem_type or
  * float32. y NULL: h alone; weight belongs to y. gate_row_stride 0: one gate for all rows. Sums are fp32: of squares, so
  * that fp32 values beyond 10^18 overflow. sum may be residual or x itself and y may be x itself; they may not overlap
- * an input otherwise. width: at most 32768. */
+ * an input otherwise. width: at most 32768. Rows that begin alike within 16 bytes, and weights that are 16-byte aligned,
+ * go in wide accesses; others element by element, up to three times as slow. */
 typedef struct sb_residual_norm_args {
   const void *x, *residual, *gate;
   void *sum, *y;
@@ -339,10 +340,11 @@ SB_API int32_t sb_residual_norm(const sb_residual_norm_args* args, void* stream)
  *   y = sum over its experts of share * down[e] (act(gate_up[e][:inner] x) * (gate_up[e][inner:] x))
  * with act(z) = z / (1 + e^-z) or z Phi(z). router [experts][width] (elem_type or float32), gate_up
  * [experts][2 * inner][width], down [experts][width][inner] (elem_type: float16 or bfloat16), rows contiguous and the
- * other strides in elements; selection_bias float32. Meant for few tokens: an expert's weights are read once for every
- * 32 of its tokens. experts: at most 512; top_k: at most 32; width and inner: multiples of 8; pointers
- * 16-byte aligned and strides multiples of 8 elements. Hidden values are held as two numbers
- * of elem_type (16 bits in bfloat16, 22 in float16, where they overflow beyond 65504). */
+ * other strides in elements; selection_bias float32. Meant for few tokens: an expert's weights are read from memory
+ * anew for every 256 tokens (2048 / top_k where that is less), and from L2 for every 32 of an expert's tokens, or 8
+ * where experts have few. experts: at most 512; top_k: at most 32; width and inner: multiples of 8; pointers
+ * 16-byte aligned and strides multiples of 8 elements. Hidden values are held as
+ * two numbers of elem_type (16 bits in bfloat16, 22 in float16, where they overflow beyond 65504). */
 #define SB_MOE_SOFTMAX 0
 #define SB_MOE_SIGMOID 1
 #define SB_MOE_SILU 0
@@ -367,7 +369,8 @@ SB_API int32_t sb_moe(const sb_moe_weights* weights, const void* x, int64_t x_ro
  * which the running sum of the kept w, in order of the index, exceeds uniform[row] (float32, [0, 1)) times their sum.
  * Settings of each row (device arrays) or, where the array is NULL, of all. temperature 0 (or less, or NaN): the first
  * of the largest. top_k 0 (or less): any number. top_p 1 (or more, or NaN) and min_p 0 (or less, or NaN): no filter;
- * top_p 0: the first of the largest. A row without a logit above -inf gives -1. Weights below 2^-43 count as 0. vocab: at most 2^21. */
+ * top_p 0: the first of the largest; the largest is kept at any min_p. A row without a logit above -inf gives -1.
+ * Weights below 2^-43 count as 0. vocab: at most 2^21. */
 typedef struct sb_sampling {
   const float *temperature_of, *top_p_of, *min_p_of;
   const int32_t* top_k_of;

@@ -13,10 +13,11 @@
 // Four kernels in a chain, each launched while the one before it runs: the router's dot products and the choice, a cluster
 // per token; the first product over (expert, features), its k split over a CTA's warps; the second over (expert, outputs,
 // part of k) into partial sums, whose weights are on their way before the first has ended; their sum in the order of a
-// token's experts. No atomics decide an order: results repeat. (All of it in one cooperative launch took 33 us, not 27, for a
-// token through 8 of 128 experts of 2048 x 768: such a launch and its three barriers cost 8 us, these four kernels 4.)
-// Measured: 13 tokens through 6 of 64 experts of 4096 x 1400 in fp16 (1.6 GB) 259 us, 6.1 TB/s; one token (75 MB) 27 us,
-// of which the router and the choice take 4.5, the lists 1, the products 18; 200 tokens of 32 experts (0.4 GB) 118 us.
+// token's experts. No atomics decide an order: results repeat. (All of it in one cooperative launch took 33 us where the chain
+// took 27, for a token through 8 of 128 experts of 2048 x 768: such a launch and its three barriers cost 8 us, these four
+// kernels 4.)
+// Measured: 13 tokens through 6 of 64 experts of 4096 x 1400 in fp16 (1.6 GB) 266 us, 6.0 TB/s; one token (75 MB) 29 us,
+// of which the router and the choice take 6, the lists 1, the products 18; 200 tokens of 32 experts (0.4 GB) 130 us.
 //
 // The router's sums, scores and their order are in fp64: a choice between experts whose scores are next to each other
 // hangs on it. Hidden values are two numbers of the weights' type, the second product's operands (see below);

@@ -19,9 +19,9 @@
 // order needs the weights of the border's bin only, and then of the part that the draw falls in.
 //
 // The weights' arithmetic (about 25 instructions each) and the cluster's barriers bound it, not the logits' bytes (12 us):
-// 256 rows of 150001 in bf16 take 30 us for the largest alone, 96 us without a filter, 107 us with top_k 50, 187 us with
+// 256 rows of 150001 in bf16 take 39 us for the largest alone, 109 us without a filter, 115 us with top_k 50, 193 us with
 // top_p 0.9 (two CTAs per SM hide part of the barriers). One row of 32000: 16 us, a chain of seven barriers. Exponentials
-// in fp64 and 64-bit atomics in place of the table and the halves: 584 us for the 187.
+// in fp64 and 64-bit atomics in place of the table and the halves: 584 us for the 193.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

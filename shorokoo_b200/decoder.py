@@ -417,7 +417,8 @@ def residual_norm(x: torch.Tensor, weight: Optional[torch.Tensor], *, bias: Opti
     type; weights and biases [width] have x's type or float32, all of them the same one; ``weight_offset`` is added
     to both weights. Without residual, gate, post_weight and scale h is x itself, or a copy where ``out`` is x; without a
     weight y is None. y is taken of h before h is rounded. ``out`` may be x, and ``residual_out`` x or residual; they may
-    not overlap an input otherwise."""
+    not overlap an input otherwise. Rows that begin alike within 16 bytes, and weights that are 16-byte aligned (whole tensors
+    are), go in wide accesses; others element by element, up to three times as slow."""
     device = _cuda(x, "x")
     dtype = x.dtype
     elem = _ELEM.get(dtype)
@@ -543,8 +544,8 @@ class MoEWeights:
 
 def moe(x: torch.Tensor, weights: MoEWeights, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The mixture-of-experts layer of x [tokens, width], of the weights' type: for each token the sum over its
-    experts of share * down (act(gate x) * (up x)). Meant for few tokens: an expert's weights are read once for every
-    32 of its tokens. Hidden values are held as two numbers of the weights' type (16 bits in bfloat16, 22 in
+    experts of share * down (act(gate x) * (up x)). Meant for few tokens: an expert's weights are read from memory anew for
+    every 256 tokens (2048 / top_k where that is less). Hidden values are held as two numbers of the weights' type (16 bits in bfloat16, 22 in
     float16, where they overflow beyond 65504). ``out`` may be x itself."""
     if not isinstance(weights, MoEWeights):
         _bad("weights must be MoEWeights")
@@ -572,7 +573,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_
     (equal logits: the lower index first); the token is the first index at which the running sum of the kept w, in order
     of the index, exceeds uniform times their sum. Each setting is a number or a tensor of one per row (float32, top_k
     int32). Temperature 0 (or less): the first of the largest; top_k 0 (or less), top_p 1 (or more) and min_p 0 (or
-    less) filter nothing. A row without a logit above -inf gives -1. Weights below 2^-43 count as 0."""
+    less) filter nothing, and at any min_p the largest is kept. A row without a logit above -inf gives -1. Weights below
+    2^-43 count as 0."""
     device = _cuda(logits, "logits")
     dtype = logits.dtype
     elem = _ELEM.get(dtype)
