@@ -17,7 +17,7 @@
 // took 27, for a token through 8 of 128 experts of 2048 x 768: such a launch and its three barriers cost 8 us, these four
 // kernels 4.)
 // Measured: 13 tokens through 6 of 64 experts of 4096 x 1400 in fp16 (1.6 GB) 266 us, 6.0 TB/s; one token (75 MB) 29 us,
-// of which the router and the choice take 6, the lists 1, the products 18; 200 tokens of 32 experts (0.4 GB) 130 us.
+// of which the router and the choice take 6, the lists 1, the products 18; 200 tokens of 32 experts (0.4 GB) 130 to 138 us.
 //
 // The router's sums, scores and their order are in fp64: a choice between experts whose scores are next to each other
 // hangs on it. Hidden values are two numbers of the weights' type, the second product's operands (see below);
@@ -352,6 +352,11 @@ template <typename T> __device__ __forceinline__ void store_hidden(const MoEArgs
   to[int64_t(a.rows) * a.w.inner] = Op<T>::round((v - Op<T>::widen(whole)) * Op<T>::kRest);
 }
 
+// The sums over both operands. (One that is infinite by its weights has no rest: infinities of another sign would make it NaN.)
+template <typename T> __device__ __forceinline__ float joined(float whole, float rest) {
+  return isfinite(whole) ? fmaf(rest, 1.f / Op<T>::kRest, whole) : whole;
+}
+
 // The two products, for up to 8 rows of an expert. Units: (entry, tile of 8 features or 16 outputs, part of k); a CTA takes
 // every gridDim.x-th, its warps every kWarps-th block of k.
 template <typename T, bool kFirst>
@@ -487,7 +492,7 @@ struct Product {
       float* all = sums + turn * kWarps * 128;
       turn ^= 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) all[warp * 128 + i * 32 + lane] = kFirst ? d[0][i] : fmaf(d[kSets - 1][i], 1.f / Op<T>::kRest, d[0][i]);
+      for (int i = 0; i < 4; ++i) all[warp * 128 + i * 32 + lane] = kFirst ? d[0][i] : joined<T>(d[0][i], d[kSets - 1][i]);
       __syncthreads();
       auto total = [&](int q) { return all[q] + all[128 + q] + all[256 + q] + all[384 + q]; };
       static_assert(kWarps == 4, "the sum above");
@@ -656,7 +661,7 @@ struct WideProduct {
               if (r < out_rows) store_hidden<T>(a, row, r, activated(a.w.gelu, d[0][n][m][i], d[0][n][m][i + 2]));
             } else {
               float* to = a.partial + (int64_t(v.part) * a.rows + row) * out_rows + r;
-              auto both = [&](int j) { return fmaf(d[kSets - 1][n][m][j], 1.f / Op<T>::kRest, d[0][n][m][j]); };
+              auto both = [&](int j) { return joined<T>(d[0][n][m][j], d[kSets - 1][n][m][j]); };
               if (r < out_rows) to[0] = both(i);
               if (r + 8 < out_rows) to[8] = both(i + 2);
             }

@@ -10,7 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from shorokoo_b200 import B200ArgumentError, B200NotSupportedError, decoder
-from test_gpu_decoder_step import BF16, FP16, FP32, U, V, check_moe, half, layer, moe_reference, norm_reference, normal, rounded, within
+from test_gpu_decoder_step import BF16, FP16, FP32, U, V, check_moe, check_sample, half, layer, moe_reference, norm_reference, normal, rounded, within
 
 pytestmark = pytest.mark.gpu
 
@@ -47,6 +47,22 @@ def test_moe_keeps_hidden_values_that_cancel(tokens, experts, top_k, width, inne
             slack[t] += s * (d.abs() @ dh + ((inner / 16 + 16) * U + 8 * V) * (d.abs() @ hidden.abs()))
     w = decoder.MoEWeights(router.cuda(), gate_up.cuda(), down.cuda(), top_k=top_k)
     within(decoder.moe(x.cuda(), w), want, rounded(want, slack, dtype), "moe")
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens,experts", [(1, 3), (40, 2)])
+def test_moe_of_infinite_weights(tokens, experts, dtype):
+    """One infinite weight behind a hidden value makes its output infinite, of the value's sign, and no other."""
+    gen = torch.Generator().manual_seed(tokens)
+    router, gate_up, down = layer(gen, experts, 64, 40, dtype)
+    x = normal(gen, (tokens, 64), dtype)
+    down[:, 17, 5] = math.inf
+    hidden = lambda e: (lambda g, u: g * torch.sigmoid(g) * u)(x.double() @ gate_up[e, 5].double(), x.double() @ gate_up[e, 45].double())
+    first = (x.double() @ router.double().t()).argmax(1)
+    sign = torch.stack([hidden(e) for e in range(experts)], 1)[torch.arange(tokens), first].sign()
+    y = decoder.moe(x.cuda(), decoder.MoEWeights(router.cuda(), gate_up.cuda(), down.cuda(), top_k=1)).cpu().double()
+    assert torch.equal(y[:, 17], sign * math.inf)
+    assert torch.isfinite(y[:, :17]).all() and torch.isfinite(y[:, 18:]).all()
 
 
 def by_logits(gen, logits, tokens, dtype, width=32, inner=40, router_type=None):
@@ -185,6 +201,14 @@ def test_sample_at_low_temperatures(temperature):
         row = top - 10 * max(temperature, abs(top) * 2.0 ** -22) * torch.rand(50001, generator=gen)
         u = torch.rand(4000, generator=gen)
         check_draws(row, u, temperature)(decoder.sample(row.cuda().expand(u.numel(), row.numel()), u.cuda(), temperature=temperature))
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-4, 1e-5])
+def test_sample_filters_at_low_temperatures(temperature):
+    gen = torch.Generator().manual_seed(8)
+    logits = 30 + max(3 * temperature, 1e-4) * torch.randn((20, 5001), generator=gen)
+    for kw in (dict(), dict(top_k=40), dict(top_k=1000), dict(top_p=0.9), dict(top_p=0.3), dict(min_p=0.05), dict(top_k=400, top_p=0.8, min_p=0.001)):
+        check_sample(logits, torch.rand(20, generator=gen), temperature=temperature, **kw)
 
 
 # ---- residual norms --------------------------------------------------------------------------
