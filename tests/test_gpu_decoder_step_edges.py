@@ -10,7 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from shorokoo_b200 import B200ArgumentError, B200NotSupportedError, decoder
-from test_gpu_decoder_step import BF16, FP16, FP32, U, V, check_moe, check_sample, half, layer, moe_reference, norm_reference, normal, rounded, within
+from test_gpu_decoder_step import BF16, FP16, FP32, U, V, check_moe, check_sample, half, layer, norm_reference, normal, rounded, within
 
 pytestmark = pytest.mark.gpu
 
